@@ -613,6 +613,98 @@ int nkv_fast_finish(const void* native, const float* native_lse, const void* lif
                     int64_t rows, int total_heads, int group_heads, int d, int dtype, void* out,
                     float* out_lse, void* stream);
 
+/* ------------------------------------------------- 8-bit block cache */
+
+/*
+ * A cache of keys and values that tokens enter one at a time or in chunks, without trained operators; several
+ * sequences of unlike lengths, query heads grouped over kv heads.  A sequence and kv head own `blocks` slots of
+ * NKV_BLOCK tokens.  Token t lies in logical block t / NKV_BLOCK, whose slot is table[t / NKV_BLOCK].  A full block holds
+ * 8-bit codes (code + 128, code in -127 .. 127) and one scale each for K and V: value = code * scale,
+ * scale = max |x| / 127 over the block's NKV_BLOCK x head_dim elements, code = rint(x / scale) (scale and quotient
+ * rounded to fp32, ties to even; all codes 0 where the scale is 0).  V is stored transposed, so that the tokens a product with V runs over lie
+ * together.  The tokens of the open block (lengths[b] % NKV_BLOCK of them) are kept as they came, in `dtype`, and are
+ * quantised once, when the block is complete: a cache does not depend on how its tokens were cut into calls.
+ * A token with an element that is not finite is held with NaN keys and zero values, and a block with such a token
+ * has a NaN key scale and a zero value scale: queries that see it get NaN, others are not touched.
+ * Arrays over [batch][kv_heads]; device memory except `lengths`.  Not in the reference, whose caches hold whole chunks.
+ */
+#define NKV_BLOCK 64
+typedef struct nkv_block_cache {
+  uint8_t* k_codes;         /* [blocks][NKV_BLOCK][head_dim] per sequence and head, by slot; 16-byte aligned */
+  uint8_t* v_codes;         /* [blocks][head_dim][NKV_BLOCK], by slot; 16-byte aligned */
+  float*   scales;          /* [blocks][2]  K and V scale, by slot; 8-byte aligned */
+  const int32_t* table;     /* [blocks]  slot of every logical block: a permutation of 0 .. blocks-1 */
+  void*    k_tail;          /* [NKV_BLOCK][head_dim] in dtype: keys of the open block; 16-byte aligned */
+  void*    v_tail;          /* [head_dim][NKV_BLOCK] in dtype: its values; 16-byte aligned */
+  const int32_t* lengths;   /* HOST [batch]: tokens of every sequence */
+  int32_t batch, kv_heads, head_dim, blocks;   /* head_dim 64 | 128 */
+  int32_t dtype;            /* NKV_BF16 | NKV_F16 */
+} nkv_block_cache;
+
+/* Rows [batch, tokens, heads, head_dim] with strides in elements; elements of a row lie together. */
+typedef struct nkv_tokens {
+  const void* data;
+  int64_t stride_batch, stride_token, stride_head;
+  int32_t heads;
+} nkv_tokens;
+
+/*
+ * Rotary positions.  table f32 [rows][rotary_dim/2][2]: cosine and sine of every position's angles (scalings for long
+ * contexts are in the table).  The first rotary_dim elements of a head row are pairs (x0, x1): elements (i, i +
+ * rotary_dim/2) in the half layout, (2i, 2i+1) in the interleaved one; y0 = x0 c - x1 s, y1 = x0 s + x1 c, products and
+ * sum rounded to fp32 one by one, one rounding to the rows' type.  positions i32 [batch][tokens]; a position outside the
+ * table makes the rotated elements NaN.
+ */
+#define NKV_ROTARY_HALF        0
+#define NKV_ROTARY_INTERLEAVED 1
+typedef struct nkv_rotation {
+  const float* table;
+  const int32_t* positions;
+  int32_t rows, rotary_dim, layout;
+} nkv_rotation;
+
+/* Rows of x (and of y, or NULL) rotated: out_x, out_y [batch, tokens, heads, head_dim] contiguous, in `dtype`
+ * (NKV_F32 | NKV_BF16 | NKV_F16); elements past rotary_dim are copied.  transposed: with -s for s, the direction that a
+ * gradient takes.  An output may be its own contiguous input. */
+int nkv_rotary(const nkv_tokens* x, void* out_x, const nkv_tokens* y, void* out_y, int dtype, int batch, int tokens,
+               int head_dim, const nkv_rotation* rotation, int transposed, void* stream);
+
+/* The first counts[b] tokens (HOST [batch]; NULL: all `tokens`) of k and v [batch, tokens, kv_heads, head_dim] put
+ * behind the lengths[b] tokens of every sequence, keys rotated on the way unless rotation is NULL (rotary_dim a multiple
+ * of 16).  The caller advances its lengths afterwards. */
+int nkv_block_append(const nkv_block_cache* cache, const nkv_tokens* k, const nkv_tokens* v, int tokens,
+                     const int32_t* counts, const nkv_rotation* rotation, void* stream);
+
+/* Values of tokens [start, stop) as rows k_out, v_out [batch, stop - start, kv_heads, head_dim] in the cache's dtype (code *
+ * scale rounded once); zero past a sequence's length. */
+int nkv_block_read(const nkv_block_cache* cache, int start, int stop, void* k_out, void* v_out, void* stream);
+
+/*
+ * Attention of q [batch, tokens, heads, head_dim] over the cache; heads a multiple of kv_heads, head h attends kv head
+ * h / (heads / kv_heads).  Query i of sequence b, of counts[b] (HOST; NULL: `tokens`), sees tokens
+ * j < lengths[b] - counts[b] + i + 1 (causal) or j < lengths[b]; queries past counts[b] see none.  out [batch, tokens, heads,
+ * head_dim] in dtype, lse f32 [batch, tokens, heads] natural log; a query that sees nothing has out 0 and lse -inf.
+ * block_weights f32 [batch][kv_heads][blocks] or NULL: += the probability that the queries of the kv head's group gave to
+ * every logical block, summed in an order that does not change.  workspace: nkv_block_attend_workspace_bytes(...)
+ * bytes of device scratch (16-byte aligned); status_word: device int32 as for the other reads.
+ */
+size_t nkv_block_attend_workspace_bytes(const nkv_block_cache* cache, int heads, int tokens, const int32_t* counts,
+                                        int causal, int with_weights);
+int nkv_block_attend(const nkv_block_cache* cache, const nkv_tokens* q, int tokens, const int32_t* counts, int causal,
+                     float scale, void* out, float* lse, float* block_weights, int32_t* status_word, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/*
+ * Room made in block tables: of the full[b] (HOST [batch]) full blocks of every sequence and kv head the first `sinks`, the
+ * last `recent` and, of the others, those of largest weight stay, `keep` in all (sinks + recent <= keep); equal weights: the
+ * lower index stays; NaN counts as larger than any number.  Kept entries come first, in order, then the open block's
+ * (partial[b] 1 | 0), then the freed ones, then the unused ones.  weights f32, table i32 [batch][kv_heads][blocks] ->
+ * weights_out (moved along, zero behind the live entries), table_out; outputs must not be the inputs.
+ */
+int nkv_block_evict(const float* weights, const int32_t* table, const int32_t* full, const int32_t* partial, int batch,
+                    int kv_heads, int blocks, int keep, int sinks, int recent, float* weights_out, int32_t* table_out,
+                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

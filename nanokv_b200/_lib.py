@@ -48,6 +48,26 @@ class Payload(ctypes.Structure):
                 ("tokens", c_int32), ("clusters", c_int32)]
 
 
+class BlockCache(ctypes.Structure):
+    """struct nkv_block_cache"""
+    _fields_ = [("k_codes", c_void_p), ("v_codes", c_void_p), ("scales", c_void_p), ("table", c_void_p),
+                ("k_tail", c_void_p), ("v_tail", c_void_p), ("lengths", POINTER(c_int32)),
+                ("batch", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("blocks", c_int32),
+                ("dtype", c_int32)]
+
+
+class Tokens(ctypes.Structure):
+    """struct nkv_tokens"""
+    _fields_ = [("data", c_void_p), ("stride_batch", c_int64), ("stride_token", c_int64), ("stride_head", c_int64),
+                ("heads", c_int32)]
+
+
+class Rotation(ctypes.Structure):
+    """struct nkv_rotation"""
+    _fields_ = [("table", c_void_p), ("positions", c_void_p), ("rows", c_int32), ("rotary_dim", c_int32),
+                ("layout", c_int32)]
+
+
 # name -> (restype, argtypes); every symbol the header declares
 SIGNATURES = {
     "nkv_status_string": (c_char_p, [c_int]),
@@ -142,6 +162,16 @@ SIGNATURES = {
     "nkv_cp_merge_peer": (c_int, [POINTER(c_void_p), POINTER(c_void_p), POINTER(c_void_p),
                                   POINTER(c_void_p), c_int, c_int64, c_int, c_int64, c_int64, c_int,
                                   c_void_p]),
+    "nkv_rotary": (c_int, [POINTER(Tokens), c_void_p, POINTER(Tokens), c_void_p, c_int, c_int, c_int, c_int,
+                           POINTER(Rotation), c_int, c_void_p]),
+    "nkv_block_append": (c_int, [POINTER(BlockCache), POINTER(Tokens), POINTER(Tokens), c_int, POINTER(c_int32),
+                                 POINTER(Rotation), c_void_p]),
+    "nkv_block_read": (c_int, [POINTER(BlockCache), c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "nkv_block_attend_workspace_bytes": (c_size_t, [POINTER(BlockCache), c_int, c_int, POINTER(c_int32), c_int, c_int]),
+    "nkv_block_attend": (c_int, [POINTER(BlockCache), POINTER(Tokens), c_int, POINTER(c_int32), c_int, c_float,
+                                 c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "nkv_block_evict": (c_int, [c_void_p, c_void_p, POINTER(c_int32), POINTER(c_int32), c_int, c_int, c_int, c_int,
+                                c_int, c_int, c_void_p, c_void_p, c_void_p]),
 }
 
 _EXCEPTIONS = {NKV_ERR_INVALID: ValueError, NKV_ERR_TOO_LARGE: ValueError}

@@ -716,4 +716,131 @@ int nkv_history_moments(const nkv_history* hist, float* latent_sum, int32_t* cen
                          static_cast<cudaStream_t>(stream));
 }
 
+static int check_rotation(const nkv_rotation* r, int head_dim, const char* name) {
+  NKV_REQUIRE(r->rows > 0 && r->table && r->positions, NKV_ERR_INVALID, "%s: rotation of %d rows without its arrays", name, r->rows);
+  NKV_REQUIRE(r->rotary_dim > 0 && r->rotary_dim % 2 == 0 && r->rotary_dim <= head_dim, NKV_ERR_INVALID,
+              "%s: rotary_dim %d must be even and at most the head width %d", name, r->rotary_dim, head_dim);
+  NKV_REQUIRE(r->layout == NKV_ROTARY_HALF || r->layout == NKV_ROTARY_INTERLEAVED, NKV_ERR_INVALID, "%s: layout %d", name, r->layout);
+  NKV_REQUIRE((reinterpret_cast<uintptr_t>(r->table) & 7) == 0, NKV_ERR_INVALID, "%s: the table must be 8-byte aligned", name);
+  return NKV_OK;
+}
+
+static int check_block_cache(const nkv_block_cache* c, const char* name) {
+  NKV_REQUIRE(c != nullptr, NKV_ERR_INVALID, "%s: cache is NULL", name);
+  NKV_REQUIRE(c->batch >= 0 && c->kv_heads > 0 && c->kv_heads <= 65535 && c->blocks > 0 && c->blocks <= (1 << 24), NKV_ERR_INVALID,
+              "%s: batch=%d kv_heads=%d blocks=%d", name, c->batch, c->kv_heads, c->blocks);
+  NKV_REQUIRE(c->head_dim == 64 || c->head_dim == 128, NKV_ERR_UNSUPPORTED, "%s: head width %d (64 and 128 are built)", name, c->head_dim);
+  NKV_REQUIRE(c->dtype == NKV_BF16 || c->dtype == NKV_F16, NKV_ERR_INVALID, "%s: the cache's dtype must be bf16 or fp16", name);
+  NKV_REQUIRE(c->k_codes && c->v_codes && c->scales && c->table && c->k_tail && c->v_tail && (c->lengths || c->batch == 0),
+              NKV_ERR_INVALID, "%s: cache with missing arrays", name);
+  NKV_REQUIRE(((reinterpret_cast<uintptr_t>(c->k_codes) | reinterpret_cast<uintptr_t>(c->v_codes) |
+                reinterpret_cast<uintptr_t>(c->k_tail) | reinterpret_cast<uintptr_t>(c->v_tail)) & 15) == 0 &&
+                  (reinterpret_cast<uintptr_t>(c->scales) & 7) == 0,
+              NKV_ERR_INVALID, "%s: codes and tails must be 16-byte aligned, scales 8-byte aligned", name);
+  for (int b = 0; b < c->batch; ++b)
+    NKV_REQUIRE(c->lengths[b] >= 0 && c->lengths[b] <= c->blocks * NKV_BLOCK, NKV_ERR_INVALID,
+                "%s: sequence %d holds %d tokens in %d blocks", name, b, c->lengths[b], c->blocks);
+  return NKV_OK;
+}
+
+static int check_counts(const nkv_block_cache* c, int tokens, const int32_t* counts, const char* name) {
+  NKV_REQUIRE(tokens >= 0, NKV_ERR_INVALID, "%s: tokens=%d", name, tokens);
+  for (int b = 0; counts && b < c->batch; ++b)
+    NKV_REQUIRE(counts[b] >= 0 && counts[b] <= tokens, NKV_ERR_INVALID, "%s: sequence %d has %d of %d tokens", name, b, counts[b], tokens);
+  return NKV_OK;
+}
+
+int nkv_rotary(const nkv_tokens* x, void* out_x, const nkv_tokens* y, void* out_y, int dtype, int batch, int tokens,
+               int head_dim, const nkv_rotation* rotation, int transposed, void* stream) {
+  NKV_REQUIRE(x && rotation && batch >= 0 && tokens >= 0 && head_dim > 0, NKV_ERR_INVALID, "rotary: batch=%d tokens=%d head width %d",
+              batch, tokens, head_dim);
+  NKV_REQUIRE(dtype == NKV_F32 || dtype == NKV_BF16 || dtype == NKV_F16, NKV_ERR_INVALID, "rotary: dtype %d", dtype);
+  NKV_REQUIRE(x->heads >= 0 && (!y || y->heads >= 0), NKV_ERR_INVALID, "rotary: heads");
+  if (batch == 0 || tokens == 0 || x->heads + (y ? y->heads : 0) == 0) return NKV_OK;
+  int rc = check_rotation(rotation, head_dim, "rotary");
+  if (rc != NKV_OK) return rc;
+  NKV_REQUIRE((x->heads == 0 || (x->data && out_x)) && (!y || y->heads == 0 || (y->data && out_y)), NKV_ERR_INVALID, "rotary: rows without data");
+  return rotary(*x, out_x, y, out_y, dtype, batch, tokens, head_dim, *rotation, transposed != 0, static_cast<cudaStream_t>(stream));
+}
+
+int nkv_block_append(const nkv_block_cache* cache, const nkv_tokens* k, const nkv_tokens* v, int tokens,
+                     const int32_t* counts, const nkv_rotation* rotation, void* stream) {
+  int rc = check_block_cache(cache, "block_append");
+  if (rc == NKV_OK) rc = check_counts(cache, tokens, counts, "block_append");
+  if (rc != NKV_OK) return rc;
+  for (int b = 0; b < cache->batch; ++b)
+    NKV_REQUIRE(static_cast<int64_t>(cache->lengths[b]) + (counts ? counts[b] : tokens) <= static_cast<int64_t>(cache->blocks) * NKV_BLOCK,
+                NKV_ERR_TOO_LARGE, "block_append: sequence %d: %d tokens and %d more do not fit %d blocks of %d", b,
+                cache->lengths[b], counts ? counts[b] : tokens, cache->blocks, NKV_BLOCK);
+  if (tokens == 0 || cache->batch == 0) return NKV_OK;
+  NKV_REQUIRE(k && v && k->data && v->data, NKV_ERR_INVALID, "block_append: no rows");
+  NKV_REQUIRE(k->heads == cache->kv_heads && v->heads == cache->kv_heads, NKV_ERR_INVALID, "block_append: %d and %d heads for a cache of %d",
+              k->heads, v->heads, cache->kv_heads);
+  if (rotation) {
+    rc = check_rotation(rotation, cache->head_dim, "block_append");
+    if (rc != NKV_OK) return rc;
+    NKV_REQUIRE(rotation->rotary_dim % 16 == 0, NKV_ERR_INVALID, "block_append: rotary_dim %d must be a multiple of 16", rotation->rotary_dim);
+  }
+  return block_append(*cache, *k, *v, tokens, counts, rotation, static_cast<cudaStream_t>(stream));
+}
+
+int nkv_block_read(const nkv_block_cache* cache, int start, int stop, void* k_out, void* v_out, void* stream) {
+  int rc = check_block_cache(cache, "block_read");
+  if (rc != NKV_OK) return rc;
+  NKV_REQUIRE(0 <= start && start <= stop && stop <= cache->blocks * NKV_BLOCK, NKV_ERR_INVALID, "block_read: tokens %d to %d of %d blocks",
+              start, stop, cache->blocks);
+  if (start == stop || cache->batch == 0) return NKV_OK;
+  NKV_REQUIRE(k_out && v_out && ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) == 0, NKV_ERR_INVALID,
+              "block_read: results must be 16-byte aligned");
+  return block_read(*cache, start, stop, k_out, v_out, static_cast<cudaStream_t>(stream));
+}
+
+static int check_attend(const nkv_block_cache* cache, int heads, int tokens, const int32_t* counts) {
+  int rc = check_block_cache(cache, "block_attend");
+  if (rc == NKV_OK) rc = check_counts(cache, tokens, counts, "block_attend");
+  if (rc != NKV_OK) return rc;
+  NKV_REQUIRE(heads > 0 && heads % cache->kv_heads == 0, NKV_ERR_INVALID, "block_attend: %d query heads over %d kv heads", heads, cache->kv_heads);
+  NKV_REQUIRE(static_cast<int64_t>(tokens) * (heads / cache->kv_heads) <= (1 << 28), NKV_ERR_TOO_LARGE, "block_attend: %d tokens of %d heads", tokens, heads);
+  return NKV_OK;
+}
+
+size_t nkv_block_attend_workspace_bytes(const nkv_block_cache* cache, int heads, int tokens, const int32_t* counts, int causal,
+                                        int with_weights) {
+  if (check_attend(cache, heads, tokens, counts) != NKV_OK || tokens == 0 || cache->batch == 0) return 0;
+  return block_attend_workspace_bytes(*cache, heads, tokens, counts, causal != 0, with_weights != 0);
+}
+
+int nkv_block_attend(const nkv_block_cache* cache, const nkv_tokens* q, int tokens, const int32_t* counts, int causal,
+                     float scale, void* out, float* lse, float* block_weights, int32_t* status_word, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  NKV_REQUIRE(q != nullptr, NKV_ERR_INVALID, "block_attend: no queries");
+  int rc = check_attend(cache, q->heads, tokens, counts);
+  if (rc != NKV_OK) return rc;
+  if (tokens == 0 || cache->batch == 0) return NKV_OK;
+  NKV_REQUIRE(q->data && out && lse && status_word, NKV_ERR_INVALID, "block_attend: queries, results or status word missing");
+  NKV_REQUIRE((reinterpret_cast<uintptr_t>(out) & 15) == 0, NKV_ERR_INVALID, "block_attend: results must be 16-byte aligned");
+  const size_t need = block_attend_workspace_bytes(*cache, q->heads, tokens, counts, causal != 0, block_weights != nullptr);
+  NKV_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0), NKV_ERR_INVALID,
+              "block_attend: workspace of %zu bytes is too small or not 16-byte aligned (%zu)", workspace_bytes, need);
+  return block_attend(*cache, *q, tokens, counts, causal != 0, scale, out, lse, block_weights, status_word, workspace,
+                      static_cast<cudaStream_t>(stream));
+}
+
+int nkv_block_evict(const float* weights, const int32_t* table, const int32_t* full, const int32_t* partial, int batch,
+                    int kv_heads, int blocks, int keep, int sinks, int recent, float* weights_out, int32_t* table_out,
+                    void* stream) {
+  NKV_REQUIRE(batch >= 0 && kv_heads >= 0 && kv_heads <= 65535 && blocks > 0 && blocks <= (1 << 24), NKV_ERR_INVALID, "block_evict: batch=%d kv_heads=%d blocks=%d",
+              batch, kv_heads, blocks);
+  NKV_REQUIRE(sinks >= 0 && recent >= 0 && static_cast<int64_t>(sinks) + recent <= keep, NKV_ERR_INVALID,
+              "block_evict: %d first and %d last blocks of %d to keep", sinks, recent, keep);
+  if (batch == 0 || kv_heads == 0) return NKV_OK;
+  NKV_REQUIRE(weights && table && full && partial && weights_out && table_out && weights != weights_out && table != table_out, NKV_ERR_INVALID,
+              "block_evict: missing arrays, or results in place of the inputs");
+  for (int b = 0; b < batch; ++b)
+    NKV_REQUIRE(full[b] >= 0 && (partial[b] == 0 || partial[b] == 1) && full[b] + partial[b] <= blocks, NKV_ERR_INVALID,
+                "block_evict: sequence %d has %d full and %d open blocks of %d", b, full[b], partial[b], blocks);
+  return block_evict(weights, table, full, partial, batch, kv_heads, blocks, keep, sinks, recent, weights_out, table_out,
+                     static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

@@ -1,0 +1,57 @@
+// What the kernels of the 8-bit block cache share.
+#pragma once
+
+#include <math_constants.h>
+
+#include "nkv_common.cuh"
+
+namespace nkv {
+
+constexpr int MAX_SEQUENCES = 128;   // sequences of one launch; longer batches are cut
+
+// lengths and token counts of a launch's sequences, passed by value
+struct Sequences {
+  int32_t length[MAX_SEQUENCES];
+  int32_t count[MAX_SEQUENCES];
+};
+
+// device arrays of nkv_block_cache from one of its sequences on
+struct BlockArrays {
+  uint8_t* k_codes;
+  uint8_t* v_codes;
+  float* scales;
+  const int32_t* table;
+  void* k_tail;
+  void* v_tail;
+  int kv_heads, blocks;
+};
+BlockArrays block_arrays(const nkv_block_cache& c, int first);
+
+// slot of a logical block among all slots; an entry outside the row's slots is taken to its end, never followed out of the arrays
+__device__ __forceinline__ size_t slot_of(const BlockArrays& c, size_t bh, int block) {
+  return bh * c.blocks + min(static_cast<unsigned>(__ldg(c.table + bh * c.blocks + block)), static_cast<unsigned>(c.blocks - 1));
+}
+
+template <int DT> struct Elem { using type = uint16_t; };
+template <> struct Elem<NKV_F32> { using type = float; };
+
+// two 16-bit elements of a word, the even one in the low half
+template <int DT>
+__device__ __forceinline__ float2 unpack2(uint32_t w) {
+  if (DT == NKV_BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if (DT == NKV_BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// value of a stored byte: 2^23 + byte is an fp32 number whose low mantissa bits are the byte
+__device__ __forceinline__ float code_value(uint32_t byte) { return __uint_as_float(0x4B000000u | byte) - 8388736.0f; }
+
+}  // namespace nkv

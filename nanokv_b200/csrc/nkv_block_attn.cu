@@ -1,0 +1,196 @@
+// Attention over the 8-bit block cache.
+#include "nkv_block.cuh"
+#include "nkv_internal.h"
+
+namespace nkv {
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// One call, from one of its sequences on.  The queries of a kv head are rows r = token * group + (head within the group).
+struct Call {
+  const uint16_t* q;
+  long long q_batch, q_token, q_head;
+  uint16_t* out;
+  float* lse;
+  float* partial;      // log2 of every (row, block)'s weight sum, or NULL: [sequence][kv head][most blocks][rows]
+  float* weights;      // block weights to add to
+  int tokens, heads, group, rows, causal, most_blocks;
+  float scale_log2;    // scale * log2(e)
+};
+
+// tokens that row r of a sequence sees
+__device__ __forceinline__ int visible_to(const Call& a, int length, int count, int r) {
+  const int t = r / a.group;
+  if (t >= count) return 0;
+  return a.causal ? max(0, min(length, length - count + t + 1)) : length;
+}
+
+// ---- CUDA cores ------------------------------------------------------------------------------------------------
+
+// The formula as it stands, in fp32: a warp per row, the rows of a block share its dequantised K and V.  Runs where the
+// tensor-core kernels are switched off, to check them.
+constexpr int ROWS = 8;
+template <int DT, int D>
+__global__ void __launch_bounds__(32 * ROWS)
+attend_plain_kernel(BlockArrays c, Call a, Sequences seqs) {
+  extern __shared__ float smem[];
+  float* const ks = smem;                            // [64][D + 1]
+  float* const vs = ks + NKV_BLOCK * (D + 1);        // [D][65]
+  float* const qs = vs + D * (NKV_BLOCK + 1);        // [ROWS][D]
+  float* const ps = qs + ROWS * D;                   // [ROWS][64]
+  const int b = blockIdx.z, h = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int length = seqs.length[b], count = seqs.count[b];
+  const int r = blockIdx.x * ROWS + warp;
+  const size_t bh = static_cast<size_t>(b) * c.kv_heads + h;
+  const bool row = r < a.rows;
+  const int token = r / a.group, head = h * a.group + r % a.group;
+  const int seen = row ? visible_to(a, length, count, r) : 0;
+  const int last = min(a.rows, (static_cast<int>(blockIdx.x) + 1) * ROWS) - 1;
+  const int seen_most = a.causal ? visible_to(a, length, count, min(last, count * a.group - 1)) : (count > 0 ? length : 0);
+  if (row)
+    for (int d = lane; d < D; d += 32)
+      qs[warp * D + d] = load_float(a.q, DT, b * a.q_batch + token * a.q_token + head * a.q_head + d);
+  float m = -INFINITY, l = 0.f, o[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) o[i] = 0.f;
+  for (int t0 = 0; t0 < seen_most; t0 += NKV_BLOCK) {
+    const int block = t0 / NKV_BLOCK;
+    __syncthreads();
+    if (t0 + NKV_BLOCK <= length) {
+      const size_t slot = slot_of(c, bh, block);
+      const float k_scale = c.scales[2 * slot], v_scale = c.scales[2 * slot + 1];
+      for (int i = threadIdx.x; i < NKV_BLOCK * D; i += 32 * ROWS) {
+        ks[i / D * (D + 1) + i % D] = code_value(c.k_codes[slot * NKV_BLOCK * D + i]) * k_scale;
+        vs[i / NKV_BLOCK * (NKV_BLOCK + 1) + i % NKV_BLOCK] = code_value(c.v_codes[slot * NKV_BLOCK * D + i]) * v_scale;
+      }
+    } else {
+      const size_t tail = bh * NKV_BLOCK * D;
+      for (int i = threadIdx.x; i < NKV_BLOCK * D; i += 32 * ROWS) {
+        ks[i / D * (D + 1) + i % D] = t0 + i / D < length ? load_float(c.k_tail, DT, tail + i) : 0.f;
+        vs[i / NKV_BLOCK * (NKV_BLOCK + 1) + i % NKV_BLOCK] = t0 + i % NKV_BLOCK < length ? load_float(c.v_tail, DT, tail + i) : 0.f;
+      }
+    }
+    __syncthreads();
+    if (t0 >= seen) continue;
+    float s[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int t = lane + 32 * j;
+      float dot = 0.f;
+      for (int d = 0; d < D; ++d) dot = fmaf(qs[warp * D + d], ks[t * (D + 1) + d], dot);
+      s[j] = t0 + t < seen ? dot * a.scale_log2 : -INFINITY;
+    }
+    // NaN has to reach the row: the maximum of a NaN and a number is the number
+    float top = fmaxf(s[0], s[1]);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    const float next = fmaxf(m, top), ref = next == -INFINITY ? 0.f : next;
+    const float alpha = exp2f(m - ref), p0 = exp2f(s[0] - ref), p1 = exp2f(s[1] - ref);
+    float sum = p0 + p1;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    if (a.partial && lane == 0) a.partial[(bh * a.most_blocks + block) * a.rows + r] = log2f(sum) + ref;
+    l = l * alpha + sum;
+    m = next;
+    ps[warp * NKV_BLOCK + lane] = p0;
+    ps[warp * NKV_BLOCK + lane + 32] = p1;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      float acc = o[i] * alpha;
+      for (int t = 0; t < NKV_BLOCK; ++t) acc = fmaf(ps[warp * NKV_BLOCK + t], vs[(lane + 32 * i) * (NKV_BLOCK + 1) + t], acc);
+      o[i] = acc;
+    }
+    __syncwarp();
+  }
+  if (!row) return;
+  const size_t at = (static_cast<size_t>(b) * a.tokens + token) * a.heads + head;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) store_float(a.out, DT, at * D + lane + 32 * i, seen > 0 ? o[i] / l : 0.f);
+  if (lane == 0) a.lse[at] = seen > 0 ? (m + log2f(l)) * LN2 : -INFINITY;
+}
+
+// weights[block] += sum over rows of 2^(partial - lse): a thread block per (block, kv head, sequence), rows in a fixed order
+__global__ void __launch_bounds__(256)
+block_weights_kernel(BlockArrays c, Call a, Sequences seqs) {
+  __shared__ float sums[8];
+  const int block = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int length = seqs.length[b], count = seqs.count[b];
+  if (block * NKV_BLOCK >= length) return;
+  const size_t bh = static_cast<size_t>(b) * c.kv_heads + h;
+  const float* partial = a.partial + (bh * a.most_blocks + block) * a.rows;
+  float sum = 0.f;
+  for (int r = threadIdx.x; r < a.rows; r += 256) {
+    if (visible_to(a, length, count, r) <= block * NKV_BLOCK) continue;
+    const float lse = a.lse[(static_cast<size_t>(b) * a.tokens + r / a.group) * a.heads + h * a.group + r % a.group];
+    sum += exp2f(partial[r] - lse * LOG2E);
+  }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x / 32] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float total = 0.f;
+    for (int w = 0; w < 8; ++w) total += sums[w];
+    a.weights[bh * c.blocks + block] += total;
+  }
+}
+
+int most_blocks_of(const nkv_block_cache& c) {
+  int most = 0;
+  for (int i = 0; i < c.batch; ++i) most = max(most, ceil_div(c.lengths[i], NKV_BLOCK));
+  return most;
+}
+
+}  // namespace
+
+size_t block_attend_workspace_bytes(const nkv_block_cache& c, int heads, int tokens, const int32_t* counts, bool causal,
+                                    bool with_weights) {
+  const size_t rows = static_cast<size_t>(tokens) * (heads / c.kv_heads);
+  return with_weights ? static_cast<size_t>(min(c.batch, MAX_SEQUENCES)) * c.kv_heads * most_blocks_of(c) * rows * 4 : 0;
+}
+
+int block_attend(const nkv_block_cache& c, const nkv_tokens& q, int tokens, const int32_t* counts, bool causal, float scale,
+                 void* out, float* lse, float* weights, int32_t* status, void* workspace, cudaStream_t stream) {
+  for (int first = 0; first < c.batch; first += MAX_SEQUENCES) {
+    const int n = min(MAX_SEQUENCES, c.batch - first);
+    Sequences seqs;
+    for (int i = 0; i < n; ++i) {
+      seqs.length[i] = c.lengths[first + i];
+      seqs.count[i] = counts ? counts[first + i] : tokens;
+    }
+    Call a;
+    a.q = static_cast<const uint16_t*>(q.data) + first * q.stride_batch;
+    a.q_batch = q.stride_batch;
+    a.q_token = q.stride_token;
+    a.q_head = q.stride_head;
+    a.out = static_cast<uint16_t*>(out) + static_cast<size_t>(first) * tokens * q.heads * c.head_dim;
+    a.lse = lse + static_cast<size_t>(first) * tokens * q.heads;
+    a.partial = weights ? static_cast<float*>(workspace) : nullptr;
+    a.weights = weights ? weights + static_cast<size_t>(first) * c.kv_heads * c.blocks : nullptr;
+    a.tokens = tokens;
+    a.heads = q.heads;
+    a.group = q.heads / c.kv_heads;
+    a.rows = tokens * a.group;
+    a.causal = causal;
+    a.most_blocks = most_blocks_of(c);
+    a.scale_log2 = scale * LOG2E;
+    const BlockArrays arrays = block_arrays(c, first);
+    auto kernel = c.head_dim == 128
+                      ? (c.dtype == NKV_BF16 ? attend_plain_kernel<NKV_BF16, 128> : attend_plain_kernel<NKV_F16, 128>)
+                      : (c.dtype == NKV_BF16 ? attend_plain_kernel<NKV_BF16, 64> : attend_plain_kernel<NKV_F16, 64>);
+    const size_t smem = sizeof(float) * (NKV_BLOCK * (c.head_dim + 1) + c.head_dim * (NKV_BLOCK + 1) +
+                                         ROWS * (c.head_dim + NKV_BLOCK));
+    NKV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    kernel<<<dim3(ceil_div(a.rows, ROWS), c.kv_heads, n), 32 * ROWS, smem, stream>>>(arrays, a, seqs);
+    NKV_LAUNCH_CHECK("attend_plain_kernel");
+    if (weights && a.most_blocks > 0) {
+      block_weights_kernel<<<dim3(a.most_blocks, c.kv_heads, n), 256, 0, stream>>>(arrays, a, seqs);
+      NKV_LAUNCH_CHECK("block_weights_kernel");
+    }
+  }
+  return NKV_OK;
+}
+
+}  // namespace nkv

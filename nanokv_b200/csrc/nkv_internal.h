@@ -68,6 +68,19 @@ int cp_merge_peer(const void* const* part_out, const float* const* part_lse, voi
                   int64_t row_end, int dtype, cudaStream_t stream, int32_t* const* flags = nullptr,
                   int rank = 0, int epoch = 0, long long budget_cycles = 0, int32_t* status = nullptr);
 
+// ---- 8-bit block cache (nkv_block_cache.cu, nkv_block_attn.cu); arguments are checked by the caller
+int rotary(const nkv_tokens& x, void* out_x, const nkv_tokens* y, void* out_y, int dtype, int batch, int tokens, int d,
+           const nkv_rotation& rotation, bool transposed, cudaStream_t stream);
+int block_append(const nkv_block_cache& c, const nkv_tokens& k, const nkv_tokens& v, int tokens, const int32_t* counts,
+                 const nkv_rotation* rotation, cudaStream_t stream);
+int block_read(const nkv_block_cache& c, int start, int stop, void* k_out, void* v_out, cudaStream_t stream);
+size_t block_attend_workspace_bytes(const nkv_block_cache& c, int heads, int tokens, const int32_t* counts, bool causal,
+                                    bool with_weights);
+int block_attend(const nkv_block_cache& c, const nkv_tokens& q, int tokens, const int32_t* counts, bool causal, float scale,
+                 void* out, float* lse, float* weights, int32_t* status, void* workspace, cudaStream_t stream);
+int block_evict(const float* weights, const int32_t* table, const int32_t* full, const int32_t* partial, int batch, int kv_heads,
+                int blocks, int keep, int sinks, int recent, float* weights_out, int32_t* table_out, cudaStream_t stream);
+
 // ---- tcgen05 / TMA kernels (nkv_tc_*.cu), bf16 operands, fp32 accumulation
 int tc_assign(const void* x_bf16, const void* centers_bf16, int S, int J, int C, void* ids,
               int id_bytes, cudaStream_t stream);

@@ -703,3 +703,117 @@ def force_simt(on: bool) -> None:
     """Triage hook: run bf16 work on the fp32 CUDA-core kernels (same rounding points)."""
     _SIMT_FORCED[0] = bool(on)
     _lib.check(_lib.library().nkv_set_bf16_path(1 if on else 0))
+
+
+# ------------------------------------------------------------------ 8-bit block cache
+BLOCK = 64   # tokens of a block (NKV_BLOCK)
+_LAYOUTS = {"half": 0, "interleaved": 1}
+
+
+def _rows(x: torch.Tensor, name: str, dtype: torch.dtype | None = None) -> _lib.Tokens:
+    """Rows [batch, tokens, heads, width] as the ABI takes them, whatever their strides but the last."""
+    if not x.is_cuda:
+        raise RuntimeError("nanokv_b200 runs on CUDA tensors only (there is no CPU path)")
+    if x.dim() != 4 or (x.stride(3) != 1 and x.shape[3] > 1):
+        raise ValueError(f"{name} must be [batch, tokens, heads, width], contiguous along the width")
+    if dtype is not None and x.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, not {x.dtype}")
+    return _lib.Tokens(x.data_ptr(), x.stride(0), x.stride(1), x.stride(2), x.shape[2])
+
+
+def _host_ints(values, count: int, name: str):
+    """Host integers, one per sequence, as the ABI takes them."""
+    if values is None:
+        return None
+    if len(values) != count:
+        raise ValueError(f"{name} must name {count} sequences; got {len(values)}")
+    return (ctypes.c_int32 * count)(*values)
+
+
+def _check_positions(positions: torch.Tensor, batch: int, tokens: int, device: torch.device) -> None:
+    if positions is None or positions.dtype != torch.int32 or tuple(positions.shape) != (batch, tokens):
+        raise ValueError(f"positions must be int32 [{batch}, {tokens}]")
+    if not positions.is_contiguous() or positions.device != device:
+        raise ValueError("positions must be contiguous, on the rows' device")
+
+
+def rotation(table: torch.Tensor, positions: torch.Tensor, layout: str) -> _lib.Rotation:
+    """struct nkv_rotation over device tensors: table f32 [rows, rotary_dim/2, 2], positions i32."""
+    _require_cuda(table, positions)
+    if table.dtype != torch.float32 or table.dim() != 3 or table.shape[2] != 2:
+        raise ValueError("rotation table must be float32 [rows, rotary_dim/2, 2]")
+    if layout not in _LAYOUTS:
+        raise ValueError(f"layout must be one of {sorted(_LAYOUTS)}; got {layout!r}")
+    return _lib.Rotation(table.data_ptr(), positions.data_ptr(), table.shape[0], 2 * table.shape[1], _LAYOUTS[layout])
+
+
+def rotary(x: torch.Tensor, y: torch.Tensor | None, table: torch.Tensor, positions: torch.Tensor, *, layout: str = "half",
+           transposed: bool = False):
+    """Rows x (and y, or None) [batch, tokens, heads, width] rotated by positions i32 [batch, tokens] in one launch
+    (nkv_rotary) -> contiguous rows.  ``transposed`` is the direction a gradient takes."""
+    xs = _rows(x, "x")
+    batch, tokens, _, width = x.shape
+    ys = out_y = None
+    if y is not None:
+        ys = _rows(y, "y", x.dtype)
+        if y.shape[:2] != x.shape[:2] or y.shape[3] != width or y.device != x.device:
+            raise ValueError(f"x and y must share batch, tokens, width and device; got {tuple(x.shape)} and {tuple(y.shape)}")
+        out_y = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    _check_positions(positions, batch, tokens, x.device)
+    if table.device != x.device:
+        raise ValueError("the rotation table must be on the rows' device")
+    rot = rotation(table, positions, layout)
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.library().nkv_rotary(xs, _ptr(out), ys, _ptr(out_y), dtype_code(x.dtype), batch, tokens, width, rot,
+                                             int(transposed), _stream(x.device)))
+    return out if y is None else (out, out_y)
+
+
+def block_append(struct: _lib.BlockCache, k: torch.Tensor, v: torch.Tensor, *, counts=None,
+                 rotation: _lib.Rotation | None = None) -> None:
+    """Tokens k, v [batch, tokens, kv_heads, width] put behind what the cache holds (nkv_block_append)."""
+    _lib.check(_lib.library().nkv_block_append(struct, _rows(k, "k"), _rows(v, "v"), k.shape[1], counts, rotation,
+                                               _stream(k.device)))
+
+
+def block_read(struct: _lib.BlockCache, start: int, stop: int, *, dtype: torch.dtype, device: torch.device):
+    """Values of tokens [start, stop) of every sequence -> k, v [batch, stop - start, kv_heads, width] (nkv_block_read)."""
+    shape = (struct.batch, max(0, stop - start), struct.kv_heads, struct.head_dim)
+    k, v = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+    _lib.check(_lib.library().nkv_block_read(struct, start, stop, _ptr(k), _ptr(v), _stream(device)))
+    return k, v
+
+
+def block_attend(struct: _lib.BlockCache, q: torch.Tensor, *, counts=None, causal: bool, scale: float,
+                 weights: torch.Tensor | None = None, status: torch.Tensor | None = None):
+    """Attention of q [batch, tokens, heads, width] over the cache (nkv_block_attend) -> (O like q, lse f32 [batch, tokens,
+    heads]); ``weights`` f32 [batch, kv_heads, blocks] is added to."""
+    rows = _rows(q, "q")
+    lib = _lib.library()
+    tokens, heads = q.shape[1], q.shape[2]
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+    nbytes = lib.nkv_block_attend_workspace_bytes(struct, heads, tokens, counts, int(causal), int(weights is not None))
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    _lib.check(lib.nkv_block_attend(struct, rows, tokens, counts, int(causal), float(scale), _ptr(out), _ptr(lse), _ptr(weights),
+                                    _ptr(status_word(q.device) if status is None else status), _ptr(workspace), nbytes,
+                                    _stream(q.device)))
+    return out, lse
+
+
+def block_evict(weights: torch.Tensor, table: torch.Tensor, full, partial, *, keep: int, sinks: int = 0, recent: int = 0):
+    """Block tables [batch, kv_heads, blocks] with the blocks of least weight freed (nkv_block_evict) -> (table, weights).
+    ``full`` / ``partial``: full and open blocks of every sequence (host integers)."""
+    device = _require_cuda(weights, table)
+    if weights.dtype != torch.float32 or table.dtype != torch.int32 or weights.dim() != 3 or weights.shape != table.shape:
+        raise ValueError("weights must be float32 and table int32, both [batch, kv_heads, blocks]")
+    if table.device != device:
+        raise ValueError("weights and table must be on one device")
+    batch, kv_heads, blocks = table.shape
+    full, partial = _host_ints(full, batch, "full"), _host_ints(partial, batch, "partial")
+    table_out, weights_out = torch.empty_like(table), torch.empty_like(weights)
+    with torch.cuda.device(device):
+        _lib.check(_lib.library().nkv_block_evict(_ptr(weights), _ptr(table), full, partial, batch, kv_heads, blocks, int(keep),
+                                                  int(sinks), int(recent), _ptr(weights_out), _ptr(table_out), _stream(device)))
+    return table_out, weights_out
