@@ -54,4 +54,32 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // value of a stored byte: 2^23 + byte is an fp32 number whose low mantissa bits are the byte
 __device__ __forceinline__ float code_value(uint32_t byte) { return __uint_as_float(0x4B000000u | byte) - 8388736.0f; }
 
+// ---- attention ----
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// One call, from one of its sequences on.  The queries of a kv head are rows r = token * group + (head within the group).
+struct Call {
+  const uint16_t* q;
+  long long q_batch, q_token, q_head;
+  uint16_t* out;
+  float* lse;
+  float* partial;      // log2 of every (row, block)'s weight sum, or NULL: [sequence][kv head][most blocks][rows]
+  float* weights;      // block weights to add to
+  int tokens, heads, group, rows, causal, most_blocks;
+  float scale_log2;    // scale * log2(e)
+};
+
+// tokens that row r of a sequence sees
+__device__ __forceinline__ int visible_to(const Call& a, int length, int count, int r) {
+  const int t = r / a.group;
+  if (t >= count) return 0;
+  return a.causal ? max(0, min(length, length - count + t + 1)) : length;
+}
+
+// few rows per kv head (nkv_block_step.cu)
+bool block_step_supported(int rows);
+size_t block_step_bytes(const Sequences& seqs, int n, int kv_heads, int rows, int d);
+int block_step(const BlockArrays& c, const Call& a, const Sequences& seqs, int n, int dtype, int d, void* workspace, int32_t* status,
+               cudaStream_t stream);
+
 }  // namespace nkv

@@ -5,27 +5,6 @@
 namespace nkv {
 namespace {
 
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-
-// One call, from one of its sequences on.  The queries of a kv head are rows r = token * group + (head within the group).
-struct Call {
-  const uint16_t* q;
-  long long q_batch, q_token, q_head;
-  uint16_t* out;
-  float* lse;
-  float* partial;      // log2 of every (row, block)'s weight sum, or NULL: [sequence][kv head][most blocks][rows]
-  float* weights;      // block weights to add to
-  int tokens, heads, group, rows, causal, most_blocks;
-  float scale_log2;    // scale * log2(e)
-};
-
-// tokens that row r of a sequence sees
-__device__ __forceinline__ int visible_to(const Call& a, int length, int count, int r) {
-  const int t = r / a.group;
-  if (t >= count) return 0;
-  return a.causal ? max(0, min(length, length - count + t + 1)) : length;
-}
-
 // ---- CUDA cores ------------------------------------------------------------------------------------------------
 
 // The formula as it stands, in fp32: a warp per row, the rows of a block share its dequantised K and V.  Runs where the
@@ -143,23 +122,42 @@ int most_blocks_of(const nkv_block_cache& c) {
   return most;
 }
 
+Sequences sequences_of(const nkv_block_cache& c, int first, int n, const int32_t* counts, int tokens) {
+  Sequences s;
+  for (int i = 0; i < n; ++i) {
+    s.length[i] = c.lengths[first + i];
+    s.count[i] = counts ? counts[first + i] : tokens;
+  }
+  return s;
+}
+
+// scratch of one launch over n sequences: the rows' weight sums per block, then the kernel's own
+struct Scratch { size_t partial, own; };
+Scratch scratch_of(const nkv_block_cache& c, const Sequences& seqs, int n, int rows, int most_blocks, bool with_weights) {
+  Scratch s{0, 0};
+  if (with_weights) s.partial = (static_cast<size_t>(n) * c.kv_heads * most_blocks * rows * 4 + 255) & ~static_cast<size_t>(255);
+  if (!simt_forced() && block_step_supported(rows)) s.own = block_step_bytes(seqs, n, c.kv_heads, rows, c.head_dim);
+  return s;
+}
+
 }  // namespace
 
 size_t block_attend_workspace_bytes(const nkv_block_cache& c, int heads, int tokens, const int32_t* counts, bool causal,
                                     bool with_weights) {
-  const size_t rows = static_cast<size_t>(tokens) * (heads / c.kv_heads);
-  return with_weights ? static_cast<size_t>(min(c.batch, MAX_SEQUENCES)) * c.kv_heads * most_blocks_of(c) * rows * 4 : 0;
+  size_t most = 0;   // launches follow one another on the stream and share it
+  for (int first = 0; first < c.batch; first += MAX_SEQUENCES) {
+    const int n = min(MAX_SEQUENCES, c.batch - first);
+    const Scratch s = scratch_of(c, sequences_of(c, first, n, counts, tokens), n, tokens * (heads / c.kv_heads), most_blocks_of(c), with_weights);
+    if (s.partial + s.own > most) most = s.partial + s.own;
+  }
+  return most;
 }
 
 int block_attend(const nkv_block_cache& c, const nkv_tokens& q, int tokens, const int32_t* counts, bool causal, float scale,
                  void* out, float* lse, float* weights, int32_t* status, void* workspace, cudaStream_t stream) {
   for (int first = 0; first < c.batch; first += MAX_SEQUENCES) {
     const int n = min(MAX_SEQUENCES, c.batch - first);
-    Sequences seqs;
-    for (int i = 0; i < n; ++i) {
-      seqs.length[i] = c.lengths[first + i];
-      seqs.count[i] = counts ? counts[first + i] : tokens;
-    }
+    const Sequences seqs = sequences_of(c, first, n, counts, tokens);
     Call a;
     a.q = static_cast<const uint16_t*>(q.data) + first * q.stride_batch;
     a.q_batch = q.stride_batch;
@@ -177,6 +175,12 @@ int block_attend(const nkv_block_cache& c, const nkv_tokens& q, int tokens, cons
     a.most_blocks = most_blocks_of(c);
     a.scale_log2 = scale * LOG2E;
     const BlockArrays arrays = block_arrays(c, first);
+    void* const own = static_cast<uint8_t*>(workspace) + scratch_of(c, seqs, n, a.rows, a.most_blocks, weights != nullptr).partial;
+    if (!simt_forced() && block_step_supported(a.rows)) {
+      const int rc = block_step(arrays, a, seqs, n, c.dtype, c.head_dim, own, status, stream);
+      if (rc != NKV_OK) return rc;
+      continue;
+    }
     auto kernel = c.head_dim == 128
                       ? (c.dtype == NKV_BF16 ? attend_plain_kernel<NKV_BF16, 128> : attend_plain_kernel<NKV_F16, 128>)
                       : (c.dtype == NKV_BF16 ? attend_plain_kernel<NKV_BF16, 64> : attend_plain_kernel<NKV_F16, 64>);
