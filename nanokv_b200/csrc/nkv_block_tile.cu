@@ -1,0 +1,802 @@
+// Attention of many query rows over the 8-bit block cache, on tcgen05.
+//
+// The rows of a kv head (its group's heads of all query tokens) are cut into units of 256: two 128-row tiles that share
+// every K and V tile.  A tile is 128 tokens, two blocks of the cache.  Four warps read its codes, turn them into the
+// cache's 16-bit type (exactly: a code is an integer below 2^7) and store them as the swizzled operands the tensor cores
+// read; no 16-bit copy of the cache exists in memory.  S = Q K^T goes to tensor memory, eight warps take the softmax (one
+// thread per row), P replaces S as the operand of O += P V.  The block scales never touch an operand.  K's multiplies the
+// scores.  V's goes into the exponent: the weight handed over is P' = 2^(s + log2 vs - m'), with m' the running maximum of
+// s + log2 vs, so that a row's weights are at most 1 (2^8 with the lazy reference) however unlike the scales of its blocks are; a block's
+// part of the row sum is the sum of its P' divided by vs again, in fp32.
+//
+// The tiles of all units form one list that the SMs take in equal runs; a unit that a run's end cuts leaves fp32 parts,
+// joined by a second launch.  Warps: 0-7 softmax, 8-11 operands, 12 MMA issue.
+#include "nkv_block.cuh"
+#include "nkv_internal.h"
+#include "nkv_tc.cuh"
+
+namespace nkv {
+namespace {
+
+using namespace tc;
+
+constexpr int QT = 128, NQ = 2, UNIT = QT * NQ;   // rows of a query tile, tiles and rows of a unit
+constexpr int TOK = 128;                          // tokens of a tile
+constexpr int STAGES = 2;                         // K / V operand stages
+constexpr int SOFTMAX_WARPS = 8, OPERAND_WARPS = 4, THREADS = 512;   // four warpgroups: the last one has only the MMA warp at work
+constexpr int SUB = 128 * 128;                    // bytes of a [128 rows x 64 elements] swizzled operand tile
+constexpr float RESCALE_THRESHOLD = 8.0f;
+// log2(1 + 2^-9) and its factor's inverse: bf16 weights are rounded by raising them half a step (in the exponent) and
+// dropping the low bits, which leaves the quarter-rate conversion unit to the exponentials
+constexpr float HALF_STEP_LOG2 = 0.0028150156070540f, HALF_STEP_INV = 0.998050682261209f;
+
+enum Bar { Q_FULL = 0, Q_FREE = 1, K_FULL = 2, K_FREE = 4, V_FULL = 6, V_FREE = 8, S_FULL = 10, P_READY = 12, P_LAST = 14,
+           PV_DONE = 16, O_FREE = 18, META_FULL = 20, NUM_BARS = 24 };
+constexpr int NMETA = 4;
+constexpr int M_SLOT = NUM_BARS * 8, M_ABORT = M_SLOT + 4, M_SCALES = 256;   // scales: [NMETA][2 blocks] float4 {ks, log2 vs, 1 / vs, -}
+
+template <int D> struct Layout {
+  static constexpr int DCH = D / 64;
+  static constexpr int Q_OFF = 1024;
+  static constexpr int K_OFF = Q_OFF + NQ * DCH * SUB;
+  static constexpr int V_OFF = K_OFF + STAGES * DCH * SUB;
+  static constexpr int V_SUB = D * 128;            // [D rows x 64 tokens]
+  static constexpr int BYTES = V_OFF + STAGES * 2 * V_SUB;
+  static constexpr int DYNAMIC = BYTES + 1024;     // room to start on 1,024 bytes
+};
+static_assert(M_SCALES + NMETA * 2 * 16 <= 1024, "meta block");
+
+// The list of tiles: sequence by sequence, kv head by kv head, unit by unit.
+struct Plan {
+  uint32_t start[MAX_SEQUENCES + 1];
+  int sequences, runs, units;      // runs: thread blocks; units per kv head
+  uint32_t run, longer;            // tiles of a run; the first `longer` have one more
+  __host__ __device__ uint32_t first_of(uint32_t i) const { return i * run + min(i, longer); }
+  __host__ __device__ uint32_t run_of(uint32_t g) const {
+    const uint32_t edge = longer * (run + 1);
+    return g < edge ? g / (run + 1) : longer + (g - edge) / run;
+  }
+};
+
+// tokens that any of rows [0, r_end) ... of a query tile sees, as tiles: rows r0 .. r0 + n - 1 of `rows`
+__host__ __device__ inline int tiles_seen(int length, int count, int group, int rows, bool causal, int r0, int n) {
+  const int r1 = min(rows, r0 + n) - 1;
+  if (r1 < r0 || r0 / group >= count) return 0;
+  const int last = min(r1 / group, count - 1);
+  const int seen = causal ? min(length, length - count + last + 1) : length;
+  return seen > 0 ? (seen + TOK - 1) / TOK : 0;
+}
+
+struct Piece {                     // a unit, or a run's part of one
+  int b, h, unit, tile0, nt, whole;   // tiles tile0 .. tile0 + nt - 1; whole: all the unit has
+};
+
+// The pieces of one run in order; every role walks the same list.
+struct Walk {
+  uint32_t g, end;
+  int b, h, unit, tiles;           // the unit that g lies in, its tiles
+  uint32_t at;                     // tiles of the unit before g
+  __device__ __forceinline__ int tiles_of(const Call& a, const Sequences& s, int bb, int u) const {
+    return tiles_seen(s.length[bb], s.count[bb], a.group, a.rows, a.causal, u * UNIT, UNIT);
+  }
+  __device__ __forceinline__ Walk(const Plan& p, const Call& a, const Sequences& s, int run, int kv_heads) {
+    g = p.first_of(run);
+    end = p.first_of(run + 1);
+    int lo = 0, hi = p.sequences - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (p.start[mid] <= g) lo = mid; else hi = mid - 1;
+    }
+    b = lo;
+    const uint32_t per_head = (p.start[b + 1] - p.start[b]) / kv_heads;
+    at = g - p.start[b];
+    h = static_cast<int>(at / per_head);
+    at -= h * per_head;
+    unit = 0;
+    while (at >= static_cast<uint32_t>(tiles = tiles_of(a, s, b, unit))) {
+      at -= tiles;
+      ++unit;
+    }
+  }
+  __device__ __forceinline__ bool next(const Plan& p, const Call& a, const Sequences& s, int kv_heads, Piece& out) {
+    if (g >= end) return false;
+    while (at >= static_cast<uint32_t>(tiles)) {   // on to the next unit that has tiles
+      at = 0;
+      if (++unit == p.units) {
+        unit = 0;
+        if (++h == kv_heads) {
+          h = 0;
+          ++b;
+        }
+      }
+      tiles = tiles_of(a, s, b, unit);
+    }
+    out.b = b;
+    out.h = h;
+    out.unit = unit;
+    out.tile0 = static_cast<int>(at);
+    out.nt = static_cast<int>(min(static_cast<uint32_t>(tiles) - at, end - g));
+    out.whole = out.nt == tiles;
+    at += out.nt;
+    g += out.nt;
+    return true;
+  }
+};
+
+// tiles of a piece that query tile i takes part in (causal: the first tile sees less than the second)
+__device__ __forceinline__ int tiles_for(const Call& a, const Sequences& s, const Piece& p, int i) {
+  return max(0, min(p.nt, tiles_seen(s.length[p.b], s.count[p.b], a.group, a.rows, a.causal, p.unit * UNIT + i * QT, QT) - p.tile0));
+}
+
+// A run holds at most one piece that starts inside a unit and one that starts with it and is cut: two places each.
+struct Parts {
+  float* o;       // [2 runs][UNIT][D], relative to 2^m'
+  float2* ml;     // [2 runs][UNIT]
+};
+
+struct Ctx { volatile int* abort_flag; };
+
+// bounded wait of a whole warp; parks in the barrier unit so that waiting warps leave the issue slots to the others
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, const Ctx& c, int code) {
+  bool ok = true;
+  if (!mbar_try_wait(bar, parity)) {
+    const long long begin = clock64();
+    while (true) {
+      if (*c.abort_flag) { ok = false; break; }
+      if (mbar_try_wait_parked(bar, parity, 1000u)) break;
+      if (clock64() - begin > WAIT_BUDGET_CYCLES) {
+        atomicCAS(const_cast<int*>(c.abort_flag), 0, code);
+        ok = false;
+        break;
+      }
+    }
+  }
+  return __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
+}
+__device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
+
+template <int DT> __host__ __device__ constexpr uint32_t idesc(int n) {
+  return (1u << 4) | (DT == NKV_BF16 ? (1u << 7) | (1u << 10) : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// four codes (plus 128) as two 16-bit pairs, exactly.  fp16: 0x64 above a byte is 1024 + byte.  bf16 has room for seven
+// bits: 0x43 above them is 128 + low bits, and the top bit decides whether 128 or 256 is subtracted.
+template <int DT>
+__device__ __forceinline__ void expand(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (DT == NKV_F16) {
+    const __half2 off = __half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+    const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+    const __half2 ha = __hsub2(*reinterpret_cast<const __half2*>(&a), off), hb = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&ha);
+    hi = *reinterpret_cast<const uint32_t*>(&hb);
+  } else {
+    const uint32_t low = w & 0x7F7F7F7Fu, top = ~w & 0x80808080u;
+    const uint32_t a = __byte_perm(low, 0x43434343u, 0x4140), b = __byte_perm(low, 0x43434343u, 0x4342);
+    const uint32_t c = __byte_perm(top, 0x43434343u, 0x4140), d = __byte_perm(top, 0x43434343u, 0x4342);
+    const __nv_bfloat162 ha = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&c));
+    const __nv_bfloat162 hb = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&d));
+    lo = *reinterpret_cast<const uint32_t*>(&ha);
+    hi = *reinterpret_cast<const uint32_t*>(&hb);
+  }
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 16 codes as 32 bytes of an operand row: two pieces, columns col .. col + 15 (col a multiple of 16)
+template <int DT>
+__device__ __forceinline__ void store_codes(uint8_t* tile, int row, int col, const uint4& raw, bool swap) {
+  uint4 p0, p1;
+  expand<DT>(raw.x, p0.x, p0.y);
+  expand<DT>(raw.y, p0.z, p0.w);
+  expand<DT>(raw.z, p1.x, p1.y);
+  expand<DT>(raw.w, p1.z, p1.w);
+  const uint32_t a0 = sw128_offset(row, col), a1 = sw128_offset(row, col + 8);
+  // the eight lanes that store together shall fill all banks: half of them take their second piece first
+  const uint4 s0 = swap ? p1 : p0, s1 = swap ? p0 : p1;
+  *reinterpret_cast<uint4*>(tile + (swap ? a1 : a0)) = s0;
+  *reinterpret_cast<uint4*>(tile + (swap ? a0 : a1)) = s1;
+}
+
+// ---- warps 8-11: queries, K and V as operands -----------------------------------------------------------------
+template <int DT, int D>
+__device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, const BlockArrays& c, const Call& a, const Sequences& seqs,
+                                             const Plan& plan, const Ctx& ctx, int q_vector) {
+  using L = Layout<D>;
+  constexpr int DCH = L::DCH, LOADS = D / 16;   // 16-byte loads of a thread per tile and tensor
+  const int tid = threadIdx.x - 32 * SOFTMAX_WARPS, lane = tid & 31;
+  float4* const scales = reinterpret_cast<float4*>(smem + M_SCALES);
+  const uint16_t sign = a.scale_log2 < 0.f ? 0x8000u : 0u;
+  Walk walk(plan, a, seqs, blockIdx.x, c.kv_heads);
+  Piece p;
+  bool ok = true;
+  int seq = 0, pieces = 0;
+  while (ok && walk.next(plan, a, seqs, c.kv_heads, p)) {
+    const size_t bh = static_cast<size_t>(p.b) * c.kv_heads + p.h;
+    const int length = seqs.length[p.b], full = length / NKV_BLOCK;
+    // ---- queries
+    if (pieces > 0) ok = wait(&bars[Q_FREE], (pieces - 1) & 1, ctx, 970);
+    if (!ok) break;
+    ++pieces;
+#pragma unroll 4
+    for (int i = tid; i < UNIT * (D / 8); i += 32 * OPERAND_WARPS) {
+      const int row = i / (D / 8), col = (i % (D / 8)) * 8, r = p.unit * UNIT + row;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (r < a.rows) {
+        const int token = r / a.group;
+        const uint16_t* src = a.q + p.b * a.q_batch + token * a.q_token + (p.h * a.group + r - token * a.group) * a.q_head + col;
+        if (q_vector) {
+          v = __ldg(reinterpret_cast<const uint4*>(src));
+        } else {
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = __ldg(src + 2 * e) | (static_cast<uint32_t>(__ldg(src + 2 * e + 1)) << 16);
+          v = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        const uint32_t flip = sign * 0x10001u;   // a negative scale is the queries' sign
+        v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+      }
+      uint8_t* tile = smem + L::Q_OFF + ((row / QT) * DCH + col / 64) * SUB;
+      *reinterpret_cast<uint4*>(tile + sw128_offset(row % QT, col % 64)) = v;
+    }
+    fence_proxy_async();
+    warp_arrive(&bars[Q_FULL], lane);
+    // ---- tiles: codes are requested one tensor ahead of their conversion, slots one tile ahead
+    uint4 kc[LOADS], vc[LOADS];
+    size_t slots[2];
+    float2 sc[2];
+    auto find = [&](int t) {        // slots and scales of tile t's blocks
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int block = 2 * (p.tile0 + t) + j;
+        slots[j] = 0;
+        sc[j] = make_float2(1.f, 1.f);
+        if (t < p.nt && block < full) {
+          slots[j] = slot_of(c, bh, block);
+          sc[j] = __ldg(reinterpret_cast<const float2*>(c.scales) + slots[j]);
+        }
+      }
+    };
+    // thread's 16 bytes i of a tile: half the loads lie in each block
+    auto fetch = [&](const uint8_t* codes, int t, const size_t (&at)[2], uint4 (&into)[LOADS]) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int j = i / (LOADS / 2), block = 2 * (p.tile0 + t) + j;
+        into[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+        if (t < p.nt && block < full)
+          into[i] = __ldg(reinterpret_cast<const uint4*>(codes + at[j] * (NKV_BLOCK * D)) + (i % (LOADS / 2)) * 128 + tid);
+      }
+    };
+    find(0);
+    size_t now[2] = {slots[0], slots[1]};
+    float2 now_sc[2] = {sc[0], sc[1]};
+    fetch(c.k_codes, 0, now, kc);
+    for (int t = 0; t < p.nt && ok; ++t, ++seq) {
+      const int stage = seq % STAGES, use = seq / STAGES;
+      fetch(c.v_codes, t, now, vc);
+      find(t + 1);
+      // ---- scales.  A block of scale 0 has only codes 0: any scale serves, and 2^-30 lies below all that 16-bit rows give
+      if (tid < 2) {
+        const float ks = tid ? now_sc[1].x : now_sc[0].x, vs = tid ? now_sc[1].y : now_sc[0].y;
+        const float lv = vs == 0.f ? -30.f : log2f(vs);
+        scales[(seq % NMETA) * 2 + tid] = make_float4(ks == 0.f ? 1.f : ks, lv, exp2f(-lv), 0.f);
+      }
+      if (tid < 32) warp_arrive(&bars[META_FULL + seq % NMETA], lane);
+      const int block0 = 2 * (p.tile0 + t);
+      // ---- K: [128 tokens x D]
+      if (use >= 1) ok = wait(&bars[K_FREE + stage], (use - 1) & 1, ctx, 971);
+      if (!ok) break;
+      uint8_t* const kt = smem + L::K_OFF + stage * DCH * SUB;
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int j = i / (LOADS / 2);
+        const int at = ((i % (LOADS / 2)) * 128 + tid) * 16, row = at / D, col = at % D;
+        if (block0 + j < full || block0 + j > full)   // (blocks behind the last one: zeros, their scores are masked)
+          store_codes<DT>(kt + (col / 64) * SUB, j * NKV_BLOCK + row, col % 64, kc[i], D == 128 && (lane & 4) != 0);
+      }
+      const int open = full - block0;                  // the open block's half of the tile, if 0 or 1
+      if (open == 0 || open == 1) {
+        const uint16_t* tail = static_cast<const uint16_t*>(c.k_tail) + bh * NKV_BLOCK * D;
+        const int held = length - full * NKV_BLOCK;
+        for (int i = tid; i < NKV_BLOCK * (D / 8); i += 32 * OPERAND_WARPS) {
+          const int row = i / (D / 8), col = (i % (D / 8)) * 8;
+          const uint4 v = row < held ? *reinterpret_cast<const uint4*>(tail + row * D + col) : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(kt + (col / 64) * SUB + sw128_offset(open * NKV_BLOCK + row, col % 64)) = v;
+        }
+      }
+      fence_proxy_async();
+      warp_arrive(&bars[K_FULL + stage], lane);
+      now[0] = slots[0]; now[1] = slots[1];
+      now_sc[0] = sc[0]; now_sc[1] = sc[1];
+      fetch(c.k_codes, t + 1, now, kc);
+      // ---- V: two [D x 64 tokens] halves
+      if (use >= 1) ok = wait(&bars[V_FREE + stage], (use - 1) & 1, ctx, 972);
+      if (!ok) break;
+      uint8_t* const vt = smem + L::V_OFF + stage * 2 * L::V_SUB;
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const int j = i / (LOADS / 2);
+        const int at = ((i % (LOADS / 2)) * 128 + tid) * 16, row = at / NKV_BLOCK, col = at % NKV_BLOCK;
+        if (block0 + j != full) store_codes<DT>(vt + j * L::V_SUB, row, col, vc[i], false);
+      }
+      if (open == 0 || open == 1) {
+        const uint16_t* tail = static_cast<const uint16_t*>(c.v_tail) + bh * NKV_BLOCK * D;
+        const int held = length - full * NKV_BLOCK;
+        for (int i = tid; i < D * (NKV_BLOCK / 8); i += 32 * OPERAND_WARPS) {
+          const int row = i / (NKV_BLOCK / 8), col = (i % (NKV_BLOCK / 8)) * 8;
+          const uint4 raw = *reinterpret_cast<const uint4*>(tail + row * NKV_BLOCK + col);
+          uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)   // tokens that are not there count as zero: what lies there may be anything
+            w[e] &= col + 2 * e + 1 < held ? 0xFFFFFFFFu : col + 2 * e < held ? 0xFFFFu : 0u;
+          *reinterpret_cast<uint4*>(vt + open * L::V_SUB + sw128_offset(row, col)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      fence_proxy_async();
+      warp_arrive(&bars[V_FULL + stage], lane);
+    }
+  }
+}
+
+// ---- warp 12: MMA issue -----------------------------------------------------------------------------------------
+template <int DT, int D>
+__device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t tmem, const Call& a, const Sequences& seqs,
+                                         const Plan& plan, const Ctx& ctx, int kv_heads) {
+  using L = Layout<D>;
+  constexpr int DCH = L::DCH;
+  const bool leader = elect_one();   // the whole warp runs the (uniform) control flow; one elected lane issues
+  const uint32_t base = smem_u32(smem);
+  auto issue_s = [&](int i, int stage) {
+#pragma unroll
+    for (int ch = 0; ch < DCH; ++ch) {
+      const uint64_t qd = make_smem_desc_sw128(base + L::Q_OFF + (i * DCH + ch) * SUB);
+      const uint64_t kd = make_smem_desc_sw128(base + L::K_OFF + (stage * DCH + ch) * SUB);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (leader) mma_bf16(tmem + i * 128, qd + 2 * k, kd + 2 * k, idesc<DT>(TOK), ch + k > 0);
+    }
+    if (leader) mma_commit(&bars[S_FULL + i]);
+  };
+  // weights of 64 tokens (a block) times V of it: [128 rows x 64] [D x 64]^T, both with the tokens running along rows
+  auto issue_pv = [&](int i, int stage, int half, bool accumulate) {
+    const uint64_t vd = make_smem_desc_sw128(base + L::V_OFF + (stage * 2 + half) * L::V_SUB);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (leader) mma_bf16_ts(tmem + 256 + i * 128, tmem + i * 128 + half * 32 + 8 * k, vd + 2 * k, idesc<DT>(D), accumulate || half + k > 0);
+    if (half == 1 && leader) mma_commit(&bars[PV_DONE + i]);
+  };
+  Walk walk(plan, a, seqs, blockIdx.x, kv_heads);
+  Piece p;
+  bool ok = true;
+  int seq = 0, pieces = 0, done[NQ] = {0, 0}, used[NQ] = {0, 0};   // tiles and pieces of each query tile so far
+  while (ok && walk.next(plan, a, seqs, kv_heads, p)) {
+    const int n[NQ] = {tiles_for(a, seqs, p, 0), tiles_for(a, seqs, p, 1)};
+    const int longest = max(n[0], n[1]);
+    ok = wait(&bars[Q_FULL], pieces & 1, ctx, 980);
+    ++pieces;
+    // which query tile is the last to use tile t
+    auto last_of = [&](int t) { return t < n[1] ? 1 : 0; };
+    for (int t = 0; t <= longest && ok; ++t) {
+      const int cur = seq + t - 1, next = seq + t;   // PV of tile t - 1 and S of tile t, query tile by query tile
+      for (int i = 0; i < NQ && ok; ++i) {
+        if (t > 0 && t - 1 < n[i]) {
+          const int stage = cur % STAGES, ci = done[i] + t - 1;
+          ok = wait(&bars[P_READY + i], ci & 1, ctx, 981);
+          ok = ok && wait(&bars[V_FULL + stage], (cur / STAGES) & 1, ctx, 982);
+          if (ok && t == 1 && used[i] > 0) ok = wait(&bars[O_FREE + i], (used[i] - 1) & 1, ctx, 983);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(i, stage, 0, t > 1);
+          ok = wait(&bars[P_LAST + i], ci & 1, ctx, 984);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(i, stage, 1, true);
+          if (i == last_of(t - 1) && leader) mma_commit(&bars[V_FREE + stage]);
+        }
+        if (t < n[i]) {
+          // S of the next tile overwrites P of this one, right behind the PV that reads it: the tensor core executes one
+          // thread's MMAs in order
+          const int stage = next % STAGES;
+          ok = wait(&bars[K_FULL + stage], (next / STAGES) & 1, ctx, 985);
+          if (!ok) break;
+          tc_fence_after();
+          issue_s(i, stage);
+          if (i == last_of(t) && leader) mma_commit(&bars[K_FREE + stage]);
+        }
+      }
+    }
+    if (!ok) break;
+    if (leader) mma_commit(&bars[Q_FREE]);
+    // tiles of the list that no query tile of the piece uses do not exist: the longest of the two is the piece's length
+    seq += p.nt;
+    for (int i = 0; i < NQ; ++i) {
+      done[i] += n[i];
+      used[i] += n[i] > 0 ? 1 : 0;
+    }
+  }
+  __syncwarp();
+}
+
+// ---- warps 0-7: softmax -------------------------------------------------------------------------------------------
+template <int DT, int D>
+__device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint32_t tmem, const Call& a, const Sequences& seqs,
+                                             const Plan& plan, const Parts& parts, const Ctx& ctx, int kv_heads) {
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+  const int wg = warp / 4, row = tid & 127;
+  const uint32_t lane_sel = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+  const uint32_t s_addr = tmem + lane_sel + wg * 128, o_addr = tmem + lane_sel + 256 + wg * 128;
+  const float4* const scales = reinterpret_cast<const float4*>(smem + M_SCALES);
+  const float scale = fabsf(a.scale_log2);
+  constexpr float RAISE = DT == NKV_BF16 ? HALF_STEP_LOG2 : 0.f, LOWER = DT == NKV_BF16 ? HALF_STEP_INV : 1.f;
+  Walk walk(plan, a, seqs, blockIdx.x, kv_heads);
+  Piece p;
+  bool ok = true, more = true;
+  int seq = 0, ci = 0;
+  auto place = [&](const Piece& pc) { return 2 * static_cast<size_t>(blockIdx.x) + (pc.tile0 == 0 ? 1 : 0); };
+  while (ok && (more = walk.next(plan, a, seqs, kv_heads, p))) {
+    const int r = p.unit * UNIT + wg * QT + row;
+    const int length = seqs.length[p.b], count = seqs.count[p.b];
+    const int seen = r < a.rows ? visible_to(a, length, count, r) : 0;
+    const int n = tiles_for(a, seqs, p, wg);
+    const size_t bh = static_cast<size_t>(p.b) * kv_heads + p.h;
+    const int token = r / a.group;
+    const size_t at = (static_cast<size_t>(p.b) * a.tokens + token) * a.heads + p.h * a.group + r - token * a.group;
+    float m = -INFINITY, l = 0.f;
+    for (int t = 0; t < n && ok; ++t, ++ci) {
+      const int meta = (seq + t) % NMETA, first = (p.tile0 + t) * TOK;
+      ok = wait(&bars[S_FULL + wg], ci & 1, ctx, 990);
+      // The scales were there before K was.  Asked for behind S_FULL only: a query tile that sat out some pieces would take
+      // a phase of long ago for the one it needs.
+      ok = ok && wait(&bars[META_FULL + meta], ((seq + t) / NMETA) & 1, ctx, 991);
+      if (!ok) break;
+      const float4 sc0 = scales[2 * meta], sc1 = scales[2 * meta + 1];
+      tc_fence_after();
+      // S of this tile was issued behind PV of the one before and its commit covers both: O is up to date
+      uint32_t raw[4][32];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) tmem_ld32_issue(s_addr + k * 32, raw[k]);
+      tmem_ld128_wait(raw[0], raw[1], raw[2], raw[3]);
+      float f0 = scale * sc0.x, f1 = scale * sc1.x;
+      const bool masked = __any_sync(0xffffffffu, first + TOK > seen) != 0;
+      if (masked) {
+        // scaled before they are masked: -inf times a scale of 0 would be NaN
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            raw[k][j] = first + 32 * k + j < seen ? __float_as_uint(__uint_as_float(raw[k][j]) * (k < 2 ? f0 : f1)) : 0xFF800000u;
+        f0 = f1 = 1.f;
+      }
+      float top[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float x = __uint_as_float(raw[k][0]), y = __uint_as_float(raw[k][1]);
+#pragma unroll
+        for (int j = 2; j < 32; j += 2) {
+          x = fmaxf(x, __uint_as_float(raw[k][j]));
+          y = fmaxf(y, __uint_as_float(raw[k][j + 1]));
+        }
+        top[k] = fmaxf(x, y);
+      }
+      const float m_new = fmaxf(m, fmaxf(fmaf(fmaxf(top[0], top[1]), f0, sc0.y), fmaf(fmaxf(top[2], top[3]), f1, sc1.y)));
+      if (__any_sync(0xffffffffu, m_new > m + RESCALE_THRESHOLD || (m == -INFINITY && m_new > m))) {
+        // move the reference: O and the sum are scaled by 2^(old - new)
+        const float alpha = m_new == -INFINITY ? 1.f : exp2f(m - m_new);
+        if (t > 0) {
+#pragma unroll 1
+          for (int cc = 0; cc < D / 32; ++cc) {
+            uint32_t v[32];
+            tmem_ld32_issue(o_addr + cc * 32, v);
+            tmem_ld32_wait(v);
+            float f[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]) * alpha;
+            tmem_st32(o_addr + cc * 32, f);
+          }
+        }
+        l *= alpha;
+        m = m_new;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+      // One pass over the scores: eight at a time, exponentials of group b, arguments of b + 1, sums and packing of b - 1.  P'
+      // (16-bit pairs) replaces S in place; the first block's half is handed over while the second is computed.
+      const uint64_t scale2[2] = {pair_f32(f0, f0), pair_f32(f1, f1)};
+      const float off0 = sc0.y - ref + RAISE, off1 = sc1.y - ref + RAISE;
+      const uint64_t off2[2] = {pair_f32(off0, off0), pair_f32(off1, off1)};
+      uint64_t sum2[2][2] = {{0ull, 0ull}, {0ull, 0ull}};
+      uint32_t packed[16];
+      uint64_t arg[2][4];
+      float w[2][8];
+      auto args = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          arg[b & 1][i] = fma_f32x2(pair_bits(raw[b >> 2][(b & 3) * 8 + 2 * i], raw[b >> 2][(b & 3) * 8 + 2 * i + 1]), scale2[b >> 3], off2[b >> 3]);
+      };
+      auto exps = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float lo, hi;
+          split_f32(arg[b & 1][i], lo, hi);
+          w[b & 1][2 * i] = exp2_fast(lo);
+          w[b & 1][2 * i + 1] = exp2_fast(hi);
+        }
+      };
+      auto finish = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float lo = w[b & 1][2 * i], hi = w[b & 1][2 * i + 1];
+          sum2[b >> 3][i & 1] = add_f32x2(sum2[b >> 3][i & 1], pair_f32(lo, hi));
+          packed[(b & 3) * 4 + i] = DT == NKV_BF16 ? __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632) : pack2<NKV_F16>(lo, hi);
+        }
+        if ((b & 3) == 3) {
+          tmem_st16(s_addr + (b >> 2) * 16, packed);
+          if (b == 7) {
+            tmem_wait_st();
+            tc_fence_before();
+            warp_arrive(&bars[P_READY + wg], lane);
+          }
+        }
+      };
+      args(0);
+#pragma unroll
+      for (int b = 0; b < 16; ++b) {
+        exps(b);
+        if (b + 1 < 16) args(b + 1);
+        if (b >= 1) finish(b - 1);
+      }
+      finish(15);
+      tmem_wait_st();
+      tc_fence_before();
+      warp_arrive(&bars[P_LAST + wg], lane);
+      float sum[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float lo, hi;
+        split_f32(add_f32x2(sum2[j][0], sum2[j][1]), lo, hi);
+        sum[j] = (lo + hi) * LOWER;
+      }
+      l += sum[0] * sc0.z + sum[1] * sc1.z;
+      if (a.partial && r < a.rows) {
+        const int block = 2 * (p.tile0 + t);
+        float* to = a.partial + (bh * a.most_blocks + block) * a.rows + r;
+        to[0] = log2f(sum[0]) + (ref - sc0.y);
+        if (block + 1 < a.most_blocks) to[a.rows] = log2f(sum[1]) + (ref - sc1.y);
+      }
+    }
+    seq += p.nt;
+    if (!ok) break;
+    // ---- the rows: results, or a part of them
+    if (n > 0) {
+      ok = wait(&bars[PV_DONE + wg], (ci - 1) & 1, ctx, 992);
+      if (!ok) break;
+      tc_fence_after();
+    }
+    const float inv = seen > 0 ? 1.f / l : 0.f;
+    float* const part = parts.o + (place(p) * UNIT + wg * QT + row) * D;
+#pragma unroll 1
+    for (int cc = 0; cc < D / 32; ++cc) {
+      uint32_t v[32];
+      if (n > 0) {
+        tmem_ld32_issue(o_addr + cc * 32, v);
+        tmem_ld32_wait(v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = 0u;
+      }
+      if (r >= a.rows) continue;
+      if (p.whole) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 8) {
+          uint32_t o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float lo = __uint_as_float(v[j + 2 * e]), hi = __uint_as_float(v[j + 2 * e + 1]);
+            o[e] = seen > 0 ? pack2<DT>(lo * inv, hi * inv) : 0u;
+          }
+          *reinterpret_cast<uint4*>(a.out + at * D + cc * 32 + j) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(part + cc * 32 + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+      }
+    }
+    if (r < a.rows) {
+      if (p.whole) a.lse[at] = seen > 0 ? (m + log2f(l)) * LN2 : -INFINITY;
+      else parts.ml[place(p) * UNIT + wg * QT + row] = make_float2(m, l);
+    }
+    if (n > 0) {
+      tc_fence_before();
+      warp_arrive(&bars[O_FREE + wg], lane);
+    }
+  }
+  // a launch that gave up: NaN for the piece it stopped in and all later ones
+  if (!ok) {
+    while (more) {
+      const int r = p.unit * UNIT + wg * QT + row, token = r / a.group;
+      if (r < a.rows) {
+        if (p.whole) a.lse[(static_cast<size_t>(p.b) * a.tokens + token) * a.heads + p.h * a.group + r - token * a.group] = CUDART_NAN_F;
+        else parts.ml[place(p) * UNIT + wg * QT + row] = make_float2(0.f, CUDART_NAN_F);
+      }
+      more = walk.next(plan, a, seqs, kv_heads, p);
+    }
+  }
+}
+
+template <int DT, int D>
+__global__ void __launch_bounds__(THREADS, 1)
+tile_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const __grid_constant__ Plan plan, Parts parts, int q_vector,
+            int32_t* status) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(smem);
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + M_SLOT);
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + M_ABORT);
+  const int warp = threadIdx.x / 32;
+  if (threadIdx.x == 0) {
+    mbar_init(&bars[Q_FULL], OPERAND_WARPS);
+    mbar_init(&bars[Q_FREE], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars[K_FULL + i], OPERAND_WARPS);
+      mbar_init(&bars[K_FREE + i], 1);
+      mbar_init(&bars[V_FULL + i], OPERAND_WARPS);
+      mbar_init(&bars[V_FREE + i], 1);
+      mbar_init(&bars[S_FULL + i], 1);
+      mbar_init(&bars[P_READY + i], QT / 32);
+      mbar_init(&bars[P_LAST + i], QT / 32);
+      mbar_init(&bars[PV_DONE + i], 1);
+      mbar_init(&bars[O_FREE + i], QT / 32);
+    }
+    for (int i = 0; i < NMETA; ++i) mbar_init(&bars[META_FULL + i], 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    fence_proxy_async();
+  }
+  if (warp == 12) tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const Ctx ctx{abort_flag};
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // 512 threads x 128 registers: 256 x 184 + 128 x 104 + 128 x 40 = 65,536
+  if (warp < SOFTMAX_WARPS) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    softmax_role<DT, D>(smem, bars, tmem, a, seqs, plan, parts, ctx, c.kv_heads);
+  } else if (warp < SOFTMAX_WARPS + OPERAND_WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    operand_role<DT, D>(smem, bars, c, a, seqs, plan, ctx, q_vector);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 12) mma_role<DT, D>(smem, bars, tmem, a, seqs, plan, ctx, c.kv_heads);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 12) tmem_dealloc(tmem, 512);
+  if (threadIdx.x == 0 && *abort_flag) atomicCAS(status, 0, *abort_flag);
+}
+
+// Joins the parts of cut units and fills the rows of units that see nothing; a thread block per (unit, kv head,
+// sequence) and 32 rows, a thread per row and 16 bytes of it.
+template <int DT, int D>
+__global__ void __launch_bounds__(256)
+join_units_kernel(Call a, const __grid_constant__ Sequences seqs, const __grid_constant__ Plan plan, Parts parts, int kv_heads, int slices) {
+  __shared__ uint32_t before;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int unit = blockIdx.x / slices, slice = blockIdx.x % slices, h = blockIdx.y, b = blockIdx.z;
+  const int length = seqs.length[b], count = seqs.count[b];
+  auto tiles_of = [&](int u) { return tiles_seen(length, count, a.group, a.rows, a.causal, u * UNIT, UNIT); };
+  const int nt = tiles_of(unit);
+  uint32_t r0 = 0, r1 = 0, begin = 0;
+  if (nt > 0) {
+    if (threadIdx.x == 0) before = 0;
+    __syncthreads();
+    uint32_t mine = 0;
+    for (int u = threadIdx.x; u < unit; u += 256) mine += tiles_of(u);
+    if (mine) atomicAdd(&before, mine);
+    __syncthreads();
+    begin = plan.start[b] + h * ((plan.start[b + 1] - plan.start[b]) / kv_heads) + before;
+    r0 = plan.run_of(begin);
+    r1 = plan.run_of(begin + nt - 1);
+    if (r0 == r1) return;   // one run had all of it and wrote the results
+  }
+  constexpr int PER_ROW = D / 8, ROWS = 256 / PER_ROW;
+  const int row0 = slice * (UNIT / slices);
+  for (int row = row0 + threadIdx.x / PER_ROW; row < row0 + UNIT / slices; row += ROWS) {
+    const int r = unit * UNIT + row, col = (threadIdx.x % PER_ROW) * 8;
+    if (r >= a.rows) break;
+    const int token = r / a.group;
+    const size_t at = (static_cast<size_t>(b) * a.tokens + token) * a.heads + h * a.group + r - token * a.group;
+    const bool any = nt > 0 && visible_to(a, length, count, r) > 0;
+    float top = -INFINITY, sum = 0.f, acc[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+    if (any) {
+      // the run the unit starts in has it as a piece that starts with the unit, the others as one that starts inside
+      auto place = [&](uint32_t run) { return (2 * static_cast<size_t>(run) + (run == r0 ? 1 : 0)) * UNIT + row; };
+      for (uint32_t run = r0; run <= r1; ++run) top = fmaxf(top, __ldcg(&parts.ml[place(run)].x));
+      const float ref = top == -INFINITY ? 0.f : top;
+      for (uint32_t run = r0; run <= r1; ++run) {
+        const float2 ml = __ldcg(&parts.ml[place(run)]);
+        const float4 lo = __ldcg(reinterpret_cast<const float4*>(parts.o + place(run) * D + col));
+        const float4 hi = __ldcg(reinterpret_cast<const float4*>(parts.o + place(run) * D + col + 4));
+        const float f = exp2f(ml.x - ref);
+        sum = fmaf(ml.y, f, sum);
+        acc[0] = fmaf(lo.x, f, acc[0]); acc[1] = fmaf(lo.y, f, acc[1]); acc[2] = fmaf(lo.z, f, acc[2]); acc[3] = fmaf(lo.w, f, acc[3]);
+        acc[4] = fmaf(hi.x, f, acc[4]); acc[5] = fmaf(hi.y, f, acc[5]); acc[6] = fmaf(hi.z, f, acc[6]); acc[7] = fmaf(hi.w, f, acc[7]);
+      }
+    }
+    const float inv = any ? 1.f / sum : 0.f;
+    uint32_t o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = pack2<DT>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    *reinterpret_cast<uint4*>(a.out + at * D + col) = make_uint4(o[0], o[1], o[2], o[3]);
+    if (col == 0) a.lse[at] = any ? (top + log2f(sum)) * LN2 : -INFINITY;
+  }
+}
+
+Plan plan_of(const Sequences& seqs, int n, int kv_heads, int group, int rows, bool causal) {
+  Plan p;
+  p.sequences = n;
+  p.units = ceil_div(rows, UNIT);
+  uint64_t total = 0;
+  for (int i = 0; i < n; ++i) {
+    p.start[i] = static_cast<uint32_t>(total);
+    uint64_t tiles = 0;
+    for (int u = 0; u < p.units; ++u) tiles += tiles_seen(seqs.length[i], seqs.count[i], group, rows, causal, u * UNIT, UNIT);
+    total += tiles * kv_heads;
+  }
+  p.start[n] = static_cast<uint32_t>(total);
+  p.runs = static_cast<int>(min(total, static_cast<uint64_t>(sm_count())));
+  p.run = p.runs ? static_cast<uint32_t>(total / p.runs) : 0;
+  p.longer = p.runs ? static_cast<uint32_t>(total % p.runs) : 0;
+  return p;
+}
+
+}  // namespace
+
+size_t block_tile_bytes(const Sequences& seqs, int n, int kv_heads, int group, int rows, bool causal, int d) {
+  return static_cast<size_t>(plan_of(seqs, n, kv_heads, group, rows, causal).runs) * 2 * UNIT * (d + 2) * sizeof(float);
+}
+
+int block_tile(const BlockArrays& c, const Call& a, const Sequences& seqs, int n, int dtype, int d, void* workspace, int32_t* status,
+               cudaStream_t stream) {
+  const Plan plan = plan_of(seqs, n, c.kv_heads, a.group, a.rows, a.causal);
+  Parts parts;
+  parts.o = static_cast<float*>(workspace);
+  parts.ml = reinterpret_cast<float2*>(parts.o + static_cast<size_t>(plan.runs) * 2 * UNIT * d);
+  const int q_vector = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_batch % 8 == 0 && a.q_token % 8 == 0 && a.q_head % 8 == 0;
+  const bool bf16 = dtype == NKV_BF16;
+  if (plan.runs > 0) {
+    auto run = [&](auto kernel, int smem) {
+      NKV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      kernel<<<plan.runs, THREADS, smem, stream>>>(c, a, seqs, plan, parts, q_vector, status);
+      NKV_LAUNCH_CHECK("tile_kernel");
+      return NKV_OK;
+    };
+    const int rc = d == 128 ? (bf16 ? run(tile_kernel<NKV_BF16, 128>, Layout<128>::DYNAMIC) : run(tile_kernel<NKV_F16, 128>, Layout<128>::DYNAMIC))
+                            : (bf16 ? run(tile_kernel<NKV_BF16, 64>, Layout<64>::DYNAMIC) : run(tile_kernel<NKV_F16, 64>, Layout<64>::DYNAMIC));
+    if (rc != NKV_OK) return rc;
+  }
+  const int slices = 8;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(plan.units * slices, c.kv_heads, n);
+  config.blockDim = dim3(256);
+  config.stream = stream;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = plan.runs > 0 ? 1 : 0;
+  auto join = d == 128 ? (bf16 ? join_units_kernel<NKV_BF16, 128> : join_units_kernel<NKV_F16, 128>)
+                       : (bf16 ? join_units_kernel<NKV_BF16, 64> : join_units_kernel<NKV_F16, 64>);
+  NKV_CUDA(cudaLaunchKernelEx(&config, join, a, seqs, plan, parts, c.kv_heads, slices));
+  return NKV_OK;
+}
+
+}  // namespace nkv
