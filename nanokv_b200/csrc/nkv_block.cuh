@@ -55,6 +55,17 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 __device__ __forceinline__ float code_value(uint32_t byte) { return __uint_as_float(0x4B000000u | byte) - 8388736.0f; }
 
 // ---- attention ----
+// Shared memory by its own addresses: a dynamic buffer aligned by hand has a generic pointer, and 16-byte accesses through
+// one are slower.
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t addr, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 // One call, from one of its sequences on.  The queries of a kv head are rows r = token * group + (head within the group).

@@ -1,16 +1,16 @@
 // Attention of many query rows over the 8-bit block cache, on tcgen05.
 //
 // The rows of a kv head (its group's heads of all query tokens) are cut into units of 256: two 128-row tiles that share
-// every K and V tile.  A tile is 128 tokens, two blocks of the cache.  Four warps read its codes, turn them into the
-// cache's 16-bit type (exactly: a code is an integer below 2^7) and store them as the swizzled operands the tensor cores
-// read; no 16-bit copy of the cache exists in memory.  S = Q K^T goes to tensor memory, eight warps take the softmax (one
+// every K and V tile.  A tile is 128 tokens, two blocks of the cache.  A warp brings its codes into a ring by bulk
+// copies; four warps turn them into the cache's 16-bit type (exactly: a code is an integer below 2^7) and store them as the
+// swizzled operands the tensor cores read; no 16-bit copy of the cache exists in memory.  S = Q K^T goes to tensor memory, eight warps take the softmax (one
 // thread per row), P replaces S as the operand of O += P V.  The block scales never touch an operand.  K's multiplies the
 // scores.  V's goes into the exponent: the weight handed over is P' = 2^(s + log2 vs - m'), with m' the running maximum of
 // s + log2 vs, so that a row's weights are at most 1 (2^8 with the lazy reference) however unlike the scales of its blocks are; a block's
 // part of the row sum is the sum of its P' divided by vs again, in fp32.
 //
 // The tiles of all units form one list that the SMs take in equal runs; a unit that a run's end cuts leaves fp32 parts,
-// joined by a second launch.  Warps: 0-7 softmax, 8-11 operands, 12 MMA issue.
+// joined by a second launch.  Warps: 0-7 softmax, 8-11 operands, 12 MMA issue, 13 codes.
 #include "nkv_block.cuh"
 #include "nkv_internal.h"
 #include "nkv_tc.cuh"
@@ -23,7 +23,7 @@ using namespace tc;
 constexpr int QT = 128, NQ = 2, UNIT = QT * NQ;   // rows of a query tile, tiles and rows of a unit
 constexpr int TOK = 128;                          // tokens of a tile
 constexpr int STAGES = 2;                         // K / V operand stages
-constexpr int SOFTMAX_WARPS = 8, OPERAND_WARPS = 4, THREADS = 512;   // four warpgroups: the last one has only the MMA warp at work
+constexpr int SOFTMAX_WARPS = 8, OPERAND_WARPS = 4, THREADS = 512;   // four warpgroups; two warps of the last have no work
 constexpr int SUB = 128 * 128;                    // bytes of a [128 rows x 64 elements] swizzled operand tile
 constexpr float RESCALE_THRESHOLD = 8.0f;
 // log2(1 + 2^-9) and its factor's inverse: bf16 weights are rounded by raising them half a step (in the exponent) and
@@ -31,9 +31,10 @@ constexpr float RESCALE_THRESHOLD = 8.0f;
 constexpr float HALF_STEP_LOG2 = 0.0028150156070540f, HALF_STEP_INV = 0.998050682261209f;
 
 enum Bar { Q_FULL = 0, Q_FREE = 1, K_FULL = 2, K_FREE = 4, V_FULL = 6, V_FREE = 8, S_FULL = 10, P_READY = 12, P_LAST = 14,
-           PV_DONE = 16, O_FREE = 18, META_FULL = 20, NUM_BARS = 24 };
-constexpr int NMETA = 4;
-constexpr int M_SLOT = NUM_BARS * 8, M_ABORT = M_SLOT + 4, M_SCALES = 256;   // scales: [NMETA][2 blocks] float4 {ks, log2 vs, 1 / vs, -}
+           PV_DONE = 16, O_FREE = 18, RAW_FULL = 20, RAW_FREE = 24, META_FULL = 28, NUM_BARS = 36 };
+// scales are written up to four tiles ahead of the softmax (two operand stages, the ring of codes)
+constexpr int NMETA = 8;
+constexpr int M_SLOT = NUM_BARS * 8, M_ABORT = M_SLOT + 4, M_SCALES = 512;   // scales: [NMETA][2 blocks] float4 {ks, log2 vs, 1 / vs, -}
 
 template <int D> struct Layout {
   static constexpr int DCH = D / 64;
@@ -41,7 +42,10 @@ template <int D> struct Layout {
   static constexpr int K_OFF = Q_OFF + NQ * DCH * SUB;
   static constexpr int V_OFF = K_OFF + STAGES * DCH * SUB;
   static constexpr int V_SUB = D * 128;            // [D rows x 64 tokens]
-  static constexpr int BYTES = V_OFF + STAGES * 2 * V_SUB;
+  static constexpr int RAW_OFF = V_OFF + STAGES * 2 * V_SUB;
+  static constexpr int RAW = TOK * D;              // codes of a tile of K or V
+  static constexpr int RAWS = D == 128 ? 2 : 4;    // ring of them
+  static constexpr int BYTES = RAW_OFF + RAWS * RAW;
   static constexpr int DYNAMIC = BYTES + 1024;     // room to start on 1,024 bytes
 };
 static_assert(M_SCALES + NMETA * 2 * 16 <= 1024, "meta block");
@@ -191,7 +195,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 
 // 16 codes as 32 bytes of an operand row: two pieces, columns col .. col + 15 (col a multiple of 16)
 template <int DT>
-__device__ __forceinline__ void store_codes(uint8_t* tile, int row, int col, const uint4& raw, bool swap) {
+__device__ __forceinline__ void store_codes(uint32_t tile, int row, int col, const uint4& raw, bool swap) {
   uint4 p0, p1;
   expand<DT>(raw.x, p0.x, p0.y);
   expand<DT>(raw.y, p0.z, p0.w);
@@ -200,8 +204,64 @@ __device__ __forceinline__ void store_codes(uint8_t* tile, int row, int col, con
   const uint32_t a0 = sw128_offset(row, col), a1 = sw128_offset(row, col + 8);
   // the eight lanes that store together shall fill all banks: half of them take their second piece first
   const uint4 s0 = swap ? p1 : p0, s1 = swap ? p0 : p1;
-  *reinterpret_cast<uint4*>(tile + (swap ? a1 : a0)) = s0;
-  *reinterpret_cast<uint4*>(tile + (swap ? a0 : a1)) = s1;
+  sts128(tile + (swap ? a1 : a0), s0);
+  sts128(tile + (swap ? a0 : a1), s1);
+}
+
+// ---- warp 13: codes and scales ---------------------------------------------------------------------------------
+template <int D>
+__device__ __forceinline__ void codes_role(uint8_t* smem, uint64_t* bars, const BlockArrays& c, const Call& a, const Sequences& seqs,
+                                           const Plan& plan, const Ctx& ctx) {
+  using L = Layout<D>;
+  constexpr uint32_t BLOCK_BYTES = NKV_BLOCK * D;
+  const int lane = threadIdx.x & 31;
+  float4* const scales = reinterpret_cast<float4*>(smem + M_SCALES);
+  Walk walk(plan, a, seqs, blockIdx.x, c.kv_heads);
+  Piece p;
+  bool ok = true;
+  int seq = 0, item = 0;
+  while (ok && walk.next(plan, a, seqs, c.kv_heads, p)) {
+    const size_t bh = static_cast<size_t>(p.b) * c.kv_heads + p.h;
+    const int full = seqs.length[p.b] / NKV_BLOCK;
+    long long slot = 0;
+    float2 sc = make_float2(1.f, 1.f);
+    for (int t = 0; t < p.nt && ok; ++t, ++seq) {
+      const int block0 = 2 * (p.tile0 + t), at = (2 * t) & 31;
+      if (at == 0) {   // lane l knows block l of the next sixteen tiles: one trip to memory for all of them
+        const int block = block0 + lane;
+        sc = make_float2(1.f, 1.f);
+        if (block < full) {
+          slot = static_cast<long long>(slot_of(c, bh, block));
+          sc = __ldg(reinterpret_cast<const float2*>(c.scales) + slot);
+        }
+      }
+      if ((lane & ~1) == at) {
+        // a block of scale 0 has only codes 0: any scale serves, and 2^-30 lies below all that 16-bit rows give
+        const float lv = sc.y == 0.f ? -30.f : log2f(sc.y);
+        scales[(seq % NMETA) * 2 + (lane & 1)] = make_float4(sc.x == 0.f ? 1.f : sc.x, lv, exp2f(-lv), 0.f);
+      }
+      warp_arrive(&bars[META_FULL + seq % NMETA], lane);
+      const long long s0 = __shfl_sync(0xffffffffu, slot, at), s1 = __shfl_sync(0xffffffffu, slot, at + 1);
+      const uint32_t blocks = min(2, max(0, full - block0));   // full ones: the open block is read where it is needed
+      for (int tensor = 0; tensor < 2 && ok; ++tensor, ++item) {
+        const int stage = item % L::RAWS;
+        if (item >= L::RAWS) ok = wait(&bars[RAW_FREE + stage], (item / L::RAWS - 1) & 1, ctx, 975);
+        if (!ok) break;
+        if (lane == 0) {
+          uint8_t* const to = smem + L::RAW_OFF + stage * L::RAW;
+          const uint8_t* const from = tensor ? c.v_codes : c.k_codes;
+          mbar_arrive_expect_tx(&bars[RAW_FULL + stage], blocks * BLOCK_BYTES);
+          if (blocks > 0) bulk_load_1d(to, from + s0 * BLOCK_BYTES, BLOCK_BYTES, &bars[RAW_FULL + stage]);
+          if (blocks > 1) bulk_load_1d(to + BLOCK_BYTES, from + s1 * BLOCK_BYTES, BLOCK_BYTES, &bars[RAW_FULL + stage]);
+        }
+        __syncwarp();
+      }
+    }
+  }
+  if (!ok) {   // copies in flight land before the block goes away
+    const long long begin = clock64();
+    while (clock64() - begin < (1ll << 21)) {}
+  }
 }
 
 // ---- warps 8-11: queries, K and V as operands -----------------------------------------------------------------
@@ -209,22 +269,37 @@ template <int DT, int D>
 __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, const BlockArrays& c, const Call& a, const Sequences& seqs,
                                              const Plan& plan, const Ctx& ctx, int q_vector) {
   using L = Layout<D>;
-  constexpr int DCH = L::DCH, LOADS = D / 16;   // 16-byte loads of a thread per tile and tensor
+  constexpr int DCH = L::DCH, LOADS = D / 16;   // 16-byte pieces of a thread per tile and tensor, half of them of each block
   const int tid = threadIdx.x - 32 * SOFTMAX_WARPS, lane = tid & 31;
-  float4* const scales = reinterpret_cast<float4*>(smem + M_SCALES);
   const uint16_t sign = a.scale_log2 < 0.f ? 0x8000u : 0u;
   Walk walk(plan, a, seqs, blockIdx.x, c.kv_heads);
   Piece p;
   bool ok = true;
-  int seq = 0, pieces = 0;
+  int seq = 0, pieces = 0, item = 0;
+  const uint32_t base = smem_u32(smem);
+  // A rolled loop on purpose: its body is fetched once, where eight copies of it would push the softmax warps' instructions
+  // out of the cache they share (a quarter of all issue slots was lost to fetching).
+  auto convert = [&](auto place, bool swap) {
+    const uint32_t from = base + L::RAW_OFF + (item % L::RAWS) * L::RAW + tid * 16;
+    uint4 next = lds128(from);
+#pragma unroll 1
+    for (int i = 0; i < LOADS; ++i) {
+      const uint4 raw = next;
+      if (i + 1 < LOADS) next = lds128(from + (i + 1) * 2048);
+      const int j = i / (LOADS / 2);
+      place(j, ((i % (LOADS / 2)) * 128 + tid) * 16, raw, swap);
+    }
+    warp_arrive(&bars[RAW_FREE + item % L::RAWS], lane);
+    ++item;
+  };
   while (ok && walk.next(plan, a, seqs, c.kv_heads, p)) {
     const size_t bh = static_cast<size_t>(p.b) * c.kv_heads + p.h;
-    const int length = seqs.length[p.b], full = length / NKV_BLOCK;
+    const int length = seqs.length[p.b], full = length / NKV_BLOCK, held = length - full * NKV_BLOCK;
     // ---- queries
     if (pieces > 0) ok = wait(&bars[Q_FREE], (pieces - 1) & 1, ctx, 970);
     if (!ok) break;
     ++pieces;
-#pragma unroll 4
+#pragma unroll 2
     for (int i = tid; i < UNIT * (D / 8); i += 32 * OPERAND_WARPS) {
       const int row = i / (D / 8), col = (i % (D / 8)) * 8, r = p.unit * UNIT + row;
       uint4 v = make_uint4(0, 0, 0, 0);
@@ -242,101 +317,67 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
         const uint32_t flip = sign * 0x10001u;   // a negative scale is the queries' sign
         v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
       }
-      uint8_t* tile = smem + L::Q_OFF + ((row / QT) * DCH + col / 64) * SUB;
-      *reinterpret_cast<uint4*>(tile + sw128_offset(row % QT, col % 64)) = v;
+      sts128(base + L::Q_OFF + ((row / QT) * DCH + col / 64) * SUB + sw128_offset(row % QT, col % 64), v);
     }
     fence_proxy_async();
     warp_arrive(&bars[Q_FULL], lane);
-    // ---- tiles: codes are requested one tensor ahead of their conversion, slots one tile ahead
-    uint4 kc[LOADS], vc[LOADS];
-    size_t slots[2];
-    float2 sc[2];
-    auto find = [&](int t) {        // slots and scales of tile t's blocks
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int block = 2 * (p.tile0 + t) + j;
-        slots[j] = 0;
-        sc[j] = make_float2(1.f, 1.f);
-        if (t < p.nt && block < full) {
-          slots[j] = slot_of(c, bh, block);
-          sc[j] = __ldg(reinterpret_cast<const float2*>(c.scales) + slots[j]);
-        }
-      }
-    };
-    // thread's 16 bytes i of a tile: half the loads lie in each block
-    auto fetch = [&](const uint8_t* codes, int t, const size_t (&at)[2], uint4 (&into)[LOADS]) {
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int j = i / (LOADS / 2), block = 2 * (p.tile0 + t) + j;
-        into[i] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-        if (t < p.nt && block < full)
-          into[i] = __ldg(reinterpret_cast<const uint4*>(codes + at[j] * (NKV_BLOCK * D)) + (i % (LOADS / 2)) * 128 + tid);
-      }
-    };
-    find(0);
-    size_t now[2] = {slots[0], slots[1]};
-    float2 now_sc[2] = {sc[0], sc[1]};
-    fetch(c.k_codes, 0, now, kc);
+    // ---- tiles
     for (int t = 0; t < p.nt && ok; ++t, ++seq) {
       const int stage = seq % STAGES, use = seq / STAGES;
-      fetch(c.v_codes, t, now, vc);
-      find(t + 1);
-      // ---- scales.  A block of scale 0 has only codes 0: any scale serves, and 2^-30 lies below all that 16-bit rows give
-      if (tid < 2) {
-        const float ks = tid ? now_sc[1].x : now_sc[0].x, vs = tid ? now_sc[1].y : now_sc[0].y;
-        const float lv = vs == 0.f ? -30.f : log2f(vs);
-        scales[(seq % NMETA) * 2 + tid] = make_float4(ks == 0.f ? 1.f : ks, lv, exp2f(-lv), 0.f);
-      }
-      if (tid < 32) warp_arrive(&bars[META_FULL + seq % NMETA], lane);
       const int block0 = 2 * (p.tile0 + t);
-      // ---- K: [128 tokens x D]
-      if (use >= 1) ok = wait(&bars[K_FREE + stage], (use - 1) & 1, ctx, 971);
+      const int open = full - block0;                  // 0 or 1: that half of the tile is not a full block
+      // ---- K: [128 tokens x D]; what lies behind the last token is masked in the scores, whatever it is
+      ok = wait(&bars[RAW_FULL + item % L::RAWS], (item / L::RAWS) & 1, ctx, 973);
+      if (ok && use >= 1) ok = wait(&bars[K_FREE + stage], (use - 1) & 1, ctx, 971);
       if (!ok) break;
-      uint8_t* const kt = smem + L::K_OFF + stage * DCH * SUB;
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int j = i / (LOADS / 2);
-        const int at = ((i % (LOADS / 2)) * 128 + tid) * 16, row = at / D, col = at % D;
-        if (block0 + j < full || block0 + j > full)   // (blocks behind the last one: zeros, their scores are masked)
-          store_codes<DT>(kt + (col / 64) * SUB, j * NKV_BLOCK + row, col % 64, kc[i], D == 128 && (lane & 4) != 0);
-      }
-      const int open = full - block0;                  // the open block's half of the tile, if 0 or 1
+      const uint32_t kt = base + L::K_OFF + stage * DCH * SUB;
+      convert([&](int j, int at, const uint4& raw, bool swap) {
+        store_codes<DT>(kt + (at % D / 64) * SUB, j * NKV_BLOCK + at / D, at % 64, raw, swap);
+      }, D == 128 && (lane & 4) != 0);
       if (open == 0 || open == 1) {
+        __syncwarp();   // (the same lanes' codes of that half went there)
         const uint16_t* tail = static_cast<const uint16_t*>(c.k_tail) + bh * NKV_BLOCK * D;
-        const int held = length - full * NKV_BLOCK;
-        for (int i = tid; i < NKV_BLOCK * (D / 8); i += 32 * OPERAND_WARPS) {
-          const int row = i / (D / 8), col = (i % (D / 8)) * 8;
-          const uint4 v = row < held ? *reinterpret_cast<const uint4*>(tail + row * D + col) : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(kt + (col / 64) * SUB + sw128_offset(open * NKV_BLOCK + row, col % 64)) = v;
+#pragma unroll 1
+        for (int i = 0; i < LOADS / 2; ++i) {
+          const int at = (i * 128 + tid) * 16, row = at / D, col = at % D;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint4 v = *reinterpret_cast<const uint4*>(tail + row * D + col + 8 * half);
+            sts128(kt + (col / 64) * SUB + sw128_offset(open * NKV_BLOCK + row, col % 64 + 8 * half), v);
+          }
         }
       }
       fence_proxy_async();
       warp_arrive(&bars[K_FULL + stage], lane);
-      now[0] = slots[0]; now[1] = slots[1];
-      now_sc[0] = sc[0]; now_sc[1] = sc[1];
-      fetch(c.k_codes, t + 1, now, kc);
-      // ---- V: two [D x 64 tokens] halves
-      if (use >= 1) ok = wait(&bars[V_FREE + stage], (use - 1) & 1, ctx, 972);
+      // ---- V: two [D x 64 tokens] halves; what lies behind the last token counts as zero: a weight of 0 times anything else
+      // might be NaN
+      ok = wait(&bars[RAW_FULL + item % L::RAWS], (item / L::RAWS) & 1, ctx, 974);
+      if (ok && use >= 1) ok = wait(&bars[V_FREE + stage], (use - 1) & 1, ctx, 972);
       if (!ok) break;
-      uint8_t* const vt = smem + L::V_OFF + stage * 2 * L::V_SUB;
-#pragma unroll
-      for (int i = 0; i < LOADS; ++i) {
-        const int j = i / (LOADS / 2);
-        const int at = ((i % (LOADS / 2)) * 128 + tid) * 16, row = at / NKV_BLOCK, col = at % NKV_BLOCK;
-        if (block0 + j != full) store_codes<DT>(vt + j * L::V_SUB, row, col, vc[i], false);
-      }
-      if (open == 0 || open == 1) {
+      const uint32_t vt = base + L::V_OFF + stage * 2 * L::V_SUB;
+      convert([&](int j, int at, const uint4& raw, bool swap) {
+        store_codes<DT>(vt + j * L::V_SUB, at / NKV_BLOCK, at % NKV_BLOCK, raw, swap);
+      }, false);
+      if (open <= 1) {
+        __syncwarp();
         const uint16_t* tail = static_cast<const uint16_t*>(c.v_tail) + bh * NKV_BLOCK * D;
-        const int held = length - full * NKV_BLOCK;
-        for (int i = tid; i < D * (NKV_BLOCK / 8); i += 32 * OPERAND_WARPS) {
-          const int row = i / (NKV_BLOCK / 8), col = (i % (NKV_BLOCK / 8)) * 8;
-          const uint4 raw = *reinterpret_cast<const uint4*>(tail + row * NKV_BLOCK + col);
-          uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        for (int j = max(open, 0); j < 2; ++j)
+#pragma unroll 1
+          for (int i = 0; i < LOADS / 2; ++i) {
+            const int at = (i * 128 + tid) * 16, row = at / NKV_BLOCK, col = at % NKV_BLOCK;
 #pragma unroll
-          for (int e = 0; e < 4; ++e)   // tokens that are not there count as zero: what lies there may be anything
-            w[e] &= col + 2 * e + 1 < held ? 0xFFFFFFFFu : col + 2 * e < held ? 0xFFFFu : 0u;
-          *reinterpret_cast<uint4*>(vt + open * L::V_SUB + sw128_offset(row, col)) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+            for (int half = 0; half < 2; ++half) {
+              uint32_t w[4] = {0, 0, 0, 0};
+              const int col8 = col + 8 * half;
+              if (j == open && col8 < held) {
+                const uint4 v = *reinterpret_cast<const uint4*>(tail + row * NKV_BLOCK + col8);
+                w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] &= col8 + 2 * e + 1 < held ? 0xFFFFFFFFu : col8 + 2 * e < held ? 0xFFFFu : 0u;
+              }
+              sts128(vt + j * L::V_SUB + sw128_offset(row, col8), make_uint4(w[0], w[1], w[2], w[3]));
+            }
+          }
       }
       fence_proxy_async();
       warp_arrive(&bars[V_FULL + stage], lane);
@@ -652,6 +693,10 @@ tile_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
       mbar_init(&bars[PV_DONE + i], 1);
       mbar_init(&bars[O_FREE + i], QT / 32);
     }
+    for (int i = 0; i < Layout<D>::RAWS; ++i) {
+      mbar_init(&bars[RAW_FULL + i], 1);
+      mbar_init(&bars[RAW_FREE + i], OPERAND_WARPS);
+    }
     for (int i = 0; i < NMETA; ++i) mbar_init(&bars[META_FULL + i], 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -674,6 +719,7 @@ tile_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 12) mma_role<DT, D>(smem, bars, tmem, a, seqs, plan, ctx, c.kv_heads);
+    if (warp == 13) codes_role<D>(smem, bars, c, a, seqs, plan, ctx);
   }
   tc_fence_before();
   __syncthreads();
