@@ -140,21 +140,19 @@ struct Parts {
 
 struct Ctx { volatile int* abort_flag; };
 
-// bounded wait of a whole warp; parks in the barrier unit so that waiting warps leave the issue slots to the others
+// Bounded wait of a whole warp.  A phase that is over costs a few instructions; otherwise the warp parks in the barrier unit, a
+// microsecond at most at a time, and leaves the issue slots to the others.  The bound is a count of those (seconds): every
+// instruction here is fetched at two dozen sites by warps that share their cache.
+constexpr int MOST_PARKED = 1 << 22;
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, const Ctx& c, int code) {
-  bool ok = true;
-  if (!mbar_try_wait(bar, parity)) {
-    const long long begin = clock64();
-    while (true) {
-      if (*c.abort_flag) { ok = false; break; }
-      if (mbar_try_wait_parked(bar, parity, 1000u)) break;
-      if (clock64() - begin > WAIT_BUDGET_CYCLES) {
-        atomicCAS(const_cast<int*>(c.abort_flag), 0, code);
-        ok = false;
-        break;
-      }
-    }
+  if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity) ? 1 : 0)) return true;
+  bool ok = false;
+#pragma unroll 1
+  for (int n = 0; n < MOST_PARKED && !ok; ++n) {
+    ok = mbar_try_wait_parked(bar, parity, 1000u);
+    if (*c.abort_flag) break;
   }
+  if (!ok) atomicCAS(const_cast<int*>(c.abort_flag), 0, code);
   return __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
 }
 __device__ __forceinline__ void warp_arrive(uint64_t* bar, int lane) {
@@ -263,7 +261,6 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
   using L = Layout<D>;
   constexpr int DCH = L::DCH, LOADS = D / 16;   // 16-byte pieces of a thread per tile and tensor, half of them of each block
   const int tid = threadIdx.x - 32 * SOFTMAX_WARPS, lane = tid & 31;
-  const uint16_t sign = a.scale_log2 < 0.f ? 0x8000u : 0u;
   Walk walk(plan, a, seqs, blockIdx.x, c.kv_heads);
   Piece p;
   bool ok = true;
@@ -334,25 +331,37 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
     if (pieces > 0) ok = wait(&bars[Q_FREE], (pieces - 1) & 1, ctx, 970);
     if (!ok) break;
     ++pieces;
-#pragma unroll 2
-    for (int i = tid; i < UNIT * (D / 8); i += 32 * OPERAND_WARPS) {
-      const int row = i / (D / 8), col = (i % (D / 8)) * 8, r = p.unit * UNIT + row;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (r < a.rows) {
-        const int token = r / a.group;
-        const uint16_t* src = a.q + p.b * a.q_batch + token * a.q_token + (p.h * a.group + r - token * a.group) * a.q_head + col;
-        if (q_vector) {
-          v = __ldg(reinterpret_cast<const uint4*>(src));
-        } else {
-          uint32_t w[4];
+    constexpr int PER_ROW = D / 8, ROWS = 32 * OPERAND_WARPS / PER_ROW, AHEAD = 8;   // rows of a pass, passes in flight
+    const int col = tid % PER_ROW * 8;
+    const uint16_t* const q_head = a.q + p.b * a.q_batch + static_cast<long long>(p.h) * a.group * a.q_head + col;
+    const uint32_t q_to = base + L::Q_OFF + (col / 64) * SUB;
+    const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;   // a negative scale is the queries' sign
+#pragma unroll 1
+    for (int row0 = tid / PER_ROW; row0 < UNIT; row0 += AHEAD * ROWS) {
+      uint4 v[AHEAD];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = __ldg(src + 2 * e) | (static_cast<uint32_t>(__ldg(src + 2 * e + 1)) << 16);
-          v = make_uint4(w[0], w[1], w[2], w[3]);
+      for (int k = 0; k < AHEAD; ++k) {
+        const int r = p.unit * UNIT + row0 + k * ROWS;
+        v[k] = make_uint4(0, 0, 0, 0);
+        if (r < a.rows) {
+          const int token = r / a.group;
+          const uint16_t* src = q_head + token * a.q_token + (r - token * a.group) * a.q_head;
+          if (q_vector) {
+            v[k] = __ldg(reinterpret_cast<const uint4*>(src));
+          } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = __ldg(src + 2 * e) | (static_cast<uint32_t>(__ldg(src + 2 * e + 1)) << 16);
+            v[k] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
         }
-        const uint32_t flip = sign * 0x10001u;   // a negative scale is the queries' sign
-        v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
       }
-      sts128(base + L::Q_OFF + ((row / QT) * DCH + col / 64) * SUB + sw128_offset(row % QT, col % 64), v);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int row = row0 + k * ROWS;
+        sts128(q_to + (row / QT) * DCH * SUB + sw128_offset(row % QT, col % 64),
+               make_uint4(v[k].x ^ flip, v[k].y ^ flip, v[k].z ^ flip, v[k].w ^ flip));
+      }
     }
     fence_proxy_async();
     warp_arrive(&bars[Q_FULL], lane);
@@ -384,24 +393,30 @@ __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t
   constexpr int DCH = L::DCH;
   const bool leader = elect_one();   // the whole warp runs the (uniform) control flow; one elected lane issues
   const uint32_t base = smem_u32(smem);
+  // operand descriptors of the first tile and stage; the others lie a whole number of 16-byte units on
+  const uint64_t q_desc = make_smem_desc_sw128(base + L::Q_OFF), k_desc = make_smem_desc_sw128(base + L::K_OFF);
+  const uint64_t v_desc = make_smem_desc_sw128(base + L::V_OFF);
   auto issue_s = [&](int i, int stage) {
+    const uint64_t qd = q_desc + static_cast<uint32_t>(i * (DCH * SUB / 16)), kd = k_desc + static_cast<uint32_t>(stage * (DCH * SUB / 16));
+    const uint32_t d = tmem + i * 128;
+    if (leader) {
 #pragma unroll
-    for (int ch = 0; ch < DCH; ++ch) {
-      const uint64_t qd = make_smem_desc_sw128(base + L::Q_OFF + (i * DCH + ch) * SUB);
-      const uint64_t kd = make_smem_desc_sw128(base + L::K_OFF + (stage * DCH + ch) * SUB);
+      for (int ch = 0; ch < DCH; ++ch)
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (leader) mma_bf16(tmem + i * 128, qd + 2 * k, kd + 2 * k, idesc<DT>(TOK), ch + k > 0);
+        for (int k = 0; k < 4; ++k)
+          mma_bf16(d, qd + ch * (SUB / 16) + 2 * k, kd + ch * (SUB / 16) + 2 * k, idesc<DT>(TOK), ch + k > 0);
+      mma_commit(&bars[S_FULL + i]);
     }
-    if (leader) mma_commit(&bars[S_FULL + i]);
   };
   // weights of 64 tokens (a block) times V of it: [128 rows x 64] [D x 64]^T, both with the tokens running along rows
   auto issue_pv = [&](int i, int stage, int half, bool accumulate) {
-    const uint64_t vd = make_smem_desc_sw128(base + L::V_OFF + (stage * 2 + half) * L::V_SUB);
+    const uint64_t vd = v_desc + static_cast<uint32_t>((stage * 2 + half) * (L::V_SUB / 16));
+    const uint32_t d = tmem + 256 + i * 128, w = tmem + i * 128 + half * 32;
+    if (leader) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (leader) mma_bf16_ts(tmem + 256 + i * 128, tmem + i * 128 + half * 32 + 8 * k, vd + 2 * k, idesc<DT>(D), accumulate || half + k > 0);
-    if (half == 1 && leader) mma_commit(&bars[PV_DONE + i]);
+      for (int k = 0; k < 4; ++k) mma_bf16_ts(d, w + 8 * k, vd + 2 * k, idesc<DT>(D), accumulate || k > 0);
+      if (half == 1) mma_commit(&bars[PV_DONE + i]);
+    }
   };
   Walk walk(plan, a, seqs, blockIdx.x, kv_heads);
   Piece p;
@@ -412,34 +427,44 @@ __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t
     const int longest = max(n[0], n[1]);
     ok = wait(&bars[Q_FULL], pieces & 1, ctx, 980);
     ++pieces;
-    // which query tile is the last to use tile t
+    // The first and the last query tile to use tile t: each K and V stage is waited for once and given back once.
+    auto first_of = [&](int t) { return t < n[0] ? 0 : 1; };
     auto last_of = [&](int t) { return t < n[1] ? 1 : 0; };
+#pragma unroll 1
     for (int t = 0; t <= longest && ok; ++t) {
-      const int cur = seq + t - 1, next = seq + t;   // PV of tile t - 1 and S of tile t, query tile by query tile
-      for (int i = 0; i < NQ && ok; ++i) {
-        if (t > 0 && t - 1 < n[i]) {
-          const int stage = cur % STAGES, ci = done[i] + t - 1;
-          ok = wait(&bars[P_READY + i], ci & 1, ctx, 981);
-          ok = ok && wait(&bars[V_FULL + stage], (cur / STAGES) & 1, ctx, 982);
-          if (ok && t == 1 && used[i] > 0) ok = wait(&bars[O_FREE + i], (used[i] - 1) & 1, ctx, 983);
+      // PV of tile t - 1 and S of tile t, query tile by query tile
+      const int now = (seq + t - 1) % STAGES, next = (seq + t) % STAGES;
+      const uint32_t now_phase = ((seq + t - 1) / STAGES) & 1, next_phase = ((seq + t) / STAGES) & 1;
+#pragma unroll 1
+      for (int i = 0; i < NQ; ++i) {
+        const int tiles = i ? n[1] : n[0];
+        if (t > 0 && t - 1 < tiles) {
+          const uint32_t phase = ((i ? done[1] : done[0]) + t - 1) & 1;
+          if (i == first_of(t - 1)) ok = wait(&bars[V_FULL + now], now_phase, ctx, 982);
+          if (t == 1) {   // the first PV of a piece overwrites O: the rows of the piece before must have been read
+            const int pieces_before = i ? used[1] : used[0];
+            if (ok && pieces_before > 0) ok = wait(&bars[O_FREE + i], (pieces_before - 1) & 1, ctx, 983);
+          }
+          ok = ok && wait(&bars[P_READY + i], phase, ctx, 981);
           if (!ok) break;
           tc_fence_after();
-          issue_pv(i, stage, 0, t > 1);
-          ok = wait(&bars[P_LAST + i], ci & 1, ctx, 984);
+          issue_pv(i, now, 0, t > 1);
+          ok = wait(&bars[P_LAST + i], phase, ctx, 984);
           if (!ok) break;
           tc_fence_after();
-          issue_pv(i, stage, 1, true);
-          if (i == last_of(t - 1) && leader) mma_commit(&bars[V_FREE + stage]);
+          issue_pv(i, now, 1, true);
+          if (i == last_of(t - 1) && leader) mma_commit(&bars[V_FREE + now]);
         }
-        if (t < n[i]) {
+        if (t < tiles) {
           // S of the next tile overwrites P of this one, right behind the PV that reads it: the tensor core executes one
           // thread's MMAs in order
-          const int stage = next % STAGES;
-          ok = wait(&bars[K_FULL + stage], (next / STAGES) & 1, ctx, 985);
-          if (!ok) break;
-          tc_fence_after();
-          issue_s(i, stage);
-          if (i == last_of(t) && leader) mma_commit(&bars[K_FREE + stage]);
+          if (i == first_of(t)) {
+            ok = wait(&bars[K_FULL + next], next_phase, ctx, 985);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          issue_s(i, next);
+          if (i == last_of(t) && leader) mma_commit(&bars[K_FREE + next]);
         }
       }
     }
@@ -700,15 +725,15 @@ tile_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
   const uint32_t tmem = *tmem_slot;
   const Ctx ctx{abort_flag};
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // 512 threads x 128 registers: 256 x 184 + 128 x 104 + 128 x 40 = 65,536
+  // 512 threads x 128 registers: 256 x 192 + 128 x 72 + 128 x 56 = 65,536
   if (warp < SOFTMAX_WARPS) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
     softmax_role<DT, D>(smem, bars, tmem, a, seqs, plan, parts, ctx, c.kv_heads);
   } else if (warp < SOFTMAX_WARPS + OPERAND_WARPS) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     operand_role<DT, D>(smem, bars, c, a, seqs, plan, ctx, q_vector);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 12) mma_role<DT, D>(smem, bars, tmem, a, seqs, plan, ctx, c.kv_heads);
     if (warp == 13) codes_role<D>(smem, bars, c, a, seqs, plan, ctx);
   }
