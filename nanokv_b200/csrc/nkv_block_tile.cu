@@ -275,26 +275,33 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
   const uint32_t v0 = v_to + sw128_offset(v_row, v_col), v1 = v_to + sw128_offset(v_row, v_col + 8);
   constexpr uint32_t K_STEP = 2048 / D * 128, V_STEP = 32 * 128;
   // The eight lanes that store together shall fill all banks: for K of 128-wide heads half of them take their second piece first.
-  const bool second_first = D == 128 && (lane & 4) != 0;
-  // One rolled loop for both on purpose: unrolled copies push the softmax warps' instructions out of the cache they share (a
-  // quarter of the issue slots went to fetching, 2.5 ms against 1.8 for 4,680 queries x 24 heads over 24,960 tokens).
-  auto convert = [&](uint32_t to0, uint32_t to1, uint32_t step) {
+  const uint32_t swap = D == 128 && (lane & 4) != 0 ? 8 : 0;
+  const uint32_t kf = swap ? k1 : k0, ks = swap ? k0 : k1;
+  // One loop for both, rolled but for pairs, on purpose: unrolled copies push the softmax warps' instructions out of the cache
+  // they share (a quarter of the issue slots went to fetching, 2.5 ms against 1.8 for 4,680 queries x 24 heads over 24,960
+  // tokens).
+  auto convert = [&](uint32_t to0, uint32_t to1, uint32_t step, uint32_t first) {
     uint32_t from = base + L::RAW_OFF + (item % L::RAWS) * L::RAW + tid * 16;
-    uint4 next = lds128(from);
 #pragma unroll 1
-    for (int i = 0; i < LOADS; ++i) {
-      const uint4 raw = next;
-      from += 2048;
-      if (i + 1 < LOADS) next = lds128(from);
-      uint4 p0, p1;
-      expand<DT>(second_first ? raw.z : raw.x, p0.x, p0.y);
-      expand<DT>(second_first ? raw.w : raw.y, p0.z, p0.w);
-      expand<DT>(second_first ? raw.x : raw.z, p1.x, p1.y);
-      expand<DT>(second_first ? raw.y : raw.w, p1.z, p1.w);
-      sts128(second_first ? to1 : to0, p0);
-      sts128(second_first ? to0 : to1, p1);
-      to0 += step;
-      to1 += step;
+    for (int i = 0; i < LOADS; i += 2) {
+      const uint2 a0 = lds64(from + first), a1 = lds64(from + (first ^ 8));
+      const uint2 b0 = lds64(from + 2048 + first), b1 = lds64(from + 2048 + (first ^ 8));
+      uint4 p0, p1, p2, p3;
+      expand<DT>(a0.x, p0.x, p0.y);
+      expand<DT>(a0.y, p0.z, p0.w);
+      expand<DT>(a1.x, p1.x, p1.y);
+      expand<DT>(a1.y, p1.z, p1.w);
+      sts128(to0, p0);
+      sts128(to1, p1);
+      expand<DT>(b0.x, p2.x, p2.y);
+      expand<DT>(b0.y, p2.z, p2.w);
+      expand<DT>(b1.x, p3.x, p3.y);
+      expand<DT>(b1.y, p3.z, p3.w);
+      sts128(to0 + step, p2);
+      sts128(to1 + step, p3);
+      from += 4096;
+      to0 += 2 * step;
+      to1 += 2 * step;
     }
     warp_arrive(&bars[RAW_FREE + item % L::RAWS], lane);
     ++item;
@@ -373,7 +380,7 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
       if (ok && use >= 1) ok = wait(&bars[(value ? V_FREE : K_FREE) + stage], (use - 1) & 1, ctx, 972 + value);
       if (!ok) break;
       const uint32_t at = stage * (value ? 2 * L::V_SUB : DCH * SUB);
-      convert((value ? v0 : k0) + at, (value ? v1 : k1) + at, value ? V_STEP : K_STEP);
+      convert((value ? v0 : kf) + at, (value ? v1 : ks) + at, value ? V_STEP : K_STEP, value ? 0 : swap);
       const int open = full - 2 * (p.tile0 + t / 2);   // 0 or 1: that half of the tile is not a full block
       if (open <= 1) {
         if (value) open_values(v_to + at, bh, open, held); else open_keys(base + L::K_OFF + at, bh, open);
@@ -725,15 +732,15 @@ tile_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
   const uint32_t tmem = *tmem_slot;
   const Ctx ctx{abort_flag};
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // 512 threads x 128 registers: 256 x 192 + 128 x 72 + 128 x 56 = 65,536
+  // 512 threads x 128 registers: 256 x 184 + 128 x 72 + 128 x 72 = 65,536
   if (warp < SOFTMAX_WARPS) {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     softmax_role<DT, D>(smem, bars, tmem, a, seqs, plan, parts, ctx, c.kv_heads);
   } else if (warp < SOFTMAX_WARPS + OPERAND_WARPS) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     operand_role<DT, D>(smem, bars, c, a, seqs, plan, ctx, q_vector);
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp == 12) mma_role<DT, D>(smem, bars, tmem, a, seqs, plan, ctx, c.kv_heads);
     if (warp == 13) codes_role<D>(smem, bars, c, a, seqs, plan, ctx);
   }
