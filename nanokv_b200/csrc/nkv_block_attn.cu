@@ -133,13 +133,13 @@ Sequences sequences_of(const nkv_block_cache& c, int first, int n, const int32_t
 
 // scratch of one launch over n sequences: the rows' weight sums per block, then the kernel's own
 struct Scratch { size_t partial, own; };
-Scratch scratch_of(const nkv_block_cache& c, const Sequences& seqs, int n, int group, int tokens, bool causal, int most_blocks, bool with_weights) {
+Scratch scratch_of(const nkv_block_cache& c, const Sequences& seqs, int n, int group, int tokens, int most_blocks, bool with_weights) {
   const int rows = group * tokens;
   Scratch s{0, 0};
   if (with_weights) s.partial = (static_cast<size_t>(n) * c.kv_heads * most_blocks * rows * 4 + 255) & ~static_cast<size_t>(255);
   if (!simt_forced())
     s.own = block_step_supported(rows) ? block_step_bytes(seqs, n, c.kv_heads, rows, c.head_dim)
-                                       : block_tile_bytes(seqs, n, c.kv_heads, group, rows, causal, c.head_dim);
+                                       : block_tile_bytes(seqs, n, c.kv_heads, most_blocks, rows, c.head_dim);
   return s;
 }
 
@@ -150,7 +150,7 @@ size_t block_attend_workspace_bytes(const nkv_block_cache& c, int heads, int tok
   size_t most = 0;   // launches follow one another on the stream and share it
   for (int first = 0; first < c.batch; first += MAX_SEQUENCES) {
     const int n = min(MAX_SEQUENCES, c.batch - first);
-    const Scratch s = scratch_of(c, sequences_of(c, first, n, counts, tokens), n, heads / c.kv_heads, tokens, causal, most_blocks_of(c), with_weights);
+    const Scratch s = scratch_of(c, sequences_of(c, first, n, counts, tokens), n, heads / c.kv_heads, tokens, most_blocks_of(c), with_weights);
     if (s.partial + s.own > most) most = s.partial + s.own;
   }
   return most;
@@ -178,7 +178,7 @@ int block_attend(const nkv_block_cache& c, const nkv_tokens& q, int tokens, cons
     a.most_blocks = most_blocks_of(c);
     a.scale_log2 = scale * LOG2E;
     const BlockArrays arrays = block_arrays(c, first);
-    void* const own = static_cast<uint8_t*>(workspace) + scratch_of(c, seqs, n, a.group, tokens, causal, a.most_blocks, weights != nullptr).partial;
+    void* const own = static_cast<uint8_t*>(workspace) + scratch_of(c, seqs, n, a.group, tokens, a.most_blocks, weights != nullptr).partial;
     if (!simt_forced() && block_step_supported(a.rows)) {
       const int rc = block_step(arrays, a, seqs, n, c.dtype, c.head_dim, own, status, stream);
       if (rc != NKV_OK) return rc;
