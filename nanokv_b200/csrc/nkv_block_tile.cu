@@ -1,14 +1,10 @@
 // Attention of many query rows over the 8-bit block cache, on tcgen05.
 //
-// The rows of a kv head (its group's heads of all query tokens) are cut into units of 256: two 128-row tiles that share every
-// block of K and V.  Bulk copies bring a block's codes into a ring; four warps turn them into the cache's 16-bit type (exactly:
-// a code is an integer below 2^7) and store them as the swizzled operands the tensor cores read.  S = Q K^T of a block goes to
-// tensor memory, eight warps take the softmax (one thread per row), P replaces S as the operand of O += P V.  Each query
-// tile has two places for S: while one block's softmax runs, the product of the block before and the scores of the block
-// behind are computed, so that neither side waits for the other's latency.  (Scores of 128 tokens at a time in one place, with
-// P handed over in halves, took 1.34 ms where this takes @@.)
-//
-// The block scales never touch an operand.  K's multiplies the
+// The rows of a kv head (its group's heads of all query tokens) are cut into units of 256: two 128-row tiles that share
+// every K and V tile.  A tile is 128 tokens, two blocks of the cache.  A warp brings its codes into a ring by bulk
+// copies; four warps turn them into the cache's 16-bit type (exactly: a code is an integer below 2^7) and store them as the
+// swizzled operands the tensor cores read; no 16-bit copy of the cache exists in memory.  S = Q K^T goes to tensor memory, eight warps take the softmax (one
+// thread per row), P replaces S as the operand of O += P V.  The block scales never touch an operand.  K's multiplies the
 // scores.  V's goes into the exponent: the weight handed over is P' = 2^(s + log2 vs - m'), with m' the running maximum of
 // s + log2 vs, so that a row's weights are at most 1 (2^8 with the lazy reference) however unlike the scales of its blocks are; a block's
 // part of the row sum is the sum of its P' divided by vs again, in fp32.
@@ -29,7 +25,8 @@ namespace {
 using namespace tc;
 
 constexpr int QT = 128, NQ = 2, UNIT = QT * NQ;   // rows of a query tile, tiles and rows of a unit
-constexpr int STAGES = 4;                         // K / V operand stages, a block each
+constexpr int TOK = 128;                          // tokens of a tile
+constexpr int STAGES = 2;                         // K / V operand stages
 constexpr int SOFTMAX_WARPS = 8, OPERAND_WARPS = 4, MMA_WARP = 12, THREADS = 448;
 constexpr int SUB = 128 * 128;                    // bytes of a [128 rows x 64 elements] swizzled operand tile
 constexpr float RESCALE_THRESHOLD = 8.0f;
@@ -37,33 +34,33 @@ constexpr float RESCALE_THRESHOLD = 8.0f;
 // dropping the low bits, which leaves the quarter-rate conversion unit to the exponentials
 constexpr float HALF_STEP_LOG2 = 0.0028150156070540f, HALF_STEP_INV = 0.998050682261209f;
 
-// (S_FULL and P_READY: query tile i, place h at 2 i + h)
-enum Bar { Q_FULL = 0, Q_FREE = 1, K_FULL = 2, K_FREE = 6, V_FULL = 10, V_FREE = 14, S_FULL = 18, P_READY = 22, PV_DONE = 26,
-           O_FREE = 28, RAW_FULL = 30, RAW_FREE = 34, O_DONE = 38, NUM_BARS = 40 };
-constexpr int NMETA = 16;        // scales are written up to eleven blocks ahead of the softmax (operand stages, the ring of codes)
-constexpr int M_SLOT = NUM_BARS * 8, M_ABORT = M_SLOT + 4, M_SCALES = 512;   // scales: [NMETA] float4 {ks, log2 vs, 1 / vs, -}
+// (P_READY: query tile i, half h of its tokens at 2 i + h)
+enum Bar { Q_FULL = 0, Q_FREE = 1, K_FULL = 2, K_FREE = 4, V_FULL = 6, V_FREE = 8, S_FULL = 10, P_READY = 12, PV_HALF = 16,
+           O_DONE = 18, O_FREE = 20, RAW_FULL = 22, RAW_FREE = 26, NUM_BARS = 30 };
+// scales are written up to four tiles ahead of the softmax (two operand stages, the ring of codes)
+constexpr int NMETA = 8;
+constexpr int M_SLOT = NUM_BARS * 8, M_ABORT = M_SLOT + 4, M_SCALES = 512;   // scales: [NMETA][2 blocks] float4 {ks, log2 vs, 1 / vs, -}
 
 template <int D> struct Layout {
   static constexpr int DCH = D / 64;
-  static constexpr int K_SUB = NKV_BLOCK * 128;    // [64 tokens x 64 elements]
-  static constexpr int OPERAND = NKV_BLOCK * D * 2;   // a block of K ([DCH][64][64 elements]) or V ([D][64 tokens])
   static constexpr int Q_OFF = 1024;
   static constexpr int K_OFF = Q_OFF + NQ * DCH * SUB;
-  static constexpr int V_OFF = K_OFF + STAGES * OPERAND;
-  static constexpr int RAW_OFF = V_OFF + STAGES * OPERAND;
-  static constexpr int RAW = NKV_BLOCK * D;        // codes of a block of K or V
-  static constexpr int RAWS = 4;                   // ring of them, K and V in turn
+  static constexpr int V_OFF = K_OFF + STAGES * DCH * SUB;
+  static constexpr int V_SUB = D * 128;            // [D rows x 64 tokens]
+  static constexpr int RAW_OFF = V_OFF + STAGES * 2 * V_SUB;
+  static constexpr int RAW = TOK * D;              // codes of a tile of K or V
+  static constexpr int RAWS = D == 128 ? 2 : 4;    // ring of them
   static constexpr int BYTES = RAW_OFF + RAWS * RAW;
   static constexpr int DYNAMIC = BYTES + 1024;     // room to start on 1,024 bytes
 };
-static_assert(M_SCALES + NMETA * 16 <= 1024, "meta block");
+static_assert(M_SCALES + NMETA * 2 * 16 <= 1024, "meta block");
 
-// The list of blocks that units attend: sequence by sequence, kv head by kv head, unit by unit.
+// The list of tiles: sequence by sequence, kv head by kv head, unit by unit.
 struct Plan {
   uint32_t start[MAX_SEQUENCES + 1];
   int sequences, runs, units;      // runs: thread blocks; units per kv head
-  int most_blocks;                 // of any sequence: the images of a head
-  uint32_t run, longer;            // blocks of a run; the first `longer` have one more
+  int most_tiles;                  // of any sequence: the images of a head
+  uint32_t run, longer;            // tiles of a run; the first `longer` have one more
   __host__ __device__ uint32_t first_of(uint32_t i) const { return i * run + min(i, longer); }
   __host__ __device__ uint32_t run_of(uint32_t g) const {
     const uint32_t edge = longer * (run + 1);
@@ -71,26 +68,26 @@ struct Plan {
   }
 };
 
-// blocks that any of rows r0 .. r0 + n - 1 sees
-__host__ __device__ inline int blocks_seen(int length, int count, int group, int rows, bool causal, int r0, int n) {
+// tokens that any of rows [0, r_end) ... of a query tile sees, as tiles: rows r0 .. r0 + n - 1 of `rows`
+__host__ __device__ inline int tiles_seen(int length, int count, int group, int rows, bool causal, int r0, int n) {
   const int r1 = min(rows, r0 + n) - 1;
   if (r1 < r0 || r0 / group >= count) return 0;
   const int last = min(r1 / group, count - 1);
   const int seen = causal ? min(length, length - count + last + 1) : length;
-  return seen > 0 ? (seen + NKV_BLOCK - 1) / NKV_BLOCK : 0;
+  return seen > 0 ? (seen + TOK - 1) / TOK : 0;
 }
 
 struct Piece {                     // a unit, or a run's part of one
-  int b, h, unit, block0, n, whole;   // blocks block0 .. block0 + n - 1; whole: all the unit has
+  int b, h, unit, tile0, nt, whole;   // tiles tile0 .. tile0 + nt - 1; whole: all the unit has
 };
 
 // The pieces of one run in order; every role walks the same list.
 struct Walk {
   uint32_t g, end;
-  int b, h, unit, blocks;          // the unit that g lies in, its blocks
-  uint32_t at;                     // blocks of the unit before g
-  __device__ __forceinline__ int blocks_of(const Call& a, const Sequences& s, int bb, int u) const {
-    return blocks_seen(s.length[bb], s.count[bb], a.group, a.rows, a.causal, u * UNIT, UNIT);
+  int b, h, unit, tiles;           // the unit that g lies in, its tiles
+  uint32_t at;                     // tiles of the unit before g
+  __device__ __forceinline__ int tiles_of(const Call& a, const Sequences& s, int bb, int u) const {
+    return tiles_seen(s.length[bb], s.count[bb], a.group, a.rows, a.causal, u * UNIT, UNIT);
   }
   __device__ __forceinline__ Walk(const Plan& p, const Call& a, const Sequences& s, int run, int kv_heads) {
     g = p.first_of(run);
@@ -106,14 +103,14 @@ struct Walk {
     h = static_cast<int>(at / per_head);
     at -= h * per_head;
     unit = 0;
-    while (at >= static_cast<uint32_t>(blocks = blocks_of(a, s, b, unit))) {
-      at -= blocks;
+    while (at >= static_cast<uint32_t>(tiles = tiles_of(a, s, b, unit))) {
+      at -= tiles;
       ++unit;
     }
   }
   __device__ __forceinline__ bool next(const Plan& p, const Call& a, const Sequences& s, int kv_heads, Piece& out) {
     if (g >= end) return false;
-    while (at >= static_cast<uint32_t>(blocks)) {   // on to the next unit that has any
+    while (at >= static_cast<uint32_t>(tiles)) {   // on to the next unit that has tiles
       at = 0;
       if (++unit == p.units) {
         unit = 0;
@@ -122,23 +119,23 @@ struct Walk {
           ++b;
         }
       }
-      blocks = blocks_of(a, s, b, unit);
+      tiles = tiles_of(a, s, b, unit);
     }
     out.b = b;
     out.h = h;
     out.unit = unit;
-    out.block0 = static_cast<int>(at);
-    out.n = static_cast<int>(min(static_cast<uint32_t>(blocks) - at, end - g));
-    out.whole = out.n == blocks;
-    at += out.n;
-    g += out.n;
+    out.tile0 = static_cast<int>(at);
+    out.nt = static_cast<int>(min(static_cast<uint32_t>(tiles) - at, end - g));
+    out.whole = out.nt == tiles;
+    at += out.nt;
+    g += out.nt;
     return true;
   }
 };
 
-// blocks of a piece that query tile i takes part in (causal: the first tile sees less than the second)
-__device__ __forceinline__ int blocks_for(const Call& a, const Sequences& s, const Piece& p, int i) {
-  return max(0, min(p.n, blocks_seen(s.length[p.b], s.count[p.b], a.group, a.rows, a.causal, p.unit * UNIT + i * QT, QT) - p.block0));
+// tiles of a piece that query tile i takes part in (causal: the first tile sees less than the second)
+__device__ __forceinline__ int tiles_for(const Call& a, const Sequences& s, const Piece& p, int i) {
+  return max(0, min(p.nt, tiles_seen(s.length[p.b], s.count[p.b], a.group, a.rows, a.causal, p.unit * UNIT + i * QT, QT) - p.tile0));
 }
 
 // A run holds at most one piece that starts inside a unit and one that starts with it and is cut: two places each.
@@ -240,88 +237,85 @@ __device__ __forceinline__ float max32(const uint32_t (&r)[32]) {
   return fmaxf(x, y);
 }
 
-// ---- warp 13: codes (or images) and scales -----------------------------------------------------------------------
+// ---- warp 13: codes and scales ---------------------------------------------------------------------------------
 template <int D, bool IMAGES>
 __device__ __forceinline__ void codes_role(uint8_t* smem, uint64_t* bars, const BlockArrays& c, const Call& a, const Sequences& seqs,
                                            const Plan& plan, const Ctx& ctx, const uint8_t* images) {
   using L = Layout<D>;
+  constexpr uint32_t BLOCK_BYTES = NKV_BLOCK * D;
   const int lane = threadIdx.x & 31;
   float4* const scales = reinterpret_cast<float4*>(smem + M_SCALES);
   Walk walk(plan, a, seqs, blockIdx.x, c.kv_heads);
   Piece p;
   bool ok = true;
-  int seq = 0;
+  int seq = 0, item = 0;
   while (ok && walk.next(plan, a, seqs, c.kv_heads, p)) {
     const size_t bh = static_cast<size_t>(p.b) * c.kv_heads + p.h;
     const int full = seqs.length[p.b] / NKV_BLOCK;
     long long slot = 0;
     float2 sc = make_float2(1.f, 1.f);
-    for (int n = 0; n < p.n && ok; ++n, ++seq) {
-      const int block = p.block0 + n, at = n & 31;
-      if (at == 0) {   // lane l knows block l of the next 32: one trip to memory for all of them
+    for (int t = 0; t < p.nt && ok; ++t, ++seq) {
+      const int block0 = 2 * (p.tile0 + t), at = (2 * t) & 31;
+      if (at == 0) {   // lane l knows block l of the next sixteen tiles: one trip to memory for all of them
+        const int block = block0 + lane;
         sc = make_float2(1.f, 1.f);
-        if (block + lane < full) {
-          slot = static_cast<long long>(slot_of(c, bh, block + lane));
+        if (block < full) {
+          slot = static_cast<long long>(slot_of(c, bh, block));
           sc = __ldg(reinterpret_cast<const float2*>(c.scales) + slot);
         }
       }
-      if (lane == at) {
+      if ((lane & ~1) == at) {
         // a block of scale 0 has only codes 0: any scale serves, and 2^-30 lies below all that 16-bit rows give
         const float lv = sc.y == 0.f ? -30.f : log2f(sc.y);
-        scales[seq % NMETA] = make_float4(sc.x == 0.f ? 1.f : sc.x, lv, exp2f(-lv), 0.f);
+        scales[(seq % NMETA) * 2 + (lane & 1)] = make_float4(sc.x == 0.f ? 1.f : sc.x, lv, exp2f(-lv), 0.f);
       }
       __syncwarp();   // ahead of the request whose completion lets S be computed
-      const long long from = __shfl_sync(0xffffffffu, slot, at);
-#pragma unroll 1
-      for (int tensor = 0; tensor < 2 && ok; ++tensor) {
-        if (IMAGES) {
-          const int stage = seq % STAGES, use = seq / STAGES;
-          uint64_t* const bar = &bars[(tensor ? V_FULL : K_FULL) + stage];
+      if (IMAGES) {
+        const int stage = seq % STAGES, use = seq / STAGES;
+        constexpr uint32_t BYTES = L::DCH * SUB;   // (as many for K as for V)
+        const uint8_t* const from = images + ((bh * plan.most_tiles + p.tile0 + t) * 2) * static_cast<size_t>(BYTES);
+        for (int tensor = 0; tensor < 2 && ok; ++tensor) {
+          uint64_t* const full_bar = &bars[(tensor ? V_FULL : K_FULL) + stage];
           if (use >= 1) ok = wait(&bars[(tensor ? V_FREE : K_FREE) + stage], (use - 1) & 1, ctx, 976);
           if (ok && lane == 0) {
-            mbar_arrive_expect_tx(bar, L::OPERAND);
-            bulk_load_1d(smem + (tensor ? L::V_OFF : L::K_OFF) + stage * L::OPERAND,
-                         images + ((bh * plan.most_blocks + block) * 2 + tensor) * static_cast<size_t>(L::OPERAND), L::OPERAND, bar);
+            mbar_arrive_expect_tx(full_bar, BYTES);
+            bulk_load_1d(smem + (tensor ? L::V_OFF : L::K_OFF) + stage * BYTES, from + tensor * BYTES, BYTES, full_bar);
           }
-        } else {
-          const int item = 2 * seq + tensor, stage = item % L::RAWS;
-          if (item >= L::RAWS) ok = wait(&bars[RAW_FREE + stage], (item / L::RAWS - 1) & 1, ctx, 975);
-          if (ok && lane == 0) {
-            if (block < full) {
-              mbar_arrive_expect_tx(&bars[RAW_FULL + stage], L::RAW);
-              bulk_load_1d(smem + L::RAW_OFF + stage * L::RAW, (tensor ? c.v_codes : c.k_codes) + from * L::RAW, L::RAW, &bars[RAW_FULL + stage]);
-            } else {
-              mbar_arrive(&bars[RAW_FULL + stage]);   // (the open block is read where it is needed)
-            }
-          }
+          __syncwarp();
+        }
+        continue;
+      }
+      const long long s0 = __shfl_sync(0xffffffffu, slot, at), s1 = __shfl_sync(0xffffffffu, slot, at + 1);
+      const uint32_t blocks = min(2, max(0, full - block0));   // full ones: the open block is read where it is needed
+      for (int tensor = 0; tensor < 2 && ok; ++tensor, ++item) {
+        const int stage = item % L::RAWS;
+        if (item >= L::RAWS) ok = wait(&bars[RAW_FREE + stage], (item / L::RAWS - 1) & 1, ctx, 975);
+        if (!ok) break;
+        if (lane == 0) {
+          uint8_t* const to = smem + L::RAW_OFF + stage * L::RAW;
+          const uint8_t* const from = tensor ? c.v_codes : c.k_codes;
+          mbar_arrive_expect_tx(&bars[RAW_FULL + stage], blocks * BLOCK_BYTES);
+          if (blocks > 0) bulk_load_1d(to, from + s0 * BLOCK_BYTES, BLOCK_BYTES, &bars[RAW_FULL + stage]);
+          if (blocks > 1) bulk_load_1d(to + BLOCK_BYTES, from + s1 * BLOCK_BYTES, BLOCK_BYTES, &bars[RAW_FULL + stage]);
         }
         __syncwarp();
       }
     }
   }
-  if (!ok) {   // copies in flight land before the thread block goes away
+  if (!ok) {   // copies in flight land before the block goes away
     const long long begin = clock64();
     while (clock64() - begin < (1ll << 21)) {}
   }
 }
 
-// ---- warps 8-11: queries, K and V as operands ---------------------------------------------------------------------
+// ---- warps 8-11: queries, K and V as operands -----------------------------------------------------------------
 template <int DT, int D, bool IMAGES>
 __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, const BlockArrays& c, const Call& a, const Sequences& seqs,
                                              const Plan& plan, const Ctx& ctx, int q_vector) {
   using L = Layout<D>;
-  constexpr int DCH = L::DCH, LOADS = D / 32;   // 16-byte pieces of a thread per block and tensor
+  constexpr int DCH = L::DCH, LOADS = D / 16;   // 16-byte pieces of a thread per tile and tensor, half of them of each block
   const int tid = threadIdx.x - 32 * SOFTMAX_WARPS, lane = tid & 31;
   const uint32_t base = smem_u32(smem);
-  // Where this thread's 16 codes of a block go, as two 16-byte pieces of an operand row: K rows are tokens of D codes, V rows
-  // columns of 64.  Its next 16 codes lie 2,048 bytes on in the ring and a whole number of 8-row groups on in the
-  // operand, so one step serves all of them.
-  const int k_row = tid * 16 / D, k_col = tid * 16 % D, v_row = tid / 4, v_col = tid % 4 * 16;
-  const uint32_t k_to = base + L::K_OFF + (k_col / 64) * L::K_SUB, v_to = base + L::V_OFF;
-  // the eight lanes that store together shall fill all banks: for K of 128-wide heads half of them take their second piece first
-  const uint32_t k_swap = D == 128 && (lane & 4) != 0 ? 8 : 0;
-  const uint32_t k0 = k_to + sw128_offset(k_row, k_col % 64 + k_swap), k1 = k_to + sw128_offset(k_row, k_col % 64 + (k_swap ^ 8));
-  const uint32_t v0 = v_to + sw128_offset(v_row, v_col), v1 = v_to + sw128_offset(v_row, v_col + 8);
   // queries: a thread has one 16-byte column of every ROWS-th row of the unit
   constexpr int PER_ROW = D / 8, ROWS = 32 * OPERAND_WARPS / PER_ROW, AHEAD = 8;
   const int q_row = tid / PER_ROW, q_col = tid % PER_ROW * 8;
@@ -330,7 +324,72 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
   Walk walk(plan, a, seqs, blockIdx.x, c.kv_heads);
   Piece p;
   bool ok = true;
-  int seq = 0, pieces = 0;
+  int seq = 0, pieces = 0, item = 0;
+  // Where this thread's 16 codes of a tile go, as two 16-byte pieces of an operand row: K rows are tokens of D codes, V rows
+  // columns of 64 per block.  Its next 16 codes lie 2,048 bytes on in the ring and a whole number of 8-row groups
+  // on in the operand, so one step serves all of them.
+  const int k_row = tid * 16 / D, k_col = tid * 16 % D, v_row = tid / 4, v_col = tid % 4 * 16;
+  const uint32_t k_to = base + L::K_OFF + (k_col / 64) * SUB, v_to = base + L::V_OFF;
+  const uint32_t k0 = k_to + sw128_offset(k_row, k_col % 64), k1 = k_to + sw128_offset(k_row, k_col % 64 + 8);
+  const uint32_t v0 = v_to + sw128_offset(v_row, v_col), v1 = v_to + sw128_offset(v_row, v_col + 8);
+  constexpr uint32_t K_STEP = 2048 / D * 128, V_STEP = 32 * 128;
+  // The eight lanes that store together shall fill all banks: for K of 128-wide heads half of them take their second piece first.
+  const uint32_t swap = D == 128 && (lane & 4) != 0 ? 8 : 0;
+  const uint32_t kf = swap ? k1 : k0, ks = swap ? k0 : k1;
+  // One loop for both, rolled but for pairs, on purpose: unrolled copies push the softmax warps' instructions out of the cache
+  // they share (a quarter of the issue slots went to fetching, 2.5 ms against 1.8 for 4,680 queries x 24 heads over 24,960
+  // tokens).
+  auto convert = [&](uint32_t to0, uint32_t to1, uint32_t step, uint32_t first) {
+    uint32_t from = base + L::RAW_OFF + (item % L::RAWS) * L::RAW + tid * 16;
+#pragma unroll 1
+    for (int i = 0; i < LOADS; i += 2) {
+      const uint2 a0 = lds64(from + first), a1 = lds64(from + (first ^ 8));
+      const uint2 b0 = lds64(from + 2048 + first), b1 = lds64(from + 2048 + (first ^ 8));
+      uint4 p0, p1, p2, p3;
+      expand<DT>(a0.x, p0.x, p0.y);
+      expand<DT>(a0.y, p0.z, p0.w);
+      expand<DT>(a1.x, p1.x, p1.y);
+      expand<DT>(a1.y, p1.z, p1.w);
+      sts128(to0, p0);
+      sts128(to1, p1);
+      expand<DT>(b0.x, p2.x, p2.y);
+      expand<DT>(b0.y, p2.z, p2.w);
+      expand<DT>(b1.x, p3.x, p3.y);
+      expand<DT>(b1.y, p3.z, p3.w);
+      sts128(to0 + step, p2);
+      sts128(to1 + step, p3);
+      from += 4096;
+      to0 += 2 * step;
+      to1 += 2 * step;
+    }
+    warp_arrive(&bars[RAW_FREE + item % L::RAWS], lane);
+    ++item;
+  };
+  // The open block, over what was converted there (by the same threads).  Keys behind its last token are masked in the scores,
+  // whatever they are; values there count as zero: a weight of 0 times anything else might be NaN.
+  auto open_keys = [&](uint32_t tile, size_t bh, int open) {
+    const uint16_t* const tail = static_cast<const uint16_t*>(c.k_tail) + bh * NKV_BLOCK * D;
+#pragma unroll 1
+    for (int i = 0; i < LOADS; ++i) {
+      const int at = ((i / 2) * 128 + tid) * 16 + (i % 2) * 8, row = at / D, col = at % D;
+      sts128(tile + (col / 64) * SUB + sw128_offset(open * NKV_BLOCK + row, col % 64), *reinterpret_cast<const uint4*>(tail + at));
+    }
+  };
+  auto open_values = [&](uint32_t tile, size_t bh, int open, int held) {
+    const uint16_t* const tail = static_cast<const uint16_t*>(c.v_tail) + bh * NKV_BLOCK * D;
+#pragma unroll 1
+    for (int i = 0; i < (2 - open) * LOADS; ++i) {     // the open block, and the one behind it where the tile has room
+      const int at = ((i % LOADS / 2) * 128 + tid) * 16 + (i % 2) * 8, row = at / NKV_BLOCK, col = at % NKV_BLOCK;
+      uint32_t w[4] = {0, 0, 0, 0};
+      if (i < LOADS && col < held) {
+        const uint4 v = *reinterpret_cast<const uint4*>(tail + at);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] &= col + 2 * e + 1 < held ? 0xFFFFFFFFu : col + 2 * e < held ? 0xFFFFu : 0u;
+      }
+      sts128(tile + (open + i / LOADS) * L::V_SUB + sw128_offset(row, col), make_uint4(w[0], w[1], w[2], w[3]));
+    }
+  };
   while (ok && walk.next(plan, a, seqs, c.kv_heads, p)) {
     const size_t bh = static_cast<size_t>(p.b) * c.kv_heads + p.h;
     const int length = seqs.length[p.b], full = length / NKV_BLOCK, held = length - full * NKV_BLOCK;
@@ -374,60 +433,27 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
     }
     fence_proxy_async();
     warp_arrive(&bars[Q_FULL], lane);
-    // ---- blocks: K, then V
+    // ---- tiles: K, then V
 #pragma unroll 1
-    for (int i = 0; i < (IMAGES ? 0 : 2 * p.n) && ok; ++i) {
-      const int value = i & 1, block_seq = seq + i / 2, stage = block_seq % STAGES, use = block_seq / STAGES;
-      const int item = 2 * seq + i, slot = item % L::RAWS;
-      ok = wait(&bars[RAW_FULL + slot], (item / L::RAWS) & 1, ctx, 971);
-      if (ok && use >= 1) ok = wait(&bars[(value ? V_FREE : K_FREE) + stage], (use - 1) & 1, ctx, 972);
+    for (int t = 0; t < (IMAGES ? 0 : 2 * p.nt) && ok; ++t) {
+      const int value = t & 1, stage = seq % STAGES, use = seq / STAGES;
+      ok = wait(&bars[RAW_FULL + item % L::RAWS], (item / L::RAWS) & 1, ctx, 971);
+      if (ok && use >= 1) ok = wait(&bars[(value ? V_FREE : K_FREE) + stage], (use - 1) & 1, ctx, 972 + value);
       if (!ok) break;
-      const uint32_t at = stage * L::OPERAND, swap = value ? 0 : k_swap, step = value ? 32 * 128 : 2048 / D * 128;
-      const uint32_t to0 = (value ? v0 : k0) + at, to1 = (value ? v1 : k1) + at, ring = base + L::RAW_OFF + slot * L::RAW + tid * 16;
-      // Rolled but for pairs, and one loop for both, on purpose: unrolled copies push the softmax warps' instructions out of the
-      // cache they share (a quarter of the issue slots went to fetching).
-#pragma unroll 1
-      for (int k = 0; k < LOADS; k += 2) {
-        const uint32_t from = ring + k * 2048, out0 = to0 + k * step, out1 = to1 + k * step;
-        const uint2 a0 = lds64(from + swap), a1 = lds64(from + (swap ^ 8)), b0 = lds64(from + 2048 + swap), b1 = lds64(from + 2048 + (swap ^ 8));
-        uint4 p0, p1;
-        expand<DT>(a0.x, p0.x, p0.y);
-        expand<DT>(a0.y, p0.z, p0.w);
-        expand<DT>(a1.x, p1.x, p1.y);
-        expand<DT>(a1.y, p1.z, p1.w);
-        sts128(out0, p0);
-        sts128(out1, p1);
-        expand<DT>(b0.x, p0.x, p0.y);
-        expand<DT>(b0.y, p0.z, p0.w);
-        expand<DT>(b1.x, p1.x, p1.y);
-        expand<DT>(b1.y, p1.z, p1.w);
-        sts128(out0 + step, p0);
-        sts128(out1 + step, p1);
-      }
-      warp_arrive(&bars[RAW_FREE + slot], lane);
-      // The open block, over what was converted there (by the same threads).  Keys behind its last token are masked in the scores,
-      // whatever they are; values there count as zero: a weight of 0 times anything else might be NaN.
-      if (p.block0 + i / 2 == full) {
-        const uint16_t* const tail = static_cast<const uint16_t*>(value ? c.v_tail : c.k_tail) + bh * NKV_BLOCK * D + tid * 16;
-#pragma unroll 1
-        for (int k = 0; k < 2 * LOADS; ++k) {
-          const uint32_t half = (k & 1) ? swap ^ 8 : swap;
-          const uint4 v = *reinterpret_cast<const uint4*>(tail + k / 2 * 2048 + half);
-          uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          const int left = value ? held - (v_col + static_cast<int>(half)) : 8;   // tokens of the piece
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] &= left > 2 * e + 1 ? 0xFFFFFFFFu : left > 2 * e ? 0xFFFFu : 0u;
-          sts128(((k & 1) ? to1 : to0) + k / 2 * step, make_uint4(w[0], w[1], w[2], w[3]));
-        }
+      const uint32_t at = stage * (value ? 2 * L::V_SUB : DCH * SUB);
+      convert((value ? v0 : kf) + at, (value ? v1 : ks) + at, value ? V_STEP : K_STEP, value ? 0 : swap);
+      const int open = full - 2 * (p.tile0 + t / 2);   // 0 or 1: that half of the tile is not a full block
+      if (open <= 1) {
+        if (value) open_values(v_to + at, bh, open, held); else open_keys(base + L::K_OFF + at, bh, open);
       }
       fence_proxy_async();
       warp_arrive(&bars[(value ? V_FULL : K_FULL) + stage], lane);
+      seq += value;
     }
-    seq += p.n;
   }
 }
 
-// ---- warp 12: MMA issue -------------------------------------------------------------------------------------------
+// ---- warp 12: MMA issue -----------------------------------------------------------------------------------------
 template <int DT, int D>
 __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t tmem, const Call& a, const Sequences& seqs,
                                          const Plan& plan, const Ctx& ctx, int kv_heads) {
@@ -438,76 +464,87 @@ __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t
   // operand descriptors of the first tile and stage; the others lie a whole number of 16-byte units on
   const uint64_t q_desc = make_smem_desc_sw128(base + L::Q_OFF), k_desc = make_smem_desc_sw128(base + L::K_OFF);
   const uint64_t v_desc = make_smem_desc_sw128(base + L::V_OFF);
-  auto issue_s = [&](int i, int place, int stage) {
-    const uint64_t qd = q_desc + static_cast<uint32_t>(i * (DCH * SUB / 16)), kd = k_desc + static_cast<uint32_t>(stage * (L::OPERAND / 16));
-    const uint32_t d = tmem + place * 64;
+  auto issue_s = [&](int i, int stage) {
+    const uint64_t qd = q_desc + static_cast<uint32_t>(i * (DCH * SUB / 16)), kd = k_desc + static_cast<uint32_t>(stage * (DCH * SUB / 16));
+    const uint32_t d = tmem + i * 128;
     if (leader) {
 #pragma unroll
       for (int ch = 0; ch < DCH; ++ch)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          mma_bf16(d, qd + ch * (SUB / 16) + 2 * k, kd + ch * (L::K_SUB / 16) + 2 * k, idesc<DT>(NKV_BLOCK), ch + k > 0);
-      mma_commit(&bars[S_FULL + place]);
+          mma_bf16(d, qd + ch * (SUB / 16) + 2 * k, kd + ch * (SUB / 16) + 2 * k, idesc<DT>(TOK), ch + k > 0);
+      mma_commit(&bars[S_FULL + i]);
     }
   };
-  // weights of a block times V of it: [128 rows x 64] [D x 64]^T, both with the tokens running along rows
-  auto issue_pv = [&](int i, int place, int stage, bool accumulate) {
-    const uint64_t vd = v_desc + static_cast<uint32_t>(stage * (L::OPERAND / 16));
-    const uint32_t d = tmem + 256 + i * 128, w = tmem + place * 64;
+  // weights of 64 tokens (a block) times V of it: [128 rows x 64] [D x 64]^T, both with the tokens running along rows
+  auto issue_pv = [&](int i, int stage, int half, bool accumulate) {
+    const uint64_t vd = v_desc + static_cast<uint32_t>((stage * 2 + half) * (L::V_SUB / 16));
+    const uint32_t d = tmem + 256 + i * 128, w = tmem + i * 128 + half * 32;
     if (leader) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) mma_bf16_ts(d, w + 8 * k, vd + 2 * k, idesc<DT>(D), accumulate || k > 0);
-      mma_commit(&bars[PV_DONE + i]);
+      if (half == 0) mma_commit(&bars[PV_HALF + i]);
     }
   };
   Walk walk(plan, a, seqs, blockIdx.x, kv_heads);
   Piece p;
   bool ok = true;
-  int seq = 0, pieces = 0, done0 = 0, done1 = 0, used0 = 0, used1 = 0;   // blocks and pieces of each query tile so far
+  int seq = 0, pieces = 0, done[NQ] = {0, 0}, used[NQ] = {0, 0};   // tiles and pieces of each query tile so far
   while (ok && walk.next(plan, a, seqs, kv_heads, p)) {
-    const int n0 = blocks_for(a, seqs, p, 0), n1 = blocks_for(a, seqs, p, 1);   // (one of them is p.n)
+    const int n[NQ] = {tiles_for(a, seqs, p, 0), tiles_for(a, seqs, p, 1)};
+    const int longest = max(n[0], n[1]);
     ok = wait(&bars[Q_FULL], pieces & 1, ctx, 980);
     ++pieces;
-    // PV of block n, then S of block n + 2 in the place that it leaves: the tensor core executes one thread's MMAs in order.
-    // Each K and V stage is waited for by the first query tile to use it and given back by the last.
+    // The first and the last query tile to use tile t: each K and V stage is waited for once and given back once.
+    auto first_of = [&](int t) { return t < n[0] ? 0 : 1; };
+    auto last_of = [&](int t) { return t < n[1] ? 1 : 0; };
 #pragma unroll 1
-    for (int n = -2; n < p.n && ok; ++n) {
-      const int now = (seq + n) % STAGES, next = (seq + n + 2) % STAGES;
+    for (int t = 0; t <= longest && ok; ++t) {
+      // PV of tile t - 1 and S of tile t, query tile by query tile
+      const int now = (seq + t - 1) % STAGES, next = (seq + t) % STAGES;
+      const uint32_t now_phase = ((seq + t - 1) / STAGES) & 1, next_phase = ((seq + t) / STAGES) & 1;
 #pragma unroll 1
       for (int i = 0; i < NQ; ++i) {
-        const int mine = i ? n1 : n0, other = i ? n0 : n1, ci = (i ? done1 : done0) + n;
-        const int place = 2 * i + (ci & 1);
-        if (n >= 0 && n < mine) {
-          if (i == 0 || n >= other) ok = wait(&bars[V_FULL + now], ((seq + n) / STAGES) & 1, ctx, 982);
-          if (n == 0) {   // the first PV of a piece overwrites O: the rows of the piece before must have been read
-            const int before = i ? used1 : used0;
-            if (ok && before > 0) ok = wait(&bars[O_FREE + i], (before - 1) & 1, ctx, 983);
+        const int tiles = i ? n[1] : n[0];
+        if (t > 0 && t - 1 < tiles) {
+          const uint32_t phase = ((i ? done[1] : done[0]) + t - 1) & 1;
+          if (i == first_of(t - 1)) ok = wait(&bars[V_FULL + now], now_phase, ctx, 982);
+          if (t == 1) {   // the first PV of a piece overwrites O: the rows of the piece before must have been read
+            const int pieces_before = i ? used[1] : used[0];
+            if (ok && pieces_before > 0) ok = wait(&bars[O_FREE + i], (pieces_before - 1) & 1, ctx, 983);
           }
-          ok = ok && wait(&bars[P_READY + place], (ci >> 1) & 1, ctx, 981);
+          ok = ok && wait(&bars[P_READY + 2 * i], phase, ctx, 981);
           if (!ok) break;
           tc_fence_after();
-          issue_pv(i, place, now, n > 0);
-          if (n == mine - 1 && leader) mma_commit(&bars[O_DONE + i]);
-          if ((i == 1 || n >= other) && leader) mma_commit(&bars[V_FREE + now]);
+          issue_pv(i, now, 0, t > 1);
+          ok = wait(&bars[P_READY + 2 * i + 1], phase, ctx, 984);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(i, now, 1, true);
+          if (t == tiles && leader) mma_commit(&bars[O_DONE + i]);
+          if (i == last_of(t - 1) && leader) mma_commit(&bars[V_FREE + now]);
         }
-        if (n + 2 < mine) {
-          if (i == 0 || n + 2 >= other) {
-            ok = wait(&bars[K_FULL + next], ((seq + n + 2) / STAGES) & 1, ctx, 985);
+        if (t < tiles) {
+          // S of the next tile overwrites P of this one, right behind the PV that reads it: the tensor core executes one
+          // thread's MMAs in order
+          if (i == first_of(t)) {
+            ok = wait(&bars[K_FULL + next], next_phase, ctx, 985);
             if (!ok) break;
             tc_fence_after();
           }
-          issue_s(i, place, next);
-          if ((i == 1 || n + 2 >= other) && leader) mma_commit(&bars[K_FREE + next]);
+          issue_s(i, next);
+          if (i == last_of(t) && leader) mma_commit(&bars[K_FREE + next]);
         }
       }
     }
     if (!ok) break;
     if (leader) mma_commit(&bars[Q_FREE]);
-    seq += p.n;
-    done0 += n0;
-    done1 += n1;
-    used0 += n0 > 0 ? 1 : 0;
-    used1 += n1 > 0 ? 1 : 0;
+    // tiles of the list that no query tile of the piece uses do not exist: the longest of the two is the piece's length
+    seq += p.nt;
+    for (int i = 0; i < NQ; ++i) {
+      done[i] += n[i];
+      used[i] += n[i] > 0 ? 1 : 0;
+    }
   }
   __syncwarp();
 }
@@ -526,28 +563,32 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
   Walk walk(plan, a, seqs, blockIdx.x, kv_heads);
   Piece p;
   bool ok = true, more = true;
-  int seq = 0, ci = 0, pieces = 0;   // blocks of the list, and blocks and pieces of this query tile
-  auto place_of = [&](const Piece& pc) { return 2 * static_cast<size_t>(blockIdx.x) + (pc.block0 == 0 ? 1 : 0); };
+  int seq = 0, ci = 0, pieces = 0;   // tiles of the list, and tiles and pieces of this query tile
+  auto place_of = [&](const Piece& pc) { return 2 * static_cast<size_t>(blockIdx.x) + (pc.tile0 == 0 ? 1 : 0); };
   while (ok && (more = walk.next(plan, a, seqs, kv_heads, p))) {
     const int r = p.unit * UNIT + wg * QT + row;
     const int length = seqs.length[p.b], count = seqs.count[p.b];
     const int seen = r < a.rows ? visible_to(a, length, count, r) : 0;
     const int seen_least = __reduce_min_sync(0xffffffffu, seen);
-    const int blocks = blocks_for(a, seqs, p, wg);
+    const int tiles = tiles_for(a, seqs, p, wg);
     const size_t bh = static_cast<size_t>(p.b) * kv_heads + p.h;
     const int token = r / a.group;
     const size_t at = (static_cast<size_t>(p.b) * a.tokens + token) * a.heads + p.h * a.group + r - token * a.group;
     float m = -INFINITY, l = 0.f;
-    for (int n = 0; n < blocks && ok; ++n, ++ci) {
-      const int place = 2 * wg + (ci & 1), first = (p.block0 + n) * NKV_BLOCK;
-      const uint32_t s_addr = tmem + lane_sel + place * 64;
-      ok = wait(&bars[S_FULL + place], (ci >> 1) & 1, ctx, 990);
-      if (!ok) break;
-      tc_fence_after();
+    // half a tile, a block of the cache, at a time
+#pragma unroll 1
+    for (int n = 0; n < 2 * tiles && ok; ++n) {
+      const int half = n & 1, block = 2 * p.tile0 + n, first = block * NKV_BLOCK;
+      const uint32_t s_addr = tmem + lane_sel + wg * 128 + half * 64, p_addr = tmem + lane_sel + wg * 128 + half * 32;
+      if (half == 0) {
+        ok = wait(&bars[S_FULL + wg], ci & 1, ctx, 990);
+        if (!ok) break;
+        tc_fence_after();
+      }
       uint32_t raw[2][32];
       tmem_ld32_issue(s_addr, raw[0]);
       tmem_ld32_issue(s_addr + 32, raw[1]);
-      const float4 sc = scales[(seq + n) % NMETA];   // (written ahead of the request for the codes that this S came from)
+      const float4 sc = scales[(2 * seq + n) % (2 * NMETA)];   // (written ahead of the request for the codes that this S came from)
       tmem_ld32_wait(raw[0]);
       tmem_ld32_wait(raw[1]);
       float f = scale * sc.x;
@@ -562,13 +603,15 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       }
       const float m_new = fmaxf(m, fmaf(fmaxf(max32(raw[0]), max32(raw[1])), f, sc.y));
       if (__any_sync(0xffffffffu, m_new > m + RESCALE_THRESHOLD || (m == -INFINITY && m_new > m))) {
-        // Move the reference: O and the sum are scaled by 2^(old - new).  PV of the block before the last was complete ahead of
-        // this S; that of the last one may still run.
+        // Move the reference: O and the sum are scaled by 2^(old - new).  S was issued behind PV of the tile before and its commit
+        // covers both; PV of this tile's first half may still run.
         const float alpha = m_new == -INFINITY ? 1.f : exp2f(m - m_new);
         if (n > 0) {
-          ok = wait(&bars[PV_DONE + wg], (ci - 1) & 1, ctx, 991);
-          if (!ok) break;
-          tc_fence_after();
+          if (half) {
+            ok = wait(&bars[PV_HALF + wg], ci & 1, ctx, 991);
+            if (!ok) break;
+            tc_fence_after();
+          }
 #pragma unroll 1
           for (int cc = 0; cc < D / 16; ++cc) {
             uint32_t v[16];
@@ -583,7 +626,7 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
         m = m_new;
       }
       // One pass over the scores: eight at a time, exponentials of group b, arguments of b + 1, sums and packing of b - 1.  P'
-      // (16-bit pairs) replaces S in place.
+      // (16-bit pairs) replaces S, the first half's of the first columns.
       const float ref = m == -INFINITY ? 0.f : m, off = sc.y - ref + RAISE;
       const uint64_t scale2 = pair_f32(f, f), off2 = pair_f32(off, off);
       uint64_t sum2[2] = {0ull, 0ull};
@@ -611,7 +654,7 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
           sum2[i & 1] = add_f32x2(sum2[i & 1], pair_f32(lo, hi));
           packed[(b & 3) * 4 + i] = DT == NKV_BF16 ? __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632) : pack2<NKV_F16>(lo, hi);
         }
-        if ((b & 3) == 3) tmem_st16(s_addr + (b >> 2) * 16, packed);
+        if ((b & 3) == 3) tmem_st16(p_addr + (b >> 2) * 16, packed);
       };
       args(0);
 #pragma unroll
@@ -623,17 +666,18 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       finish(7);
       tmem_wait_st();
       tc_fence_before();
-      warp_arrive(&bars[P_READY + place], lane);
+      warp_arrive(&bars[P_READY + 2 * wg + half], lane);
       float lo, hi;
       split_f32(add_f32x2(sum2[0], sum2[1]), lo, hi);
       const float sum = (lo + hi) * LOWER;
       l = fmaf(sum, sc.z, l);
-      if (a.partial && r < a.rows) a.partial[(bh * a.most_blocks + p.block0 + n) * a.rows + r] = log2f(sum) + (ref - sc.y);
+      if (a.partial && r < a.rows && block < a.most_blocks) a.partial[(bh * a.most_blocks + block) * a.rows + r] = log2f(sum) + (ref - sc.y);
+      ci += half;
     }
-    seq += p.n;
+    seq += p.nt;
     if (!ok) break;
     // ---- the rows: results, or a part of them
-    if (blocks > 0) {
+    if (tiles > 0) {
       ok = wait(&bars[O_DONE + wg], pieces & 1, ctx, 992);
       ++pieces;
       if (!ok) break;
@@ -644,7 +688,7 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
 #pragma unroll 1
     for (int cc = 0; cc < D / 32; ++cc) {
       uint32_t v[32];
-      if (blocks > 0) {
+      if (tiles > 0) {
         tmem_ld32_issue(o_addr + cc * 32, v);
         tmem_ld32_wait(v);
       } else {
@@ -672,7 +716,7 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       if (p.whole) a.lse[at] = seen > 0 ? (m + log2f(l)) * LN2 : -INFINITY;
       else parts.ml[place_of(p) * UNIT + wg * QT + row] = make_float2(m, l);
     }
-    if (blocks > 0) {
+    if (tiles > 0) {
       tc_fence_before();
       warp_arrive(&bars[O_FREE + wg], lane);
     }
@@ -703,20 +747,20 @@ tile_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
   if (threadIdx.x == 0) {
     mbar_init(&bars[Q_FULL], OPERAND_WARPS);
     mbar_init(&bars[Q_FREE], 1);
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i) {
       mbar_init(&bars[K_FULL + i], IMAGES ? 1 : OPERAND_WARPS);
       mbar_init(&bars[K_FREE + i], 1);
       mbar_init(&bars[V_FULL + i], IMAGES ? 1 : OPERAND_WARPS);
       mbar_init(&bars[V_FREE + i], 1);
       mbar_init(&bars[S_FULL + i], 1);
+      mbar_init(&bars[PV_HALF + i], 1);
+      mbar_init(&bars[O_DONE + i], 1);
+      mbar_init(&bars[O_FREE + i], QT / 32);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&bars[P_READY + i], QT / 32);
       mbar_init(&bars[RAW_FULL + i], 1);
       mbar_init(&bars[RAW_FREE + i], OPERAND_WARPS);
-    }
-    for (int i = 0; i < NQ; ++i) {
-      mbar_init(&bars[PV_DONE + i], 1);
-      mbar_init(&bars[O_DONE + i], 1);
-      mbar_init(&bars[O_FREE + i], QT / 32);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -732,51 +776,58 @@ tile_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp < SOFTMAX_WARPS) softmax_role<DT, D>(smem, bars, tmem, a, seqs, plan, parts, ctx, c.kv_heads);
   else if (warp < SOFTMAX_WARPS + OPERAND_WARPS) operand_role<DT, D, IMAGES>(smem, bars, c, a, seqs, plan, ctx, q_vector);
-  else if (warp == MMA_WARP) mma_role<DT, D>(smem, bars, tmem, a, seqs, plan, ctx, c.kv_heads);
-  else codes_role<D, IMAGES>(smem, bars, c, a, seqs, plan, ctx, images);
+  else if (warp > MMA_WARP) codes_role<D, IMAGES>(smem, bars, c, a, seqs, plan, ctx, images);
+  else mma_role<DT, D>(smem, bars, tmem, a, seqs, plan, ctx, c.kv_heads);
   tc_fence_before();
   __syncthreads();
   if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
   if (threadIdx.x == 0 && *abort_flag) atomicCAS(status, 0, *abort_flag);
 }
 
-// Blocks of all heads as operand images: [head][block][K, V], laid out as the tensor cores read them from shared memory.  A
-// thread block per cache block and tensor; a thread stores eight elements of an operand row at a time.  Bound: memory, three
+// Tiles of all heads as operand images: [head][tile][K, V] of DCH * SUB bytes, laid out as the tensor cores read them from shared
+// memory.  A thread block per tile and tensor; a thread stores eight elements of an operand row at a time.  Bound: memory, three
 // bytes a code.
 template <int DT, int D>
 __global__ void __launch_bounds__(256)
-expand_kernel(BlockArrays c, const __grid_constant__ Sequences seqs, int most_blocks, uint8_t* images) {
+expand_kernel(BlockArrays c, const __grid_constant__ Sequences seqs, int most_tiles, uint8_t* images) {
   using L = Layout<D>;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int block = blockIdx.x >> 1, tensor = blockIdx.x & 1, h = blockIdx.y, b = blockIdx.z;
+  const int tile = blockIdx.x >> 1, tensor = blockIdx.x & 1, h = blockIdx.y, b = blockIdx.z;
   const int length = seqs.length[b], full = length / NKV_BLOCK, held = length - full * NKV_BLOCK;
-  if (block * NKV_BLOCK >= length) return;
+  if (tile * TOK >= length) return;
   const size_t bh = static_cast<size_t>(b) * c.kv_heads + h;
-  uint8_t* const to = images + ((bh * most_blocks + block) * 2 + tensor) * static_cast<size_t>(L::OPERAND);
-  asm volatile("griddepcontrol.wait;" ::: "memory");   // the launches before may still write the cache and read these images
-  const uint8_t* codes = nullptr;
-  if (block < full) codes = (tensor ? c.v_codes : c.k_codes) + slot_of(c, bh, block) * (NKV_BLOCK * D);
-  const uint16_t* const tail = static_cast<const uint16_t*>(tensor ? c.v_tail : c.k_tail) + bh * NKV_BLOCK * D;
+  constexpr uint32_t BYTES = L::DCH * SUB;
+  uint8_t* const to = images + ((bh * most_tiles + tile) * 2 + tensor) * static_cast<size_t>(BYTES);
+  // the launch before may still read these images
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    const int at = (i * 256 + threadIdx.x) * 8;       // element of the block: [64][D] of K, [D][64] of V
-    const int row = tensor ? at / NKV_BLOCK : at / D, col = tensor ? at % NKV_BLOCK : at % D;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (codes != nullptr) {
-      const uint2 raw = __ldg(reinterpret_cast<const uint2*>(codes + at));
-      expand<DT>(raw.x, v.x, v.y);
-      expand<DT>(raw.y, v.z, v.w);
-    } else {   // values behind the last token count as zero: a weight of 0 times anything else might be NaN
-      const int left = tensor ? held - col : row < held ? 8 : 0;
-      if (left > 0) {
-        v = *reinterpret_cast<const uint4*>(tail + at);
-        uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  for (int j = 0; j < 2; ++j) {
+    const int block = 2 * tile + j;
+    const uint8_t* codes = nullptr;
+    if (block < full) codes = (tensor ? c.v_codes : c.k_codes) + slot_of(c, bh, block) * (NKV_BLOCK * D);
+    const uint16_t* const tail = static_cast<const uint16_t*>(tensor ? c.v_tail : c.k_tail) + bh * NKV_BLOCK * D;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] &= left > 2 * e + 1 ? 0xFFFFFFFFu : left > 2 * e ? 0xFFFFu : 0u;
-        v = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int i = 0; i < D / 32; ++i) {
+      const int at = (i * 256 + threadIdx.x) * 8;       // element of the block: [64][D] of K, [D][64] of V
+      const int row = tensor ? at / NKV_BLOCK : at / D, col = tensor ? at % NKV_BLOCK : at % D;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (codes != nullptr) {
+        const uint2 raw = __ldg(reinterpret_cast<const uint2*>(codes + at));
+        expand<DT>(raw.x, v.x, v.y);
+        expand<DT>(raw.y, v.z, v.w);
+      } else if (block == full) {   // values behind the last token count as zero: a weight of 0 times anything else might be NaN
+        const int left = tensor ? held - col : row < held ? 8 : 0;
+        if (left > 0) {
+          v = *reinterpret_cast<const uint4*>(tail + at);
+          uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] &= left > 2 * e + 1 ? 0xFFFFFFFFu : left > 2 * e ? 0xFFFFu : 0u;
+          v = make_uint4(w[0], w[1], w[2], w[3]);
+        }
       }
+      const uint32_t place = tensor ? j * L::V_SUB + sw128_offset(row, col) : (col / 64) * SUB + sw128_offset(j * NKV_BLOCK + row, col % 64);
+      *reinterpret_cast<uint4*>(to + place) = v;
     }
-    *reinterpret_cast<uint4*>(to + (tensor ? 0 : (col / 64) * L::K_SUB) + sw128_offset(row, col % 64)) = v;
   }
 }
 
@@ -789,19 +840,19 @@ join_units_kernel(Call a, const __grid_constant__ Sequences seqs, const __grid_c
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int unit = blockIdx.x / slices, slice = blockIdx.x % slices, h = blockIdx.y, b = blockIdx.z;
   const int length = seqs.length[b], count = seqs.count[b];
-  auto blocks_of = [&](int u) { return blocks_seen(length, count, a.group, a.rows, a.causal, u * UNIT, UNIT); };
-  const int blocks = blocks_of(unit);
+  auto tiles_of = [&](int u) { return tiles_seen(length, count, a.group, a.rows, a.causal, u * UNIT, UNIT); };
+  const int nt = tiles_of(unit);
   uint32_t r0 = 0, r1 = 0, begin = 0;
-  if (blocks > 0) {
+  if (nt > 0) {
     if (threadIdx.x == 0) before = 0;
     __syncthreads();
     uint32_t mine = 0;
-    for (int u = threadIdx.x; u < unit; u += 256) mine += blocks_of(u);
+    for (int u = threadIdx.x; u < unit; u += 256) mine += tiles_of(u);
     if (mine) atomicAdd(&before, mine);
     __syncthreads();
     begin = plan.start[b] + h * ((plan.start[b + 1] - plan.start[b]) / kv_heads) + before;
     r0 = plan.run_of(begin);
-    r1 = plan.run_of(begin + blocks - 1);
+    r1 = plan.run_of(begin + nt - 1);
     if (r0 == r1) return;   // one run had all of it and wrote the results
   }
   constexpr int PER_ROW = D / 8, ROWS = 256 / PER_ROW;
@@ -811,7 +862,7 @@ join_units_kernel(Call a, const __grid_constant__ Sequences seqs, const __grid_c
     if (r >= a.rows) break;
     const int token = r / a.group;
     const size_t at = (static_cast<size_t>(b) * a.tokens + token) * a.heads + h * a.group + r - token * a.group;
-    const bool any = blocks > 0 && visible_to(a, length, count, r) > 0;
+    const bool any = nt > 0 && visible_to(a, length, count, r) > 0;
     float top = -INFINITY, sum = 0.f, acc[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.f;
@@ -843,14 +894,14 @@ Plan plan_of(const Sequences& seqs, int n, int kv_heads, int group, int rows, bo
   Plan p;
   p.sequences = n;
   p.units = ceil_div(rows, UNIT);
-  p.most_blocks = 0;
+  p.most_tiles = 0;
   uint64_t total = 0;
   for (int i = 0; i < n; ++i) {
     p.start[i] = static_cast<uint32_t>(total);
-    p.most_blocks = max(p.most_blocks, ceil_div(seqs.length[i], NKV_BLOCK));
-    uint64_t blocks = 0;
-    for (int u = 0; u < p.units; ++u) blocks += blocks_seen(seqs.length[i], seqs.count[i], group, rows, causal, u * UNIT, UNIT);
-    total += blocks * kv_heads;
+    p.most_tiles = max(p.most_tiles, ceil_div(seqs.length[i], TOK));
+    uint64_t tiles = 0;
+    for (int u = 0; u < p.units; ++u) tiles += tiles_seen(seqs.length[i], seqs.count[i], group, rows, causal, u * UNIT, UNIT);
+    total += tiles * kv_heads;
   }
   p.start[n] = static_cast<uint32_t>(total);
   p.runs = static_cast<int>(min(total, static_cast<uint64_t>(sm_count())));
@@ -865,7 +916,7 @@ Plan plan_of(const Sequences& seqs, int n, int kv_heads, int group, int rows, bo
 constexpr int UNITS_FOR_IMAGES = 4;
 constexpr size_t IMAGE_BYTES = static_cast<size_t>(64) << 20;   // scratch for images, one head at least
 
-size_t head_image_bytes(int most_blocks, int d) { return static_cast<size_t>(most_blocks) * 2 * NKV_BLOCK * d * 2; }
+size_t head_image_bytes(int most_blocks, int d) { return static_cast<size_t>((most_blocks + 1) / 2) * 2 * TOK * d * 2; }
 size_t part_bytes(int runs, int d) { return static_cast<size_t>(runs) * 2 * UNIT * (d + 2) * sizeof(float); }
 
 // one launch: sequences and heads as they are given
@@ -886,12 +937,12 @@ int launch(const BlockArrays& c, const Call& a, const Sequences& seqs, int n, in
   config.attrs = &attribute;
   if (plan.runs > 0) {
     if (images) {
-      config.gridDim = dim3(2 * plan.most_blocks, c.kv_heads, n);
+      config.gridDim = dim3(2 * plan.most_tiles, c.kv_heads, n);
       config.blockDim = dim3(256);
       config.numAttrs = 1;
       auto expand = wide ? (bf16 ? expand_kernel<NKV_BF16, 128> : expand_kernel<NKV_F16, 128>)
                          : (bf16 ? expand_kernel<NKV_BF16, 64> : expand_kernel<NKV_F16, 64>);
-      NKV_CUDA(cudaLaunchKernelEx(&config, expand, c, seqs, plan.most_blocks, image));
+      NKV_CUDA(cudaLaunchKernelEx(&config, expand, c, seqs, plan.most_tiles, image));
     }
     auto run = [&](auto kernel, int smem) {
       NKV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
