@@ -90,29 +90,43 @@ attend_plain_kernel(BlockArrays c, Call a, Sequences seqs) {
   if (lane == 0) a.lse[at] = seen > 0 ? (m + log2f(l)) * LN2 : -INFINITY;
 }
 
-// weights[block] += sum over rows of 2^(partial - lse): a thread block per (block, kv head, sequence), rows in a fixed order
+// weights[block] += sum over rows of 2^(partial - lse), rows in a fixed order: a thread block per WEIGHT_BLOCKS blocks of a kv
+// head, so that a row's lse, scattered over the query heads, is fetched once for all of them.  Bound: memory, four bytes a row and
+// block.
+constexpr int WEIGHT_BLOCKS = 4;
 __global__ void __launch_bounds__(256)
 block_weights_kernel(BlockArrays c, Call a, Sequences seqs) {
-  __shared__ float sums[8];
-  const int block = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  __shared__ float sums[WEIGHT_BLOCKS][8];
+  const int block0 = blockIdx.x * WEIGHT_BLOCKS, h = blockIdx.y, b = blockIdx.z;
   const int length = seqs.length[b], count = seqs.count[b];
-  if (block * NKV_BLOCK >= length) return;
+  const int blocks = min(WEIGHT_BLOCKS, (length + NKV_BLOCK - 1) / NKV_BLOCK - block0);
+  if (blocks <= 0 || count <= 0) return;
   const size_t bh = static_cast<size_t>(b) * c.kv_heads + h;
-  const float* partial = a.partial + (bh * a.most_blocks + block) * a.rows;
-  float sum = 0.f;
-  for (int r = threadIdx.x; r < a.rows; r += 256) {
-    if (visible_to(a, length, count, r) <= block * NKV_BLOCK) continue;
-    const float lse = a.lse[(static_cast<size_t>(b) * a.tokens + r / a.group) * a.heads + h * a.group + r % a.group];
-    sum += exp2f(partial[r] - lse * LOG2E);
+  const float* const partial = a.partial + (bh * a.most_blocks + block0) * a.rows;
+  const float* const lse = a.lse + static_cast<size_t>(b) * a.tokens * a.heads + h * a.group;
+  // the first token that sees anything of these blocks
+  const int first = a.causal ? max(0, block0 * NKV_BLOCK - (length - count)) : 0;
+  float sum[WEIGHT_BLOCKS] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (int r = first * a.group + threadIdx.x; r < count * a.group; r += 256) {
+    const int token = r / a.group;
+    const float ref = lse[static_cast<size_t>(token) * a.heads + r - token * a.group] * LOG2E;
+    const int seen = visible_to(a, length, count, r) - block0 * NKV_BLOCK;
+#pragma unroll
+    for (int k = 0; k < WEIGHT_BLOCKS; ++k)
+      if (k < blocks && seen > k * NKV_BLOCK) sum[k] += exp2f(partial[static_cast<size_t>(k) * a.rows + r] - ref);
   }
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-  if ((threadIdx.x & 31) == 0) sums[threadIdx.x / 32] = sum;
+  for (int k = 0; k < WEIGHT_BLOCKS; ++k) {
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], x);
+    if ((threadIdx.x & 31) == 0) sums[k][threadIdx.x / 32] = sum[k];
+  }
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (threadIdx.x < blocks) {
     float total = 0.f;
-    for (int w = 0; w < 8; ++w) total += sums[w];
-    a.weights[bh * c.blocks + block] += total;
+    for (int w = 0; w < 8; ++w) total += sums[threadIdx.x][w];
+    a.weights[bh * c.blocks + block0 + threadIdx.x] += total;
   }
 }
 
@@ -198,7 +212,7 @@ int block_attend(const nkv_block_cache& c, const nkv_tokens& q, int tokens, cons
       NKV_LAUNCH_CHECK("attend_plain_kernel");
     }
     if (weights && a.most_blocks > 0) {
-      block_weights_kernel<<<dim3(a.most_blocks, c.kv_heads, n), 256, 0, stream>>>(arrays, a, seqs);
+      block_weights_kernel<<<dim3(ceil_div(a.most_blocks, WEIGHT_BLOCKS), c.kv_heads, n), 256, 0, stream>>>(arrays, a, seqs);
       NKV_LAUNCH_CHECK("block_weights_kernel");
     }
   }

@@ -219,6 +219,19 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
                : "memory");
 }
 
+// 32 bytes of a result row, in one store where they start on as many: a warp's rows lie apart, and what its stores cost is the
+// lines that each of them touches
+__device__ __forceinline__ void store32(void* to, const uint32_t (&v)[8], bool wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                 "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+  } else {
+    static_cast<uint4*>(to)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+    static_cast<uint4*>(to)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+  }
+}
+
 // 16 bytes of a row that may start anywhere
 __device__ __forceinline__ uint4 gather16(const uint16_t* src) {
   uint32_t w[4];
@@ -317,7 +330,7 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
   const int tid = threadIdx.x - 32 * SOFTMAX_WARPS, lane = tid & 31;
   const uint32_t base = smem_u32(smem);
   // queries: a thread has one 16-byte column of every ROWS-th row of the unit
-  constexpr int PER_ROW = D / 8, ROWS = 32 * OPERAND_WARPS / PER_ROW, AHEAD = 8;
+  constexpr int PER_ROW = D / 8, ROWS = 32 * OPERAND_WARPS / PER_ROW, AHEAD = 16;
   const int q_row = tid / PER_ROW, q_col = tid % PER_ROW * 8;
   const uint32_t q_to = base + L::Q_OFF + (q_col / 64) * SUB;
   const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;   // a negative scale is the queries' sign
@@ -393,42 +406,40 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
   while (ok && walk.next(plan, a, seqs, c.kv_heads, p)) {
     const size_t bh = static_cast<size_t>(p.b) * c.kv_heads + p.h;
     const int length = seqs.length[p.b], full = length / NKV_BLOCK, held = length - full * NKV_BLOCK;
-    // ---- queries
-    if (pieces > 0) ok = wait(&bars[Q_FREE], (pieces - 1) & 1, ctx, 970);
-    if (!ok) break;
-    ++pieces;
-    {
-      const uint16_t* const q_head = a.q + p.b * a.q_batch + static_cast<long long>(p.h) * a.group * a.q_head + q_col;
-      int r = p.unit * UNIT + q_row, token = r / a.group, head = r - token * a.group;
-      const int token_step = ROWS / a.group, head_step = ROWS - token_step * a.group;
-      auto next_row = [&]() {
+    // ---- queries: the first rows are on their way while the piece before still reads its own
+    const uint16_t* const q_head = a.q + p.b * a.q_batch + static_cast<long long>(p.h) * a.group * a.q_head + q_col;
+    int r = p.unit * UNIT + q_row, token = r / a.group, head = r - token * a.group;
+    const int token_step = ROWS / a.group, head_step = ROWS - token_step * a.group;
+#pragma unroll 1
+    for (int row0 = q_row; row0 < UNIT && ok; row0 += AHEAD * ROWS) {
+      uint4 v[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const uint16_t* const src = q_head + token * a.q_token + head * a.q_head;
+        v[k] = make_uint4(0, 0, 0, 0);
+        if (q_vector && r < a.rows) v[k] = __ldg(reinterpret_cast<const uint4*>(src));
         r += ROWS;
         token += token_step;
         head += head_step;
         if (head >= a.group) { head -= a.group; ++token; }
-      };
-      auto put = [&](int row, const uint4& v) {
+      }
+      if (row0 == q_row && pieces > 0) ok = wait(&bars[Q_FREE], (pieces - 1) & 1, ctx, 970);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int row = row0 + k * ROWS;
+        sts128(q_to + (row / QT) * DCH * SUB + sw128_offset(row % QT, q_col % 64),
+               make_uint4(v[k].x ^ flip, v[k].y ^ flip, v[k].z ^ flip, v[k].w ^ flip));
+      }
+    }
+    if (!ok) break;
+    ++pieces;
+    if (!q_vector) {   // rows that start anywhere
+#pragma unroll 1
+      for (int row = q_row; row < UNIT; row += ROWS) {
+        const int at = p.unit * UNIT + row, t = at / a.group;
+        if (at >= a.rows) break;
+        const uint4 v = gather16(q_head + t * a.q_token + (at - t * a.group) * a.q_head);
         sts128(q_to + (row / QT) * DCH * SUB + sw128_offset(row % QT, q_col % 64), make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip));
-      };
-      if (q_vector) {
-#pragma unroll 1
-        for (int row0 = q_row; row0 < UNIT; row0 += AHEAD * ROWS) {
-          uint4 v[AHEAD];
-#pragma unroll
-          for (int k = 0; k < AHEAD; ++k) {
-            v[k] = make_uint4(0, 0, 0, 0);
-            if (r < a.rows) v[k] = __ldg(reinterpret_cast<const uint4*>(q_head + token * a.q_token + head * a.q_head));
-            next_row();
-          }
-#pragma unroll
-          for (int k = 0; k < AHEAD; ++k) put(row0 + k * ROWS, v[k]);
-        }
-      } else {
-#pragma unroll 1
-        for (int row = q_row; row < UNIT; row += ROWS) {
-          put(row, r < a.rows ? gather16(q_head + token * a.q_token + head * a.q_head) : make_uint4(0, 0, 0, 0));
-          next_row();
-        }
       }
     }
     fence_proxy_async();
@@ -467,24 +478,21 @@ __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t
   auto issue_s = [&](int i, int stage) {
     const uint64_t qd = q_desc + static_cast<uint32_t>(i * (DCH * SUB / 16)), kd = k_desc + static_cast<uint32_t>(stage * (DCH * SUB / 16));
     const uint32_t d = tmem + i * 128;
-    if (leader) {
 #pragma unroll
-      for (int ch = 0; ch < DCH; ++ch)
+    for (int ch = 0; ch < DCH; ++ch)
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          mma_bf16(d, qd + ch * (SUB / 16) + 2 * k, kd + ch * (SUB / 16) + 2 * k, idesc<DT>(TOK), ch + k > 0);
-      mma_commit(&bars[S_FULL + i]);
-    }
+      for (int k = 0; k < 4; ++k)
+        if (leader) mma_bf16(d, qd + ch * (SUB / 16) + 2 * k, kd + ch * (SUB / 16) + 2 * k, idesc<DT>(TOK), ch + k > 0);
+    if (leader) mma_commit(&bars[S_FULL + i]);
   };
   // weights of 64 tokens (a block) times V of it: [128 rows x 64] [D x 64]^T, both with the tokens running along rows
   auto issue_pv = [&](int i, int stage, int half, bool accumulate) {
     const uint64_t vd = v_desc + static_cast<uint32_t>((stage * 2 + half) * (L::V_SUB / 16));
     const uint32_t d = tmem + 256 + i * 128, w = tmem + i * 128 + half * 32;
-    if (leader) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) mma_bf16_ts(d, w + 8 * k, vd + 2 * k, idesc<DT>(D), accumulate || k > 0);
-      if (half == 0) mma_commit(&bars[PV_HALF + i]);
-    }
+    for (int k = 0; k < 4; ++k)
+      if (leader) mma_bf16_ts(d, w + 8 * k, vd + 2 * k, idesc<DT>(D), accumulate || k > 0);
+    if (half == 0 && leader) mma_commit(&bars[PV_HALF + i]);
   };
   Walk walk(plan, a, seqs, blockIdx.x, kv_heads);
   Piece p;
@@ -503,7 +511,7 @@ __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t
       // PV of tile t - 1 and S of tile t, query tile by query tile
       const int now = (seq + t - 1) % STAGES, next = (seq + t) % STAGES;
       const uint32_t now_phase = ((seq + t - 1) / STAGES) & 1, next_phase = ((seq + t) / STAGES) & 1;
-#pragma unroll 1
+#pragma unroll
       for (int i = 0; i < NQ; ++i) {
         const int tiles = i ? n[1] : n[0];
         if (t > 0 && t - 1 < tiles) {
@@ -684,6 +692,7 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       tc_fence_after();
     }
     const float inv = seen > 0 ? 1.f / l : 0.f;
+    const bool wide_out = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0, wide_part = (reinterpret_cast<uintptr_t>(parts.o) & 31) == 0;
     float* const part = parts.o + (place_of(p) * UNIT + wg * QT + row) * D;
 #pragma unroll 1
     for (int cc = 0; cc < D / 32; ++cc) {
@@ -698,18 +707,21 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       if (r >= a.rows) continue;
       if (p.whole) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-          uint32_t o[4];
+        for (int j = 0; j < 32; j += 16) {
+          uint32_t o[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
+          for (int e = 0; e < 8; ++e) {
             const float lo = __uint_as_float(v[j + 2 * e]), hi = __uint_as_float(v[j + 2 * e + 1]);
             o[e] = seen > 0 ? pack2<DT>(lo * inv, hi * inv) : 0u;
           }
-          *reinterpret_cast<uint4*>(a.out + at * D + cc * 32 + j) = make_uint4(o[0], o[1], o[2], o[3]);
+          store32(a.out + at * D + cc * 32 + j, o, wide_out);
         }
       } else {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) *reinterpret_cast<uint4*>(part + cc * 32 + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+        for (int j = 0; j < 32; j += 8) {
+          const uint32_t o[8] = {v[j], v[j + 1], v[j + 2], v[j + 3], v[j + 4], v[j + 5], v[j + 6], v[j + 7]};
+          store32(part + cc * 32 + j, o, wide_part);
+        }
       }
     }
     if (r < a.rows) {
