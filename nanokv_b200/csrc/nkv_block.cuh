@@ -83,6 +83,7 @@ struct Call {
   float* weights;      // block weights to add to
   int tokens, heads, group, rows, causal, most_blocks;
   float scale_log2;    // scale * log2(e)
+  int q_vector;        // the queries' rows start on 16 bytes
 };
 
 // tokens that row r of a sequence sees
@@ -93,7 +94,7 @@ __device__ __forceinline__ int visible_to(const Call& a, int length, int count, 
 }
 
 // few rows per kv head (nkv_block_step.cu)
-bool block_step_supported(int rows);
+bool block_step_supported(int rows, int d);
 size_t block_step_bytes(const Sequences& seqs, int n, int kv_heads, int rows, int d);
 int block_step(const BlockArrays& c, const Call& a, const Sequences& seqs, int n, int dtype, int d, void* workspace, int32_t* status,
                cudaStream_t stream);

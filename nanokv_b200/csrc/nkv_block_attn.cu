@@ -93,10 +93,10 @@ attend_plain_kernel(BlockArrays c, Call a, Sequences seqs) {
 // weights[block] += sum over rows of 2^(partial - lse), rows in a fixed order: a thread block per WEIGHT_BLOCKS blocks of a kv
 // head, so that a row's lse, scattered over the query heads, is fetched once for all of them.  Bound: memory, four bytes a row and
 // block.
-constexpr int WEIGHT_BLOCKS = 4;
-__global__ void __launch_bounds__(256)
+constexpr int WEIGHT_BLOCKS = 2, WEIGHT_THREADS = 512;
+__global__ void __launch_bounds__(WEIGHT_THREADS)
 block_weights_kernel(BlockArrays c, Call a, Sequences seqs) {
-  __shared__ float sums[WEIGHT_BLOCKS][8];
+  __shared__ float sums[WEIGHT_BLOCKS][WEIGHT_THREADS / 32];
   const int block0 = blockIdx.x * WEIGHT_BLOCKS, h = blockIdx.y, b = blockIdx.z;
   const int length = seqs.length[b], count = seqs.count[b];
   const int blocks = min(WEIGHT_BLOCKS, (length + NKV_BLOCK - 1) / NKV_BLOCK - block0);
@@ -106,9 +106,9 @@ block_weights_kernel(BlockArrays c, Call a, Sequences seqs) {
   const float* const lse = a.lse + static_cast<size_t>(b) * a.tokens * a.heads + h * a.group;
   // the first token that sees anything of these blocks
   const int first = a.causal ? max(0, block0 * NKV_BLOCK - (length - count)) : 0;
-  float sum[WEIGHT_BLOCKS] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-  for (int r = first * a.group + threadIdx.x; r < count * a.group; r += 256) {
+  float sum[WEIGHT_BLOCKS] = {};
+#pragma unroll 4
+  for (int r = first * a.group + threadIdx.x; r < count * a.group; r += WEIGHT_THREADS) {
     const int token = r / a.group;
     const float ref = lse[static_cast<size_t>(token) * a.heads + r - token * a.group] * LOG2E;
     const int seen = visible_to(a, length, count, r) - block0 * NKV_BLOCK;
@@ -125,7 +125,7 @@ block_weights_kernel(BlockArrays c, Call a, Sequences seqs) {
   __syncthreads();
   if (threadIdx.x < blocks) {
     float total = 0.f;
-    for (int w = 0; w < 8; ++w) total += sums[threadIdx.x][w];
+    for (int w = 0; w < WEIGHT_THREADS / 32; ++w) total += sums[threadIdx.x][w];
     a.weights[bh * c.blocks + block0 + threadIdx.x] += total;
   }
 }
@@ -152,7 +152,7 @@ Scratch scratch_of(const nkv_block_cache& c, const Sequences& seqs, int n, int g
   Scratch s{0, 0};
   if (with_weights) s.partial = (static_cast<size_t>(n) * c.kv_heads * most_blocks * rows * 4 + 255) & ~static_cast<size_t>(255);
   if (!simt_forced())
-    s.own = block_step_supported(rows) ? block_step_bytes(seqs, n, c.kv_heads, rows, c.head_dim)
+    s.own = block_step_supported(rows, c.head_dim) ? block_step_bytes(seqs, n, c.kv_heads, rows, c.head_dim)
                                        : block_tile_bytes(seqs, n, c.kv_heads, most_blocks, rows, c.head_dim);
   return s;
 }
@@ -191,9 +191,10 @@ int block_attend(const nkv_block_cache& c, const nkv_tokens& q, int tokens, cons
     a.causal = causal;
     a.most_blocks = most_blocks_of(c);
     a.scale_log2 = scale * LOG2E;
+    a.q_vector = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_batch % 8 == 0 && a.q_token % 8 == 0 && a.q_head % 8 == 0;
     const BlockArrays arrays = block_arrays(c, first);
     void* const own = static_cast<uint8_t*>(workspace) + scratch_of(c, seqs, n, a.group, tokens, a.most_blocks, weights != nullptr).partial;
-    if (!simt_forced() && block_step_supported(a.rows)) {
+    if (!simt_forced() && block_step_supported(a.rows, c.head_dim)) {
       const int rc = block_step(arrays, a, seqs, n, c.dtype, c.head_dim, own, status, stream);
       if (rc != NKV_OK) return rc;
       continue;
@@ -212,7 +213,7 @@ int block_attend(const nkv_block_cache& c, const nkv_tokens& q, int tokens, cons
       NKV_LAUNCH_CHECK("attend_plain_kernel");
     }
     if (weights && a.most_blocks > 0) {
-      block_weights_kernel<<<dim3(ceil_div(a.most_blocks, WEIGHT_BLOCKS), c.kv_heads, n), 256, 0, stream>>>(arrays, a, seqs);
+      block_weights_kernel<<<dim3(ceil_div(a.most_blocks, WEIGHT_BLOCKS), c.kv_heads, n), WEIGHT_THREADS, 0, stream>>>(arrays, a, seqs);
       NKV_LAUNCH_CHECK("block_weights_kernel");
     }
   }

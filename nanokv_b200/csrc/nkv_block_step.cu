@@ -1,6 +1,6 @@
 // Attention of few query rows over the 8-bit block cache: the read of a decoding step.
 //
-// The rows of a kv head are its group's heads of all query tokens, up to 16.  Every byte of the cache is used once per
+// The rows of a kv head are its group's heads of all query tokens, up to 16 (32 of heads of 64).  Every byte of the cache is used once per
 // row, so memory is the bound, and the work is cut by bytes: the blocks of all sequences and kv heads form one list, and
 // each warp takes an equal run of it, whatever heads and sequences that run cuts through.  A warp is on its own: its
 // blocks arrive by bulk copies in a ring that only it uses, it keeps the running softmax of its rows in registers, and
@@ -101,7 +101,7 @@ __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i ==
 // the tokens of an 8 x 8 piece of scores: with them a lane's four neighbouring bytes of a V row are its operand as they lie
 __device__ __forceinline__ int token_of(int tile, int hi, int row) { return 16 * (row >> 1) + 4 * tile + 2 * hi + (row & 1); }
 
-// NT: 8-wide groups of rows (1 or 2)
+// NT: 8-wide groups of rows
 template <int DT, int D, int NT>
 __global__ void __launch_bounds__(32 * WARPS, CTAS_PER_SM)
 step_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const __grid_constant__ Plan plan, Parts parts,
@@ -177,9 +177,27 @@ step_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
 #pragma unroll
       for (int ch = 0; ch < CHUNKS; ++ch)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          x[ch][e] = in ? load_float(row, DT, 64 * ch + 16 * t4 + e) : 0.f;
-          top = fmaxf(top, fabsf(x[ch][e]));
+        for (int e = 0; e < 16; e += 8) {
+          const uint16_t* const src = row + 64 * ch + 16 * t4 + e;
+          uint32_t w[4] = {0, 0, 0, 0};
+          if (in && a.q_vector) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(src));
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+          } else if (in) {
+#pragma unroll 1
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t pair = __ldg(src + 2 * k) | (static_cast<uint32_t>(__ldg(src + 2 * k + 1)) << 16);
+#pragma unroll
+              for (int kk = 0; kk < 4; ++kk) w[kk] = kk == k ? pair : w[kk];
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = unpack2<DT>(w[k]);
+            x[ch][e + 2 * k] = f.x;
+            x[ch][e + 2 * k + 1] = f.y;
+            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
         }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -384,30 +402,39 @@ step_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
       const uint16_t* kt = static_cast<const uint16_t*>(c.k_tail) + tail;
       const uint16_t* vt = static_cast<const uint16_t*>(c.v_tail) + tail;
       const int held = seqs.length[b] - t0;
+      // (64 columns at a time, all loads of them in flight: one warp has this block, and the others wait for it)
 #pragma unroll 1
-      for (int ch = 0; ch < CHUNKS; ++ch)
-#pragma unroll 1
-        for (int w = 0; w < 4; ++w) {
-          const int d0 = 64 * ch + 16 * t4 + 4 * w;
-          uint32_t q2[NT][2];
+      for (int ch = 0; ch < CHUNKS; ++ch) {
+        uint2 k_lo[4][4], k_hi[4][4], q2[NT][4];
+        const int d0 = 64 * ch + 16 * t4;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const int r = 8 * nt + g8, token = r / a.group;
-            q2[nt][0] = q2[nt][1] = 0;
-            if (r < a.rows) {
-              const uint16_t* row = a.q + b * a.q_batch + token * a.q_token + (h * a.group + r - token * a.group) * a.q_head + d0;
-              q2[nt][0] = __ldg(row) | (static_cast<uint32_t>(__ldg(row + 1)) << 16);
-              q2[nt][1] = __ldg(row + 2) | (static_cast<uint32_t>(__ldg(row + 3)) << 16);
-            }
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            k_lo[i][w] = *reinterpret_cast<const uint2*>(kt + token_of(i, 0, g8) * D + d0 + 4 * w);
+            k_hi[i][w] = *reinterpret_cast<const uint2*>(kt + token_of(i, 1, g8) * D + d0 + 4 * w);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint2 lo = *reinterpret_cast<const uint2*>(kt + token_of(i, 0, g8) * D + d0);
-            const uint2 hi = *reinterpret_cast<const uint2*>(kt + token_of(i, 1, g8) * D + d0);
+        for (int nt = 0; nt < NT; ++nt) {
+          const int r = 8 * nt + g8, token = r / a.group;
+          const uint16_t* const row = a.q + b * a.q_batch + token * a.q_token + (h * a.group + r - token * a.group) * a.q_head + d0;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816<DT == NKV_BF16>(s[nt][i], lo.x, hi.x, lo.y, hi.y, q2[nt][0], q2[nt][1]);
+          for (int w = 0; w < 4; ++w) {
+            q2[nt][w] = make_uint2(0, 0);
+            if (r < a.rows && a.q_vector) q2[nt][w] = __ldg(reinterpret_cast<const uint2*>(row + 4 * w));
+            else if (r < a.rows)
+              q2[nt][w] = make_uint2(__ldg(row + 4 * w) | (static_cast<uint32_t>(__ldg(row + 4 * w + 1)) << 16),
+                                     __ldg(row + 4 * w + 2) | (static_cast<uint32_t>(__ldg(row + 4 * w + 3)) << 16));
           }
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma16816<DT == NKV_BF16>(s[nt][i], k_lo[i][w].x, k_hi[i][w].x, k_lo[i][w].y, k_hi[i][w].y, q2[nt][w].x, q2[nt][w].y);
+      }
       // `factor` carries the rows' powers of two and the sign of the scale is in the operand: neither is here
       float kept[NT][2];
 #pragma unroll
@@ -464,12 +491,16 @@ step_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
   if (head_b >= 0) store_part(head_b, head_h);
 }
 
-// Joins the parts of one kv head's rows: a thread block per head.  With weights, every block's share of the rows'
-// attention as well, rows in a fixed order.
+// Joins the parts of `slice` rows of a kv head.  A thread has four columns of a row; where the rows leave threads over, the parts
+// are dealt out to several of them.  With weights, every block's share of the rows' attention as well,
+// rows in a fixed order.
+constexpr int JOIN_THREADS = 512;
 template <int DT, int D>
-__global__ void __launch_bounds__(256)
-join_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const __grid_constant__ Plan plan, Parts parts) {
-  __shared__ float lse2[16];
+__global__ void __launch_bounds__(JOIN_THREADS)
+join_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const __grid_constant__ Plan plan, Parts parts, int slice) {
+  __shared__ float lse2[32];
+  __shared__ float4 accs[JOIN_THREADS];
+  __shared__ float2 mls[JOIN_THREADS];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int h = blockIdx.x, b = blockIdx.y;
   const int length = seqs.length[b], count = seqs.count[b];
@@ -477,40 +508,57 @@ join_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
   const size_t bh = static_cast<size_t>(b) * c.kv_heads + h;
   const uint32_t begin = plan.start[b] + h * n;
   const uint32_t w0 = n ? plan.worker_of(begin) : 0u, w1 = n ? plan.worker_of(begin + n - 1) : 0u;
-  for (int i = threadIdx.x; i < a.rows * (D / 4); i += 256) {
-    const int r = i / (D / 4), col = (i % (D / 4)) * 4;
-    const int token = r / a.group, head = h * a.group + r % a.group;
-    const size_t at = (static_cast<size_t>(b) * a.tokens + token) * a.heads + head;
-    const bool any = visible_to(a, length, count, r) > 0;
+  constexpr int COLS = D / 4;
+  const int row0 = blockIdx.z * slice, wanted = min(slice, a.rows - row0) * COLS;
+  const int groups = max(1, min(JOIN_THREADS / wanted, static_cast<int>(w1 - w0) + 1));   // threads that share the parts of four columns
+  for (int base = 0; base < wanted; base += JOIN_THREADS) {
+    const int i = groups > 1 ? threadIdx.x % wanted : base + threadIdx.x, group = groups > 1 ? threadIdx.x / wanted : 0;
+    const bool in = i < wanted && group < groups;
+    const int r = row0 + i / COLS, col = (i % COLS) * 4;
+    const bool any = in && visible_to(a, length, count, r) > 0;
     float top = -INFINITY, sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float m, float l, const float4& o) {
+      const float next = fmaxf(top, m), ref = next == -INFINITY ? 0.f : next, f = exp2f(top - ref), g = exp2f(m - ref);
+      top = next;
+      sum = fmaf(sum, f, l * g);
+      acc.x = fmaf(acc.x, f, o.x * g);
+      acc.y = fmaf(acc.y, f, o.y * g);
+      acc.z = fmaf(acc.z, f, o.z * g);
+      acc.w = fmaf(acc.w, f, o.w * g);
+    };
     if (any) {
 #pragma unroll 4
-      for (uint32_t w = w0; w <= w1; ++w) top = fmaxf(top, __ldcg(&parts.ml[(w + bh) * a.rows + r].x));
-      const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll 4
-      for (uint32_t w = w0; w <= w1; ++w) {
+      for (uint32_t w = w0 + group; w <= w1; w += groups) {
         const float2 ml = __ldcg(&parts.ml[(w + bh) * a.rows + r]);
-        const float4 part = __ldcg(reinterpret_cast<const float4*>(parts.o + ((w + bh) * a.rows + r) * D + col));
-        const float f = exp2f(ml.x - ref);
-        sum = fmaf(ml.y, f, sum);
-        acc.x = fmaf(part.x, f, acc.x);
-        acc.y = fmaf(part.y, f, acc.y);
-        acc.z = fmaf(part.z, f, acc.z);
-        acc.w = fmaf(part.w, f, acc.w);
+        add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4*>(parts.o + ((w + bh) * a.rows + r) * D + col)));
       }
     }
-    const float inv = any ? 1.f / sum : 0.f;
-    *reinterpret_cast<uint2*>(a.out + at * D + col) = make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
-    if (col == 0) {
-      const float v = any ? top + log2f(sum) : -INFINITY;
-      a.lse[at] = v * LN2;
-      lse2[r] = v;
+    for (int left = groups; left > 1;) {
+      const int half = (left + 1) / 2;
+      accs[threadIdx.x] = acc;
+      mls[threadIdx.x] = make_float2(top, sum);
+      __syncthreads();
+      const int other = threadIdx.x + half * wanted;
+      if (any && group + half < left) add(mls[other].x, mls[other].y, accs[other]);
+      __syncthreads();
+      left = half;
+    }
+    if (in && group == 0) {
+      const int token = r / a.group, head = h * a.group + r - token * a.group;
+      const size_t at = (static_cast<size_t>(b) * a.tokens + token) * a.heads + head;
+      const float inv = any ? 1.f / sum : 0.f;
+      *reinterpret_cast<uint2*>(a.out + at * D + col) = make_uint2(pack2<DT>(acc.x * inv, acc.y * inv), pack2<DT>(acc.z * inv, acc.w * inv));
+      if (col == 0) {
+        const float v = any ? top + log2f(sum) : -INFINITY;
+        a.lse[at] = v * LN2;
+        lse2[r] = v;
+      }
     }
   }
   if (a.weights == nullptr) return;
   __syncthreads();
-  for (uint32_t block = threadIdx.x; block < n; block += 256) {
+  for (uint32_t block = threadIdx.x; block < n; block += JOIN_THREADS) {
     const float* partial = a.partial + (bh * a.most_blocks + block) * a.rows;
     float sum = 0.f;
     for (int r = 0; r < a.rows; ++r)
@@ -540,7 +588,8 @@ size_t parts_of(const Plan& p, int kv_heads) { return p.workers + static_cast<si
 
 }  // namespace
 
-bool block_step_supported(int rows) { return rows <= 16; }
+// four groups of eight rows of 64 columns take as many registers as two of 128
+bool block_step_supported(int rows, int d) { return rows <= (d == 64 ? 32 : 16); }
 
 // bytes of the parts of one launch
 size_t block_step_bytes(const Sequences& seqs, int n, int kv_heads, int rows, int d) {
@@ -560,17 +609,24 @@ int block_step(const BlockArrays& c, const Call& a, const Sequences& seqs, int n
       NKV_LAUNCH_CHECK("step_kernel");
       return NKV_OK;
     };
-    const bool bf16 = dtype == NKV_BF16, wide = d == 128, two = a.rows > 8;
-    const int rc = wide ? (bf16 ? (two ? run(step_kernel<NKV_BF16, 128, 2>) : run(step_kernel<NKV_BF16, 128, 1>))
-                                : (two ? run(step_kernel<NKV_F16, 128, 2>) : run(step_kernel<NKV_F16, 128, 1>)))
-                        : (bf16 ? (two ? run(step_kernel<NKV_BF16, 64, 2>) : run(step_kernel<NKV_BF16, 64, 1>))
-                                : (two ? run(step_kernel<NKV_F16, 64, 2>) : run(step_kernel<NKV_F16, 64, 1>)));
+    const bool bf16 = dtype == NKV_BF16;
+    const int groups = ceil_div(a.rows, 8);
+    int rc;
+    if (d == 128) rc = groups == 1 ? (bf16 ? run(step_kernel<NKV_BF16, 128, 1>) : run(step_kernel<NKV_F16, 128, 1>))
+                                   : (bf16 ? run(step_kernel<NKV_BF16, 128, 2>) : run(step_kernel<NKV_F16, 128, 2>));
+    else if (groups == 1) rc = bf16 ? run(step_kernel<NKV_BF16, 64, 1>) : run(step_kernel<NKV_F16, 64, 1>);
+    else if (groups == 2) rc = bf16 ? run(step_kernel<NKV_BF16, 64, 2>) : run(step_kernel<NKV_F16, 64, 2>);
+    else if (groups == 3) rc = bf16 ? run(step_kernel<NKV_BF16, 64, 3>) : run(step_kernel<NKV_F16, 64, 3>);
+    else rc = bf16 ? run(step_kernel<NKV_BF16, 64, 4>) : run(step_kernel<NKV_F16, 64, 4>);
     if (rc != NKV_OK) return rc;
   }
   // the joining launch is set up under the first one's tail and waits for its results
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(c.kv_heads, n);
-  config.blockDim = dim3(256);
+  // few heads: their rows are cut too (not with weights, which take all rows of a head)
+  const int slices = a.weights ? 1 : min(a.rows, max(1, 2 * sm_count() / (c.kv_heads * n)));
+  const int slice = ceil_div(a.rows, slices);
+  config.gridDim = dim3(c.kv_heads, n, ceil_div(a.rows, slice));
+  config.blockDim = dim3(JOIN_THREADS);
   config.stream = stream;
   cudaLaunchAttribute attribute;
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -579,7 +635,7 @@ int block_step(const BlockArrays& c, const Call& a, const Sequences& seqs, int n
   config.numAttrs = plan.workers > 0 ? 1 : 0;
   auto join = d == 128 ? (dtype == NKV_BF16 ? join_kernel<NKV_BF16, 128> : join_kernel<NKV_F16, 128>)
                        : (dtype == NKV_BF16 ? join_kernel<NKV_BF16, 64> : join_kernel<NKV_F16, 64>);
-  NKV_CUDA(cudaLaunchKernelEx(&config, join, c, a, seqs, plan, parts));
+  NKV_CUDA(cudaLaunchKernelEx(&config, join, c, a, seqs, plan, parts, slice));
   return NKV_OK;
 }
 

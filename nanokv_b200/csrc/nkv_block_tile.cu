@@ -324,7 +324,7 @@ __device__ __forceinline__ void codes_role(uint8_t* smem, uint64_t* bars, const 
 // ---- warps 8-11: queries, K and V as operands -----------------------------------------------------------------
 template <int DT, int D, bool IMAGES>
 __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, const BlockArrays& c, const Call& a, const Sequences& seqs,
-                                             const Plan& plan, const Ctx& ctx, int q_vector) {
+                                             const Plan& plan, const Ctx& ctx) {
   using L = Layout<D>;
   constexpr int DCH = L::DCH, LOADS = D / 16;   // 16-byte pieces of a thread per tile and tensor, half of them of each block
   const int tid = threadIdx.x - 32 * SOFTMAX_WARPS, lane = tid & 31;
@@ -417,7 +417,7 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
       for (int k = 0; k < AHEAD; ++k) {
         const uint16_t* const src = q_head + token * a.q_token + head * a.q_head;
         v[k] = make_uint4(0, 0, 0, 0);
-        if (q_vector && r < a.rows) v[k] = __ldg(reinterpret_cast<const uint4*>(src));
+        if (a.q_vector && r < a.rows) v[k] = __ldg(reinterpret_cast<const uint4*>(src));
         r += ROWS;
         token += token_step;
         head += head_step;
@@ -433,7 +433,7 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
     }
     if (!ok) break;
     ++pieces;
-    if (!q_vector) {   // rows that start anywhere
+    if (!a.q_vector) {   // rows that start anywhere
 #pragma unroll 1
       for (int row = q_row; row < UNIT; row += ROWS) {
         const int at = p.unit * UNIT + row, t = at / a.group;
@@ -749,7 +749,7 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
 template <int DT, int D, bool IMAGES>
 __global__ void __launch_bounds__(THREADS, 1)
 tile_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const __grid_constant__ Plan plan, Parts parts, const uint8_t* images,
-            int q_vector, int32_t* status) {
+            int32_t* status) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem);
@@ -787,7 +787,7 @@ tile_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
   if (IMAGES) asm volatile("griddepcontrol.wait;" ::: "memory");   // the images are written by the launch before
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp < SOFTMAX_WARPS) softmax_role<DT, D>(smem, bars, tmem, a, seqs, plan, parts, ctx, c.kv_heads);
-  else if (warp < SOFTMAX_WARPS + OPERAND_WARPS) operand_role<DT, D, IMAGES>(smem, bars, c, a, seqs, plan, ctx, q_vector);
+  else if (warp < SOFTMAX_WARPS + OPERAND_WARPS) operand_role<DT, D, IMAGES>(smem, bars, c, a, seqs, plan, ctx);
   else if (warp > MMA_WARP) codes_role<D, IMAGES>(smem, bars, c, a, seqs, plan, ctx, images);
   else mma_role<DT, D>(smem, bars, tmem, a, seqs, plan, ctx, c.kv_heads);
   tc_fence_before();
@@ -939,7 +939,6 @@ int launch(const BlockArrays& c, const Call& a, const Sequences& seqs, int n, in
   parts.o = static_cast<float*>(workspace);
   parts.ml = reinterpret_cast<float2*>(parts.o + static_cast<size_t>(plan.runs) * 2 * UNIT * d);
   uint8_t* const image = static_cast<uint8_t*>(workspace) + part_bytes(sm_count(), d);
-  const int q_vector = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_batch % 8 == 0 && a.q_token % 8 == 0 && a.q_head % 8 == 0;
   const bool bf16 = dtype == NKV_BF16, wide = d == 128;
   cudaLaunchAttribute attribute;
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -962,7 +961,7 @@ int launch(const BlockArrays& c, const Call& a, const Sequences& seqs, int n, in
       config.blockDim = dim3(THREADS);
       config.dynamicSmemBytes = smem;
       config.numAttrs = images ? 1 : 0;
-      NKV_CUDA(cudaLaunchKernelEx(&config, kernel, c, a, seqs, plan, parts, static_cast<const uint8_t*>(image), q_vector, status));
+      NKV_CUDA(cudaLaunchKernelEx(&config, kernel, c, a, seqs, plan, parts, static_cast<const uint8_t*>(image), status));
       config.dynamicSmemBytes = 0;
       return NKV_OK;
     };
