@@ -51,6 +51,13 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// (a NaN among them is passed over, as by fmaxf)
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+
 // value of a stored byte: 2^23 + byte is an fp32 number whose low mantissa bits are the byte
 __device__ __forceinline__ float code_value(uint32_t byte) { return __uint_as_float(0x4B000000u | byte) - 8388736.0f; }
 

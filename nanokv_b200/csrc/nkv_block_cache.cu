@@ -179,6 +179,27 @@ __device__ __forceinline__ uint4 load_piece(const uint16_t* row, int d0, bool ve
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// entries of eight neighbouring pairs from the one of element d0 on (half layout); rows of the table start on 16 bytes where its
+// base does, as dim is a multiple of 16
+__device__ __forceinline__ void turns_of(const Rotation& rot, int position, int d0, float2 (&cs)[8]) {
+  const bool in = static_cast<unsigned>(position) < static_cast<unsigned>(rot.rows);
+  const float2* const from = rot.table + static_cast<size_t>(in ? position : 0) * (rot.dim / 2) + d0;
+  if ((reinterpret_cast<uintptr_t>(rot.table) & 15) == 0) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(from + e));
+      cs[e] = make_float2(v.x, v.y);
+      cs[e + 1] = make_float2(v.z, v.w);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) cs[e] = __ldg(from + e);
+  }
+  if (!in)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) cs[e] = make_float2(CUDART_NAN_F, CUDART_NAN_F);
+}
+
 template <int DT>
 __device__ __forceinline__ uint4 rotated_piece(const uint16_t* row, int d0, bool vector, const Rotation& rot, int position) {
   const uint4 raw = load_piece<DT>(row, d0, vector);
@@ -216,20 +237,42 @@ __device__ __forceinline__ bool not_finite(const uint4& v) {
   return bad;
 }
 
-// Code (plus 128) of x for a block scale: rint(x / scale).  x * inv is within 2 ulp of the IEEE quotient, less than 1e-4 at
-// 127, so only products that near to a half take the division; rint is the addition of 1.5 * 2^23 + 128, whose low
-// byte is the code.  A scale too small for its reciprocal divides always, and clamps: such a scale is a subnormal
-// number, a coarse multiple of the maximum / 127.
-__device__ __forceinline__ uint32_t code_of(float x, float scale, float inv) {
+// Codes (plus 128) of eight elements for a block scale: rint(x / scale), quotient rounded to fp32.  fma(x, inv, 1.5 * 2^23 + 128) is
+// the exact x * inv rounded to an integer, whose low byte is the code; x * inv is within 2 ulp of the quotient, less than 1e-4 at
+// 127, so only pieces with an element that near to a half take the division.  exact: the scale is too small for its
+// reciprocal; such a scale is a subnormal number, a coarse multiple of the maximum / 127, and its codes are clamped.
+__device__ __forceinline__ uint2 codes_of(const float (&x)[8], float scale, float inv, bool exact) {
   constexpr float MAGIC = 12583040.0f;
-  float q = x * inv;
-  float t = __fadd_rn(q, MAGIC);
-  if (fabsf(q - (t - MAGIC)) > 0.4999f || !(inv < 1e37f)) {
-    q = fminf(fmaxf(__fdiv_rn(x, scale), -127.f), 127.f);
-    t = __fadd_rn(q, MAGIC);
+  const uint64_t inv2 = pair_f32(inv, inv), magic2 = pair_f32(MAGIC, MAGIC), minus2 = pair_f32(-MAGIC, -MAGIC), neg2 = pair_f32(-inv, -inv);
+  uint32_t t[8];
+  float worst = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const uint64_t v = pair_f32(x[e], x[e + 1]), sum = fma_f32x2(v, inv2, magic2);
+    float d0, d1, t0, t1;
+    split_f32(fma_f32x2(v, neg2, add_f32x2(sum, minus2)), d0, d1);   // rounded less exact
+    split_f32(sum, t0, t1);
+    worst = max3(worst, fabsf(d0), fabsf(d1));
+    t[e] = __float_as_uint(t0);
+    t[e + 1] = __float_as_uint(t1);
   }
-  return __float_as_uint(t) & 0xFFu;
+  if (worst > 0.4999f || exact) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t[e] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fdiv_rn(x[e], scale), -127.f), 127.f), MAGIC));
+  }
+  uint2 w;
+  w.x = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+  w.y = __byte_perm(__byte_perm(t[4], t[5], 0x0040), __byte_perm(t[6], t[7], 0x0040), 0x5410);
+  return w;
 }
+
+// largest magnitudes of the two halves, as bits: those of 16-bit floating-point numbers are ordered as the numbers are, and what
+// is not finite comes out as NOT_FINITE or more
+__device__ __forceinline__ uint32_t magnitude(const uint4& v) {
+  constexpr uint32_t M = 0x7FFF7FFFu;
+  return __vmaxu2(__vmaxu2(v.x & M, v.y & M), __vmaxu2(v.z & M, v.w & M));
+}
+template <int DT> constexpr uint32_t NOT_FINITE = DT == NKV_BF16 ? 0x7F80u : 0x7C00u;
 
 struct AppendSide {
   const uint16_t* x;
@@ -237,15 +280,18 @@ struct AppendSide {
   int vector;   // rows and strides on 16 bytes
 };
 
-// One block of one sequence and head that the call touches.  A thread holds eight columns of four neighbouring tokens, so
-// that four codes of a column make a word of the transposed V block.  A block that the call completes takes its old
-// tokens from the tail; one that stays open only gets its new tokens stored there.
+// One block of one sequence and head that the call touches.  K: a thread has the pieces p and p + D / 16 of a token's row, which
+// are each other's partners where all of a head turns in the half layout, in two passes of 32 tokens.  V: it has eight
+// columns of four neighbouring tokens, so that four codes of a column make a word of the transposed block.  A block that
+// the call completes takes its old tokens from the tail; one that stays open only gets its new tokens stored there.
+// Bound: memory (24,967 tokens x 40 heads x 128 rotated and written: @@ us); with the pairs of a head turned twice, table entries
+// fetched one by one and a division's test per element it was the arithmetic, 503 us.
 template <int DT, int D>
-__global__ void __launch_bounds__(2 * D)
+__global__ void __launch_bounds__(2 * D, 512 / D)
 append_kernel(BlockArrays c, AppendSide k, AppendSide v, Rotation rot, int tokens, Sequences seqs) {
-  constexpr int PIECES = D / 8, THREADS = 2 * D;
+  constexpr int PIECES = D / 8, PAIRS = PIECES / 2, THREADS = 2 * D, WARPS = THREADS / 32;
   __shared__ uint32_t words[D * 16];        // [column][16 words of 4 tokens], word index xor column / 8
-  __shared__ float reduced[2][THREADS / 32];
+  __shared__ uint32_t reduced[2][WARPS];
   const int b = blockIdx.z, h = blockIdx.y;
   const int length = seqs.length[b], count = seqs.count[b];
   const int block = length / NKV_BLOCK + blockIdx.x;
@@ -253,84 +299,119 @@ append_kernel(BlockArrays c, AppendSide k, AppendSide v, Rotation rot, int token
   if (t0 >= length + count || block >= c.blocks || count <= 0) return;
   const int held = max(0, length - t0), filled = min(NKV_BLOCK, length + count - t0);
   const bool whole = filled == NKV_BLOCK;
-  const int piece = threadIdx.x % PIECES, group = threadIdx.x / PIECES, lane = threadIdx.x & 31;
-  const int d0 = piece * 8;
+  const int lane = threadIdx.x & 31;
   const size_t bh = static_cast<size_t>(b) * c.kv_heads + h;
   uint16_t* const k_tail = static_cast<uint16_t*>(c.k_tail) + bh * NKV_BLOCK * D;
   uint16_t* const v_tail = static_cast<uint16_t*>(c.v_tail) + bh * NKV_BLOCK * D;
-  uint4 kp[4], vp[4];
-  uint32_t bad_tokens = 0;
+  // ---- K
+  const int pair = threadIdx.x % PAIRS, d_lo = pair * 8, d_hi = d_lo + D / 2;
+  const int k_token = threadIdx.x / PAIRS;   // and 32 on
+  const bool partners = rot.dim == D && rot.layout == NKV_ROTARY_HALF && k.vector != 0;
+  uint4 kp[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int t = k_token + 32 * i;
+    kp[i][0] = kp[i][1] = make_uint4(0, 0, 0, 0);
+    if (t >= held && t < filled) {
+      const long long n = t0 + t - length;   // token of the call
+      const uint16_t* const row = k.x + b * k.stride_batch + n * k.stride_token + h * k.stride_head;
+      const int position = rot.dim > 0 ? __ldg(rot.positions + static_cast<size_t>(b) * tokens + n) : 0;
+      if (partners) {
+        const uint4 lo = load_piece<DT>(row, d_lo, true), hi = load_piece<DT>(row, d_hi, true);
+        float2 cs[8];
+        turns_of(rot, position, d_lo, cs);
+        float x[8], y[8];
+        Piece<DT>::unpack(lo, x);
+        Piece<DT>::unpack(hi, y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float x0 = x[e], x1 = y[e];
+          x[e] = turn_first(x0, x1, cs[e]);
+          y[e] = turn_second(x0, x1, cs[e]);
+        }
+        kp[i][0] = Piece<DT>::pack(x);
+        kp[i][1] = Piece<DT>::pack(y);
+      } else {
+        kp[i][0] = rot.dim > 0 ? rotated_piece<DT>(row, d_lo, k.vector != 0, rot, position) : load_piece<DT>(row, d_lo, k.vector != 0);
+        kp[i][1] = rot.dim > 0 ? rotated_piece<DT>(row, d_hi, k.vector != 0, rot, position) : load_piece<DT>(row, d_hi, k.vector != 0);
+      }
+    } else if (whole && t < held) {
+      kp[i][0] = *reinterpret_cast<const uint4*>(k_tail + t * D + d_lo);
+      kp[i][1] = *reinterpret_cast<const uint4*>(k_tail + t * D + d_hi);
+    }
+  }
+  // ---- V
+  const int piece = threadIdx.x % PIECES, group = threadIdx.x / PIECES, d0 = piece * 8;
+  uint4 vp[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int t = 4 * group + i;
-    kp[i] = vp[i] = make_uint4(0, 0, 0, 0);
+    vp[i] = make_uint4(0, 0, 0, 0);
     if (t >= held && t < filled) {
-      const long long n = t0 + t - length;   // token of the call
-      const uint16_t* kr = k.x + b * k.stride_batch + n * k.stride_token + h * k.stride_head;
-      const uint16_t* vr = v.x + b * v.stride_batch + n * v.stride_token + h * v.stride_head;
-      const int position = rot.dim > 0 && d0 < rot.dim ? __ldg(rot.positions + static_cast<size_t>(b) * tokens + n) : 0;
-      kp[i] = rot.dim > 0 ? rotated_piece<DT>(kr, d0, k.vector != 0, rot, position) : load_piece<DT>(kr, d0, k.vector != 0);
-      vp[i] = load_piece<DT>(vr, d0, v.vector != 0);
+      const uint16_t* const row = v.x + b * v.stride_batch + static_cast<long long>(t0 + t - length) * v.stride_token + h * v.stride_head;
+      vp[i] = load_piece<DT>(row, d0, v.vector != 0);
     } else if (whole && t < held) {
-      kp[i] = *reinterpret_cast<const uint4*>(k_tail + t * D + d0);
       uint32_t w[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         w[e] = v_tail[(d0 + 2 * e) * NKV_BLOCK + t] | (static_cast<uint32_t>(v_tail[(d0 + 2 * e + 1) * NKV_BLOCK + t]) << 16);
       vp[i] = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    // a token with an element that is not finite: NaN keys, zero values (all pieces of a token lie in one warp)
-    const uint32_t flags = __ballot_sync(0xffffffffu, not_finite<DT>(kp[i]) || not_finite<DT>(vp[i]));
-    const uint32_t mine = (PIECES == 32 ? 0xffffffffu : ((1u << PIECES) - 1u) << (lane / PIECES * PIECES));
-    if (flags & mine) {
-      kp[i] = make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);
-      vp[i] = make_uint4(0, 0, 0, 0);
-      bad_tokens |= 1u << i;
-    }
   }
   if (!whole) {
+    // a token with an element that is not finite: NaN keys, zero values
+    __shared__ uint32_t bad_tokens[2];
+    if (threadIdx.x < 2) bad_tokens[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (not_finite<DT>(kp[i][0]) || not_finite<DT>(kp[i][1])) atomicOr(&bad_tokens[i], 1u << k_token);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (not_finite<DT>(vp[i])) atomicOr(&bad_tokens[(4 * group + i) >> 5], 1u << ((4 * group + i) & 31));
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (bad_tokens[i] >> k_token & 1) kp[i][0] = kp[i][1] = make_uint4(0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu, 0x7FFF7FFFu);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (bad_tokens[(4 * group + i) >> 5] >> ((4 * group + i) & 31) & 1) vp[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = k_token + 32 * i;
+      if (t < held || t >= filled) continue;
+      *reinterpret_cast<uint4*>(k_tail + t * D + d_lo) = kp[i][0];
+      *reinterpret_cast<uint4*>(k_tail + t * D + d_hi) = kp[i][1];
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int t = 4 * group + i;
       if (t < held || t >= filled) continue;
-      *reinterpret_cast<uint4*>(k_tail + t * D + d0) = kp[i];
       const uint32_t w[4] = {vp[i].x, vp[i].y, vp[i].z, vp[i].w};
 #pragma unroll
       for (int e = 0; e < 8; ++e) v_tail[(d0 + e) * NKV_BLOCK + t] = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
     }
     return;
   }
-  // ---- the block's scales
-  float kmax = 0.f, vmax = 0.f;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float x[8];
-    if (!(bad_tokens & (1u << i))) {
-      Piece<DT>::unpack(kp[i], x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) kmax = fmaxf(kmax, fabsf(x[e]));
-    }
-    Piece<DT>::unpack(vp[i], x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) vmax = fmaxf(vmax, fabsf(x[e]));
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    kmax = fmaxf(kmax, __shfl_xor_sync(0xffffffffu, kmax, o));
-    vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
-  }
+  // ---- the block's scales; one with an element that is not finite: NaN for K, zero for V
+  uint32_t k_most = __vmaxu2(__vmaxu2(magnitude(kp[0][0]), magnitude(kp[0][1])), __vmaxu2(magnitude(kp[1][0]), magnitude(kp[1][1])));
+  uint32_t v_most = __vmaxu2(__vmaxu2(magnitude(vp[0]), magnitude(vp[1])), __vmaxu2(magnitude(vp[2]), magnitude(vp[3])));
+  k_most = __reduce_max_sync(0xffffffffu, max(k_most & 0xFFFFu, k_most >> 16));
+  v_most = __reduce_max_sync(0xffffffffu, max(v_most & 0xFFFFu, v_most >> 16));
   if (lane == 0) {
-    reduced[0][threadIdx.x / 32] = kmax;
-    reduced[1][threadIdx.x / 32] = vmax;
+    reduced[0][threadIdx.x / 32] = k_most;
+    reduced[1][threadIdx.x / 32] = v_most;
   }
-  const bool bad = __syncthreads_or(bad_tokens != 0) != 0;
+  __syncthreads();
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
-    kmax = fmaxf(kmax, reduced[0][w]);
-    vmax = fmaxf(vmax, reduced[1][w]);
+  for (int w = 0; w < WARPS; ++w) {
+    k_most = max(k_most, reduced[0][w]);
+    v_most = max(v_most, reduced[1][w]);
   }
-  const float k_scale = bad ? 0.f : __fdiv_rn(kmax, 127.f), v_scale = bad ? 0.f : __fdiv_rn(vmax, 127.f);
+  const bool bad = max(k_most, v_most) >= NOT_FINITE<DT>;
+  const float k_scale = bad ? 0.f : __fdiv_rn(unpack2<DT>(k_most).x, 127.f), v_scale = bad ? 0.f : __fdiv_rn(unpack2<DT>(v_most).x, 127.f);
   const float k_inv = __frcp_rn(k_scale), v_inv = __frcp_rn(v_scale);
+  const bool k_exact = !(k_inv < 1e37f), v_exact = !(v_inv < 1e37f);
   const size_t slot = slot_of(c, bh, block);
   if (threadIdx.x == 0) {
     c.scales[2 * slot] = bad ? CUDART_NAN_F : k_scale;
@@ -338,26 +419,34 @@ append_kernel(BlockArrays c, AppendSide k, AppendSide v, Rotation rot, int token
   }
   // ---- codes: K rows as they are, V through shared memory
   uint8_t* const k_codes = c.k_codes + slot * NKV_BLOCK * D;
-  uint32_t column[8];   // four tokens of each of this thread's columns
 #pragma unroll
-  for (int e = 0; e < 8; ++e) column[e] = 0;
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      float x[8];
+      uint2 w = make_uint2(0x80808080u, 0x80808080u);
+      Piece<DT>::unpack(kp[i][half], x);
+      if (k_scale > 0.f) w = codes_of(x, k_scale, k_inv, k_exact);
+      *reinterpret_cast<uint2*>(k_codes + (k_token + 32 * i) * D + (half ? d_hi : d_lo)) = w;
+    }
+  uint2 vw[4];   // codes of the thread's columns, token by token
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float x[8];
-    uint32_t word[2] = {0x80808080u, 0x80808080u};
-    if (k_scale > 0.f) {
-      Piece<DT>::unpack(kp[i], x);
-      word[0] = word[1] = 0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) word[e / 4] |= code_of(x[e], k_scale, k_inv) << (8 * (e & 3));
-    }
-    *reinterpret_cast<uint2*>(k_codes + (4 * group + i) * D + d0) = make_uint2(word[0], word[1]);
     Piece<DT>::unpack(vp[i], x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) column[e] |= (v_scale > 0.f ? code_of(x[e], v_scale, v_inv) : 128u) << (8 * i);
+    vw[i] = v_scale > 0.f ? codes_of(x, v_scale, v_inv, v_exact) : make_uint2(0x80808080u, 0x80808080u);
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) words[(d0 + e) * 16 + (group ^ (piece & 15))] = column[e];
+  for (int half = 0; half < 2; ++half) {   // four columns: a 4 x 4 transposition of bytes
+    const uint32_t w0 = half ? vw[0].y : vw[0].x, w1 = half ? vw[1].y : vw[1].x, w2 = half ? vw[2].y : vw[2].x, w3 = half ? vw[3].y : vw[3].x;
+    const uint32_t a = __byte_perm(w0, w1, 0x5140), e = __byte_perm(w0, w1, 0x7362);
+    const uint32_t f = __byte_perm(w2, w3, 0x5140), g = __byte_perm(w2, w3, 0x7362);
+    const int col = d0 + 4 * half, at = group ^ (piece & 15);
+    words[(col + 0) * 16 + at] = __byte_perm(a, f, 0x5410);
+    words[(col + 1) * 16 + at] = __byte_perm(a, f, 0x7632);
+    words[(col + 2) * 16 + at] = __byte_perm(e, g, 0x5410);
+    words[(col + 3) * 16 + at] = __byte_perm(e, g, 0x7632);
+  }
   __syncthreads();
   uint32_t* const v_codes = reinterpret_cast<uint32_t*>(c.v_codes + slot * NKV_BLOCK * D);
 #pragma unroll

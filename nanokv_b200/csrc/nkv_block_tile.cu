@@ -197,13 +197,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// (a NaN among them is passed over, as by fmaxf)
-__device__ __forceinline__ float max3(float x, float y, float z) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
-  return r;
-}
-
 // 16 columns of this thread's TMEM lane
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
