@@ -630,6 +630,175 @@ evict_kernel(const float* weights, const int32_t* table, int blocks, int keep, i
   }
 }
 
+// The same for rows of 257 to 2,048 entries, whose keys stay in registers, sixteen neighbouring entries to a thread.  The
+// digits begin at the highest bit in which keys differ (weights share most of their exponents, and counts of equal digits
+// collide), and end as soon as all that is left of a digit stays.  Two prefix sums then place every entry.  32 x 40 rows
+// of 1,564: 18.6 us, 25.6 with the kernel above.
+constexpr int SMALL_THREADS = 128, EVICT_ITEMS = 16;
+__global__ void __launch_bounds__(SMALL_THREADS)
+evict_small_kernel(const float* weights, const int32_t* table, int blocks, int keep, int sinks, int recent, float* weights_out,
+                   int32_t* table_out, Sequences seqs) {
+  constexpr int WARPS = SMALL_THREADS / 32;
+  __shared__ float staged[SMALL_THREADS * (EVICT_ITEMS + 1)];
+  __shared__ int32_t slots[SMALL_THREADS * (EVICT_ITEMS + 1)];
+  __shared__ uint16_t order[SMALL_THREADS * EVICT_ITEMS];
+  __shared__ int counts[256];
+  __shared__ uint32_t extremes[2][WARPS];
+  __shared__ uint32_t s_threshold;
+  __shared__ int s_need;
+  __shared__ int sums[2][WARPS];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int full = seqs.length[blockIdx.y], partial = seqs.count[blockIdx.y];
+  const size_t base = (static_cast<size_t>(blockIdx.y) * gridDim.x + blockIdx.x) * blocks;
+  weights += base; table += base; weights_out += base; table_out += base;
+  const int lo = min(sinks, full), hi = max(lo, full - recent);   // candidates [lo, hi)
+  const int live = full + partial, kept_total = min(keep, full) + partial;
+  // coalesced in, sixteen neighbours (one word of padding behind them) out
+#pragma unroll 4
+  for (int i = tid; i < blocks; i += SMALL_THREADS) {
+    staged[i + i / EVICT_ITEMS] = weights[i];
+    slots[i + i / EVICT_ITEMS] = table[i];
+  }
+  __syncthreads();
+  uint32_t key[EVICT_ITEMS];
+  uint32_t candidates = 0;
+#pragma unroll
+  for (int k = 0; k < EVICT_ITEMS; ++k) {
+    const int i = tid * EVICT_ITEMS + k;
+    key[k] = i < live ? weight_key(staged[tid * (EVICT_ITEMS + 1) + k]) : 0u;
+    if (i >= lo && i < hi) candidates |= 1u << k;
+  }
+  int need = keep - (lo + full - hi);   // candidates that stay
+  uint32_t threshold = 0xFFFFFFFFu;
+  int equals = 0;                       // candidates at the threshold that stay; others stay above it
+  const bool all = keep >= full;
+  if (!all && need > 0) {
+    uint32_t most = 0, least = 0xFFFFFFFFu;
+#pragma unroll
+    for (int k = 0; k < EVICT_ITEMS; ++k)
+      if (candidates >> k & 1) {
+        most = max(most, key[k]);
+        least = min(least, key[k]);
+      }
+    most = __reduce_max_sync(0xffffffffu, most);
+    least = __reduce_min_sync(0xffffffffu, least);
+    if (lane == 0) {
+      extremes[0][warp] = most;
+      extremes[1][warp] = least;
+    }
+    counts[tid] = counts[tid + 128] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < WARPS; ++x) {
+      most = max(most, extremes[0][x]);
+      least = min(least, extremes[1][x]);
+    }
+    int top = 32 - __clz(most ^ least);            // bits that are still open
+    threshold = top < 32 ? most >> top << top : 0u;
+    equals = need;                                 // (all keys equal: the first of them)
+#pragma unroll 1
+    while (top > 0) {
+      const int shift = max(0, top - 8);
+      const uint32_t digits = (1u << (top - shift)) - 1u;
+      const uint32_t prefix = top < 32 ? threshold >> top : 0u;
+#pragma unroll
+      for (int k = 0; k < EVICT_ITEMS; ++k)
+        if ((candidates >> k & 1) && (top == 32 || key[k] >> top == prefix)) atomicAdd(&counts[(key[k] >> shift) & digits], 1);
+      __syncthreads();
+      if (warp == 0) {
+        // 8 digits per lane, from the largest down: lane l has digits 255 - 8 l ... 248 - 8 l
+        int own = 0, here[8];
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          here[x] = counts[255 - 8 * lane - x];
+          own += here[x];
+        }
+        int above = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, above, o);
+          if (lane >= o) above += up;
+        }
+        above -= own;
+        if (above < need && above + own >= need) {
+          int left = need - above, digit = 255 - 8 * lane, inside = 0;
+          bool found = false;
+#pragma unroll
+          for (int x = 0; x < 8; ++x)
+            if (!found) {
+              if (left <= here[x]) {
+                found = true;
+                inside = here[x];
+                digit -= x;
+              } else {
+                left -= here[x];
+              }
+            }
+          s_threshold = threshold | (static_cast<uint32_t>(digit) << shift);
+          s_need = inside == left ? -1 : left;   // -1: everything of this digit stays
+        }
+      }
+      __syncthreads();
+      threshold = s_threshold;
+      const int left = s_need;
+      top = shift;
+      if (left < 0) {                            // keys of the digit and above stay: none is compared further
+        --threshold;                             // (a key of 0 would be -NaN's: there is none)
+        equals = 0;
+        break;
+      }
+      need = equals = left;
+      counts[tid] = counts[tid + 128] = 0;
+      __syncthreads();
+    }
+  }
+  // exclusive prefix sum over the thread block
+  auto before = [&](int own, int which) {
+    int sum = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    if (lane == 31) sums[which][warp] = sum;
+    __syncthreads();
+    int first = sum - own;
+#pragma unroll
+    for (int x = 0; x < WARPS; ++x)
+      if (x < warp) first += sums[which][x];
+    return first;
+  };
+  uint32_t eq = 0, kept = 0;
+#pragma unroll
+  for (int k = 0; k < EVICT_ITEMS; ++k)
+    if ((candidates >> k & 1) && key[k] == threshold) eq |= 1u << k;
+  int rank = before(__popc(eq), 0);
+#pragma unroll
+  for (int k = 0; k < EVICT_ITEMS; ++k) {
+    const int i = tid * EVICT_ITEMS + k;
+    const bool stays = all || !(candidates >> k & 1) || key[k] > threshold || ((eq >> k & 1) && rank < equals);
+    if (i < live && stays) kept |= 1u << k;
+    rank += eq >> k & 1;
+  }
+  int at = before(__popc(kept), 1);
+#pragma unroll
+  for (int k = 0; k < EVICT_ITEMS; ++k) {
+    const int i = tid * EVICT_ITEMS + k;
+    if (i < blocks) {
+      const bool stays = kept >> k & 1;
+      const int to = i >= live ? i : (stays ? at : kept_total + i - at);
+      order[to] = tid * (EVICT_ITEMS + 1) + k;
+      at += stays;
+    }
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int i = tid; i < blocks; i += SMALL_THREADS) {   // and coalesced out
+    table_out[i] = slots[order[i]];
+    weights_out[i] = i < kept_total ? staged[order[i]] : 0.f;
+  }
+}
+
 // Sequences of a launch, passed by value: no upload, no device state that a call would have to order against others.
 Sequences sequences_of(const nkv_block_cache& c, int first, int count, const int32_t* counts, int tokens) {
   Sequences s;
@@ -757,8 +926,11 @@ int block_evict(const float* weights, const int32_t* table, const int32_t* full,
       seqs.count[i] = partial[first + i];
     }
     const size_t skip = static_cast<size_t>(first) * kv_heads * blocks;
-    evict_kernel<<<dim3(kv_heads, n), EVICT_THREADS, 0, stream>>>(weights + skip, table + skip, blocks, keep, sinks, recent,
-                                                                  weights_out + skip, table_out + skip, seqs);
+    // one round of the plain kernel's threads: it is shorter there (8 rows of 132: 4.4 us, 5.9)
+    const bool small = blocks > EVICT_THREADS && blocks <= EVICT_ITEMS * SMALL_THREADS;
+    auto kernel = small ? evict_small_kernel : evict_kernel;
+    kernel<<<dim3(kv_heads, n), small ? SMALL_THREADS : EVICT_THREADS, 0, stream>>>(weights + skip, table + skip, blocks, keep, sinks, recent,
+                                                            weights_out + skip, table_out + skip, seqs);
     NKV_LAUNCH_CHECK("evict_kernel");
   }
   return NKV_OK;
