@@ -15,6 +15,7 @@ different streams, as with any tensor.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -75,17 +76,21 @@ class BlockCache:
         self.dtype, self.device = k_tail.dtype, k_codes.device
         self.k_codes, self.v_codes, self.scales, self.table = k_codes, v_codes, scales, table
         self.k_tail, self.v_tail, self.weights = k_tail, v_tail, weights
-        self._lengths = ops._host_ints([int(n) for n in lengths], batch, "lengths")
-        if any(not 0 <= n <= self.capacity for n in self._lengths):
-            raise ValueError(f"lengths must lie in 0 .. {self.capacity}; got {list(self._lengths)}")
-        # which block's first rows the tail holds: how far back a rewind can go
-        self._tail = [(n // BLOCK, n % BLOCK) for n in self._lengths]
+        lengths = [int(n) for n in lengths]
+        if len(lengths) != batch:
+            raise ValueError(f"lengths must name {batch} sequences; got {len(lengths)}")
+        if any(not 0 <= n <= self.capacity for n in lengths):
+            raise ValueError(f"lengths must lie in 0 .. {self.capacity}; got {lengths}")
+        self._lengths = lengths
+        # the token behind the last whose row is in 16 bits (those of its block ahead of it are, too): how far back a rewind can go
+        self._tail = list(lengths)
+        self._array = (ctypes.c_int32 * batch)(*lengths)   # the lengths as the library reads them
         self._refresh()
 
     def _refresh(self) -> None:
         self._struct = _lib.BlockCache(
             self.k_codes.data_ptr(), self.v_codes.data_ptr(), self.scales.data_ptr(), self.table.data_ptr(),
-            self.k_tail.data_ptr(), self.v_tail.data_ptr(), self._lengths, self.batch, self.kv_heads, self.head_dim,
+            self.k_tail.data_ptr(), self.v_tail.data_ptr(), self._array, self.batch, self.kv_heads, self.head_dim,
             self.blocks, ops.dtype_code(self.dtype))
 
     # ------------------------------------------------------------------ bookkeeping
@@ -97,6 +102,10 @@ class BlockCache:
     def lengths(self) -> list[int]:
         """Tokens that every sequence holds."""
         return list(self._lengths)
+
+    def _set_lengths(self, lengths: list[int]) -> None:
+        self._lengths = lengths
+        self._array[:] = lengths
 
     def _rows_of(self, x: torch.Tensor, name: str) -> int:
         if x.dim() != 4 or x.shape[0] != self.batch or x.shape[3] != self.head_dim:
@@ -122,37 +131,46 @@ class BlockCache:
                 raise ValueError(f"the rotation is for heads of {rotary.head_dim} on {rotary.table.device}")
             ops._check_positions(positions, self.batch, tokens, self.device)
             rotation = ops.rotation(rotary.table, positions, rotary.layout)
-        counts = ops._host_ints(counts, self.batch, "counts")
-        with torch.cuda.device(self.device):
-            ops.block_append(self._struct, k, v, counts=counts, rotation=rotation)
-        for b in range(self.batch):
-            added = tokens if counts is None else counts[b]
-            n = self._lengths[b] + added
-            if added and n % BLOCK:
-                self._tail[b] = (n // BLOCK, n % BLOCK)
-            self._lengths[b] = n
+        ints = ops._host_ints(counts, self.batch, "counts")
+        with ops._On(self.device):
+            ops.block_append(self._struct, k, v, counts=ints, rotation=rotation)
+        added = [tokens] * self.batch if counts is None else list(counts)
+        longer = [n + more for n, more in zip(self._lengths, added)]
+        self._tail = [n if more and n % BLOCK else t for n, more, t in zip(longer, added, self._tail)]
+        self._set_lengths(longer)
 
     def rewind(self, lengths) -> None:
         """Every sequence cut back to its first ``lengths[b]`` tokens, as after a draft that was not accepted.  A cut may fall
         between blocks, or among the rows that the open block's 16-bit store still holds; weights of blocks that
         are given up go back to zero."""
+        lengths = list(lengths)
         if len(lengths) != self.batch:
             raise ValueError(f"lengths must name {self.batch} sequences; got {len(lengths)}")
-        for b, n in enumerate(lengths):
-            block, rows = self._tail[b]
-            if not 0 <= n <= self._lengths[b]:
-                raise ValueError(f"sequence {b} holds {self._lengths[b]} tokens; it cannot be cut to {n}")
-            if n != self._lengths[b] and n % BLOCK and not (n // BLOCK == block and n % BLOCK <= rows):
-                raise ValueError(f"sequence {b} cannot be cut to {n}: the rows of block {n // BLOCK} are not in 16 bits any more")
-        for b, n in enumerate(lengths):
-            if -(-n // BLOCK) < -(-self._lengths[b] // BLOCK):
-                self.weights[b, :, -(-n // BLOCK):] = 0
-            self._lengths[b] = n
+        if lengths == self._lengths:
+            return
+        # (sequences mostly stand alike: each kind of cut is looked at once)
+        for n, now, tail in dict.fromkeys(zip(lengths, self._lengths, self._tail)):
+            if not 0 <= n <= now:
+                raise ValueError(f"a sequence that holds {now} tokens cannot be cut to {n}")
+            if n != now and n % BLOCK and not (n // BLOCK == tail // BLOCK and n <= tail):
+                raise ValueError(f"a sequence cannot be cut to {n}: the rows of its block {n // BLOCK} are not in 16 bits any more")
+        left = [-(-n // BLOCK) for n in lengths]
+        held = [-(-n // BLOCK) for n in self._lengths]
+        if left != held:
+            if min(left) == max(left):
+                self.weights[:, :, left[0]:] = 0
+            else:
+                for b, n in enumerate(left):
+                    if n < held[b]:
+                        self.weights[b, :, n:] = 0
+        # rows in 16 bits of tokens that are given up count no longer
+        self._tail = [t if t <= n else (n if n % BLOCK else 0) for n, t in zip(lengths, self._tail)]
+        self._set_lengths(lengths)
 
     def read(self, start: int, stop: int):
         """k, v [batch, stop - start, kv_heads, head_dim]: the values that the cache holds for tokens [start, stop), zero past
         a sequence's length; for callers with an attention of their own."""
-        with torch.cuda.device(self.device):
+        with ops._On(self.device):
             return ops.block_read(self._struct, int(start), int(stop), dtype=self.dtype, device=self.device)
 
     # ------------------------------------------------------------------ attention and eviction
@@ -171,7 +189,7 @@ class BlockCache:
             raise ValueError(f"weights must be contiguous float32 [{self.batch}, {self.kv_heads}, {self.blocks}] on {self.device}")
         if status is not None:
             ops._require_cuda(status)
-        with torch.cuda.device(self.device):
+        with ops._On(self.device):
             return ops.block_attend(self._struct, q, counts=ops._host_ints(counts, self.batch, "counts"), causal=causal,
                                     scale=1.0 / math.sqrt(self.head_dim) if scale is None else scale, weights=weights,
                                     status=status)
@@ -182,10 +200,12 @@ class BlockCache:
         full = [n // BLOCK for n in self._lengths]
         partial = [int(n % BLOCK > 0) for n in self._lengths]
         self.table, self.weights = ops.block_evict(self.weights, self.table, full, partial, keep=keep, sinks=sinks, recent=recent)
+        lengths = list(self._lengths)
         for b, n in enumerate(full):
             if n <= keep:
                 continue
             # the rows in 16 bits move with the open block; those of a block that is complete are given up
-            self._tail[b] = (keep, self._tail[b][1]) if self._tail[b][0] == n and partial[b] else (keep, 0)
-            self._lengths[b] = keep * BLOCK + self._lengths[b] % BLOCK
+            self._tail[b] = keep * BLOCK + self._tail[b] % BLOCK if self._tail[b] // BLOCK == n and partial[b] else 0
+            lengths[b] = keep * BLOCK + lengths[b] % BLOCK
+        self._set_lengths(lengths)
         self._refresh()

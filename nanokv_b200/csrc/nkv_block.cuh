@@ -100,6 +100,9 @@ __device__ __forceinline__ int visible_to(const Call& a, int length, int count, 
   return a.causal ? max(0, min(length, length - count + t + 1)) : length;
 }
 
+// dynamic shared memory allowed to a kernel: asked for once per kernel and device, not with every call (nkv_block_attn.cu)
+cudaError_t allow_shared(const void* kernel, int bytes);
+
 // few rows per kv head (nkv_block_step.cu)
 bool block_step_supported(int rows, int d);
 size_t block_step_bytes(const Sequences& seqs, int n, int kv_heads, int rows, int d);

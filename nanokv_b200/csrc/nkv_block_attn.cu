@@ -1,4 +1,6 @@
 // Attention over the 8-bit block cache.
+#include <atomic>
+
 #include "nkv_block.cuh"
 #include "nkv_internal.h"
 
@@ -159,6 +161,26 @@ Scratch scratch_of(const nkv_block_cache& c, const Sequences& seqs, int n, int g
 
 }  // namespace
 
+cudaError_t allow_shared(const void* kernel, int bytes) {
+  constexpr int DEVICES = 64, KERNELS = 32;
+  static std::atomic<const void*> known[DEVICES][KERNELS];
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return err;
+  std::atomic<const void*>* const row = device < DEVICES ? known[device] : nullptr;
+  for (int i = 0; row && i < KERNELS; ++i) {
+    const void* const k = row[i].load(std::memory_order_acquire);
+    if (k == kernel) return cudaSuccess;
+    if (k == nullptr) break;
+  }
+  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  for (int i = 0; row && err == cudaSuccess && i < KERNELS; ++i) {
+    const void* none = nullptr;
+    if (row[i].compare_exchange_strong(none, kernel) || none == kernel) break;
+  }
+  return err;
+}
+
 size_t block_attend_workspace_bytes(const nkv_block_cache& c, int heads, int tokens, const int32_t* counts, bool causal,
                                     bool with_weights) {
   size_t most = 0;   // launches follow one another on the stream and share it
@@ -208,7 +230,7 @@ int block_attend(const nkv_block_cache& c, const nkv_tokens& q, int tokens, cons
                         : (c.dtype == NKV_BF16 ? attend_plain_kernel<NKV_BF16, 64> : attend_plain_kernel<NKV_F16, 64>);
       const size_t smem = sizeof(float) * (NKV_BLOCK * (c.head_dim + 1) + c.head_dim * (NKV_BLOCK + 1) +
                                            ROWS * (c.head_dim + NKV_BLOCK));
-      NKV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+      NKV_CUDA(allow_shared(reinterpret_cast<const void*>(kernel), static_cast<int>(smem)));
       kernel<<<dim3(ceil_div(a.rows, ROWS), c.kv_heads, n), 32 * ROWS, smem, stream>>>(arrays, a, seqs);
       NKV_LAUNCH_CHECK("attend_plain_kernel");
     }

@@ -604,7 +604,7 @@ int block_step(const BlockArrays& c, const Call& a, const Sequences& seqs, int n
   parts.ml = reinterpret_cast<float2*>(parts.o + parts_of(plan, c.kv_heads) * a.rows * d);
   if (plan.workers > 0) {
     auto run = [&](auto kernel) {
-      NKV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, STEP_SMEM));
+      NKV_CUDA(allow_shared(reinterpret_cast<const void*>(kernel), STEP_SMEM));
       kernel<<<ceil_div(plan.workers, WARPS), 32 * WARPS, STEP_SMEM, stream>>>(c, a, seqs, plan, parts, status);
       NKV_LAUNCH_CHECK("step_kernel");
       return NKV_OK;

@@ -949,7 +949,7 @@ int launch(const BlockArrays& c, const Call& a, const Sequences& seqs, int n, in
       NKV_CUDA(cudaLaunchKernelEx(&config, expand, c, seqs, plan.most_tiles, image));
     }
     auto run = [&](auto kernel, int smem) {
-      NKV_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      NKV_CUDA(allow_shared(reinterpret_cast<const void*>(kernel), smem));
       config.gridDim = dim3(plan.runs);
       config.blockDim = dim3(THREADS);
       config.dynamicSmemBytes = smem;

@@ -32,6 +32,11 @@ def _stream(device: torch.device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def _raw_stream(device: torch.device):
+    """The same of a tensor's device, without the stream object: a few microseconds of a call that takes the GPU as many."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _require_cuda(*tensors: torch.Tensor) -> torch.device:
     device = None
     for tensor in tensors:
@@ -714,11 +719,31 @@ def _rows(x: torch.Tensor, name: str, dtype: torch.dtype | None = None) -> _lib.
     """Rows [batch, tokens, heads, width] as the ABI takes them, whatever their strides but the last."""
     if not x.is_cuda:
         raise RuntimeError("nanokv_b200 runs on CUDA tensors only (there is no CPU path)")
-    if x.dim() != 4 or (x.stride(3) != 1 and x.shape[3] > 1):
-        raise ValueError(f"{name} must be [batch, tokens, heads, width], contiguous along the width")
+    if x.dim() != 4:
+        raise ValueError(f"{name} must be [batch, tokens, heads, width]; got {list(x.shape)}")
+    batch, token, head, element = x.stride()
+    if element != 1 and x.shape[3] > 1:
+        raise ValueError(f"{name} must be contiguous along the width")
     if dtype is not None and x.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, not {x.dtype}")
-    return _lib.Tokens(x.data_ptr(), x.stride(0), x.stride(1), x.stride(2), x.shape[2])
+    return _lib.Tokens(x.data_ptr(), batch, token, head, x.shape[2])
+
+
+class _On:
+    """The device of a call made current for its launches.  The common case, that it is already, costs a comparison."""
+    __slots__ = ("index", "before")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.index is not None and self.index != self.before:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *_):
+        if self.index is not None and self.index != self.before:
+            torch.cuda.set_device(self.before)
 
 
 def _host_ints(values, count: int, name: str):
@@ -764,9 +789,9 @@ def rotary(x: torch.Tensor, y: torch.Tensor | None, table: torch.Tensor, positio
         raise ValueError("the rotation table must be on the rows' device")
     rot = rotation(table, positions, layout)
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
-        _lib.check(_lib.library().nkv_rotary(xs, _ptr(out), ys, _ptr(out_y), dtype_code(x.dtype), batch, tokens, width, rot,
-                                             int(transposed), _stream(x.device)))
+    with _On(x.device):
+        _lib.check(_lib.library().nkv_rotary(xs, out.data_ptr(), ys, None if y is None else out_y.data_ptr(), dtype_code(x.dtype), batch, tokens, width, rot,
+                                             int(transposed), _raw_stream(x.device)))
     return out if y is None else (out, out_y)
 
 
@@ -774,14 +799,14 @@ def block_append(struct: _lib.BlockCache, k: torch.Tensor, v: torch.Tensor, *, c
                  rotation: _lib.Rotation | None = None) -> None:
     """Tokens k, v [batch, tokens, kv_heads, width] put behind what the cache holds (nkv_block_append)."""
     _lib.check(_lib.library().nkv_block_append(struct, _rows(k, "k"), _rows(v, "v"), k.shape[1], counts, rotation,
-                                               _stream(k.device)))
+                                               _raw_stream(k.device)))
 
 
 def block_read(struct: _lib.BlockCache, start: int, stop: int, *, dtype: torch.dtype, device: torch.device):
     """Values of tokens [start, stop) of every sequence -> k, v [batch, stop - start, kv_heads, width] (nkv_block_read)."""
     shape = (struct.batch, max(0, stop - start), struct.kv_heads, struct.head_dim)
     k, v = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
-    _lib.check(_lib.library().nkv_block_read(struct, start, stop, _ptr(k), _ptr(v), _stream(device)))
+    _lib.check(_lib.library().nkv_block_read(struct, start, stop, k.data_ptr(), v.data_ptr(), _raw_stream(device)))
     return k, v
 
 
@@ -798,7 +823,7 @@ def block_attend(struct: _lib.BlockCache, q: torch.Tensor, *, counts=None, causa
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     _lib.check(lib.nkv_block_attend(struct, rows, tokens, counts, int(causal), float(scale), _ptr(out), _ptr(lse), _ptr(weights),
                                     _ptr(status_word(q.device) if status is None else status), _ptr(workspace), nbytes,
-                                    _stream(q.device)))
+                                    _raw_stream(q.device)))
     return out, lse
 
 
@@ -813,7 +838,7 @@ def block_evict(weights: torch.Tensor, table: torch.Tensor, full, partial, *, ke
     batch, kv_heads, blocks = table.shape
     full, partial = _host_ints(full, batch, "full"), _host_ints(partial, batch, "partial")
     table_out, weights_out = torch.empty_like(table), torch.empty_like(weights)
-    with torch.cuda.device(device):
+    with _On(device):
         _lib.check(_lib.library().nkv_block_evict(_ptr(weights), _ptr(table), full, partial, batch, kv_heads, blocks, int(keep),
-                                                  int(sinks), int(recent), _ptr(weights_out), _ptr(table_out), _stream(device)))
+                                                  int(sinks), int(recent), _ptr(weights_out), _ptr(table_out), _raw_stream(device)))
     return table_out, weights_out

@@ -163,6 +163,20 @@ def test_rewind_and_append_again():
     assert cache.lengths == [64, 0]
 
 
+def test_rows_of_tokens_that_were_given_up_are_not_cut_back_to():
+    k, v = (randn(1, 256, 1, 64, seed=s, dtype=torch.bfloat16).cuda() for s in (1, 2))
+    cache = BlockCache(1, 1, 64, 256)
+    cache.append(k[:, :104], v[:, :104])
+    cache.rewind([0])
+    cache.append(k[:, 128:256], v[:, 128:256])       # block 1 again, complete at once: 16-bit rows of it are the old ones
+    with pytest.raises(ValueError, match="cannot be cut"):
+        cache.rewind([100])
+    cache.rewind([64])
+    cache.append(k[:, :20], v[:, :20])
+    cache.rewind([70])
+    assert torch.equal(cache.read(64, 70)[0], k[:, :6])
+
+
 def test_rewind_gives_up_the_weights_of_dropped_blocks():
     cache, hk, hv = filled([200], 1, 64, torch.bfloat16, 3)
     cache.weights.fill_(1.0)
