@@ -154,8 +154,7 @@ class BlockCache:
                 raise ValueError(f"a sequence that holds {now} tokens cannot be cut to {n}")
             if n != now and n % BLOCK and not (n // BLOCK == tail // BLOCK and n <= tail):
                 raise ValueError(f"a sequence cannot be cut to {n}: the rows of its block {n // BLOCK} are not in 16 bits any more")
-        left = [-(-n // BLOCK) for n in lengths]
-        held = [-(-n // BLOCK) for n in self._lengths]
+        left, held = ([(n + BLOCK - 1) // BLOCK for n in some] for some in (lengths, self._lengths))
         if left != held:
             if min(left) == max(left):
                 self.weights[:, :, left[0]:] = 0

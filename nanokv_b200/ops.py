@@ -783,12 +783,12 @@ def rotary(x: torch.Tensor, y: torch.Tensor | None, table: torch.Tensor, positio
         ys = _rows(y, "y", x.dtype)
         if y.shape[:2] != x.shape[:2] or y.shape[3] != width or y.device != x.device:
             raise ValueError(f"x and y must share batch, tokens, width and device; got {tuple(x.shape)} and {tuple(y.shape)}")
-        out_y = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+        out_y = torch.empty_like(y, memory_format=torch.contiguous_format)
     _check_positions(positions, batch, tokens, x.device)
     if table.device != x.device:
         raise ValueError("the rotation table must be on the rows' device")
     rot = rotation(table, positions, layout)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
     with _On(x.device):
         _lib.check(_lib.library().nkv_rotary(xs, out.data_ptr(), ys, None if y is None else out_y.data_ptr(), dtype_code(x.dtype), batch, tokens, width, rot,
                                              int(transposed), _raw_stream(x.device)))
@@ -805,7 +805,7 @@ def block_append(struct: _lib.BlockCache, k: torch.Tensor, v: torch.Tensor, *, c
 def block_read(struct: _lib.BlockCache, start: int, stop: int, *, dtype: torch.dtype, device: torch.device):
     """Values of tokens [start, stop) of every sequence -> k, v [batch, stop - start, kv_heads, width] (nkv_block_read)."""
     shape = (struct.batch, max(0, stop - start), struct.kv_heads, struct.head_dim)
-    k, v = (torch.empty(shape, dtype=dtype, device=device) for _ in range(2))
+    k, v = torch.empty((2, *shape), dtype=dtype, device=device).unbind(0)
     _lib.check(_lib.library().nkv_block_read(struct, start, stop, k.data_ptr(), v.data_ptr(), _raw_stream(device)))
     return k, v
 
@@ -817,8 +817,8 @@ def block_attend(struct: _lib.BlockCache, q: torch.Tensor, *, counts=None, causa
     rows = _rows(q, "q")
     lib = _lib.library()
     tokens, heads = q.shape[1], q.shape[2]
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = q.new_empty(q.shape[:3], dtype=torch.float32)
     nbytes = lib.nkv_block_attend_workspace_bytes(struct, heads, tokens, counts, int(causal), int(weights is not None))
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     _lib.check(lib.nkv_block_attend(struct, rows, tokens, counts, int(causal), float(scale), _ptr(out), _ptr(lse), _ptr(weights),
