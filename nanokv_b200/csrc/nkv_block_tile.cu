@@ -53,6 +53,7 @@ template <int D> struct Layout {
   static constexpr int BYTES = RAW_OFF + RAWS * RAW;
   static constexpr int DYNAMIC = BYTES + 1024;     // room to start on 1,024 bytes
 };
+static_assert(STAGES == 2, "the MMA warp's stages are told by a bit");
 static_assert(M_SCALES + NMETA * 2 * 16 <= 1024, "meta block");
 
 // The list of tiles: sequence by sequence, kv head by kv head, unit by unit.
@@ -153,6 +154,18 @@ constexpr int MOST_PARKED = 1 << 20;
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, const Ctx& c, int code) {
   if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity) ? 1 : 0)) return true;
   bool ok = false;
+#pragma unroll 1
+  for (int n = 0; n < MOST_PARKED && !ok; ++n) {
+    ok = mbar_try_wait_parked(bar, parity, 1000u);
+    if (*c.abort_flag) break;
+  }
+  if (!ok) atomicCAS(const_cast<int*>(c.abort_flag), 0, code);
+  return __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
+}
+// The same for two or three barriers at once, a lane each: one trip to shared memory instead of three.
+__device__ __forceinline__ bool wait_lanes(uint64_t* bar, uint32_t parity, bool want, const Ctx& c, int code) {
+  bool ok = !want || mbar_try_wait(bar, parity);
+  if (__all_sync(0xffffffffu, ok ? 1 : 0)) return true;
 #pragma unroll 1
   for (int n = 0; n < MOST_PARKED && !ok; ++n) {
     ok = mbar_try_wait_parked(bar, parity, 1000u);
@@ -458,7 +471,7 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
 }
 
 // ---- warp 12: MMA issue -----------------------------------------------------------------------------------------
-template <int DT, int D>
+template <int DT, int D, bool IMAGES>
 __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t tmem, const Call& a, const Sequences& seqs,
                                          const Plan& plan, const Ctx& ctx, int kv_heads) {
   using L = Layout<D>;
@@ -468,8 +481,8 @@ __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t
   // operand descriptors of the first tile and stage; the others lie a whole number of 16-byte units on
   const uint64_t q_desc = make_smem_desc_sw128(base + L::Q_OFF), k_desc = make_smem_desc_sw128(base + L::K_OFF);
   const uint64_t v_desc = make_smem_desc_sw128(base + L::V_OFF);
-  auto issue_s = [&](int i, int stage) {
-    const uint64_t qd = q_desc + static_cast<uint32_t>(i * (DCH * SUB / 16)), kd = k_desc + static_cast<uint32_t>(stage * (DCH * SUB / 16));
+  auto issue_s = [&](int i, uint32_t stage) {
+    const uint64_t qd = q_desc + static_cast<uint32_t>(i * (DCH * SUB / 16)), kd = k_desc + stage * static_cast<uint32_t>(DCH * SUB / 16);
     const uint32_t d = tmem + i * 128;
 #pragma unroll
     for (int ch = 0; ch < DCH; ++ch)
@@ -479,8 +492,8 @@ __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t
     if (leader) mma_commit(&bars[S_FULL + i]);
   };
   // weights of 64 tokens (a block) times V of it: [128 rows x 64] [D x 64]^T, both with the tokens running along rows
-  auto issue_pv = [&](int i, int stage, int half, bool accumulate) {
-    const uint64_t vd = v_desc + static_cast<uint32_t>((stage * 2 + half) * (L::V_SUB / 16));
+  auto issue_pv = [&](int i, uint32_t stage, int half, bool accumulate) {
+    const uint64_t vd = v_desc + (stage * 2 + half) * static_cast<uint32_t>(L::V_SUB / 16);
     const uint32_t d = tmem + 256 + i * 128, w = tmem + i * 128 + half * 32;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -490,7 +503,9 @@ __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t
   Walk walk(plan, a, seqs, blockIdx.x, kv_heads);
   Piece p;
   bool ok = true;
-  int seq = 0, pieces = 0, done[NQ] = {0, 0}, used[NQ] = {0, 0};   // tiles and pieces of each query tile so far
+  const uint32_t lane = threadIdx.x & 31;
+  uint32_t seq = 0;
+  int pieces = 0, done[NQ] = {0, 0}, used[NQ] = {0, 0};   // tiles and pieces of each query tile so far
   while (ok && walk.next(plan, a, seqs, kv_heads, p)) {
     const int n[NQ] = {tiles_for(a, seqs, p, 0), tiles_for(a, seqs, p, 1)};
     const int longest = max(n[0], n[1]);
@@ -501,10 +516,43 @@ __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t
     auto last_of = [&](int t) { return t < n[1] ? 1 : 0; };
 #pragma unroll 1
     for (int t = 0; t <= longest && ok; ++t) {
-      // PV of tile t - 1 and S of tile t, query tile by query tile
-      const int now = (seq + t - 1) % STAGES, next = (seq + t) % STAGES;
+      // PV of tile t - 1 and S of tile t, query tile by query tile.  Between the first and the last tiles that both take part in
+      // there is nothing to decide, and what the codes' arrival allows is waited for with the first weights.
+#pragma unroll 1
+      for (; t > 1 && t < min(n[0], n[1]); ++t) {
+        const uint32_t now = (seq + t - 1) & 1, next = now ^ 1, now_phase = (seq + t - 1) >> 1 & 1, next_phase = (seq + t) >> 1 & 1;
+        const uint32_t phase0 = (done[0] + t - 1) & 1, phase1 = (done[1] + t - 1) & 1;
+        uint64_t* const bar = &bars[lane == 0 ? P_READY : lane == 1 ? V_FULL + now : K_FULL + next];
+        ok = wait_lanes(bar, lane == 0 ? phase0 : lane == 1 ? now_phase : next_phase, lane < (IMAGES ? 3u : 2u), ctx, 981);
+        if (!ok) break;
+        tc_fence_after();
+        issue_pv(0, now, 0, true);
+        ok = wait(&bars[P_READY + 1], phase0, ctx, 984);
+        if (!ok) break;
+        tc_fence_after();
+        issue_pv(0, now, 1, true);
+        if (!IMAGES) {   // K is converted just ahead of its use
+          ok = wait(&bars[K_FULL + next], next_phase, ctx, 985);
+          if (!ok) break;
+          tc_fence_after();
+        }
+        issue_s(0, next);
+        ok = wait(&bars[P_READY + 2], phase1, ctx, 981);
+        if (!ok) break;
+        tc_fence_after();
+        issue_pv(1, now, 0, true);
+        ok = wait(&bars[P_READY + 3], phase1, ctx, 984);
+        if (!ok) break;
+        tc_fence_after();
+        issue_pv(1, now, 1, true);
+        if (leader) mma_commit(&bars[V_FREE + now]);
+        issue_s(1, next);
+        if (leader) mma_commit(&bars[K_FREE + next]);
+      }
+      if (!ok) break;
+      const uint32_t now = (seq + t - 1) % STAGES, next = (seq + t) % STAGES;
       const uint32_t now_phase = ((seq + t - 1) / STAGES) & 1, next_phase = ((seq + t) / STAGES) & 1;
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < NQ; ++i) {
         const int tiles = i ? n[1] : n[0];
         if (t > 0 && t - 1 < tiles) {
@@ -782,7 +830,7 @@ tile_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
   if (warp < SOFTMAX_WARPS) softmax_role<DT, D>(smem, bars, tmem, a, seqs, plan, parts, ctx, c.kv_heads);
   else if (warp < SOFTMAX_WARPS + OPERAND_WARPS) operand_role<DT, D, IMAGES>(smem, bars, c, a, seqs, plan, ctx);
   else if (warp > MMA_WARP) codes_role<D, IMAGES>(smem, bars, c, a, seqs, plan, ctx, images);
-  else mma_role<DT, D>(smem, bars, tmem, a, seqs, plan, ctx, c.kv_heads);
+  else mma_role<DT, D, IMAGES>(smem, bars, tmem, a, seqs, plan, ctx, c.kv_heads);
   tc_fence_before();
   __syncthreads();
   if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
