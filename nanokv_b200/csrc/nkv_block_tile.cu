@@ -56,12 +56,18 @@ template <int D> struct Layout {
 static_assert(STAGES == 2, "the MMA warp's stages are told by a bit");
 static_assert(M_SCALES + NMETA * 2 * 16 <= 1024, "meta block");
 
-// The list of tiles: sequence by sequence, kv head by kv head, unit by unit.
+// A unit costs a run as much as PIECE_TILES tiles on top of its own: its queries' way in, the first softmax with nothing beside it,
+// its rows' way out.  Causal units of a prompt's start have few tiles, and runs of equally many tiles would take up to twenty of them
+// or three.  (2 x 4,095 queries x 32 heads of their own tokens: @@)
+constexpr uint32_t PIECE_TILES = 3;
+__host__ __device__ inline uint32_t cost_of(int tiles) { return tiles > 0 ? tiles + PIECE_TILES : 0; }
+
+// The list of tiles: sequence by sequence, kv head by kv head, unit by unit, with PIECE_TILES places ahead of a unit's.
 struct Plan {
   uint32_t start[MAX_SEQUENCES + 1];
   int sequences, runs, units;      // runs: thread blocks; units per kv head
   int most_tiles;                  // of any sequence: the images of a head
-  uint32_t run, longer;            // tiles of a run; the first `longer` have one more
+  uint32_t run, longer;            // places of a run; the first `longer` have one more
   __host__ __device__ uint32_t first_of(uint32_t i) const { return i * run + min(i, longer); }
   __host__ __device__ uint32_t run_of(uint32_t g) const {
     const uint32_t edge = longer * (run + 1);
@@ -86,7 +92,7 @@ struct Piece {                     // a unit, or a run's part of one
 struct Walk {
   uint32_t g, end;
   int b, h, unit, tiles;           // the unit that g lies in, its tiles
-  uint32_t at;                     // tiles of the unit before g
+  uint32_t at;                     // places of the unit before g
   __device__ __forceinline__ int tiles_of(const Call& a, const Sequences& s, int bb, int u) const {
     return tiles_seen(s.length[bb], s.count[bb], a.group, a.rows, a.causal, u * UNIT, UNIT);
   }
@@ -104,32 +110,37 @@ struct Walk {
     h = static_cast<int>(at / per_head);
     at -= h * per_head;
     unit = 0;
-    while (at >= static_cast<uint32_t>(tiles = tiles_of(a, s, b, unit))) {
-      at -= tiles;
+    while (at >= cost_of(tiles = tiles_of(a, s, b, unit))) {
+      at -= cost_of(tiles);
       ++unit;
     }
   }
   __device__ __forceinline__ bool next(const Plan& p, const Call& a, const Sequences& s, int kv_heads, Piece& out) {
-    if (g >= end) return false;
-    while (at >= static_cast<uint32_t>(tiles)) {   // on to the next unit that has tiles
-      at = 0;
-      if (++unit == p.units) {
-        unit = 0;
-        if (++h == kv_heads) {
-          h = 0;
-          ++b;
+    uint32_t from, to;
+    do {
+      if (g >= end) return false;
+      while (at >= cost_of(tiles)) {   // on to the next unit that has tiles
+        at = 0;
+        if (++unit == p.units) {
+          unit = 0;
+          if (++h == kv_heads) {
+            h = 0;
+            ++b;
+          }
         }
+        tiles = tiles_of(a, s, b, unit);
       }
-      tiles = tiles_of(a, s, b, unit);
-    }
+      from = at;
+      to = min(cost_of(tiles), at + (end - g));
+      g += to - from;
+      at = to;
+    } while (to <= PIECE_TILES);     // (the run's end, ahead of the unit's tiles)
     out.b = b;
     out.h = h;
     out.unit = unit;
-    out.tile0 = static_cast<int>(at);
-    out.nt = static_cast<int>(min(static_cast<uint32_t>(tiles) - at, end - g));
+    out.tile0 = static_cast<int>(max(from, PIECE_TILES) - PIECE_TILES);
+    out.nt = static_cast<int>(to - PIECE_TILES) - out.tile0;
     out.whole = out.nt == tiles;
-    at += out.nt;
-    g += out.nt;
     return true;
   }
 };
@@ -900,10 +911,10 @@ join_units_kernel(Call a, const __grid_constant__ Sequences seqs, const __grid_c
     if (threadIdx.x == 0) before = 0;
     __syncthreads();
     uint32_t mine = 0;
-    for (int u = threadIdx.x; u < unit; u += 256) mine += tiles_of(u);
+    for (int u = threadIdx.x; u < unit; u += 256) mine += cost_of(tiles_of(u));
     if (mine) atomicAdd(&before, mine);
     __syncthreads();
-    begin = plan.start[b] + h * ((plan.start[b + 1] - plan.start[b]) / kv_heads) + before;
+    begin = plan.start[b] + h * ((plan.start[b + 1] - plan.start[b]) / kv_heads) + before + PIECE_TILES;
     r0 = plan.run_of(begin);
     r1 = plan.run_of(begin + nt - 1);
     if (r0 == r1) return;   // one run had all of it and wrote the results
@@ -953,7 +964,7 @@ Plan plan_of(const Sequences& seqs, int n, int kv_heads, int group, int rows, bo
     p.start[i] = static_cast<uint32_t>(total);
     p.most_tiles = max(p.most_tiles, ceil_div(seqs.length[i], TOK));
     uint64_t tiles = 0;
-    for (int u = 0; u < p.units; ++u) tiles += tiles_seen(seqs.length[i], seqs.count[i], group, rows, causal, u * UNIT, UNIT);
+    for (int u = 0; u < p.units; ++u) tiles += cost_of(tiles_seen(seqs.length[i], seqs.count[i], group, rows, causal, u * UNIT, UNIT));
     total += tiles * kv_heads;
   }
   p.start[n] = static_cast<uint32_t>(total);
