@@ -110,7 +110,7 @@ int block_step(const BlockArrays& c, const Call& a, const Sequences& seqs, int n
                cudaStream_t stream);
 
 // many rows per kv head (nkv_block_tile.cu)
-size_t block_tile_bytes(const Sequences& seqs, int n, int kv_heads, int most_blocks, int rows, int d);
+size_t block_tile_bytes(int d);
 int block_tile(const BlockArrays& c, const Call& a, const Sequences& seqs, int n, int dtype, int d, void* workspace, int32_t* status,
                cudaStream_t stream);
 

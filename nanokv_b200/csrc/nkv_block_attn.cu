@@ -155,7 +155,7 @@ Scratch scratch_of(const nkv_block_cache& c, const Sequences& seqs, int n, int g
   if (with_weights) s.partial = (static_cast<size_t>(n) * c.kv_heads * most_blocks * rows * 4 + 255) & ~static_cast<size_t>(255);
   if (!simt_forced())
     s.own = block_step_supported(rows, c.head_dim) ? block_step_bytes(seqs, n, c.kv_heads, rows, c.head_dim)
-                                       : block_tile_bytes(seqs, n, c.kv_heads, most_blocks, rows, c.head_dim);
+                                       : block_tile_bytes(c.head_dim);
   return s;
 }
 

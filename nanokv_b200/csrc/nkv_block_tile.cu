@@ -9,10 +9,6 @@
 // s + log2 vs, so that a row's weights are at most 1 (2^8 with the lazy reference) however unlike the scales of its blocks are; a block's
 // part of the row sum is the sum of its P' divided by vs again, in fp32.
 //
-// Expanding a tile costs about as much as attending it once.  Heads with many units (from UNITS_FOR_IMAGES on) have their tiles
-// expanded once by a kernel of its own, as operand images in scratch memory that a bulk copy brings to where the tensor
-// cores read them; the scratch is kept small enough for L2 and the heads are taken in batches that fit it.
-//
 // The tiles of all units form one list that the SMs take in equal runs; a unit that a run's end cuts leaves fp32 parts,
 // joined by a second launch.  Warps: 0-7 softmax, 8-11 operands, 12 MMA issue, 13 codes.
 #include "nkv_block.cuh"
@@ -30,9 +26,6 @@ constexpr int STAGES = 2;                         // K / V operand stages
 constexpr int SOFTMAX_WARPS = 8, OPERAND_WARPS = 4, MMA_WARP = 12, THREADS = 448;
 constexpr int SUB = 128 * 128;                    // bytes of a [128 rows x 64 elements] swizzled operand tile
 constexpr float RESCALE_THRESHOLD = 8.0f;
-// log2(1 + 2^-9) and its factor's inverse: bf16 weights are rounded by raising them half a step (in the exponent) and
-// dropping the low bits, which leaves the quarter-rate conversion unit to the exponentials
-constexpr float HALF_STEP_LOG2 = 0.0028150156070540f, HALF_STEP_INV = 0.998050682261209f;
 
 // (P_READY: query tile i, half h of its tokens at 2 i + h)
 enum Bar { Q_FULL = 0, Q_FREE = 1, K_FULL = 2, K_FREE = 4, V_FULL = 6, V_FREE = 8, S_FULL = 10, P_READY = 12, PV_HALF = 16,
@@ -66,7 +59,7 @@ __host__ __device__ inline uint32_t cost_of(int tiles) { return tiles > 0 ? tile
 struct Plan {
   uint32_t start[MAX_SEQUENCES + 1];
   int sequences, runs, units;      // runs: thread blocks; units per kv head
-  int most_tiles;                  // of any sequence: the images of a head
+  bool fits;                       // places are counted in 32 bits
   uint32_t run, longer;            // places of a run; the first `longer` have one more
   __host__ __device__ uint32_t first_of(uint32_t i) const { return i * run + min(i, longer); }
   __host__ __device__ uint32_t run_of(uint32_t g) const {
@@ -173,8 +166,8 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, const Ctx& 
   if (!ok) atomicCAS(const_cast<int*>(c.abort_flag), 0, code);
   return __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
 }
-// The same for two or three barriers at once, a lane each: one trip to shared memory instead of three.
-__device__ __forceinline__ bool wait_lanes(uint64_t* bar, uint32_t parity, bool want, const Ctx& c, int code) {
+// The same for two barriers at once, a lane each: one trip to shared memory instead of two.
+__device__ __forceinline__ bool wait_both(uint64_t* bar, uint32_t parity, bool want, const Ctx& c, int code) {
   bool ok = !want || mbar_try_wait(bar, parity);
   if (__all_sync(0xffffffffu, ok ? 1 : 0)) return true;
 #pragma unroll 1
@@ -268,9 +261,9 @@ __device__ __forceinline__ float max32(const uint32_t (&r)[32]) {
 }
 
 // ---- warp 13: codes and scales ---------------------------------------------------------------------------------
-template <int D, bool IMAGES>
+template <int D>
 __device__ __forceinline__ void codes_role(uint8_t* smem, uint64_t* bars, const BlockArrays& c, const Call& a, const Sequences& seqs,
-                                           const Plan& plan, const Ctx& ctx, const uint8_t* images) {
+                                           const Plan& plan, const Ctx& ctx) {
   using L = Layout<D>;
   constexpr uint32_t BLOCK_BYTES = NKV_BLOCK * D;
   const int lane = threadIdx.x & 31;
@@ -300,21 +293,6 @@ __device__ __forceinline__ void codes_role(uint8_t* smem, uint64_t* bars, const 
         scales[(seq % NMETA) * 2 + (lane & 1)] = make_float4(sc.x == 0.f ? 1.f : sc.x, lv, exp2f(-lv), 0.f);
       }
       __syncwarp();   // ahead of the request whose completion lets S be computed
-      if (IMAGES) {
-        const int stage = seq % STAGES, use = seq / STAGES;
-        constexpr uint32_t BYTES = L::DCH * SUB;   // (as many for K as for V)
-        const uint8_t* const from = images + ((bh * plan.most_tiles + p.tile0 + t) * 2) * static_cast<size_t>(BYTES);
-        for (int tensor = 0; tensor < 2 && ok; ++tensor) {
-          uint64_t* const full_bar = &bars[(tensor ? V_FULL : K_FULL) + stage];
-          if (use >= 1) ok = wait(&bars[(tensor ? V_FREE : K_FREE) + stage], (use - 1) & 1, ctx, 976);
-          if (ok && lane == 0) {
-            mbar_arrive_expect_tx(full_bar, BYTES);
-            bulk_load_1d(smem + (tensor ? L::V_OFF : L::K_OFF) + stage * BYTES, from + tensor * BYTES, BYTES, full_bar);
-          }
-          __syncwarp();
-        }
-        continue;
-      }
       const long long s0 = __shfl_sync(0xffffffffu, slot, at), s1 = __shfl_sync(0xffffffffu, slot, at + 1);
       const uint32_t blocks = min(2, max(0, full - block0));   // full ones: the open block is read where it is needed
       for (int tensor = 0; tensor < 2 && ok; ++tensor, ++item) {
@@ -339,7 +317,7 @@ __device__ __forceinline__ void codes_role(uint8_t* smem, uint64_t* bars, const 
 }
 
 // ---- warps 8-11: queries, K and V as operands -----------------------------------------------------------------
-template <int DT, int D, bool IMAGES>
+template <int DT, int D>
 __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, const BlockArrays& c, const Call& a, const Sequences& seqs,
                                              const Plan& plan, const Ctx& ctx) {
   using L = Layout<D>;
@@ -463,7 +441,7 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
     warp_arrive(&bars[Q_FULL], lane);
     // ---- tiles: K, then V
 #pragma unroll 1
-    for (int t = 0; t < (IMAGES ? 0 : 2 * p.nt) && ok; ++t) {
+    for (int t = 0; t < 2 * p.nt && ok; ++t) {
       const int value = t & 1, stage = seq % STAGES, use = seq / STAGES;
       ok = wait(&bars[RAW_FULL + item % L::RAWS], (item / L::RAWS) & 1, ctx, 971);
       if (ok && use >= 1) ok = wait(&bars[(value ? V_FREE : K_FREE) + stage], (use - 1) & 1, ctx, 972 + value);
@@ -482,7 +460,7 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
 }
 
 // ---- warp 12: MMA issue -----------------------------------------------------------------------------------------
-template <int DT, int D, bool IMAGES>
+template <int DT, int D>
 __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t tmem, const Call& a, const Sequences& seqs,
                                          const Plan& plan, const Ctx& ctx, int kv_heads) {
   using L = Layout<D>;
@@ -528,13 +506,12 @@ __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t
 #pragma unroll 1
     for (int t = 0; t <= longest && ok; ++t) {
       // PV of tile t - 1 and S of tile t, query tile by query tile.  Between the first and the last tiles that both take part in
-      // there is nothing to decide, and what the codes' arrival allows is waited for with the first weights.
+      // there is nothing to decide, and V is waited for with the first weights.
 #pragma unroll 1
       for (; t > 1 && t < min(n[0], n[1]); ++t) {
         const uint32_t now = (seq + t - 1) & 1, next = now ^ 1, now_phase = (seq + t - 1) >> 1 & 1, next_phase = (seq + t) >> 1 & 1;
         const uint32_t phase0 = (done[0] + t - 1) & 1, phase1 = (done[1] + t - 1) & 1;
-        uint64_t* const bar = &bars[lane == 0 ? P_READY : lane == 1 ? V_FULL + now : K_FULL + next];
-        ok = wait_lanes(bar, lane == 0 ? phase0 : lane == 1 ? now_phase : next_phase, lane < (IMAGES ? 3u : 2u), ctx, 981);
+        ok = wait_both(lane == 0 ? &bars[P_READY] : &bars[V_FULL + now], lane == 0 ? phase0 : now_phase, lane < 2, ctx, 981);
         if (!ok) break;
         tc_fence_after();
         issue_pv(0, now, 0, true);
@@ -542,11 +519,9 @@ __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t
         if (!ok) break;
         tc_fence_after();
         issue_pv(0, now, 1, true);
-        if (!IMAGES) {   // K is converted just ahead of its use
-          ok = wait(&bars[K_FULL + next], next_phase, ctx, 985);
-          if (!ok) break;
-          tc_fence_after();
-        }
+        ok = wait(&bars[K_FULL + next], next_phase, ctx, 985);   // (converted just ahead of its use)
+        if (!ok) break;
+        tc_fence_after();
         issue_s(0, next);
         ok = wait(&bars[P_READY + 2], phase1, ctx, 981);
         if (!ok) break;
@@ -619,7 +594,6 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
   const uint32_t o_addr = tmem + lane_sel + 256 + wg * 128;
   const float4* const scales = reinterpret_cast<const float4*>(smem + M_SCALES);
   const float scale = fabsf(a.scale_log2);
-  constexpr float RAISE = DT == NKV_BF16 ? HALF_STEP_LOG2 : 0.f, LOWER = DT == NKV_BF16 ? HALF_STEP_INV : 1.f;
   Walk walk(plan, a, seqs, blockIdx.x, kv_heads);
   Piece p;
   bool ok = true, more = true;
@@ -687,7 +661,7 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       }
       // One pass over the scores: eight at a time, exponentials of group b, arguments of b + 1, sums and packing of b - 1.  P'
       // (16-bit pairs) replaces S, the first half's of the first columns.
-      const float ref = m == -INFINITY ? 0.f : m, off = sc.y - ref + RAISE;
+      const float ref = m == -INFINITY ? 0.f : m, off = sc.y - ref;
       const uint64_t scale2 = pair_f32(f, f), off2 = pair_f32(off, off);
       uint64_t sum2[2] = {0ull, 0ull};
       uint32_t packed[16];
@@ -712,7 +686,7 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
         for (int i = 0; i < 4; ++i) {
           const float lo = w[b & 1][2 * i], hi = w[b & 1][2 * i + 1];
           sum2[i & 1] = add_f32x2(sum2[i & 1], pair_f32(lo, hi));
-          packed[(b & 3) * 4 + i] = DT == NKV_BF16 ? __byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632) : pack2<NKV_F16>(lo, hi);
+          packed[(b & 3) * 4 + i] = pack2<DT>(lo, hi);
         }
         if ((b & 3) == 3) tmem_st16(p_addr + (b >> 2) * 16, packed);
       };
@@ -729,7 +703,7 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       warp_arrive(&bars[P_READY + 2 * wg + half], lane);
       float lo, hi;
       split_f32(add_f32x2(sum2[0], sum2[1]), lo, hi);
-      const float sum = (lo + hi) * LOWER;
+      const float sum = lo + hi;
       l = fmaf(sum, sc.z, l);
       if (a.partial && r < a.rows && block < a.most_blocks) a.partial[(bh * a.most_blocks + block) * a.rows + r] = log2f(sum) + (ref - sc.y);
       ci += half;
@@ -798,10 +772,9 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
   }
 }
 
-template <int DT, int D, bool IMAGES>
+template <int DT, int D>
 __global__ void __launch_bounds__(THREADS, 1)
-tile_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const __grid_constant__ Plan plan, Parts parts, const uint8_t* images,
-            int32_t* status) {
+tile_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const __grid_constant__ Plan plan, Parts parts, int32_t* status) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem);
@@ -812,9 +785,9 @@ tile_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
     mbar_init(&bars[Q_FULL], OPERAND_WARPS);
     mbar_init(&bars[Q_FREE], 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars[K_FULL + i], IMAGES ? 1 : OPERAND_WARPS);
+      mbar_init(&bars[K_FULL + i], OPERAND_WARPS);
       mbar_init(&bars[K_FREE + i], 1);
-      mbar_init(&bars[V_FULL + i], IMAGES ? 1 : OPERAND_WARPS);
+      mbar_init(&bars[V_FULL + i], OPERAND_WARPS);
       mbar_init(&bars[V_FREE + i], 1);
       mbar_init(&bars[S_FULL + i], 1);
       mbar_init(&bars[PV_HALF + i], 1);
@@ -836,63 +809,15 @@ tile_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   const Ctx ctx{abort_flag};
-  if (IMAGES) asm volatile("griddepcontrol.wait;" ::: "memory");   // the images are written by the launch before
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp < SOFTMAX_WARPS) softmax_role<DT, D>(smem, bars, tmem, a, seqs, plan, parts, ctx, c.kv_heads);
-  else if (warp < SOFTMAX_WARPS + OPERAND_WARPS) operand_role<DT, D, IMAGES>(smem, bars, c, a, seqs, plan, ctx);
-  else if (warp > MMA_WARP) codes_role<D, IMAGES>(smem, bars, c, a, seqs, plan, ctx, images);
-  else mma_role<DT, D, IMAGES>(smem, bars, tmem, a, seqs, plan, ctx, c.kv_heads);
+  else if (warp < SOFTMAX_WARPS + OPERAND_WARPS) operand_role<DT, D>(smem, bars, c, a, seqs, plan, ctx);
+  else if (warp > MMA_WARP) codes_role<D>(smem, bars, c, a, seqs, plan, ctx);
+  else mma_role<DT, D>(smem, bars, tmem, a, seqs, plan, ctx, c.kv_heads);
   tc_fence_before();
   __syncthreads();
   if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
   if (threadIdx.x == 0 && *abort_flag) atomicCAS(status, 0, *abort_flag);
-}
-
-// Tiles of all heads as operand images: [head][tile][K, V] of DCH * SUB bytes, laid out as the tensor cores read them from shared
-// memory.  A thread block per tile and tensor; a thread stores eight elements of an operand row at a time.  Bound: memory, three
-// bytes a code.
-template <int DT, int D>
-__global__ void __launch_bounds__(256)
-expand_kernel(BlockArrays c, const __grid_constant__ Sequences seqs, int most_tiles, uint8_t* images) {
-  using L = Layout<D>;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int tile = blockIdx.x >> 1, tensor = blockIdx.x & 1, h = blockIdx.y, b = blockIdx.z;
-  const int length = seqs.length[b], full = length / NKV_BLOCK, held = length - full * NKV_BLOCK;
-  if (tile * TOK >= length) return;
-  const size_t bh = static_cast<size_t>(b) * c.kv_heads + h;
-  constexpr uint32_t BYTES = L::DCH * SUB;
-  uint8_t* const to = images + ((bh * most_tiles + tile) * 2 + tensor) * static_cast<size_t>(BYTES);
-  // the launch before may still read these images
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int block = 2 * tile + j;
-    const uint8_t* codes = nullptr;
-    if (block < full) codes = (tensor ? c.v_codes : c.k_codes) + slot_of(c, bh, block) * (NKV_BLOCK * D);
-    const uint16_t* const tail = static_cast<const uint16_t*>(tensor ? c.v_tail : c.k_tail) + bh * NKV_BLOCK * D;
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      const int at = (i * 256 + threadIdx.x) * 8;       // element of the block: [64][D] of K, [D][64] of V
-      const int row = tensor ? at / NKV_BLOCK : at / D, col = tensor ? at % NKV_BLOCK : at % D;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (codes != nullptr) {
-        const uint2 raw = __ldg(reinterpret_cast<const uint2*>(codes + at));
-        expand<DT>(raw.x, v.x, v.y);
-        expand<DT>(raw.y, v.z, v.w);
-      } else if (block == full) {   // values behind the last token count as zero: a weight of 0 times anything else might be NaN
-        const int left = tensor ? held - col : row < held ? 8 : 0;
-        if (left > 0) {
-          v = *reinterpret_cast<const uint4*>(tail + at);
-          uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] &= left > 2 * e + 1 ? 0xFFFFFFFFu : left > 2 * e ? 0xFFFFu : 0u;
-          v = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
-      const uint32_t place = tensor ? j * L::V_SUB + sw128_offset(row, col) : (col / 64) * SUB + sw128_offset(j * NKV_BLOCK + row, col % 64);
-      *reinterpret_cast<uint4*>(to + place) = v;
-    }
-  }
 }
 
 // Joins the parts of cut units and fills the rows of units that see nothing; a thread block per (unit, kv head,
@@ -958,16 +883,15 @@ Plan plan_of(const Sequences& seqs, int n, int kv_heads, int group, int rows, bo
   Plan p;
   p.sequences = n;
   p.units = ceil_div(rows, UNIT);
-  p.most_tiles = 0;
   uint64_t total = 0;
   for (int i = 0; i < n; ++i) {
     p.start[i] = static_cast<uint32_t>(total);
-    p.most_tiles = max(p.most_tiles, ceil_div(seqs.length[i], TOK));
     uint64_t tiles = 0;
     for (int u = 0; u < p.units; ++u) tiles += cost_of(tiles_seen(seqs.length[i], seqs.count[i], group, rows, causal, u * UNIT, UNIT));
     total += tiles * kv_heads;
   }
   p.start[n] = static_cast<uint32_t>(total);
+  p.fits = total <= UINT32_MAX;
   p.runs = static_cast<int>(min(total, static_cast<uint64_t>(sm_count())));
   p.run = p.runs ? static_cast<uint32_t>(total / p.runs) : 0;
   p.longer = p.runs ? static_cast<uint32_t>(total % p.runs) : 0;
@@ -975,112 +899,44 @@ Plan plan_of(const Sequences& seqs, int n, int kv_heads, int group, int rows, bo
 }
 
 
-// From this many units per kv head on a tile is expanded once for all of them.  A tile attended with its conversion costs an SM 2.4
-// us, without 1.8, and its image about 2 us of the memory's time (D 128).
-constexpr int UNITS_FOR_IMAGES = 4;
-constexpr size_t IMAGE_BYTES = static_cast<size_t>(64) << 20;   // scratch for images, one head at least
-
-size_t head_image_bytes(int most_blocks, int d) { return static_cast<size_t>((most_blocks + 1) / 2) * 2 * TOK * d * 2; }
 size_t part_bytes(int runs, int d) { return static_cast<size_t>(runs) * 2 * UNIT * (d + 2) * sizeof(float); }
 
-// one launch: sequences and heads as they are given
-int launch(const BlockArrays& c, const Call& a, const Sequences& seqs, int n, int dtype, int d, void* workspace, bool images, int32_t* status,
-           cudaStream_t stream) {
+}  // namespace
+
+size_t block_tile_bytes(int d) { return part_bytes(sm_count(), d); }
+
+int block_tile(const BlockArrays& c, const Call& a, const Sequences& seqs, int n, int dtype, int d, void* workspace, int32_t* status,
+               cudaStream_t stream) {
   const Plan plan = plan_of(seqs, n, c.kv_heads, a.group, a.rows, a.causal);
+  NKV_REQUIRE(plan.fits, NKV_ERR_TOO_LARGE, "block_attend: more tiles of %d x %d than 32 bits count", UNIT, TOK);
   Parts parts;
   parts.o = static_cast<float*>(workspace);
   parts.ml = reinterpret_cast<float2*>(parts.o + static_cast<size_t>(plan.runs) * 2 * UNIT * d);
-  uint8_t* const image = static_cast<uint8_t*>(workspace) + part_bytes(sm_count(), d);
   const bool bf16 = dtype == NKV_BF16, wide = d == 128;
+  if (plan.runs > 0) {
+    auto run = [&](auto kernel, int smem) {
+      NKV_CUDA(allow_shared(reinterpret_cast<const void*>(kernel), smem));
+      kernel<<<plan.runs, THREADS, smem, stream>>>(c, a, seqs, plan, parts, status);
+      NKV_CUDA(cudaGetLastError());
+      return NKV_OK;
+    };
+    const int rc = wide ? (bf16 ? run(tile_kernel<NKV_BF16, 128>, Layout<128>::DYNAMIC) : run(tile_kernel<NKV_F16, 128>, Layout<128>::DYNAMIC))
+                        : (bf16 ? run(tile_kernel<NKV_BF16, 64>, Layout<64>::DYNAMIC) : run(tile_kernel<NKV_F16, 64>, Layout<64>::DYNAMIC));
+    if (rc != NKV_OK) return rc;
+  }
   cudaLaunchAttribute attribute;
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config = {};
-  config.stream = stream;
-  config.attrs = &attribute;
-  if (plan.runs > 0) {
-    if (images) {
-      config.gridDim = dim3(2 * plan.most_tiles, c.kv_heads, n);
-      config.blockDim = dim3(256);
-      config.numAttrs = 1;
-      auto expand = wide ? (bf16 ? expand_kernel<NKV_BF16, 128> : expand_kernel<NKV_F16, 128>)
-                         : (bf16 ? expand_kernel<NKV_BF16, 64> : expand_kernel<NKV_F16, 64>);
-      NKV_CUDA(cudaLaunchKernelEx(&config, expand, c, seqs, plan.most_tiles, image));
-    }
-    auto run = [&](auto kernel, int smem) {
-      NKV_CUDA(allow_shared(reinterpret_cast<const void*>(kernel), smem));
-      config.gridDim = dim3(plan.runs);
-      config.blockDim = dim3(THREADS);
-      config.dynamicSmemBytes = smem;
-      config.numAttrs = images ? 1 : 0;
-      NKV_CUDA(cudaLaunchKernelEx(&config, kernel, c, a, seqs, plan, parts, static_cast<const uint8_t*>(image), status));
-      config.dynamicSmemBytes = 0;
-      return NKV_OK;
-    };
-    int rc;
-    if (images)
-      rc = wide ? (bf16 ? run(tile_kernel<NKV_BF16, 128, true>, Layout<128>::DYNAMIC) : run(tile_kernel<NKV_F16, 128, true>, Layout<128>::DYNAMIC))
-                : (bf16 ? run(tile_kernel<NKV_BF16, 64, true>, Layout<64>::DYNAMIC) : run(tile_kernel<NKV_F16, 64, true>, Layout<64>::DYNAMIC));
-    else
-      rc = wide ? (bf16 ? run(tile_kernel<NKV_BF16, 128, false>, Layout<128>::DYNAMIC) : run(tile_kernel<NKV_F16, 128, false>, Layout<128>::DYNAMIC))
-                : (bf16 ? run(tile_kernel<NKV_BF16, 64, false>, Layout<64>::DYNAMIC) : run(tile_kernel<NKV_F16, 64, false>, Layout<64>::DYNAMIC));
-    if (rc != NKV_OK) return rc;
-  }
   const int slices = 8;
+  cudaLaunchConfig_t config = {};
   config.gridDim = dim3(plan.units * slices, c.kv_heads, n);
   config.blockDim = dim3(256);
+  config.stream = stream;
+  config.attrs = &attribute;
   config.numAttrs = plan.runs > 0 ? 1 : 0;
   auto join = wide ? (bf16 ? join_units_kernel<NKV_BF16, 128> : join_units_kernel<NKV_F16, 128>)
                    : (bf16 ? join_units_kernel<NKV_BF16, 64> : join_units_kernel<NKV_F16, 64>);
   NKV_CUDA(cudaLaunchKernelEx(&config, join, a, seqs, plan, parts, c.kv_heads, slices));
-  return NKV_OK;
-}
-
-}  // namespace
-
-size_t block_tile_bytes(const Sequences& seqs, int n, int kv_heads, int most_blocks, int rows, int d) {
-  size_t bytes = part_bytes(sm_count(), d);
-  if (ceil_div(rows, UNIT) >= UNITS_FOR_IMAGES) {
-    const size_t head = head_image_bytes(most_blocks, d), all = head * kv_heads * n;
-    bytes += all < IMAGE_BYTES ? all : (head > IMAGE_BYTES ? head : IMAGE_BYTES);
-  }
-  return bytes;
-}
-
-int block_tile(const BlockArrays& c, const Call& a, const Sequences& seqs, int n, int dtype, int d, void* workspace, int32_t* status,
-               cudaStream_t stream) {
-  if (ceil_div(a.rows, UNIT) < UNITS_FOR_IMAGES) return launch(c, a, seqs, n, dtype, d, workspace, false, status, stream);
-  // as many whole sequences as the scratch holds; of a sequence that does not fit, as many heads
-  const size_t head = head_image_bytes(a.most_blocks, d);
-  const int heads = head ? static_cast<int>(min(static_cast<size_t>(c.kv_heads) * n, IMAGE_BYTES / head > 0 ? IMAGE_BYTES / head : 1)) : c.kv_heads * n;
-  const int together = heads / c.kv_heads;
-  const size_t block = static_cast<size_t>(NKV_BLOCK) * d;
-  for (int b = 0; b < n; b += max(1, together)) {
-    const int count = min(max(1, together), n - b), step = together > 0 ? c.kv_heads : heads;
-    Sequences part;
-    for (int i = 0; i < count; ++i) {
-      part.length[i] = seqs.length[b + i];
-      part.count[i] = seqs.count[b + i];
-    }
-    for (int h = 0; h < c.kv_heads; h += step) {
-      BlockArrays cc = c;
-      Call ca = a;
-      const size_t bh = static_cast<size_t>(b) * c.kv_heads + h;
-      cc.k_codes += bh * c.blocks * block;
-      cc.v_codes += bh * c.blocks * block;
-      cc.scales += bh * c.blocks * 2;
-      cc.table += bh * c.blocks;
-      cc.k_tail = static_cast<uint16_t*>(c.k_tail) + bh * block;
-      cc.v_tail = static_cast<uint16_t*>(c.v_tail) + bh * block;
-      cc.kv_heads = min(step, c.kv_heads - h);
-      ca.q += b * a.q_batch + static_cast<long long>(h) * a.group * a.q_head;
-      ca.out += (static_cast<size_t>(b) * a.tokens * a.heads + static_cast<size_t>(h) * a.group) * d;
-      ca.lse += static_cast<size_t>(b) * a.tokens * a.heads + static_cast<size_t>(h) * a.group;
-      if (a.partial) ca.partial += bh * a.most_blocks * a.rows;
-      const int rc = launch(cc, ca, part, count, dtype, d, workspace, true, status, stream);
-      if (rc != NKV_OK) return rc;
-    }
-  }
   return NKV_OK;
 }
 
