@@ -349,7 +349,7 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
   // tokens).
   auto convert = [&](uint32_t to0, uint32_t to1, uint32_t step, uint32_t first) {
     uint32_t from = base + L::RAW_OFF + (item % L::RAWS) * L::RAW + tid * 16;
-#pragma unroll 1
+#pragma unroll 2
     for (int i = 0; i < LOADS; i += 2) {
       const uint2 a0 = lds64(from + first), a1 = lds64(from + (first ^ 8));
       const uint2 b0 = lds64(from + 2048 + first), b1 = lds64(from + 2048 + (first ^ 8));
@@ -659,45 +659,25 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
         l *= alpha;
         m = m_new;
       }
-      // One pass over the scores: eight at a time, exponentials of group b, arguments of b + 1, sums and packing of b - 1.  P'
-      // (16-bit pairs) replaces S, the first half's of the first columns.
+      // P' (16-bit pairs) replaces S, the first half's of the first columns.  (The compiler interleaves the groups: spelling out
+      // exponentials of one beside arguments and sums of its neighbours changes nothing.)
       const float ref = m == -INFINITY ? 0.f : m, off = sc.y - ref;
       const uint64_t scale2 = pair_f32(f, f), off2 = pair_f32(off, off);
       uint64_t sum2[2] = {0ull, 0ull};
-      uint32_t packed[16];
-      uint64_t arg[2][4];
-      float w[2][8];
-      auto args = [&](int b) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          arg[b & 1][i] = fma_f32x2(pair_bits(raw[b >> 2][(b & 3) * 8 + 2 * i], raw[b >> 2][(b & 3) * 8 + 2 * i + 1]), scale2, off2);
-      };
-      auto exps = [&](int b) {
+      for (int k = 0; k < 2; ++k) {
+        uint32_t packed[16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 16; ++i) {
           float lo, hi;
-          split_f32(arg[b & 1][i], lo, hi);
-          w[b & 1][2 * i] = exp2_fast(lo);
-          w[b & 1][2 * i + 1] = exp2_fast(hi);
-        }
-      };
-      auto finish = [&](int b) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float lo = w[b & 1][2 * i], hi = w[b & 1][2 * i + 1];
+          split_f32(fma_f32x2(pair_bits(raw[k][2 * i], raw[k][2 * i + 1]), scale2, off2), lo, hi);
+          lo = exp2_fast(lo);
+          hi = exp2_fast(hi);
           sum2[i & 1] = add_f32x2(sum2[i & 1], pair_f32(lo, hi));
-          packed[(b & 3) * 4 + i] = pack2<DT>(lo, hi);
+          packed[i] = pack2<DT>(lo, hi);
         }
-        if ((b & 3) == 3) tmem_st16(p_addr + (b >> 2) * 16, packed);
-      };
-      args(0);
-#pragma unroll
-      for (int b = 0; b < 8; ++b) {
-        exps(b);
-        if (b + 1 < 8) args(b + 1);
-        if (b >= 1) finish(b - 1);
+        tmem_st16(p_addr + k * 16, packed);
       }
-      finish(7);
       tmem_wait_st();
       tc_fence_before();
       warp_arrive(&bars[P_READY + 2 * wg + half], lane);
