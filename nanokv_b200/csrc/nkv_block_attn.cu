@@ -94,7 +94,7 @@ attend_plain_kernel(BlockArrays c, Call a, Sequences seqs) {
 
 // weights[block] += sum over rows of 2^(partial - lse), rows in a fixed order: a thread block per WEIGHT_BLOCKS blocks of a kv
 // head, so that a row's lse, scattered over the query heads, is fetched once for all of them.  Bound: memory, four bytes a row and
-// block.
+// block (16 heads of 16,380 rows x 64 blocks: 67 MB, part of it still in L2, in 29 us).
 constexpr int WEIGHT_BLOCKS = 2, WEIGHT_THREADS = 512;
 __global__ void __launch_bounds__(WEIGHT_THREADS)
 block_weights_kernel(BlockArrays c, Call a, Sequences seqs) {

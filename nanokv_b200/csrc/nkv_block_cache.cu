@@ -65,7 +65,8 @@ struct Piece {
 };
 
 // A thread takes two 16-byte pieces whose elements are each other's partners (or two that are only copied).
-// HEADS heads per thread share the table entries; one where the call is short of threads.
+// HEADS heads per thread share the table entries; one where the call is short of threads.  Bound: memory (24,960 tokens x 24
+// heads x 128, interleaved, half of each head turned: 307 MB in and out in 102 us, 6.0 TB/s).
 template <int DT, int HEADS>
 __global__ void __launch_bounds__(256)
 rotary_kernel(RotarySide a, RotarySide b, int batch, int tokens, int d, Rotation rot, int transposed) {
@@ -237,29 +238,40 @@ __device__ __forceinline__ bool not_finite(const uint4& v) {
   return bad;
 }
 
-// Codes (plus 128) of eight elements for a block scale: rint(x / scale), quotient rounded to fp32.  fma(x, inv, 1.5 * 2^23 + 128) is
-// the exact x * inv rounded to an integer, whose low byte is the code; x * inv is within 2 ulp of the quotient, less than 1e-4 at
-// 127, so only pieces with an element that near to a half take the division.  exact: the scale is too small for its
-// reciprocal; such a scale is a subnormal number, a coarse multiple of the maximum / 127, and its codes are clamped.
-__device__ __forceinline__ uint2 codes_of(const float (&x)[8], float scale, float inv, bool exact) {
+// A block's scale as codes_of takes it.  Scales below 1e-20 are lifted by 2^64, and the elements with them, so that no residual
+// falls below the normal numbers.
+struct Quotient {
+  float scale, inv, lift;   // inv: the reciprocal, rounded to nearest; lift: 1 or 2^64
+  __device__ __forceinline__ explicit Quotient(float s) {
+    lift = s < 1e-20f ? 18446744073709551616.f : 1.f;
+    scale = s * lift;
+    inv = __frcp_rn(scale);
+  }
+};
+
+// Codes (plus 128) of eight elements: rint(x / scale), quotient rounded to fp32.  The quotient comes from the reciprocal y by one
+// step of Markstein's division: q = x y, then q + (x - q scale) y with the residual exact.  It is x / scale correctly rounded for
+// every 16-bit x and every scale that is a 16-bit number / 127 (they are few enough to have been compared one by one).  Adding
+// 1.5 * 2^23 + 128 rounds it to an integer, whose low byte is the code.  A subnormal scale is a coarse multiple of the
+// maximum / 127: there the codes are clamped.
+__device__ __forceinline__ uint2 codes_of(float (&x)[8], const Quotient& by) {
   constexpr float MAGIC = 12583040.0f;
-  const uint64_t inv2 = pair_f32(inv, inv), magic2 = pair_f32(MAGIC, MAGIC), minus2 = pair_f32(-MAGIC, -MAGIC), neg2 = pair_f32(-inv, -inv);
+  const uint64_t inv2 = pair_f32(by.inv, by.inv), neg2 = pair_f32(-by.scale, -by.scale), magic2 = pair_f32(MAGIC, MAGIC);
+  if (by.lift != 1.f)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= by.lift;
   uint32_t t[8];
-  float worst = 0.f;
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
-    const uint64_t v = pair_f32(x[e], x[e + 1]), sum = fma_f32x2(v, inv2, magic2);
-    float d0, d1, t0, t1;
-    split_f32(fma_f32x2(v, neg2, add_f32x2(sum, minus2)), d0, d1);   // rounded less exact
-    split_f32(sum, t0, t1);
-    worst = max3(worst, fabsf(d0), fabsf(d1));
+    const uint64_t v = pair_f32(x[e], x[e + 1]), q = fma_f32x2(v, inv2, 0ull);
+    float t0, t1;
+    split_f32(add_f32x2(fma_f32x2(fma_f32x2(q, neg2, v), inv2, q), magic2), t0, t1);
     t[e] = __float_as_uint(t0);
     t[e + 1] = __float_as_uint(t1);
   }
-  if (worst > 0.4999f || exact) {
+  if (by.lift != 1.f)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) t[e] = __float_as_uint(__fadd_rn(fminf(fmaxf(__fdiv_rn(x[e], scale), -127.f), 127.f), MAGIC));
-  }
+    for (int e = 0; e < 8; ++e) t[e] = __float_as_uint(fminf(fmaxf(__uint_as_float(t[e]), MAGIC - 127.f), MAGIC + 127.f));
   uint2 w;
   w.x = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
   w.y = __byte_perm(__byte_perm(t[4], t[5], 0x0040), __byte_perm(t[6], t[7], 0x0040), 0x5410);
@@ -274,6 +286,12 @@ __device__ __forceinline__ uint32_t magnitude(const uint4& v) {
 }
 template <int DT> constexpr uint32_t NOT_FINITE = DT == NKV_BF16 ? 0x7F80u : 0x7C00u;
 
+// 16 bytes from memory to shared memory; the thread that asked for them may read them once they have landed
+__device__ __forceinline__ void copy16_async(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_landed() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 struct AppendSide {
   const uint16_t* x;
   long long stride_batch, stride_token, stride_head;
@@ -284,14 +302,16 @@ struct AppendSide {
 // are each other's partners where all of a head turns in the half layout, in two passes of 32 tokens.  V: it has eight
 // columns of four neighbouring tokens, so that four codes of a column make a word of the transposed block.  A block that
 // the call completes takes its old tokens from the tail; one that stays open only gets its new tokens stored there.
-// Bound: memory (24,967 tokens x 40 heads x 128 rotated and written: @@ us); with the pairs of a head turned twice, table entries
-// fetched one by one and a division's test per element it was the arithmetic, 503 us.
+// Rows come in past the registers, all at once; the table entries, fetched by position, are what the rotation waits for.
+// Bound: the arithmetic, then memory (24,967 tokens x 40 heads x 128 rotated and written: 767 MB in and out in 177 us,
+// 4.3 TB/s; 227 with a division where a quotient lay near a half, 238 with rows in registers, 503 before pairs were turned once).
 template <int DT, int D>
-__global__ void __launch_bounds__(2 * D, 512 / D)
+__global__ void __launch_bounds__(2 * D, 640 / D)
 append_kernel(BlockArrays c, AppendSide k, AppendSide v, Rotation rot, int tokens, Sequences seqs) {
   constexpr int PIECES = D / 8, PAIRS = PIECES / 2, THREADS = 2 * D, WARPS = THREADS / 32;
-  __shared__ uint32_t words[D * 16];        // [column][16 words of 4 tokens], word index xor column / 8
+  __shared__ __align__(16) uint4 k_rows[NKV_BLOCK * PIECES], v_rows[NKV_BLOCK * PIECES];   // a thread's own pieces, on their way in
   __shared__ uint32_t reduced[2][WARPS];
+  uint32_t* const words = reinterpret_cast<uint32_t*>(k_rows);   // later: [column][16 words of 4 tokens], word index xor column / 8
   const int b = blockIdx.z, h = blockIdx.y;
   const int length = seqs.length[b], count = seqs.count[b];
   const int block = length / NKV_BLOCK + blockIdx.x;
@@ -303,26 +323,51 @@ append_kernel(BlockArrays c, AppendSide k, AppendSide v, Rotation rot, int token
   const size_t bh = static_cast<size_t>(b) * c.kv_heads + h;
   uint16_t* const k_tail = static_cast<uint16_t*>(c.k_tail) + bh * NKV_BLOCK * D;
   uint16_t* const v_tail = static_cast<uint16_t*>(c.v_tail) + bh * NKV_BLOCK * D;
-  // ---- K
   const int pair = threadIdx.x % PAIRS, d_lo = pair * 8, d_hi = d_lo + D / 2;
   const int k_token = threadIdx.x / PAIRS;   // and 32 on
+  const int piece = threadIdx.x % PIECES, group = threadIdx.x / PIECES, d0 = piece * 8;
   const bool partners = rot.dim == D && rot.layout == NKV_ROTARY_HALF && k.vector != 0;
+  const bool k_ahead = k.vector != 0 && (partners || rot.dim == 0), v_ahead = v.vector != 0;
+  const uint16_t* const k_row = k.x + b * k.stride_batch + h * k.stride_head;
+  const uint16_t* const v_row = v.x + b * v.stride_batch + h * v.stride_head;
+  // ---- all rows that start on 16 bytes, past the registers and at once
+  if (k_ahead)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = k_token + 32 * i;
+      if (t < held || t >= filled) continue;
+      const uint16_t* const row = k_row + static_cast<long long>(t0 + t - length) * k.stride_token;
+      copy16_async(&k_rows[t * PIECES + pair], row + d_lo);
+      copy16_async(&k_rows[t * PIECES + pair + PAIRS], row + d_hi);
+    }
+  if (v_ahead)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int t = 4 * group + i;
+      if (t < held || t >= filled) continue;
+      copy16_async(&v_rows[t * PIECES + piece], v_row + static_cast<long long>(t0 + t - length) * v.stride_token + d0);
+    }
+  int position[2] = {0, 0};
+  if (rot.dim > 0)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = k_token + 32 * i;
+      if (t >= held && t < filled) position[i] = __ldg(rot.positions + static_cast<size_t>(b) * tokens + (t0 + t - length));
+    }
+  // ---- K
   uint4 kp[2][2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int t = k_token + 32 * i;
     kp[i][0] = kp[i][1] = make_uint4(0, 0, 0, 0);
     if (t >= held && t < filled) {
-      const long long n = t0 + t - length;   // token of the call
-      const uint16_t* const row = k.x + b * k.stride_batch + n * k.stride_token + h * k.stride_head;
-      const int position = rot.dim > 0 ? __ldg(rot.positions + static_cast<size_t>(b) * tokens + n) : 0;
       if (partners) {
-        const uint4 lo = load_piece<DT>(row, d_lo, true), hi = load_piece<DT>(row, d_hi, true);
         float2 cs[8];
-        turns_of(rot, position, d_lo, cs);
+        turns_of(rot, position[i], d_lo, cs);
+        copies_landed();
         float x[8], y[8];
-        Piece<DT>::unpack(lo, x);
-        Piece<DT>::unpack(hi, y);
+        Piece<DT>::unpack(k_rows[t * PIECES + pair], x);
+        Piece<DT>::unpack(k_rows[t * PIECES + pair + PAIRS], y);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float x0 = x[e], x1 = y[e];
@@ -331,9 +376,14 @@ append_kernel(BlockArrays c, AppendSide k, AppendSide v, Rotation rot, int token
         }
         kp[i][0] = Piece<DT>::pack(x);
         kp[i][1] = Piece<DT>::pack(y);
+      } else if (k_ahead) {
+        copies_landed();
+        kp[i][0] = k_rows[t * PIECES + pair];
+        kp[i][1] = k_rows[t * PIECES + pair + PAIRS];
       } else {
-        kp[i][0] = rot.dim > 0 ? rotated_piece<DT>(row, d_lo, k.vector != 0, rot, position) : load_piece<DT>(row, d_lo, k.vector != 0);
-        kp[i][1] = rot.dim > 0 ? rotated_piece<DT>(row, d_hi, k.vector != 0, rot, position) : load_piece<DT>(row, d_hi, k.vector != 0);
+        const uint16_t* const row = k_row + static_cast<long long>(t0 + t - length) * k.stride_token;
+        kp[i][0] = rot.dim > 0 ? rotated_piece<DT>(row, d_lo, k.vector != 0, rot, position[i]) : load_piece<DT>(row, d_lo, k.vector != 0);
+        kp[i][1] = rot.dim > 0 ? rotated_piece<DT>(row, d_hi, k.vector != 0, rot, position[i]) : load_piece<DT>(row, d_hi, k.vector != 0);
       }
     } else if (whole && t < held) {
       kp[i][0] = *reinterpret_cast<const uint4*>(k_tail + t * D + d_lo);
@@ -341,15 +391,14 @@ append_kernel(BlockArrays c, AppendSide k, AppendSide v, Rotation rot, int token
     }
   }
   // ---- V
-  const int piece = threadIdx.x % PIECES, group = threadIdx.x / PIECES, d0 = piece * 8;
+  copies_landed();
   uint4 vp[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int t = 4 * group + i;
     vp[i] = make_uint4(0, 0, 0, 0);
     if (t >= held && t < filled) {
-      const uint16_t* const row = v.x + b * v.stride_batch + static_cast<long long>(t0 + t - length) * v.stride_token + h * v.stride_head;
-      vp[i] = load_piece<DT>(row, d0, v.vector != 0);
+      vp[i] = v_ahead ? v_rows[t * PIECES + piece] : load_piece<DT>(v_row + static_cast<long long>(t0 + t - length) * v.stride_token, d0, false);
     } else if (whole && t < held) {
       uint32_t w[4];
 #pragma unroll
@@ -403,15 +452,11 @@ append_kernel(BlockArrays c, AppendSide k, AppendSide v, Rotation rot, int token
     reduced[1][threadIdx.x / 32] = v_most;
   }
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < WARPS; ++w) {
-    k_most = max(k_most, reduced[0][w]);
-    v_most = max(v_most, reduced[1][w]);
-  }
+  k_most = __reduce_max_sync(0xffffffffu, reduced[0][lane % WARPS]);
+  v_most = __reduce_max_sync(0xffffffffu, reduced[1][lane % WARPS]);
   const bool bad = max(k_most, v_most) >= NOT_FINITE<DT>;
   const float k_scale = bad ? 0.f : __fdiv_rn(unpack2<DT>(k_most).x, 127.f), v_scale = bad ? 0.f : __fdiv_rn(unpack2<DT>(v_most).x, 127.f);
-  const float k_inv = __frcp_rn(k_scale), v_inv = __frcp_rn(v_scale);
-  const bool k_exact = !(k_inv < 1e37f), v_exact = !(v_inv < 1e37f);
+  const Quotient k_by(k_scale), v_by(v_scale);
   const size_t slot = slot_of(c, bh, block);
   if (threadIdx.x == 0) {
     c.scales[2 * slot] = bad ? CUDART_NAN_F : k_scale;
@@ -426,7 +471,7 @@ append_kernel(BlockArrays c, AppendSide k, AppendSide v, Rotation rot, int token
       float x[8];
       uint2 w = make_uint2(0x80808080u, 0x80808080u);
       Piece<DT>::unpack(kp[i][half], x);
-      if (k_scale > 0.f) w = codes_of(x, k_scale, k_inv, k_exact);
+      if (k_scale > 0.f) w = codes_of(x, k_by);
       *reinterpret_cast<uint2*>(k_codes + (k_token + 32 * i) * D + (half ? d_hi : d_lo)) = w;
     }
   uint2 vw[4];   // codes of the thread's columns, token by token
@@ -434,7 +479,7 @@ append_kernel(BlockArrays c, AppendSide k, AppendSide v, Rotation rot, int token
   for (int i = 0; i < 4; ++i) {
     float x[8];
     Piece<DT>::unpack(vp[i], x);
-    vw[i] = v_scale > 0.f ? codes_of(x, v_scale, v_inv, v_exact) : make_uint2(0x80808080u, 0x80808080u);
+    vw[i] = v_scale > 0.f ? codes_of(x, v_by) : make_uint2(0x80808080u, 0x80808080u);
   }
 #pragma unroll
   for (int half = 0; half < 2; ++half) {   // four columns: a 4 x 4 transposition of bytes
@@ -458,7 +503,8 @@ append_kernel(BlockArrays c, AppendSide k, AppendSide v, Rotation rot, int token
 
 // ---- read ------------------------------------------------------------------------------------------------------
 
-// One block of one sequence and head as rows; the same split as append, the other way round.
+// One block of one sequence and head as rows; the same split as append, the other way round.  Bound: memory (24,960 tokens x 40
+// heads x 128: 767 MB in and out in 124 us, 6.2 TB/s).
 template <int DT, int D>
 __global__ void __launch_bounds__(2 * D)
 read_kernel(BlockArrays c, int start, int stop, uint16_t* k_out, uint16_t* v_out, Sequences seqs) {
@@ -851,8 +897,9 @@ int rotary(const nkv_tokens& x, void* out_x, const nkv_tokens* y, void* out_y, i
       const long long total = rows * units * (ceil_div(a.heads, heads) + ceil_div(b.heads, heads));
       kernel<<<static_cast<unsigned>((total + 255) / 256), 256, 0, stream>>>(a, b, batch, tokens, d, rot, transposed);
     };
-    // four heads per thread share the table entries once that still leaves every SM its 2,048 threads
-    const bool many = rows * units * (a.heads + b.heads) >= 4ll * 2048 * sm_count();
+    // four heads per thread share the table entries once that still leaves every SM a block of threads (one / four heads per
+    // thread, bf16: 32 tokens x 48 heads of 128 2.5 / 3.0 us, 1,024 x 32 10.2 / 8.2, 24,960 x 24 77.8 / 57.3)
+    const bool many = rows * units * (a.heads + b.heads) >= 4ll * 256 * sm_count();
     if (dtype == NKV_F32) many ? run(rotary_kernel<NKV_F32, 4>, 4) : run(rotary_kernel<NKV_F32, 1>, 1);
     else if (dtype == NKV_BF16) many ? run(rotary_kernel<NKV_BF16, 4>, 4) : run(rotary_kernel<NKV_BF16, 1>, 1);
     else many ? run(rotary_kernel<NKV_F16, 4>, 4) : run(rotary_kernel<NKV_F16, 1>, 1);

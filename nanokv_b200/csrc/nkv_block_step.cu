@@ -11,6 +11,10 @@
 // by two instructions per pair (a byte beside 0x64 is the number 1024 + byte; 1152 is subtracted, exactly), queries are
 // scaled by a power of two per row into the middle of fp16's range, weights are at most 1.  The block scales are
 // applied in fp32: K's to the scores, V's as the block's product is added to the running result.
+//
+// Measured: 40 heads of 128 over 99,840 tokens, one row each: 1.02 GB in 163 us, 6.3 TB/s.  8 heads of 32 ragged sequences
+// of up to 16,411 tokens, five rows each: 0.61 GB in 105 us, 5.8 TB/s.  8 heads of 64 of 8 sequences of up to 8,191, twenty rows
+// each: 38 MB in 18.5 us, six of them the fixed cost of a launch and the rest the arithmetic of twenty rows a byte.
 #include "nkv_block.cuh"
 #include "nkv_internal.h"
 #include "nkv_tc.cuh"
@@ -588,7 +592,9 @@ size_t parts_of(const Plan& p, int kv_heads) { return p.workers + static_cast<si
 
 }  // namespace
 
-// four groups of eight rows of 64 columns take as many registers as two of 128
+// Up to as many rows as a warp's registers hold: four groups of eight rows of 64 columns, two of 128.  The tile kernel costs the
+// same for one row as for 128 (24,960 tokens x 24 heads of 128, here / there: 1 row 49 / 94 us, 16 rows 59 / 96, and 98 there for 17
+// to 48; heads of 64: 1 row 31 / 86, 32 rows 57 / 86).
 bool block_step_supported(int rows, int d) { return rows <= (d == 64 ? 32 : 16); }
 
 // bytes of the parts of one launch
