@@ -56,7 +56,7 @@ static_assert(M_SCALES + NMETA * 2 * 16 <= 1024, "meta block");
 
 // A unit costs a run as much as PIECE_TILES tiles on top of its own: its queries' way in, the first softmax with nothing beside it,
 // its rows' way out.  Causal units of a prompt's start have few tiles, and runs of equally many tiles would take up to twenty of them
-// or three (2 x 4,095 queries x 32 heads over their own tokens, costs of 0 / 2 / 3 / 4 / 6: 455 / 403 / 393 / 401 / 412 us).
+// or three (2 x 4,095 queries x 32 heads over their own tokens, costs of 0 / 2 / 3 / 4 / 5: 474 / 412 / 409 / 418 / 422 us).
 constexpr uint32_t PIECE_TILES = 3;
 __host__ __device__ inline uint32_t cost_of(int tiles) { return tiles > 0 ? tiles + PIECE_TILES : 0; }
 
