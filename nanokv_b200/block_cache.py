@@ -130,7 +130,7 @@ class BlockCache:
             if rotary.head_dim != self.head_dim or rotary.table.device != self.device:
                 raise ValueError(f"the rotation is for heads of {rotary.head_dim} on {rotary.table.device}")
             ops._check_positions(positions, self.batch, tokens, self.device)
-            rotation = ops.rotation(rotary.table, positions, rotary.layout)
+            rotation = ops._turns(rotary.table, positions, rotary.layout)
         ints = ops._host_ints(counts, self.batch, "counts")
         with ops._On(self.device):
             ops.block_append(self._struct, k, v, counts=ints, rotation=rotation)

@@ -764,12 +764,21 @@ def _check_positions(positions: torch.Tensor, batch: int, tokens: int, device: t
 
 def rotation(table: torch.Tensor, positions: torch.Tensor, layout: str) -> _lib.Rotation:
     """struct nkv_rotation over device tensors: table f32 [rows, rotary_dim/2, 2], positions i32."""
-    _require_cuda(table, positions)
-    if table.dtype != torch.float32 or table.dim() != 3 or table.shape[2] != 2:
+    _require_cuda(positions)
+    return _turns(table, positions, layout)
+
+
+def _turns(table: torch.Tensor, positions: torch.Tensor, layout: str) -> _lib.Rotation:
+    """``rotation`` for positions that were checked already."""
+    rows, half, pair = table.shape if table.dim() == 3 else (0, 0, 0)
+    if pair != 2 or table.dtype != torch.float32:
         raise ValueError("rotation table must be float32 [rows, rotary_dim/2, 2]")
-    if layout not in _LAYOUTS:
+    if not table.is_contiguous() or not table.is_cuda:
+        _require_cuda(table)
+    code = _LAYOUTS.get(layout)
+    if code is None:
         raise ValueError(f"layout must be one of {sorted(_LAYOUTS)}; got {layout!r}")
-    return _lib.Rotation(table.data_ptr(), positions.data_ptr(), table.shape[0], 2 * table.shape[1], _LAYOUTS[layout])
+    return _lib.Rotation(table.data_ptr(), positions.data_ptr(), rows, 2 * half, code)
 
 
 def rotary(x: torch.Tensor, y: torch.Tensor | None, table: torch.Tensor, positions: torch.Tensor, *, layout: str = "half",
@@ -787,7 +796,7 @@ def rotary(x: torch.Tensor, y: torch.Tensor | None, table: torch.Tensor, positio
     _check_positions(positions, batch, tokens, x.device)
     if table.device != x.device:
         raise ValueError("the rotation table must be on the rows' device")
-    rot = rotation(table, positions, layout)
+    rot = _turns(table, positions, layout)
     out = torch.empty_like(x, memory_format=torch.contiguous_format)
     with _On(x.device):
         _lib.check(_lib.library().nkv_rotary(xs, out.data_ptr(), ys, None if y is None else out_y.data_ptr(), dtype_code(x.dtype), batch, tokens, width, rot,
@@ -818,12 +827,13 @@ def block_attend(struct: _lib.BlockCache, q: torch.Tensor, *, counts=None, causa
     lib = _lib.library()
     tokens, heads = q.shape[1], q.shape[2]
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = q.new_empty(q.shape[:3], dtype=torch.float32)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
     nbytes = lib.nkv_block_attend_workspace_bytes(struct, heads, tokens, counts, int(causal), int(weights is not None))
     workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    _lib.check(lib.nkv_block_attend(struct, rows, tokens, counts, int(causal), float(scale), _ptr(out), _ptr(lse), _ptr(weights),
-                                    _ptr(status_word(q.device) if status is None else status), _ptr(workspace), nbytes,
-                                    _raw_stream(q.device)))
+    word = status_word(q.device) if status is None else status
+    _lib.check(lib.nkv_block_attend(struct, rows, tokens, counts, int(causal), float(scale), out.data_ptr(), lse.data_ptr(),
+                                    None if weights is None else weights.data_ptr(), word.data_ptr(),
+                                    workspace.data_ptr() if nbytes else None, nbytes, _raw_stream(q.device)))
     return out, lse
 
 
@@ -839,6 +849,7 @@ def block_evict(weights: torch.Tensor, table: torch.Tensor, full, partial, *, ke
     full, partial = _host_ints(full, batch, "full"), _host_ints(partial, batch, "partial")
     table_out, weights_out = torch.empty_like(table), torch.empty_like(weights)
     with _On(device):
-        _lib.check(_lib.library().nkv_block_evict(_ptr(weights), _ptr(table), full, partial, batch, kv_heads, blocks, int(keep),
-                                                  int(sinks), int(recent), _ptr(weights_out), _ptr(table_out), _raw_stream(device)))
+        _lib.check(_lib.library().nkv_block_evict(weights.data_ptr(), table.data_ptr(), full, partial, batch, kv_heads, blocks,
+                                                  int(keep), int(sinks), int(recent), weights_out.data_ptr(),
+                                                  table_out.data_ptr(), _raw_stream(device)))
     return table_out, weights_out
