@@ -1,9 +1,11 @@
 // The 8-bit block cache without its attention: tokens in (append), rows out (read), blocks freed (evict), and the rotary
 // positions of queries and keys.  All four are bound by memory, the small calls by the latency of a launch.
 #include "nkv_block.cuh"
+#include "nkv_block_plan.h"
 #include "nkv_internal.h"
 
 namespace nkv {
+static_assert(BLOCK_TOKENS == NKV_BLOCK, "one block size");
 namespace {
 
 // ---- rotary positions -----------------------------------------------------------------------------------------
@@ -301,22 +303,23 @@ struct AppendSide {
 // One block of one sequence and head that the call touches.  K: a thread has the pieces p and p + D / 16 of a token's row, which
 // are each other's partners where all of a head turns in the half layout, in two passes of 32 tokens.  V: it has eight
 // columns of four neighbouring tokens, so that four codes of a column make a word of the transposed block.  A block that
-// the call completes takes its old tokens from the tail; one that stays open only gets its new tokens stored there.
+// the call completes takes its old tokens from the tail; one that stays open only gets its new tokens stored there, in a
+// second launch where the first one reads old tokens of the same tail.
 // Rows come in past the registers, all at once; the table entries, fetched by position, are what the rotation waits for.
 // Bound: the arithmetic, then memory (24,967 tokens x 40 heads x 128 rotated and written: 767 MB in and out in 177 us,
 // 4.3 TB/s; 227 with a division where a quotient lay near a half, 238 with rows in registers, 503 before pairs were turned once).
 template <int DT, int D>
 __global__ void __launch_bounds__(2 * D, 640 / D)
-append_kernel(BlockArrays c, AppendSide k, AppendSide v, Rotation rot, int tokens, Sequences seqs) {
+append_kernel(BlockArrays c, AppendSide k, AppendSide v, Rotation rot, int tokens, Sequences seqs, bool second_launch) {
   constexpr int PIECES = D / 8, PAIRS = PIECES / 2, THREADS = 2 * D, WARPS = THREADS / 32;
   __shared__ __align__(16) uint4 k_rows[NKV_BLOCK * PIECES], v_rows[NKV_BLOCK * PIECES];   // a thread's own pieces, on their way in
   __shared__ uint32_t reduced[2][WARPS];
   uint32_t* const words = reinterpret_cast<uint32_t*>(k_rows);   // later: [column][16 words of 4 tokens], word index xor column / 8
   const int b = blockIdx.z, h = blockIdx.y;
   const int length = seqs.length[b], count = seqs.count[b];
-  const int block = length / NKV_BLOCK + blockIdx.x;
+  const int block = append_block(length, count, blockIdx.x, second_launch);
+  if (block < 0) return;
   const int t0 = block * NKV_BLOCK;         // first token of the block
-  if (t0 >= length + count || block >= c.blocks || count <= 0) return;
   const int held = max(0, length - t0), filled = min(NKV_BLOCK, length + count - t0);
   const bool whole = filled == NKV_BLOCK;
   const int lane = threadIdx.x & 31;
@@ -930,20 +933,24 @@ int block_append(const nkv_block_cache& c, const nkv_tokens& k, const nkv_tokens
     const int n = min(MAX_SEQUENCES, c.batch - first);
     const Sequences seqs = sequences_of(c, first, n, counts, tokens);
     int touched = 0;
-    for (int i = 0; i < n; ++i)
-      if (seqs.count[i] > 0)
-        touched = max(touched, (seqs.length[i] + seqs.count[i] - 1) / NKV_BLOCK - seqs.length[i] / NKV_BLOCK + 1);
+    bool twice = false;
+    for (int i = 0; i < n; ++i) {
+      touched = max(touched, append_blocks(seqs.length[i], seqs.count[i]));
+      twice |= append_twice(seqs.length[i], seqs.count[i]);
+    }
     if (touched == 0) continue;
     AppendSide kf = ks, vf = vs;
     kf.x += first * ks.stride_batch;
     vf.x += first * vs.stride_batch;
     Rotation rf = rot;
     if (rotation) rf.positions += static_cast<size_t>(first) * tokens;
-    const dim3 grid(touched, c.kv_heads, n);
     auto kernel = c.head_dim == 128 ? (c.dtype == NKV_BF16 ? append_kernel<NKV_BF16, 128> : append_kernel<NKV_F16, 128>)
                                     : (c.dtype == NKV_BF16 ? append_kernel<NKV_BF16, 64> : append_kernel<NKV_F16, 64>);
-    kernel<<<grid, 2 * c.head_dim, 0, stream>>>(block_arrays(c, first), kf, vf, rf, tokens, seqs);
-    NKV_LAUNCH_CHECK("append_kernel");
+    for (int launch = 0; launch < (twice ? 2 : 1); ++launch) {
+      const dim3 grid(launch ? 1 : touched, c.kv_heads, n);
+      kernel<<<grid, 2 * c.head_dim, 0, stream>>>(block_arrays(c, first), kf, vf, rf, tokens, seqs, launch == 1);
+      NKV_LAUNCH_CHECK("append_kernel");
+    }
   }
   return NKV_OK;
 }
