@@ -6,9 +6,11 @@
 // swizzled operands the tensor cores read; no 16-bit copy of the cache exists in memory.  S = Q K^T goes to tensor memory,
 // eight warps take the softmax (one thread per row), P replaces S as the operand of O += P V.  The block scales never touch
 // an operand.  K's multiplies the scores.  V's goes into the exponent: the weight handed over is P' = 2^(s + log2 vs - m'),
-// with m' the running maximum of s + log2 vs, so that a row's weights are at most 1 (2^8 with the lazy reference) however
-// unlike the scales of its blocks are; a block's part of the row sum is the sum of its P' divided by vs again, in fp32.
-// P' is rounded to the cache's 16-bit type, as the tensor cores take it; sums, maxima and O stay in fp32.
+// with m' a reference that follows the running maximum of s + log2 vs, so that a row's weights stay in their type's range however
+// unlike the scales of its blocks are: in bf16 it lies 86 below, which leaves O the rest of fp32's exponents for values far below
+// the largest (2^200 of them).  Values of the open block come to the codes' size by a power of two, which is its vs.  The row sum has a reference of its own, c, near the running maximum of s: a block's part
+// is the sum of its P' times 2^(m' - log2 vs - c), or, where vs lies so far below the others that P' leaves fp32, the sum of
+// 2^(s - c) itself.  P' is rounded to the cache's 16-bit type, as the tensor cores take it; sums, maxima and O stay in fp32.
 //
 // Measured: 4,680 queries x 24 heads of 128 over 24,960 tokens 1.43 ms (1,000 TFLOP/s) one call at a time, 1.50 without pause
 // (the clock sinks); the MMAs alone, with weights that nothing computes, take 1.07.  Bound: the chain of one query tile, softmax of
@@ -30,14 +32,21 @@ constexpr int TOK = 128;                          // tokens of a tile
 constexpr int STAGES = 2;                         // K / V operand stages
 constexpr int SOFTMAX_WARPS = 8, OPERAND_WARPS = 4, MMA_WARP = 12, THREADS = 448;
 constexpr int SUB = 128 * 128;                    // bytes of a [128 rows x 64 elements] swizzled operand tile
+// m' below the maximum when it is set, and how far the maximum may rise before it is set again: P' up to 2^94 times codes times
+// 2^26 tokens are fp32 numbers
+template <int DT> constexpr float RAISE = DT == NKV_BF16 ? 86.0f : 0.0f;
 constexpr float RESCALE_THRESHOLD = 8.0f;
+// c may lag the scores by this much (sums stay below 2^16 times the number of tokens), and P' is what counts in the sum as long
+// as it stands for at most this power of two of 2^c: weights down to 2^-46 are numbers in it then
+constexpr float SUM_THRESHOLD = 16.0f, MOST_APART = 80.0f;
+constexpr float NOTHING = -3e38f;                 // either reference before the first score: below all, and a number
 
 // (P_READY: query tile i, half h of its tokens at 2 i + h)
 enum Bar { Q_FULL = 0, Q_FREE = 1, K_FULL = 2, K_FREE = 4, V_FULL = 6, V_FREE = 8, S_FULL = 10, P_READY = 12, PV_HALF = 16,
            O_DONE = 18, O_FREE = 20, RAW_FULL = 22, RAW_FREE = 26, NUM_BARS = 30 };
 // scales are written up to four tiles ahead of the softmax (two operand stages, the ring of codes)
 constexpr int NMETA = 8;
-constexpr int M_SLOT = NUM_BARS * 8, M_ABORT = M_SLOT + 4, M_SCALES = 512;   // scales: [NMETA][2 blocks] float4 {ks, log2 vs, 1 / vs, -}
+constexpr int M_SLOT = NUM_BARS * 8, M_ABORT = M_SLOT + 4, M_SCALES = 512;   // scales: [NMETA][2 blocks] float2 {ks, log2 vs}
 
 template <int D> struct Layout {
   static constexpr int DCH = D / 64;
@@ -52,7 +61,7 @@ template <int D> struct Layout {
   static constexpr int DYNAMIC = BYTES + 1024;     // room to start on 1,024 bytes
 };
 static_assert(STAGES == 2, "the MMA warp's stages are told by a bit");
-static_assert(M_SCALES + NMETA * 2 * 16 <= 1024, "meta block");
+static_assert(M_SCALES + NMETA * 2 * 8 <= 1024, "meta block");
 
 // A unit costs a run as much as PIECE_TILES tiles on top of its own: its queries' way in, the first softmax with nothing beside it,
 // its rows' way out.  Causal units of a prompt's start have few tiles, and runs of equally many tiles would take up to twenty of them
@@ -151,7 +160,7 @@ __device__ __forceinline__ int tiles_for(const Call& a, const Sequences& s, cons
 // A run holds at most one piece that starts inside a unit and one that starts with it and is cut: two places each.
 struct Parts {
   float* o;       // [2 runs][UNIT][D], relative to 2^m'
-  float2* ml;     // [2 runs][UNIT]
+  float4* ml;     // [2 runs][UNIT] m', row sum relative to 2^c, c, -
 };
 
 struct Ctx { volatile int* abort_flag; };
@@ -266,20 +275,40 @@ __device__ __forceinline__ float max32(const uint32_t (&r)[32]) {
 }
 
 // ---- warp 13: codes and scales ---------------------------------------------------------------------------------
+// The open block's values as bf16 operands are multiplied by 2^-e, which takes the largest of its `held` tokens to [64, 128): e for
+// a whole warp.  (fp16 has no exponents to spare for that, and no values that would need it.)
 template <int D>
+__device__ __forceinline__ float open_exponent(const uint16_t* tail, int held, int lane) {
+  uint32_t most = 0;
+#pragma unroll 8
+  for (int at = 8 * lane; at < D * NKV_BLOCK; at += 256) {
+    const int col = at % NKV_BLOCK;   // (behind the last token there may be anything)
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(tail + at));
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (col + 2 * e < held) most = max(most, w[e] & 0x7FFFu);
+      if (col + 2 * e + 1 < held) most = max(most, w[e] >> 16 & 0x7FFFu);
+    }
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  return most == 0 ? -60.f : static_cast<float>(max(-120, ilogbf(__uint_as_float(most << 16)) - 6));
+}
+
+template <int DT, int D>
 __device__ __forceinline__ void codes_role(uint8_t* smem, uint64_t* bars, const BlockArrays& c, const Call& a, const Sequences& seqs,
                                            const Plan& plan, const Ctx& ctx) {
   using L = Layout<D>;
   constexpr uint32_t BLOCK_BYTES = NKV_BLOCK * D;
   const int lane = threadIdx.x & 31;
-  float4* const scales = reinterpret_cast<float4*>(smem + M_SCALES);
+  float2* const scales = reinterpret_cast<float2*>(smem + M_SCALES);
   Walk walk(plan, a, seqs, blockIdx.x, c.kv_heads);
   Piece p;
   bool ok = true;
   int seq = 0, item = 0;
   while (ok && walk.next(plan, a, seqs, c.kv_heads, p)) {
     const size_t bh = static_cast<size_t>(p.b) * c.kv_heads + p.h;
-    const int full = seqs.length[p.b] / NKV_BLOCK;
+    const int full = seqs.length[p.b] / NKV_BLOCK, held = seqs.length[p.b] - full * NKV_BLOCK;
     long long slot = 0;
     float2 sc = make_float2(1.f, 1.f);
     for (int t = 0; t < p.nt && ok; ++t, ++seq) {
@@ -293,9 +322,13 @@ __device__ __forceinline__ void codes_role(uint8_t* smem, uint64_t* bars, const 
         }
       }
       if ((lane & ~1) == at) {
-        // a block of scale 0 has only codes 0: any scale serves, and 2^-30 lies below all that 16-bit rows give
-        const float lv = sc.y == 0.f ? -30.f : log2f(sc.y);
-        scales[(seq % NMETA) * 2 + (lane & 1)] = make_float4(sc.x == 0.f ? 1.f : sc.x, lv, exp2f(-lv), 0.f);
+        // a block of scale 0 has only codes 0: any scale serves, and a small one leaves the reference to the others
+        scales[(seq % NMETA) * 2 + (lane & 1)] = make_float2(sc.x == 0.f ? 1.f : sc.x, sc.y == 0.f ? -60.f : log2f(sc.y));
+      }
+      if (DT == NKV_BF16 && full - block0 <= 1 && held > 0) {
+        const float e = open_exponent<D>(static_cast<const uint16_t*>(c.v_tail) + bh * NKV_BLOCK * D, held, lane);
+        __syncwarp();
+        if (lane == 0) scales[(seq % NMETA) * 2 + full - block0] = make_float2(1.f, e);
       }
       __syncwarp();   // ahead of the request whose completion lets S be computed
       const long long s0 = __shfl_sync(0xffffffffu, slot, at), s1 = __shfl_sync(0xffffffffu, slot, at + 1);
@@ -388,7 +421,10 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
       sts128(tile + (col / 64) * SUB + sw128_offset(open * NKV_BLOCK + row, col % 64), *reinterpret_cast<const uint4*>(tail + at));
     }
   };
+  const float2* const scales = reinterpret_cast<const float2*>(smem + M_SCALES);
   auto open_values = [&](uint32_t tile, size_t bh, int open, int held) {
+    const int e = DT == NKV_BF16 ? static_cast<int>(scales[(seq % NMETA) * 2 + open].y) : 0;   // (written ahead of the tile's codes)
+    const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
     const uint16_t* const tail = static_cast<const uint16_t*>(c.v_tail) + bh * NKV_BLOCK * D;
 #pragma unroll 1
     for (int i = 0; i < (2 - open) * LOADS; ++i) {     // the open block, and the one behind it where the tile has room
@@ -398,7 +434,11 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
         const uint4 v = *reinterpret_cast<const uint4*>(tail + at);
         w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] &= col + 2 * e + 1 < held ? 0xFFFFFFFFu : col + 2 * e < held ? 0xFFFFu : 0u;
+        for (int j = 0; j < 4; ++j) {
+          w[j] &= col + 2 * j + 1 < held ? 0xFFFFFFFFu : col + 2 * j < held ? 0xFFFFu : 0u;
+          const float2 f = unpack2<DT>(w[j]);
+          if (DT == NKV_BF16) w[j] = pack2<DT>(f.x * down, f.y * down);
+        }
       }
       sts128(tile + (open + i / LOADS) * L::V_SUB + sw128_offset(row, col), make_uint4(w[0], w[1], w[2], w[3]));
     }
@@ -597,7 +637,7 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
   const int wg = warp / 4, row = tid & 127;
   const uint32_t lane_sel = static_cast<uint32_t>(32 * (warp & 3)) << 16;
   const uint32_t o_addr = tmem + lane_sel + 256 + wg * 128;
-  const float4* const scales = reinterpret_cast<const float4*>(smem + M_SCALES);
+  const float2* const scales = reinterpret_cast<const float2*>(smem + M_SCALES);
   const float scale = fabsf(a.scale_log2);
   Walk walk(plan, a, seqs, blockIdx.x, kv_heads);
   Piece p;
@@ -613,11 +653,13 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
     const size_t bh = static_cast<size_t>(p.b) * kv_heads + p.h;
     const int token = r / a.group;
     const size_t at = (static_cast<size_t>(p.b) * a.tokens + token) * a.heads + p.h * a.group + r - token * a.group;
-    float m = -INFINITY, l = 0.f;
+    float m = NOTHING, l = 0.f, c = NOTHING;   // m' and the row sum relative to 2^c
     // half a tile, a block of the cache, at a time
 #pragma unroll 1
     for (int n = 0; n < 2 * tiles && ok; ++n) {
       const int half = n & 1, block = 2 * p.tile0 + n, first = block * NKV_BLOCK;
+      auto partial_at = [&]() { return a.partial + (bh * a.most_blocks + block) * a.rows + r; };
+      const bool partial_wanted = a.partial && r < a.rows && block < a.most_blocks;
       const uint32_t s_addr = tmem + lane_sel + wg * 128 + half * 64, p_addr = tmem + lane_sel + wg * 128 + half * 32;
       if (half == 0) {
         ok = wait(&bars[S_FULL + wg], ci & 1, ctx, 990);
@@ -627,7 +669,7 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       uint32_t raw[2][32];
       tmem_ld32_issue(s_addr, raw[0]);
       tmem_ld32_issue(s_addr + 32, raw[1]);
-      const float4 sc = scales[(2 * seq + n) % (2 * NMETA)];   // (written ahead of the request for the codes that this S came from)
+      const float2 sc = scales[(2 * seq + n) % (2 * NMETA)];   // (written ahead of the request for the codes that this S came from)
       tmem_ld32_wait(raw[0]);
       tmem_ld32_wait(raw[1]);
       float f = scale * sc.x;
@@ -640,11 +682,13 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
             raw[k][j] = first + 32 * k + j < seen ? __float_as_uint(__uint_as_float(raw[k][j]) * f) : 0xFF800000u;
         f = 1.f;
       }
-      const float m_new = fmaxf(m, fmaf(fmaxf(max32(raw[0]), max32(raw[1])), f, sc.y));
-      if (__any_sync(0xffffffffu, m_new > m + RESCALE_THRESHOLD || (m == -INFINITY && m_new > m))) {
-        // Move the reference: O and the sum are scaled by 2^(old - new).  S was issued behind PV of the tile before and its commit
+      const float top = fmaxf(max32(raw[0]), max32(raw[1])) * f;
+      float off = sc.y - m, rise = m - sc.y - c;   // rise: log2 of what P' counts in the row sum
+      if (__any_sync(0xffffffffu, top + off > RAISE<DT> + RESCALE_THRESHOLD || top - c > SUM_THRESHOLD || rise > MOST_APART)) {
+        // Move the references: O and the sum are scaled by 2^(old - new).  S was issued behind PV of the tile before and its commit
         // covers both; PV of this tile's first half may still run.
-        const float alpha = m_new == -INFINITY ? 1.f : exp2f(m - m_new);
+        const float m_new = fmaxf(m, top + sc.y - RAISE<DT>), c_new = fmaxf(c, top);
+        const float alpha = exp2f(0.5f * (m - m_new));   // twice: the whole may leave fp32 where O does not
         if (n > 0) {
           if (half) {
             ok = wait(&bars[PV_HALF + wg], ci & 1, ctx, 991);
@@ -656,17 +700,35 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
             uint32_t v[16];
             tmem_ld16(o_addr + cc * 16, v);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
+            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha * alpha);
             tmem_st16(o_addr + cc * 16, v);
           }
           tmem_wait_st();
         }
-        l *= alpha;
+        l *= exp2f(c - c_new);
         m = m_new;
+        c = c_new;
+        off = sc.y - m;
+        rise = m - sc.y - c;
+        if (__any_sync(0xffffffffu, rise > MOST_APART)) {   // the sum apart from P', from scores read again (a short loop)
+          float own = 0.f;
+#pragma unroll 1
+          for (int cc = 0; cc < 4; ++cc) {
+            uint32_t v[16];
+            tmem_ld16(s_addr + 16 * cc, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (first + 16 * cc + j < seen) own += exp2_fast(fmaf(__uint_as_float(v[j]), scale * sc.x, -c));
+          }
+          if (rise > MOST_APART) {
+            l += own;
+            if (partial_wanted) *partial_at() = log2f(own) + c;
+            rise = -INFINITY;
+          }
+        }
       }
       // P' (16-bit pairs) replaces S, the first half's of the first columns.  (The compiler interleaves the groups: spelling out
       // exponentials of one beside arguments and sums of its neighbours changes nothing.)
-      const float ref = m == -INFINITY ? 0.f : m, off = sc.y - ref;
       const uint64_t scale2 = pair_f32(f, f), off2 = pair_f32(off, off);
       uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll
@@ -689,8 +751,8 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       float lo, hi;
       split_f32(add_f32x2(sum2[0], sum2[1]), lo, hi);
       const float sum = lo + hi;
-      l = fmaf(sum, sc.z, l);
-      if (a.partial && r < a.rows && block < a.most_blocks) a.partial[(bh * a.most_blocks + block) * a.rows + r] = log2f(sum) + (ref - sc.y);
+      l = fmaf(sum, exp2_fast(rise), l);
+      if (partial_wanted && rise > -INFINITY) *partial_at() = log2f(sum) - off;
       ci += half;
     }
     seq += p.nt;
@@ -702,7 +764,8 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       if (!ok) break;
       tc_fence_after();
     }
-    const float inv = seen > 0 ? 1.f / l : 0.f;
+    const float half = exp2f(0.5f * (m - c)), inv = half / l;   // in two factors: 2^(m' - c) alone may leave fp32
+    const uint64_t half2 = pair_f32(half, half), inv2 = pair_f32(inv, inv), zero2 = pair_f32(-0.f, -0.f);
     const bool wide_out = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0, wide_part = (reinterpret_cast<uintptr_t>(parts.o) & 31) == 0;
     float* const part = parts.o + (place_of(p) * UNIT + wg * QT + row) * D;
 #pragma unroll 1
@@ -722,8 +785,9 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
           uint32_t o[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float lo = __uint_as_float(v[j + 2 * e]), hi = __uint_as_float(v[j + 2 * e + 1]);
-            o[e] = seen > 0 ? pack2<DT>(lo * inv, hi * inv) : 0u;
+            float lo, hi;
+            split_f32(fma_f32x2(fma_f32x2(pair_bits(v[j + 2 * e], v[j + 2 * e + 1]), half2, zero2), inv2, zero2), lo, hi);
+            o[e] = seen > 0 ? pack2<DT>(lo, hi) : 0u;
           }
           store32(a.out + at * D + cc * 32 + j, o, wide_out);
         }
@@ -736,8 +800,8 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       }
     }
     if (r < a.rows) {
-      if (p.whole) a.lse[at] = seen > 0 ? (m + log2f(l)) * LN2 : -INFINITY;
-      else parts.ml[place_of(p) * UNIT + wg * QT + row] = make_float2(m, l);
+      if (p.whole) a.lse[at] = seen > 0 ? (c + log2f(l)) * LN2 : -INFINITY;
+      else parts.ml[place_of(p) * UNIT + wg * QT + row] = make_float4(m, l, c, 0.f);
     }
     if (tiles > 0) {
       tc_fence_before();
@@ -750,7 +814,7 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       const int r = p.unit * UNIT + wg * QT + row, token = r / a.group;
       if (r < a.rows) {
         if (p.whole) a.lse[(static_cast<size_t>(p.b) * a.tokens + token) * a.heads + p.h * a.group + r - token * a.group] = CUDART_NAN_F;
-        else parts.ml[place_of(p) * UNIT + wg * QT + row] = make_float2(0.f, CUDART_NAN_F);
+        else parts.ml[place_of(p) * UNIT + wg * QT + row] = make_float4(0.f, CUDART_NAN_F, 0.f, 0.f);
       }
       more = walk.next(plan, a, seqs, kv_heads, p);
     }
@@ -797,7 +861,7 @@ tile_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (warp < SOFTMAX_WARPS) softmax_role<DT, D>(smem, bars, tmem, a, seqs, plan, parts, ctx, c.kv_heads);
   else if (warp < SOFTMAX_WARPS + OPERAND_WARPS) operand_role<DT, D>(smem, bars, c, a, seqs, plan, ctx);
-  else if (warp > MMA_WARP) codes_role<D>(smem, bars, c, a, seqs, plan, ctx);
+  else if (warp > MMA_WARP) codes_role<DT, D>(smem, bars, c, a, seqs, plan, ctx);
   else mma_role<DT, D>(smem, bars, tmem, a, seqs, plan, ctx, c.kv_heads);
   tc_fence_before();
   __syncthreads();
@@ -837,30 +901,34 @@ join_units_kernel(Call a, const __grid_constant__ Sequences seqs, const __grid_c
     const int token = r / a.group;
     const size_t at = (static_cast<size_t>(b) * a.tokens + token) * a.heads + h * a.group + r - token * a.group;
     const bool any = nt > 0 && visible_to(a, length, count, r) > 0;
-    float top = -INFINITY, sum = 0.f, acc[8];
+    float top = -INFINITY, sum_top = -INFINITY, sum = 0.f, acc[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[e] = 0.f;
     if (any) {
       // the run the unit starts in has it as a piece that starts with the unit, the others as one that starts inside
       auto place = [&](uint32_t run) { return (2 * static_cast<size_t>(run) + (run == r0 ? 1 : 0)) * UNIT + row; };
-      for (uint32_t run = r0; run <= r1; ++run) top = fmaxf(top, __ldcg(&parts.ml[place(run)].x));
-      const float ref = top == -INFINITY ? 0.f : top;
       for (uint32_t run = r0; run <= r1; ++run) {
-        const float2 ml = __ldcg(&parts.ml[place(run)]);
+        const float4 ml = __ldcg(&parts.ml[place(run)]);
+        top = fmaxf(top, ml.x);
+        sum_top = fmaxf(sum_top, ml.z);
+      }
+      for (uint32_t run = r0; run <= r1; ++run) {
+        const float4 ml = __ldcg(&parts.ml[place(run)]);
         const float4 lo = __ldcg(reinterpret_cast<const float4*>(parts.o + place(run) * D + col));
         const float4 hi = __ldcg(reinterpret_cast<const float4*>(parts.o + place(run) * D + col + 4));
-        const float f = exp2f(ml.x - ref);
-        sum = fmaf(ml.y, f, sum);
-        acc[0] = fmaf(lo.x, f, acc[0]); acc[1] = fmaf(lo.y, f, acc[1]); acc[2] = fmaf(lo.z, f, acc[2]); acc[3] = fmaf(lo.w, f, acc[3]);
-        acc[4] = fmaf(hi.x, f, acc[4]); acc[5] = fmaf(hi.y, f, acc[5]); acc[6] = fmaf(hi.z, f, acc[6]); acc[7] = fmaf(hi.w, f, acc[7]);
+        const float f = exp2f(0.5f * (ml.x - top));   // twice, as in the kernel above
+        sum = fmaf(ml.y, exp2f(ml.z - sum_top), sum);
+        const float part[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = fmaf(part[e] * f, f, acc[e]);
       }
     }
-    const float inv = any ? 1.f / sum : 0.f;
+    const float half = any ? exp2f(0.5f * (top - sum_top)) : 0.f, inv = any ? half / sum : 0.f;
     uint32_t o[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = pack2<DT>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+    for (int e = 0; e < 4; ++e) o[e] = pack2<DT>(acc[2 * e] * half * inv, acc[2 * e + 1] * half * inv);
     *reinterpret_cast<uint4*>(a.out + at * D + col) = make_uint4(o[0], o[1], o[2], o[3]);
-    if (col == 0) a.lse[at] = any ? (top + log2f(sum)) * LN2 : -INFINITY;
+    if (col == 0) a.lse[at] = any ? (sum_top + log2f(sum)) * LN2 : -INFINITY;
   }
 }
 
@@ -884,7 +952,7 @@ Plan plan_of(const Sequences& seqs, int n, int kv_heads, int group, int rows, bo
 }
 
 
-size_t part_bytes(int runs, int d) { return static_cast<size_t>(runs) * 2 * UNIT * (d + 2) * sizeof(float); }
+size_t part_bytes(int runs, int d) { return static_cast<size_t>(runs) * 2 * UNIT * (d + 4) * sizeof(float); }
 
 }  // namespace
 
@@ -896,7 +964,7 @@ int block_tile(const BlockArrays& c, const Call& a, const Sequences& seqs, int n
   NKV_REQUIRE(plan.fits, NKV_ERR_TOO_LARGE, "block_attend: more tiles of %d x %d than 32 bits count", UNIT, TOK);
   Parts parts;
   parts.o = static_cast<float*>(workspace);
-  parts.ml = reinterpret_cast<float2*>(parts.o + static_cast<size_t>(plan.runs) * 2 * UNIT * d);
+  parts.ml = reinterpret_cast<float4*>(parts.o + static_cast<size_t>(plan.runs) * 2 * UNIT * d);
   const bool bf16 = dtype == NKV_BF16, wide = d == 128;
   if (plan.runs > 0) {
     auto run = [&](auto kernel, int smem) {
