@@ -9,8 +9,10 @@
 // Scores are computed as S^T = K Q^T and the result as O^T = V^T P^T: the codes are the 16-row operand of the tensor
 // cores, the rows the 8-wide one, so that one row costs half of what the other way round would.  Codes become fp16
 // by two instructions per pair (a byte beside 0x64 is the number 1024 + byte; 1152 is subtracted, exactly), queries are
-// scaled by a power of two per row into the middle of fp16's range, weights are at most 1.  The block scales are
-// applied in fp32: K's to the scores, V's as the block's product is added to the running result.
+// scaled by a power of two per row into the middle of fp16's range.  Weights become 16-bit numbers relative to the largest of
+// their own block and row, which is 2^7: 2^-21 of it keeps all its bits, 2^-32 is still a number, however small the block's weights are
+// beside others'.  The block scales are applied in fp32: K's to the scores, V's, with the block's own weight, as its
+// product is added to the running result.
 //
 // Measured: 40 heads of 128 over 99,840 tokens, one row each: 1.02 GB in 163 us, 6.3 TB/s.  8 heads of 32 ragged sequences
 // of up to 16,411 tokens, five rows each: 0.61 GB in 105 us, 5.8 TB/s.  8 heads of 64 of 8 sequences of up to 8,191, twenty rows
@@ -29,6 +31,7 @@ constexpr int RING_BYTES = 24576;                 // per warp: three K or V bloc
 template <int D> constexpr int SLOT = NKV_BLOCK * D;
 template <int D> constexpr int STAGES = RING_BYTES / SLOT<D>;
 constexpr int STEP_SMEM = WARPS * RING_BYTES + 1024;
+constexpr float RAISE = 7.f;                      // log2 of a block's largest weight as a 16-bit number
 
 // Where the blocks of a launch's sequences lie in the list, and how the list is cut.
 struct Plan {
@@ -256,9 +259,10 @@ step_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
       }
   };
 
-  // softmax of one block: s -> P^T operand (fp16, or the cache's type for an open block)
+  // softmax of one block: s -> P^T operand (fp16, or the cache's type for an open block), relative to the block's largest; alpha and
+  // share: what the results so far and the block's product count from now on
   auto softmax = [&](float (&s)[NT][4][4], int t0, float k_scale, int b, int h, int block, uint32_t (&pb)[NT][4][2], float (&alpha)[NT][2],
-                     bool plain_type) {
+                     float (&share)[NT][2], bool plain_type) {
     const bool masked = t0 + NKV_BLOCK > seen_least;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -277,9 +281,10 @@ step_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], x));
-        const float next = fmaxf(m[nt][e], top[e]);
-        ref[e] = next == -INFINITY ? 0.f : next;
-        alpha[nt][e] = exp2_fast(m[nt][e] - ref[e]);
+        const float next = fmaxf(m[nt][e], top[e]), now = next == -INFINITY ? 0.f : next;
+        alpha[nt][e] = exp2_fast(m[nt][e] - now);
+        share[nt][e] = exp2_fast(top[e] - now - RAISE);
+        ref[e] = (top[e] == -INFINITY ? 0.f : top[e]) - RAISE;
         m[nt][e] = next;
       }
 #pragma unroll
@@ -296,7 +301,7 @@ step_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        l[nt][e] = l[nt][e] * alpha[nt][e] + sum[e];
+        l[nt][e] = fmaf(sum[e], share[nt][e], l[nt][e] * alpha[nt][e]);
         if (a.partial) {
           float total = sum[e];
 #pragma unroll
@@ -310,9 +315,9 @@ step_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
   };
 
   // result += block product
-  auto add = [&](int nt, int j, const float (&part)[4], const float (&alpha)[2], float v_scale) {
+  auto add = [&](int nt, int j, const float (&part)[4], const float (&alpha)[2], const float (&share)[2]) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[nt][j][e] = fmaf(part[e], v_scale, o[nt][j][e] * alpha[e & 1]);
+    for (int e = 0; e < 4; ++e) o[nt][j][e] = fmaf(part[e], share[e & 1], o[nt][j][e] * alpha[e & 1]);
   };
 
   float2 scales = make_float2(0.f, 0.f);   // lane l: of block window + l
@@ -339,7 +344,7 @@ step_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
     }
     float s[NT][4][4];
     uint32_t pb[NT][4][2];
-    float alpha[NT][2];
+    float alpha[NT][2], share[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -372,7 +377,11 @@ step_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
       __syncwarp();
       ++got;
       request();
-      softmax(s, t0, k_scale, b, h, block, pb, alpha, false);
+      softmax(s, t0, k_scale, b, h, block, pb, alpha, share, false);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) share[nt][e] *= v_scale;
       // ---- O^T = V^T P^T: columns x rows
       ok = tc::wait_all(full + got % STAGES<D>, (got / STAGES<D>) & 1, abort_flag, 961);
       if (!ok) break;
@@ -395,7 +404,7 @@ step_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
           for (int nt = 0; nt < NT; ++nt) mma16816<false>(part[nt], a0, a1, a2, a3, pb[nt][w][0], pb[nt][w][1]);
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) add(nt, j, part[nt], alpha[nt], v_scale);
+        for (int nt = 0; nt < NT; ++nt) add(nt, j, part[nt], alpha[nt], share[nt]);
       }
       __syncwarp();
       ++got;
@@ -450,7 +459,7 @@ step_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
         }
       const int least = seen_least;
       seen_least = min(seen_least, 0);   // tokens behind the last one are masked
-      softmax(s, t0, 1.f, b, h, block, pb, alpha, true);
+      softmax(s, t0, 1.f, b, h, block, pb, alpha, share, true);
       seen_least = least;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -475,7 +484,7 @@ step_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
             mma16816<DT == NKV_BF16>(part[nt], lo.x & keep0, hi.x & keep0, lo.y & keep1, hi.y & keep1, pb[nt][w][0], pb[nt][w][1]);
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) add(nt, j, part[nt], alpha[nt], 1.f);
+        for (int nt = 0; nt < NT; ++nt) add(nt, j, part[nt], alpha[nt], share[nt]);
       }
     }
   }

@@ -93,3 +93,33 @@ def test_small_values_with_the_largest_scores(tokens):
     q[..., 0] = 8.0
     v = sized(n, [10.0 ** (-7 * i) for i in range(6)], 2, heads=1, dim=dim)
     check(k.to(torch.bfloat16), v, q.to(torch.bfloat16), causal=False, scale=1.0, least=2.0 ** -126)
+
+
+# batch and kv heads: enough of them that a warp of the kernel for few rows works on many blocks of one head
+@pytest.mark.parametrize("batch,heads,n,tokens,dtype", [(8, 40, 8192, 1, torch.bfloat16), (8, 40, 8192, 1, torch.float16),
+                                                        (8, 40, 8192, 3, torch.bfloat16), (8, 40, 8192, 3, torch.float16),
+                                                        (1, 1, 30000, 140, torch.bfloat16)])
+@pytest.mark.parametrize("nats", [14.0, 18.0])
+def test_many_keys_far_below_one(nats, batch, heads, n, tokens, dtype):
+    """One key takes all but a little of every row and has no value; the result is what thousands of others leave."""
+    dim = 64
+    k, q, v = (randn(batch, n, heads, dim, seed=1, std=0.3), randn(batch, tokens, 2 * heads, dim, seed=3, std=0.3),
+               1 + randn(batch, n, heads, dim, seed=2))
+    k[..., 0], q[..., 0] = 0.0, 8.0
+    k[:, 1000, :, 0], v[:, 1000] = nats / 8, 0.0
+    # fp16 holds a weight to 2^-25 at worst, of numbers that reach 2^7 at least where the largest weight is 1
+    check(k.to(dtype), v.to(dtype), q.to(dtype), causal=False, scale=1.0, least=n * 2.0 ** -32 * float(v.abs().max()))
+
+
+@pytest.mark.parametrize("batch,heads,tokens", [(32, 40, 1), (32, 40, 4), (1, 1, 140)])
+@pytest.mark.parametrize("large", [1e6, 1e8, 1e12])
+def test_large_values_under_small_weights(large, batch, heads, tokens):
+    """Keys 18 nats lower whose values are larger by as much and more: the result is theirs as well."""
+    n, dim = 64 * 6 + 10, 64
+    k, q = randn(batch, n, heads, dim, seed=1, std=0.3), randn(batch, tokens, 2 * heads, dim, seed=3, std=0.3)
+    k[..., 0], q[..., 0] = 3.0, 6.0
+    k[:, 64:128, :, 0] = k[:, 256:320, :, 0] = 0.0
+    v = randn(batch, n, heads, dim, seed=2)
+    v[:, 64:128] *= large
+    v[:, 256:320] *= large
+    check(k.to(torch.bfloat16), v.to(torch.bfloat16), q.to(torch.bfloat16), causal=False, scale=1.0)
