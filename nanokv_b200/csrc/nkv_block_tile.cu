@@ -7,9 +7,10 @@
 // eight warps take the softmax (one thread per row), P replaces S as the operand of O += P V.  The block scales never touch
 // an operand.  K's multiplies the scores.  V's goes into the exponent: the weight handed over is P' = 2^(s + log2 vs - m'),
 // with m' a reference that follows the running maximum of s + log2 vs, so that a row's weights stay in their type's range however
-// unlike the scales of its blocks are: in bf16 it lies 86 below, which leaves O the rest of fp32's exponents for values far below
-// the largest (2^200 of them).  Values of the open block come to the codes' size by a power of two, which is its vs.  The row sum has a reference of its own, c, near the running maximum of s: a block's part
-// is the sum of its P' times 2^(m' - log2 vs - c), or, where vs lies so far below the others that P' leaves fp32, the sum of
+// unlike the scales of its blocks are.  It lies below the maximum, in bf16 by 86, which leaves O the rest of fp32's exponents for
+// values far below the largest (2^200 of them).  Values of the open block come to the codes' size by a power of two, which is
+// its vs (bf16; fp16 values are taken as they are).  The row sum has a reference of its own, c, near the running maximum of s: a
+// block's part is the sum of its P' times 2^(m' - log2 vs - c), or, where vs lies so far below the others that P' leaves fp32, the sum of
 // 2^(s - c) itself.  P' is rounded to the cache's 16-bit type, as the tensor cores take it; sums, maxima and O stay in fp32.
 //
 // Measured: 4,680 queries x 24 heads of 128 over 24,960 tokens 1.43 ms (1,000 TFLOP/s) one call at a time, 1.50 without pause
@@ -32,9 +33,9 @@ constexpr int TOK = 128;                          // tokens of a tile
 constexpr int STAGES = 2;                         // K / V operand stages
 constexpr int SOFTMAX_WARPS = 8, OPERAND_WARPS = 4, MMA_WARP = 12, THREADS = 448;
 constexpr int SUB = 128 * 128;                    // bytes of a [128 rows x 64 elements] swizzled operand tile
-// m' below the maximum when it is set, and how far the maximum may rise before it is set again: P' up to 2^94 times codes times
-// 2^26 tokens are fp32 numbers
-template <int DT> constexpr float RAISE = DT == NKV_BF16 ? 86.0f : 0.0f;
+// m' below the maximum when it is set, and how far the maximum may rise before it is set again.  bf16: P' up to 2^94 times codes
+// times 2^26 tokens are fp32 numbers.  fp16: P' up to 2^15, so that 2^-21 of the largest keeps all its bits and 2^-32 is a number.
+template <int DT> constexpr float RAISE = DT == NKV_BF16 ? 86.0f : 7.0f;
 constexpr float RESCALE_THRESHOLD = 8.0f;
 // c may lag the scores by this much (sums stay below 2^16 times the number of tokens), and P' is what counts in the sum as long
 // as it stands for at most this power of two of 2^c: weights down to 2^-46 are numbers in it then

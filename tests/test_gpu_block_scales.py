@@ -95,10 +95,11 @@ def test_small_values_with_the_largest_scores(tokens):
     check(k.to(torch.bfloat16), v, q.to(torch.bfloat16), causal=False, scale=1.0, least=2.0 ** -126)
 
 
-# batch and kv heads: enough of them that a warp of the kernel for few rows works on many blocks of one head
+# batch and kv heads: enough of them that one worker of either kernel takes many blocks of one head
 @pytest.mark.parametrize("batch,heads,n,tokens,dtype", [(8, 40, 8192, 1, torch.bfloat16), (8, 40, 8192, 1, torch.float16),
                                                         (8, 40, 8192, 3, torch.bfloat16), (8, 40, 8192, 3, torch.float16),
-                                                        (1, 1, 30000, 140, torch.bfloat16)])
+                                                        (1, 1, 30000, 140, torch.bfloat16), (1, 40, 8192, 140, torch.bfloat16),
+                                                        (1, 40, 8192, 140, torch.float16)])
 @pytest.mark.parametrize("nats", [14.0, 18.0])
 def test_many_keys_far_below_one(nats, batch, heads, n, tokens, dtype):
     """One key takes all but a little of every row and has no value; the result is what thousands of others leave."""
@@ -123,3 +124,14 @@ def test_large_values_under_small_weights(large, batch, heads, tokens):
     v[:, 64:128] *= large
     v[:, 256:320] *= large
     check(k.to(torch.bfloat16), v.to(torch.bfloat16), q.to(torch.bfloat16), causal=False, scale=1.0)
+
+
+@pytest.mark.parametrize("tokens", TOKENS)
+def test_unlike_scales_in_fp16(tokens):
+    """Blocks whose values are 2^-14 and 2^-20 of others', some of them with the larger weights."""
+    n, dim = 64 * 7 + 10, 64
+    k, q = randn(1, n, 1, dim, seed=1, std=0.3), randn(1, tokens, 2, dim, seed=3, std=0.3)
+    k[..., 0], q[..., 0] = 0.0, 4.0
+    k[:, 64:128, :, 0] = 2.0
+    v = sized(n, [1.0, 2.0 ** -14, 2.0 ** -20, 100.0, 2.0 ** -14, 0.0, 2.0 ** -10, 1.0], 2, heads=1, dim=dim, dtype=torch.float16)
+    check(k.to(torch.float16), v, q.to(torch.float16), causal=tokens == 140, scale=1.0, least=n * 2.0 ** -32 * float(v.abs().max()))
