@@ -198,7 +198,11 @@ class BlockCache:
         those that ``weights`` ranks highest for the kv head at hand; the open block stays as well."""
         full = [n // BLOCK for n in self._lengths]
         partial = [int(n % BLOCK > 0) for n in self._lengths]
-        self.table, self.weights = ops.block_evict(self.weights, self.table, full, partial, keep=keep, sinks=sinks, recent=recent)
+        before = self.table, self.weights
+        self.table, self.weights = ops.block_evict(*reversed(before), full, partial, keep=keep, sinks=sinks, recent=recent)
+        # nobody else may hold them: their memory is not to be used again before this stream is past the call
+        for t in before:
+            t.record_stream(torch.cuda.current_stream(self.device))
         lengths = list(self._lengths)
         for b, n in enumerate(full):
             if n <= keep:
