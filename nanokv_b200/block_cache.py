@@ -170,7 +170,7 @@ class BlockCache:
         """k, v [batch, stop - start, kv_heads, head_dim]: the values that the cache holds for tokens [start, stop), zero past
         a sequence's length; for callers with an attention of their own."""
         with ops._On(self.device):
-            return ops.block_read(self._struct, int(start), int(stop), dtype=self.dtype, device=self.device)
+            return ops.block_read(self._struct, start, stop, dtype=self.dtype, device=self.device)
 
     # ------------------------------------------------------------------ attention and eviction
     def attend(self, q: torch.Tensor, *, counts=None, causal: bool = True, scale: float | None = None,

@@ -752,7 +752,16 @@ def _host_ints(values, count: int, name: str):
         return None
     if len(values) != count:
         raise ValueError(f"{name} must name {count} sequences; got {len(values)}")
+    if count and not (min(values) >= -2 ** 31 and max(values) < 2 ** 31):     # (ctypes would cut them off)
+        raise ValueError(f"{name} must be integers of 32 bits; got {list(values)}")
     return (ctypes.c_int32 * count)(*values)
+
+
+def _int32(value, name: str) -> int:
+    value = int(value)
+    if not -2 ** 31 <= value < 2 ** 31:
+        raise ValueError(f"{name} must be an integer of 32 bits; got {value}")
+    return value
 
 
 def _check_positions(positions: torch.Tensor, batch: int, tokens: int, device: torch.device) -> None:
@@ -813,6 +822,7 @@ def block_append(struct: _lib.BlockCache, k: torch.Tensor, v: torch.Tensor, *, c
 
 def block_read(struct: _lib.BlockCache, start: int, stop: int, *, dtype: torch.dtype, device: torch.device):
     """Values of tokens [start, stop) of every sequence -> k, v [batch, stop - start, kv_heads, width] (nkv_block_read)."""
+    start, stop = _int32(start, "start"), _int32(stop, "stop")
     shape = (struct.batch, max(0, stop - start), struct.kv_heads, struct.head_dim)
     k, v = torch.empty((2, *shape), dtype=dtype, device=device).unbind(0)
     _lib.check(_lib.library().nkv_block_read(struct, start, stop, k.data_ptr(), v.data_ptr(), _raw_stream(device)))
@@ -847,9 +857,10 @@ def block_evict(weights: torch.Tensor, table: torch.Tensor, full, partial, *, ke
         raise ValueError("weights and table must be on one device")
     batch, kv_heads, blocks = table.shape
     full, partial = _host_ints(full, batch, "full"), _host_ints(partial, batch, "partial")
+    keep, sinks, recent = _int32(keep, "keep"), _int32(sinks, "sinks"), _int32(recent, "recent")
     table_out, weights_out = torch.empty_like(table), torch.empty_like(weights)
     with _On(device):
         _lib.check(_lib.library().nkv_block_evict(weights.data_ptr(), table.data_ptr(), full, partial, batch, kv_heads, blocks,
-                                                  int(keep), int(sinks), int(recent), weights_out.data_ptr(),
+                                                  keep, sinks, recent, weights_out.data_ptr(),
                                                   table_out.data_ptr(), _raw_stream(device)))
     return table_out, weights_out
