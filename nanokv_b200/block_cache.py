@@ -104,8 +104,12 @@ class BlockCache:
         return list(self._lengths)
 
     def _set_lengths(self, lengths: list[int]) -> None:
+        try:
+            self._array[:] = lengths
+        except TypeError:
+            self._array[:] = self._lengths
+            raise
         self._lengths = lengths
-        self._array[:] = lengths
 
     def _rows_of(self, x: torch.Tensor, name: str) -> int:
         if x.dim() != 4 or x.shape[0] != self.batch or x.shape[3] != self.head_dim:
@@ -155,6 +159,7 @@ class BlockCache:
             if n != now and n % BLOCK and not (n // BLOCK == tail // BLOCK and n <= tail):
                 raise ValueError(f"a sequence cannot be cut to {n}: the rows of its block {n // BLOCK} are not in 16 bits any more")
         left, held = ([(n + BLOCK - 1) // BLOCK for n in some] for some in (lengths, self._lengths))
+        self._set_lengths(lengths)
         if left != held:
             if min(left) == max(left):
                 self.weights[:, :, left[0]:] = 0
@@ -164,7 +169,6 @@ class BlockCache:
                         self.weights[b, :, n:] = 0
         # rows in 16 bits of tokens that are given up count no longer
         self._tail = [t if t <= n else (n if n % BLOCK else 0) for n, t in zip(lengths, self._tail)]
-        self._set_lengths(lengths)
 
     def read(self, start: int, stop: int):
         """k, v [batch, stop - start, kv_heads, head_dim]: the values that the cache holds for tokens [start, stop), zero past
