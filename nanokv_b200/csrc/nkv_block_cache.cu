@@ -253,7 +253,7 @@ struct Quotient {
 
 // Codes (plus 128) of eight elements: rint(x / scale), quotient rounded to fp32.  The quotient comes from the reciprocal y by one
 // step of Markstein's division: q = x y, then q + (x - q scale) y with the residual exact.  It is x / scale correctly rounded for
-// every 16-bit x and every scale that is a 16-bit number / 127 (they are few enough to have been compared one by one).  Adding
+// every 16-bit x and every scale that is a 16-bit number / 127 (the tests compare all of them).  Adding
 // 1.5 * 2^23 + 128 rounds it to an integer, whose low byte is the code.  A subnormal scale is a coarse multiple of the
 // maximum / 127: there the codes are clamped.
 __device__ __forceinline__ uint2 codes_of(float (&x)[8], const Quotient& by) {
