@@ -9,11 +9,14 @@ namespace nkv {
 
 constexpr int MAX_SEQUENCES = 128;   // sequences of one launch; longer batches are cut
 
-// lengths and token counts of a launch's sequences, passed by value
+// Lengths and token counts of a launch's sequences, passed by value: no upload, no device state that a call would have to order
+// against others.
 struct Sequences {
   int32_t length[MAX_SEQUENCES];
   int32_t count[MAX_SEQUENCES];
 };
+// of `count` sequences from `first` on; counts NULL: `tokens` each
+Sequences sequences_of(const nkv_block_cache& c, int first, int count, const int32_t* counts, int tokens);
 
 // device arrays of nkv_block_cache from one of its sequences on
 struct BlockArrays {

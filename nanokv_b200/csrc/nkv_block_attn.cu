@@ -138,15 +138,6 @@ int most_blocks_of(const nkv_block_cache& c) {
   return most;
 }
 
-Sequences sequences_of(const nkv_block_cache& c, int first, int n, const int32_t* counts, int tokens) {
-  Sequences s;
-  for (int i = 0; i < n; ++i) {
-    s.length[i] = c.lengths[first + i];
-    s.count[i] = counts ? counts[first + i] : tokens;
-  }
-  return s;
-}
-
 // scratch of one launch over n sequences: the rows' weight sums per block, then the kernel's own
 struct Scratch { size_t partial, own; };
 Scratch scratch_of(const nkv_block_cache& c, const Sequences& seqs, int n, int group, int tokens, int most_blocks, bool with_weights) {

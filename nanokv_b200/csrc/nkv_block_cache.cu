@@ -848,7 +848,12 @@ evict_small_kernel(const float* weights, const int32_t* table, int blocks, int k
   }
 }
 
-// Sequences of a launch, passed by value: no upload, no device state that a call would have to order against others.
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+
+// ---- host ------------------------------------------------------------------------------------------------------
+
 Sequences sequences_of(const nkv_block_cache& c, int first, int count, const int32_t* counts, int tokens) {
   Sequences s;
   for (int i = 0; i < count; ++i) {
@@ -857,12 +862,6 @@ Sequences sequences_of(const nkv_block_cache& c, int first, int count, const int
   }
   return s;
 }
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-
-}  // namespace
-
-// ---- host ------------------------------------------------------------------------------------------------------
 
 BlockArrays block_arrays(const nkv_block_cache& c, int first) {
   const size_t heads = static_cast<size_t>(first) * c.kv_heads, slots = heads * c.blocks;
