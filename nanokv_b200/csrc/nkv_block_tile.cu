@@ -280,20 +280,21 @@ __device__ __forceinline__ float max32(const uint32_t (&r)[32]) {
 // a whole warp.  (fp16 has no exponents to spare for that, and no values that would need it.)
 template <int D>
 __device__ __forceinline__ float open_exponent(const uint16_t* tail, int held, int lane) {
-  uint32_t most = 0;
+  const int col = 8 * lane % NKV_BLOCK;   // the lane's eight tokens are the same in every row; behind the last one there may be anything
+  uint32_t keep[4], tops[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) keep[e] = (col + 2 * e < held ? 0x7FFFu : 0u) | (col + 2 * e + 1 < held ? 0x7FFF0000u : 0u);
 #pragma unroll 8
   for (int at = 8 * lane; at < D * NKV_BLOCK; at += 256) {
-    const int col = at % NKV_BLOCK;   // (behind the last token there may be anything)
     const uint4 v = __ldg(reinterpret_cast<const uint4*>(tail + at));
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (col + 2 * e < held) most = max(most, w[e] & 0x7FFFu);
-      if (col + 2 * e + 1 < held) most = max(most, w[e] >> 16 & 0x7FFFu);
-    }
+    for (int e = 0; e < 4; ++e) tops[e] = __vmaxu2(tops[e], w[e] & keep[e]);   // bits of magnitudes are ordered as these are
   }
-  most = __reduce_max_sync(0xffffffffu, most);
-  return most == 0 ? -60.f : static_cast<float>(max(-120, ilogbf(__uint_as_float(most << 16)) - 6));
+  tops[0] = __vmaxu2(__vmaxu2(tops[0], tops[1]), __vmaxu2(tops[2], tops[3]));
+  const uint32_t most = __reduce_max_sync(0xffffffffu, max(tops[0] & 0xFFFFu, tops[0] >> 16));
+  const int exponent = most >= 0x80u ? static_cast<int>(most >> 7) - 127 : 31 - __clz(most) - 133;   // (subnormal numbers: by their bits)
+  return most == 0 ? -60.f : static_cast<float>(min(121, max(-120, exponent - 6)));
 }
 
 template <int DT, int D>
