@@ -31,7 +31,7 @@ constexpr int RING_BYTES = 24576;                 // per warp: three K or V bloc
 template <int D> constexpr int SLOT = NKV_BLOCK * D;
 template <int D> constexpr int STAGES = RING_BYTES / SLOT<D>;
 constexpr int STEP_SMEM = WARPS * RING_BYTES + 1024;
-constexpr float RAISE = 7.f;                      // log2 of a block's largest weight as a 16-bit number
+constexpr float RAISE = 7.f;                      // log2 of a block's largest weight as an fp16 number (as a bf16 one: 0)
 
 // Where the blocks of a launch's sequences lie in the list, and how the list is cut.
 struct Plan {
@@ -264,6 +264,7 @@ step_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
   auto softmax = [&](float (&s)[NT][4][4], int t0, float k_scale, int b, int h, int block, uint32_t (&pb)[NT][4][2], float (&alpha)[NT][2],
                      float (&share)[NT][2], bool plain_type) {
     const bool masked = t0 + NKV_BLOCK > seen_least;
+    const float raise = plain_type && DT == NKV_BF16 ? 0.f : RAISE;   // (bf16 values may leave no room for it)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float top[2] = {-INFINITY, -INFINITY};
@@ -283,8 +284,8 @@ step_kernel(BlockArrays c, Call a, const __grid_constant__ Sequences seqs, const
         for (int x = 4; x < 32; x <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], x));
         const float next = fmaxf(m[nt][e], top[e]), now = next == -INFINITY ? 0.f : next;
         alpha[nt][e] = exp2_fast(m[nt][e] - now);
-        share[nt][e] = exp2_fast(top[e] - now - RAISE);
-        ref[e] = (top[e] == -INFINITY ? 0.f : top[e]) - RAISE;
+        share[nt][e] = exp2_fast(top[e] - now - raise);
+        ref[e] = (top[e] == -INFINITY ? 0.f : top[e]) - raise;
         m[nt][e] = next;
       }
 #pragma unroll

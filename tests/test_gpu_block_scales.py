@@ -135,3 +135,14 @@ def test_unlike_scales_in_fp16(tokens):
     k[:, 64:128, :, 0] = 2.0
     v = sized(n, [1.0, 2.0 ** -14, 2.0 ** -20, 100.0, 2.0 ** -14, 0.0, 2.0 ** -10, 1.0], 2, heads=1, dim=dim, dtype=torch.float16)
     check(k.to(torch.float16), v, q.to(torch.float16), causal=tokens == 140, scale=1.0, least=n * 2.0 ** -32 * float(v.abs().max()))
+
+
+@pytest.mark.parametrize("tokens", [1, 140])
+@pytest.mark.parametrize("held", [1, 2, 33, 63])
+@pytest.mark.parametrize("size", [1e36, 1e30, 1e-30, 1e-39, 0.0])
+def test_an_open_block_of_any_size(size, held, tokens):
+    """Values of the open block far above and far below the others'; what lies behind its last token is left over."""
+    n, dim = 64 * 3 + held, 128
+    v = sized(n, [1.0, 1.0, 1.0, size], 2)
+    k, q = (randn(1, m, h, dim, seed=s, dtype=torch.bfloat16) for m, h, s in ((n, 2, 1), (tokens, 4, 3)))
+    check(k, v, q, least=2.0 ** -133)
