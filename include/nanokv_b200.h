@@ -685,8 +685,11 @@ int nkv_block_read(const nkv_block_cache* cache, int start, int stop, void* k_ou
  * j < lengths[b] - counts[b] + i + 1 (causal) or j < lengths[b]; queries past counts[b] see none.  out [batch, tokens, heads,
  * head_dim] in dtype, lse f32 [batch, tokens, heads] natural log; a query that sees nothing has out 0 and lse -inf.
  * block_weights f32 [batch][kv_heads][blocks] or NULL: += the probability that the queries of the kv head's group gave to
- * every logical block, summed in an order that does not change.  workspace: nkv_block_attend_workspace_bytes(...)
- * bytes of device scratch (16-byte aligned); status_word: device int32 as for the other reads.
+ * every logical block, summed in an order that does not change; it takes 4 bytes of scratch per query head's row and block
+ * (24,960 queries x 64 heads over as many tokens: 2.5 GB), so long prompts are better attended in chunks.  workspace:
+ * nkv_block_attend_workspace_bytes(...) bytes of device scratch (16-byte aligned); status_word: device int32 as for the
+ * other reads.  Weights of attention enter the product with V as 16-bit numbers, in the cache's dtype or fp16, relative to a
+ * reference near their largest; sums, maxima and results are fp32 until they are rounded once.
  */
 size_t nkv_block_attend_workspace_bytes(const nkv_block_cache* cache, int heads, int tokens, const int32_t* counts,
                                         int causal, int with_weights);

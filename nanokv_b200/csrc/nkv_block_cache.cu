@@ -308,6 +308,8 @@ struct AppendSide {
 // Rows come in past the registers, all at once; the table entries, fetched by position, are what the rotation waits for.
 // Bound: the arithmetic, then memory (24,967 tokens x 40 heads x 128 rotated and written: 767 MB in and out in 177 us,
 // 4.3 TB/s; 227 with a division where a quotient lay near a half, 238 with rows in registers, 503 before pairs were turned once).
+// The second launch: 1,560 tokens x 40 heads behind 24 others take 22.2 us, 15.7 behind none; the same thread block going on
+// with the new open block instead took 26.6.
 template <int DT, int D>
 __global__ void __launch_bounds__(2 * D, 640 / D)
 append_kernel(BlockArrays c, AppendSide k, AppendSide v, Rotation rot, int tokens, Sequences seqs, bool second_launch) {
@@ -682,7 +684,8 @@ evict_kernel(const float* weights, const int32_t* table, int blocks, int keep, i
 // The same for rows of 257 to 2,048 entries, whose keys stay in registers, sixteen neighbouring entries to a thread.  The
 // digits begin at the highest bit in which keys differ (weights share most of their exponents, and counts of equal digits
 // collide), and end as soon as all that is left of a digit stays.  Two prefix sums then place every entry.  32 x 40 rows
-// of 1,564: 18.6 us, 25.6 with the kernel above.
+// of 1,564: 18.6 us, 25.6 with the kernel above, which has the longer rows (32 x 40 of 2,048 here 19.6 us, of 2,100 there 29.3, of
+// 4,096 53).
 constexpr int SMALL_THREADS = 128, EVICT_ITEMS = 16;
 __global__ void __launch_bounds__(SMALL_THREADS)
 evict_small_kernel(const float* weights, const int32_t* table, int blocks, int keep, int sinks, int recent, float* weights_out,

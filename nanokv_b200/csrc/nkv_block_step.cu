@@ -14,9 +14,10 @@
 // beside others'.  The block scales are applied in fp32: K's to the scores, V's, with the block's own weight, as its
 // product is added to the running result.
 //
-// Measured: 40 heads of 128 over 99,840 tokens, one row each: 1.02 GB in 163 us, 6.3 TB/s.  8 heads of 32 ragged sequences
-// of up to 16,411 tokens, five rows each: 0.61 GB in 105 us, 5.8 TB/s.  8 heads of 64 of 8 sequences of up to 8,191, twenty rows
-// each: 38 MB in 18.5 us, six of them the fixed cost of a launch and the rest the arithmetic of twenty rows a byte.
+// Measured, both launches, among other calls: 40 heads of 128 over 99,840 tokens, one row each: 1.02 GB in 166 us, 6.2 TB/s.  8 heads
+// of 32 ragged sequences of up to 16,411 tokens, five rows each: 0.61 GB in 113 to 117 us, 5.3 TB/s.  8 heads of 64 of 8
+// sequences of up to 8,191, twenty rows each: 38 MB in 25.6 us, about half of them the two launches' fixed cost and the rest the
+// arithmetic of twenty rows a byte.
 #include "nkv_block.cuh"
 #include "nkv_internal.h"
 #include "nkv_tc.cuh"
@@ -603,8 +604,8 @@ size_t parts_of(const Plan& p, int kv_heads) { return p.workers + static_cast<si
 }  // namespace
 
 // Up to as many rows as a warp's registers hold: four groups of eight rows of 64 columns, two of 128.  The tile kernel costs the
-// same for one row as for 128 (24,960 tokens x 24 heads of 128, here / there: 1 row 49 / 94 us, 16 rows 59 / 96, and 98 there for 17
-// to 48; heads of 64: 1 row 31 / 86, 32 rows 57 / 86).
+// same for one row as for 128 (single calls, 24,960 tokens x 24 heads of 128: 1 row 48 us and 16 rows 56 here, 17 to 128 rows 97 to
+// 101 there; heads of 64: 1 row 32, 24 rows 48 and 32 rows 62 here, 33 rows 87 there).
 bool block_step_supported(int rows, int d) { return rows <= (d == 64 ? 32 : 16); }
 
 // bytes of the parts of one launch
