@@ -708,6 +708,60 @@ int nkv_block_evict(const float* weights, const int32_t* table, const int32_t* f
                     int kv_heads, int blocks, int keep, int sinks, int recent, float* weights_out, int32_t* table_out,
                     void* stream);
 
+/* ------------------------------------------------- paged 16-bit cache */
+
+/*
+ * A cache of keys and values as they came, in 16 bits, in pages that all sequences take from one pool.  Token j of sequence b
+ * is row j % page of page table[b][j / page].  A sequence holds lengths[b] settled tokens; behind them stand the pending ones of
+ * the step at hand (a decoded token, a chunk, a draft), which become settled when the caller adds them to lengths.  Table and
+ * lengths are DEVICE memory, shared by the caches of all layers: a step that was captured into a graph can be replayed while
+ * they grow.  The host does not see what they hold, so the kernels check it: a token without a page (an entry outside 0 .. pages-1, or
+ * no entry) is not written, reads as keys and values of zero, and leaves status 920 in the status word, as do lengths, counts and paths out of
+ * range; no access leaves the arrays.  Two sequences may name one page as long as neither writes to it.
+ */
+typedef struct nkv_page_cache {
+  void*    k_pages;         /* [pages][kv_heads][page][head_dim] in dtype; 16-byte aligned */
+  void*    v_pages;         /* likewise */
+  const int32_t* table;     /* [batch][row_pages] */
+  const int32_t* lengths;   /* [batch] */
+  int32_t batch, row_pages, pages, page;   /* page 16 | 32 | 64 | 128 tokens */
+  int32_t kv_heads, head_dim;              /* head_dim 64 | 128 */
+  int32_t dtype;            /* NKV_BF16 | NKV_F16 */
+} nkv_page_cache;
+
+/* The first counts[b] (DEVICE i32 [batch]; NULL: all `tokens`) of k and v [batch, tokens, kv_heads, head_dim] written as pending
+ * tokens, behind the settled ones.  With a rotation (rotary_dim a multiple of 16) keys are turned on the way, and so are the queries q
+ * [batch, tokens, heads, head_dim], all of them, to q_out (contiguous, 16-byte aligned); q NULL: none.  rotation->positions NULL: token t of sequence b is
+ * at position lengths[b] + t. */
+int nkv_page_append(const nkv_page_cache* cache, const nkv_tokens* k, const nkv_tokens* v, const nkv_tokens* q, void* q_out,
+                    int tokens, const int32_t* counts, const nkv_rotation* rotation, int32_t* status_word, void* stream);
+
+/*
+ * Attention of pending queries q [batch, tokens, heads, head_dim] over the cache; heads a multiple of kv_heads, head h attends kv
+ * head h / (heads / kv_heads).  Query i of sequence b, of counts[b] (DEVICE; NULL: `tokens`), sees the settled tokens and, of the
+ * pending ones j < counts[b]: those whose bit j % 32 of word j / 32 of row i of `mask` is set (u32 [tokens][ceil(tokens / 32)], the next
+ * sequence's mask_stride words on, 0: one mask for all); without a mask those j <= i (causal) or all.  out [batch, tokens, heads, head_dim]
+ * in dtype, lse f32 [batch, tokens, heads] natural log; a query that sees nothing, or only scores of -inf, or lies past counts[b] has out 0
+ * and lse -inf.  What a query does not see has no part in its result, also where it is not finite.  Weights enter the product with V
+ * in dtype; sums, maxima and results are fp32 until they are rounded once.  workspace: nkv_page_attend_workspace_bytes(...) bytes
+ * of device scratch (16-byte aligned), no two calls in flight on the same.
+ */
+size_t nkv_page_attend_workspace_bytes(const nkv_page_cache* cache, int heads, int tokens);
+int nkv_page_attend(const nkv_page_cache* cache, const nkv_tokens* q, int tokens, const int32_t* counts, const uint32_t* mask,
+                    int64_t mask_stride, int causal, float scale, void* out, float* lse, int32_t* status_word, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* The accepted path of a draft: rows of pending tokens path[b][j] (DEVICE i32 [batch][accepted], ascending), j < counts[b] (DEVICE; NULL:
+ * `accepted`), moved to pending places j, in all `count` caches (HOST array; they share batch, table, lengths and shape; layers).
+ * Lengths stay as they are: the caller adds counts to them, once for all layers. */
+int nkv_page_keep(const nkv_page_cache* caches, int count, const int32_t* path, int accepted, const int32_t* counts,
+                  int32_t* status_word, void* stream);
+
+/* What every node of a draft sees: parents i32 [batch][tokens], each before its node, -1 for a node that follows the settled tokens ->
+ * mask u32 [batch][tokens][ceil(tokens / 32)], the bits of a node and its ancestors, and depth i32 [batch][tokens], how
+ * many ancestors it has.  tokens <= 4096.  A parent that does not come before its node counts as -1 and leaves status 921. */
+int nkv_tree_mask(const int32_t* parents, int batch, int tokens, uint32_t* mask, int32_t* depth, int32_t* status_word, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

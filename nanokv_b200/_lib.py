@@ -56,6 +56,13 @@ class BlockCache(ctypes.Structure):
                 ("dtype", c_int32)]
 
 
+class PageCache(ctypes.Structure):
+    """struct nkv_page_cache"""
+    _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p), ("table", c_void_p), ("lengths", c_void_p),
+                ("batch", c_int32), ("row_pages", c_int32), ("pages", c_int32), ("page", c_int32),
+                ("kv_heads", c_int32), ("head_dim", c_int32), ("dtype", c_int32)]
+
+
 class Tokens(ctypes.Structure):
     """struct nkv_tokens"""
     _fields_ = [("data", c_void_p), ("stride_batch", c_int64), ("stride_token", c_int64), ("stride_head", c_int64),
@@ -172,6 +179,13 @@ SIGNATURES = {
                                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "nkv_block_evict": (c_int, [c_void_p, c_void_p, POINTER(c_int32), POINTER(c_int32), c_int, c_int, c_int, c_int,
                                 c_int, c_int, c_void_p, c_void_p, c_void_p]),
+    "nkv_page_append": (c_int, [POINTER(PageCache), POINTER(Tokens), POINTER(Tokens), POINTER(Tokens), c_void_p, c_int, c_void_p,
+                                POINTER(Rotation), c_void_p, c_void_p]),
+    "nkv_page_attend_workspace_bytes": (c_size_t, [POINTER(PageCache), c_int, c_int]),
+    "nkv_page_attend": (c_int, [POINTER(PageCache), POINTER(Tokens), c_int, c_void_p, c_void_p, c_int64, c_int, c_float, c_void_p,
+                                c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "nkv_page_keep": (c_int, [POINTER(PageCache), c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    "nkv_tree_mask": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p]),
 }
 
 _EXCEPTIONS = {NKV_ERR_INVALID: ValueError, NKV_ERR_TOO_LARGE: ValueError}
@@ -204,6 +218,7 @@ def check(status: int) -> None:
 
 
 STATUS_SCORE_RANGE = 950
+STATUS_PAGE, STATUS_TREE = 920, 921
 
 
 def check_device_status(word: int) -> None:
@@ -211,12 +226,18 @@ def check_device_status(word: int) -> None:
 
     The reads and the row decode write the site code of a bounded wait that gave up (its rows are then not
     results: their LSE is NaN, decoded rows are NaN), or STATUS_SCORE_RANGE when a row's scores left the window of the
-    online softmax (that row's LSE is NaN).  NKV_OK from the launching call only says that the
+    online softmax (that row's LSE is NaN).  The operators of the paged cache write STATUS_PAGE or STATUS_TREE where
+    device arrays that the host does not see hold what they cannot follow.  NKV_OK from the launching call only says that the
     launch was accepted; the word is valid once the stream has been synchronised."""
     if word == 0:
         return
     if word == STATUS_SCORE_RANGE:
         raise RuntimeError("nanokv_b200: attention scores of a row rose more than 2^96 above the "
                            "maximum of the tiles before them; that row's LSE is NaN")
+    if word == STATUS_PAGE:
+        raise RuntimeError("nanokv_b200: paged cache: a token without a page, or a length, count or path out of range; "
+                           "that token was not written, or read as zeros")
+    if word == STATUS_TREE:
+        raise RuntimeError("nanokv_b200: tree_mask: a parent that does not come before its node was taken as -1")
     kind = library().nkv_status_string(NKV_ERR_DEVICE_WAIT).decode()
     raise RuntimeError(f"nanokv_b200: {kind}: wait site {word}")

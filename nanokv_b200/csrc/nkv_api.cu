@@ -843,4 +843,107 @@ int nkv_block_evict(const float* weights, const int32_t* table, const int32_t* f
                      static_cast<cudaStream_t>(stream));
 }
 
+static int check_page_cache(const nkv_page_cache* c, const char* name) {
+  NKV_REQUIRE(c != nullptr, NKV_ERR_INVALID, "%s: cache is NULL", name);
+  NKV_REQUIRE(c->batch >= 0 && c->batch <= 65535 && c->kv_heads > 0 && c->kv_heads <= 65535, NKV_ERR_INVALID, "%s: batch=%d kv_heads=%d", name,
+              c->batch, c->kv_heads);
+  NKV_REQUIRE(c->page == 16 || c->page == 32 || c->page == 64 || c->page == 128, NKV_ERR_INVALID,
+              "%s: pages of %d tokens (16, 32, 64 and 128 are built)", name, c->page);
+  NKV_REQUIRE(c->pages > 0 && c->row_pages > 0 && static_cast<int64_t>(c->row_pages) * c->page <= (1 << 30) &&
+                  static_cast<int64_t>(c->pages) * c->kv_heads * c->page <= INT32_MAX,
+              NKV_ERR_INVALID, "%s: %d pages, %d entries a sequence", name, c->pages, c->row_pages);
+  NKV_REQUIRE(c->head_dim == 64 || c->head_dim == 128, NKV_ERR_UNSUPPORTED, "%s: head width %d (64 and 128 are built)", name, c->head_dim);
+  NKV_REQUIRE(c->dtype == NKV_BF16 || c->dtype == NKV_F16, NKV_ERR_INVALID, "%s: the cache's dtype must be bf16 or fp16", name);
+  NKV_REQUIRE(c->k_pages && c->v_pages && c->table && c->lengths, NKV_ERR_INVALID, "%s: cache with missing arrays", name);
+  NKV_REQUIRE(((reinterpret_cast<uintptr_t>(c->k_pages) | reinterpret_cast<uintptr_t>(c->v_pages)) & 15) == 0, NKV_ERR_INVALID,
+              "%s: pages must be 16-byte aligned", name);
+  return NKV_OK;
+}
+
+int nkv_page_append(const nkv_page_cache* cache, const nkv_tokens* k, const nkv_tokens* v, const nkv_tokens* q, void* q_out,
+                    int tokens, const int32_t* counts, const nkv_rotation* rotation, int32_t* status_word, void* stream) {
+  int rc = check_page_cache(cache, "page_append");
+  if (rc != NKV_OK) return rc;
+  NKV_REQUIRE(tokens >= 0 && tokens <= (1 << 28), NKV_ERR_INVALID, "page_append: tokens=%d", tokens);
+  if (tokens == 0 || cache->batch == 0) return NKV_OK;
+  NKV_REQUIRE(k && v && k->data && v->data && status_word, NKV_ERR_INVALID, "page_append: rows or status word missing");
+  NKV_REQUIRE(k->heads == cache->kv_heads && v->heads == cache->kv_heads, NKV_ERR_INVALID, "page_append: %d and %d heads for a cache of %d",
+              k->heads, v->heads, cache->kv_heads);
+  if (q) {
+    NKV_REQUIRE(rotation != nullptr, NKV_ERR_INVALID, "page_append: queries without a rotation");
+    NKV_REQUIRE(q->heads > 0 && q->heads <= 65535 && q->data && q_out && (reinterpret_cast<uintptr_t>(q_out) & 15) == 0, NKV_ERR_INVALID,
+                "page_append: %d query heads, queries or their results missing or not 16-byte aligned", q->heads);
+  }
+  if (rotation) {
+    nkv_rotation turns = *rotation;
+    if (!turns.positions) turns.positions = cache->lengths;   // (they follow the lengths)
+    rc = check_rotation(&turns, cache->head_dim, "page_append");
+    if (rc != NKV_OK) return rc;
+    NKV_REQUIRE(rotation->rotary_dim % 16 == 0, NKV_ERR_INVALID, "page_append: rotary_dim %d must be a multiple of 16", rotation->rotary_dim);
+  }
+  const int64_t units = static_cast<int64_t>(cache->batch) * tokens * (2ll * cache->kv_heads + (q ? q->heads : 0)) * (cache->head_dim / 16);
+  NKV_REQUIRE(units <= (1ll << 38), NKV_ERR_TOO_LARGE, "page_append: %d sequences of %d tokens", cache->batch, tokens);
+  return page_append(*cache, *k, *v, q, q_out, tokens, counts, rotation, status_word, static_cast<cudaStream_t>(stream));
+}
+
+static int check_page_attend(const nkv_page_cache* cache, int heads, int tokens) {
+  int rc = check_page_cache(cache, "page_attend");
+  if (rc != NKV_OK) return rc;
+  NKV_REQUIRE(heads > 0 && heads % cache->kv_heads == 0, NKV_ERR_INVALID, "page_attend: %d query heads over %d kv heads", heads, cache->kv_heads);
+  NKV_REQUIRE(tokens >= 0 && static_cast<int64_t>(tokens) * (heads / cache->kv_heads) <= (1 << 28), NKV_ERR_TOO_LARGE,
+              "page_attend: %d tokens of %d heads", tokens, heads);
+  return NKV_OK;
+}
+
+size_t nkv_page_attend_workspace_bytes(const nkv_page_cache* cache, int heads, int tokens) {
+  if (check_page_attend(cache, heads, tokens) != NKV_OK || cache->batch == 0 || tokens == 0) return 0;
+  return page_attend_workspace_bytes(*cache, heads, tokens);
+}
+
+int nkv_page_attend(const nkv_page_cache* cache, const nkv_tokens* q, int tokens, const int32_t* counts, const uint32_t* mask,
+                    int64_t mask_stride, int causal, float scale, void* out, float* lse, int32_t* status_word, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  NKV_REQUIRE(q != nullptr, NKV_ERR_INVALID, "page_attend: no queries");
+  int rc = check_page_attend(cache, q->heads, tokens);
+  if (rc != NKV_OK) return rc;
+  if (tokens == 0 || cache->batch == 0) return NKV_OK;
+  NKV_REQUIRE(q->data && out && lse && status_word, NKV_ERR_INVALID, "page_attend: queries, results or status word missing");
+  NKV_REQUIRE((reinterpret_cast<uintptr_t>(out) & 15) == 0, NKV_ERR_INVALID, "page_attend: results must be 16-byte aligned");
+  const int64_t words = (static_cast<int64_t>(tokens) + 31) / 32 * tokens;
+  NKV_REQUIRE(!mask || mask_stride == 0 || mask_stride >= words, NKV_ERR_INVALID, "page_attend: masks of %lld words lie %lld apart",
+              static_cast<long long>(words), static_cast<long long>(mask_stride));
+  NKV_REQUIRE(scale - scale == 0.f, NKV_ERR_INVALID, "page_attend: scale is not finite");
+  const size_t need = page_attend_workspace_bytes(*cache, q->heads, tokens);
+  NKV_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0)), NKV_ERR_INVALID,
+              "page_attend: workspace of %zu bytes is too small or not 16-byte aligned (%zu)", workspace_bytes, need);
+  return page_attend(*cache, *q, tokens, counts, mask, mask_stride, causal != 0, scale, out, lse, status_word, workspace,
+                     static_cast<cudaStream_t>(stream));
+}
+
+int nkv_page_keep(const nkv_page_cache* caches, int count, const int32_t* path, int accepted, const int32_t* counts,
+                  int32_t* status_word, void* stream) {
+  NKV_REQUIRE(count >= 0 && accepted >= 0, NKV_ERR_INVALID, "page_keep: %d caches, %d tokens", count, accepted);
+  NKV_REQUIRE(caches || count == 0, NKV_ERR_INVALID, "page_keep: cache is NULL");
+  for (int i = 0; i < count; ++i) {
+    const int rc = check_page_cache(caches + i, "page_keep");
+    if (rc != NKV_OK) return rc;
+    const nkv_page_cache &a = caches[0], &b = caches[i];
+    NKV_REQUIRE(a.batch == b.batch && a.row_pages == b.row_pages && a.pages == b.pages && a.page == b.page && a.kv_heads == b.kv_heads &&
+                    a.head_dim == b.head_dim && a.table == b.table && a.lengths == b.lengths,
+                NKV_ERR_INVALID, "page_keep: cache %d does not share the table and shape of the first", i);
+    for (int j = 0; j < i; ++j)   // (its rows would be moved twice)
+      NKV_REQUIRE(caches[j].k_pages != b.k_pages && caches[j].v_pages != b.v_pages, NKV_ERR_INVALID, "page_keep: caches %d and %d are one", j, i);
+  }
+  if (count == 0 || accepted == 0 || caches[0].batch == 0) return NKV_OK;
+  NKV_REQUIRE(path && status_word, NKV_ERR_INVALID, "page_keep: path or status word missing");
+  return page_keep(caches, count, path, accepted, counts, status_word, static_cast<cudaStream_t>(stream));
+}
+
+int nkv_tree_mask(const int32_t* parents, int batch, int tokens, uint32_t* mask, int32_t* depth, int32_t* status_word, void* stream) {
+  NKV_REQUIRE(batch >= 0 && batch <= 65535 && tokens >= 0 && tokens <= 4096, NKV_ERR_INVALID, "tree_mask: batch=%d tokens=%d", batch, tokens);
+  if (batch == 0 || tokens == 0) return NKV_OK;
+  NKV_REQUIRE(parents && mask && depth && status_word, NKV_ERR_INVALID, "tree_mask: arrays missing");
+  return tree_mask(parents, batch, tokens, mask, depth, status_word, static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

@@ -81,6 +81,17 @@ int block_attend(const nkv_block_cache& c, const nkv_tokens& q, int tokens, cons
 int block_evict(const float* weights, const int32_t* table, const int32_t* full, const int32_t* partial, int batch, int kv_heads,
                 int blocks, int keep, int sinks, int recent, float* weights_out, int32_t* table_out, cudaStream_t stream);
 
+// ---- paged 16-bit cache (nkv_page_cache.cu, nkv_page_attn.cu)
+int page_append(const nkv_page_cache& c, const nkv_tokens& k, const nkv_tokens& v, const nkv_tokens* q, void* q_out, int tokens,
+                const int32_t* counts, const nkv_rotation* rotation, int32_t* status, cudaStream_t stream);
+int page_keep(const nkv_page_cache* caches, int count, const int32_t* path, int accepted, const int32_t* counts, int32_t* status,
+              cudaStream_t stream);
+int tree_mask(const int32_t* parents, int batch, int tokens, uint32_t* mask, int32_t* depth, int32_t* status, cudaStream_t stream);
+size_t page_attend_workspace_bytes(const nkv_page_cache& c, int heads, int tokens);
+int page_attend(const nkv_page_cache& c, const nkv_tokens& q, int tokens, const int32_t* counts, const uint32_t* mask,
+                int64_t mask_stride, bool causal, float scale, void* out, float* lse, int32_t* status, void* workspace,
+                cudaStream_t stream);
+
 // ---- tcgen05 / TMA kernels (nkv_tc_*.cu), bf16 operands, fp32 accumulation
 int tc_assign(const void* x_bf16, const void* centers_bf16, int S, int J, int C, void* ids,
               int id_bytes, cudaStream_t stream);

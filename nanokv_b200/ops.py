@@ -864,3 +864,81 @@ def block_evict(weights: torch.Tensor, table: torch.Tensor, full, partial, *, ke
                                                   keep, sinks, recent, weights_out.data_ptr(),
                                                   table_out.data_ptr(), _raw_stream(device)))
     return table_out, weights_out
+
+
+# ------------------------------------------------------------------ paged 16-bit cache
+PAGES = (16, 32, 64, 128)   # tokens of a page
+
+
+def _device_ints(x: torch.Tensor | None, shape: tuple, name: str, device: torch.device) -> int | None:
+    """Address of int32 device memory that calls read when they run, not when they are made."""
+    if x is None:
+        return None
+    if not isinstance(x, torch.Tensor) or x.dtype != torch.int32 or tuple(x.shape) != shape:
+        raise ValueError(f"{name} must be an int32 tensor {list(shape)}")
+    if not x.is_contiguous() or x.device != device:
+        raise ValueError(f"{name} must be contiguous, on {device}")
+    return x.data_ptr()
+
+
+def page_append(struct: _lib.PageCache, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None, *, counts=None,
+                rotation: _lib.Rotation | None = None):
+    """Pending tokens k, v [batch, tokens, kv_heads, width] put behind the settled ones (nkv_page_append) -> q rotated, or None."""
+    out = None if q is None else torch.empty_like(q, memory_format=torch.contiguous_format)
+    _lib.check(_lib.library().nkv_page_append(
+        struct, _rows(k, "k"), _rows(v, "v"), None if q is None else _rows(q, "q"), None if q is None else out.data_ptr(),
+        k.shape[1], _device_ints(counts, (struct.batch,), "counts", k.device), rotation, status_word(k.device).data_ptr(),
+        _raw_stream(k.device)))
+    return out
+
+
+def page_attend(struct: _lib.PageCache, q: torch.Tensor, *, counts=None, tree: torch.Tensor | None = None, causal: bool = True,
+                scale: float, status: torch.Tensor | None = None):
+    """Attention of pending queries q [batch, tokens, heads, width] (nkv_page_attend) -> (O like q, lse f32 [batch, tokens,
+    heads]).  ``tree`` i32 [tokens, words] or [batch, tokens, words]: bits of the pending tokens that each query sees."""
+    rows = _rows(q, "q")
+    batch, tokens, heads, _ = q.shape
+    words, stride = -(-tokens // 32), 0
+    if tree is not None:
+        shared = tree.dim() == 2
+        bits = _device_ints(tree, (tokens, words) if shared else (batch, tokens, words), "tree", q.device)
+        stride = 0 if shared else tokens * words
+    lib = _lib.library()
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
+    nbytes = lib.nkv_page_attend_workspace_bytes(struct, heads, tokens)
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    word = status_word(q.device) if status is None else status
+    _lib.check(lib.nkv_page_attend(
+        struct, rows, tokens, _device_ints(counts, (batch,), "counts", q.device), None if tree is None else bits, stride, int(causal),
+        float(scale), out.data_ptr(), lse.data_ptr(), word.data_ptr(), workspace.data_ptr() if nbytes else None, nbytes,
+        _raw_stream(q.device)))
+    return out, lse
+
+
+def page_keep(structs, path: torch.Tensor, counts: torch.Tensor | None = None) -> None:
+    """Rows of the pending tokens that ``path`` i32 [batch, accepted] lists moved to the front of them, in every cache
+    (nkv_page_keep)."""
+    batch, accepted = structs[0].batch, path.shape[1]
+    caches = (_lib.PageCache * len(structs))(*structs)
+    device = path.device
+    _lib.check(_lib.library().nkv_page_keep(
+        caches, len(structs), _device_ints(path, (batch, accepted), "path", device), accepted,
+        _device_ints(counts, (batch,), "counts", device), status_word(device).data_ptr(), _raw_stream(device)))
+
+
+def tree_mask(parents: torch.Tensor):
+    """What the nodes of a draft see (nkv_tree_mask): parents i32 [tokens] or [batch, tokens], each before its node, -1 for one
+    that follows the settled tokens -> (mask i32 [.., tokens, ceil(tokens / 32)] with the bits of a node and its ancestors, depth
+    i32 [.., tokens])."""
+    device = _require_cuda(parents)
+    if parents.dtype != torch.int32 or parents.dim() not in (1, 2):
+        raise ValueError(f"parents must be int32 [tokens] or [batch, tokens]; got {parents.dtype} {list(parents.shape)}")
+    tokens = parents.shape[-1]
+    mask = torch.empty(*parents.shape, -(-tokens // 32), dtype=torch.int32, device=device)
+    depth = torch.empty_like(parents)
+    with _On(device):
+        _lib.check(_lib.library().nkv_tree_mask(
+            parents.data_ptr(), parents.shape[0] if parents.dim() == 2 else 1, tokens, mask.data_ptr(), depth.data_ptr(),
+            status_word(device).data_ptr(), _raw_stream(device)))
+    return mask, depth
