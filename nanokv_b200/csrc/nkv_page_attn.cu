@@ -5,7 +5,8 @@
 namespace nkv {
 namespace {
 
-// The formula as it stands, in fp32: a warp per row, the rows of a thread block share 64 tokens of K and V at a time.
+// The formula as it stands, in fp32: a warp per row, the rows of a thread block share 64 tokens of K and V at a time.  Runs where the
+// tensor-core kernel is switched off, to check it.
 constexpr int ROWS = 8, STEP = 64;
 template <int DT, int D>
 __global__ void __launch_bounds__(32 * ROWS)
@@ -85,7 +86,9 @@ page_plain_kernel(PageArrays c, PageCall a, int32_t* status) {
 
 }  // namespace
 
-size_t page_attend_workspace_bytes(const nkv_page_cache& c, int heads, int tokens) { return 0; }
+size_t page_attend_workspace_bytes(const nkv_page_cache& c, int heads, int tokens) {
+  return page_tile_bytes(heads / c.kv_heads * tokens, c.head_dim);   // launches follow one another on the stream and share it
+}
 
 int page_attend(const nkv_page_cache& c, const nkv_tokens& q, int tokens, const int32_t* counts, const uint32_t* mask,
                 int64_t mask_stride, bool causal, float scale, void* out, float* lse, int32_t* status, void* workspace,
@@ -111,6 +114,11 @@ int page_attend(const nkv_page_cache& c, const nkv_tokens& q, int tokens, const 
     a.scale_log2 = scale * LOG2E;
     a.q_vector = (reinterpret_cast<uintptr_t>(a.q) & 15) == 0 && a.q_batch % 8 == 0 && a.q_token % 8 == 0 && a.q_head % 8 == 0;
     const PageArrays arrays = page_arrays(c, first);
+    if (!simt_forced()) {
+      const int rc = page_tile(arrays, a, n, c.dtype, c.head_dim, workspace, status, stream);
+      if (rc != NKV_OK) return rc;
+      continue;
+    }
     auto kernel = c.head_dim == 128 ? (c.dtype == NKV_BF16 ? page_plain_kernel<NKV_BF16, 128> : page_plain_kernel<NKV_F16, 128>)
                                     : (c.dtype == NKV_BF16 ? page_plain_kernel<NKV_BF16, 64> : page_plain_kernel<NKV_F16, 64>);
     const int smem = static_cast<int>(sizeof(float)) * (STEP * (2 * c.head_dim + 1) + ROWS * (c.head_dim + STEP));

@@ -1,0 +1,855 @@
+// Attention over the paged 16-bit cache, on tcgen05.
+//
+// The rows of a kv head (its group's heads of all pending tokens) are the left operand of both products: S = Q K^T of a tile
+// of 128 tokens goes to tensor memory, eight warps take the softmax (a thread per row), P replaces S as the operand of O += P V.  One
+// warp brings K and V as they lie, page by page, into a ring of swizzled tiles.  Two forms, by the rows a kv head has:
+//
+//   wide    more than 128: units of 256 rows, two query tiles that share every K and V tile, four warps each.
+//   narrow  up to 128, one query tile; the two groups of four warps take the even and the odd tiles of its tokens, each with sums of
+//           its own.  With at most 128 / COPIES rows, COPIES of them stand in the query tile one below the other, and
+//           every copy takes its share of a tile's tokens: the weights of the others are stored as zeros.  That cuts what one
+//           thread does per tile, which is what a tile takes.  The sums of all are joined in shared memory.
+//
+// Softmax: P' = 2^(s - m) with a reference m that follows the running maximum of the scaled scores, s; it moves when P' would pass
+// 2^8 times what it was set to.  bf16: set so that the sum of a row's P' stays below 1, O = sum P' V then below the largest |V|, any
+// number of bf16.  fp16: P' up to 2^15, so that weights down to 2^-29 of the largest keep all their bits.  P' is rounded to the cache's
+// type, as the tensor cores take it; the row sum, the maximum and O stay in fp32.
+//
+// Pending tokens that some row does not see, and whatever lies in a page behind a sequence's last token, are masked in the scores.  A weight
+// of 0 times a value that is not finite would be NaN, so four warps look at the V tiles with such tokens: values behind the
+// last token become 0 in shared memory, and so do values that are not finite; rows that see them get them added at the end, from memory.
+//
+// Table, lengths and counts are read by the kernel: every thread block makes the plan (nkv_page_plan.h) for itself.  The tiles of all
+// units form one list that the SMs take in equal runs; a unit that a run's end cuts leaves fp32 parts, joined by a second launch.
+// Warps: 0-7 softmax, 8-11 queries and masked values, 12 MMA issue, 13 pages.
+#include "nkv_internal.h"
+#include "nkv_page.cuh"
+#include "nkv_tile.cuh"
+
+namespace nkv {
+namespace {
+
+using namespace tc;
+using page::Piece;
+using page::Plan;
+using page::Shape;
+using page::TOK;
+using page::Walk;
+
+constexpr int QT = 128;                           // rows of a query tile
+constexpr int SUB = 128 * 128;                    // bytes of a [128 rows x 64 elements] swizzled tile
+constexpr int SOFTMAX_WARPS = 8, OPERAND_WARPS = 4, MMA_WARP = 12, THREADS = 448;
+constexpr float RESCALE_THRESHOLD = 8.0f;
+constexpr float NOTHING = -3e38f;                 // the reference before the first score: below all, and a number
+
+// (P_READY: chain i, half h of a tile's tokens at 2 i + h)
+enum Bar { Q_FULL = 0, Q_FREE = 1, S_FULL = 2, P_READY = 4, PV_HALF = 8, O_DONE = 10, O_FREE = 12, FULL = 14, FREE = 24, CLEAN = 34, DRAINED = 44, NUM_BARS = 45 };
+constexpr int M_SLOT = NUM_BARS * 8, M_ABORT = M_SLOT + 4, M_STRAY = M_SLOT + 8, M_EXTENTS = 384;
+constexpr int M_START = M_EXTENTS + page::MOST_SEQUENCES * static_cast<int>(sizeof(page::Extent)), META = 2048;
+static_assert(M_STRAY + 4 <= M_EXTENTS && M_START + 4 * (page::MOST_SEQUENCES + 1) <= META && page::MOST_SEQUENCES < 128, "meta block");
+
+// COPIES 0: the wide form
+template <int D, int COPIES> struct Layout {
+  static constexpr bool NARROW = COPIES > 0;
+  static constexpr int QTILES = NARROW ? 1 : 2, UNIT = QTILES * QT;
+  static constexpr int DCH = D / 64;
+  static constexpr int STAGE = DCH * SUB, STAGES = D == 128 ? 5 : 10;
+  static constexpr int LEAD = NARROW ? 2 : 1;      // K tiles ahead of the first V tile in the ring
+  static constexpr int Q_OFF = META;
+  static constexpr int RING_OFF = Q_OFF + QTILES * DCH * SUB;
+  static constexpr int ML_OFF = RING_OFF + STAGES * STAGE;             // narrow: references and sums of 256 threads
+  static constexpr int JOIN_OFF = ML_OFF + (NARROW ? 256 * 8 : 0);     // narrow: 16 columns of O of 256 threads, a row of 17 each
+  static constexpr int BYTES = JOIN_OFF + (NARROW ? 256 * 17 * 4 : 0);
+  static constexpr int DYNAMIC = BYTES + 1024;     // room to start on 1,024 bytes
+  static constexpr int HALVES = COPIES >= 2 ? 1 : 2, WIDTH = COPIES == 4 ? 32 : 64;   // tokens that a thread takes at a time
+};
+static_assert(Layout<128, 0>::DYNAMIC <= 232448 && Layout<64, 0>::DYNAMIC <= 232448, "shared memory");
+
+// places of a piece's tiles in the ring: LEAD tiles of K, then a V tile and a K tile in turn
+template <class L> __device__ __forceinline__ uint32_t place_of_k(uint32_t t) { return t < L::LEAD ? t : 2 * t - L::LEAD + 1; }
+template <class L> __device__ __forceinline__ uint32_t place_of_v(uint32_t t, uint32_t nt) { return t + min(nt, L::LEAD + t); }
+// the n-th tile of a piece in the ring
+template <class L> __device__ __forceinline__ int ring_tile(int n, int nt, bool& value) {
+  const int lead = min(nt, L::LEAD), k = n - lead, pairs = max(0, nt - L::LEAD);   // K ahead; V 0, K lead, V 1, ...; then V alone
+  value = k >= 0 && (k >= 2 * pairs || (k & 1) == 0);
+  return k < 0 ? n : k >= 2 * pairs ? k - pairs : value ? k / 2 : k / 2 + L::LEAD;
+}
+
+// steps of chain i of a piece, and the tile of a step: query tile i over the tiles it sees, or every other tile
+template <class L> __device__ __forceinline__ int steps_of(const Shape& s, const Extent& e, const Piece& p, int i) {
+  if (L::NARROW) return (p.nt - i + 1) / 2;
+  return max(0, min(p.nt, page::tiles_seen(s, e, p.unit * L::UNIT + i * QT, QT) - p.tile0));
+}
+template <class L> __device__ __forceinline__ int tile_of(int i, int step) { return L::NARROW ? 2 * step + i : step; }
+
+// tokens from the first on that all rows of a unit see, where they are asked for
+__device__ __forceinline__ int seen_by_all(const Shape& s, const Extent& e, const Piece& p) {
+  return page::sees_all_before(s.sight, e, p.unit * s.unit / s.group);
+}
+
+// A run holds at most one piece that starts inside a unit and one that starts with it and is cut: two places each.  Behind them what
+// the second launch needs of the plan.
+struct Parts {
+  float* o;             // [2 runs][unit rows][D], relative to 2^m
+  float2* ml;           // [2 runs][unit rows] m, row sum
+  page::Extent* extents;
+  uint32_t* start;
+};
+
+struct TileCall : PageCall {
+  Shape shape;
+  int sequences;
+};
+
+// ---- warp 13: pages ------------------------------------------------------------------------------------------------
+template <int D, int COPIES>
+__device__ __forceinline__ void page_role(uint8_t* smem, uint64_t* bars, const CUtensorMap* map_k, const CUtensorMap* map_v, const PageArrays& c,
+                                          const TileCall& a, const Plan& plan, const Ctx& ctx, int32_t* status) {
+  using L = Layout<D, COPIES>;
+  const int lane = threadIdx.x & 31, rows = 1 << c.shift, per_tile = TOK >> c.shift;
+  const int nowhere = c.pages * c.kv_heads << c.shift;   // behind the last row of the pool: read as zeros
+  if (lane == 0) {
+    prefetch_tensormap(map_k);
+    prefetch_tensormap(map_v);
+  }
+  Walk walk(plan, a.shape, blockIdx.x);
+  Piece p;
+  bool ok = true, bad = false;
+  uint32_t item = 0;
+  while (ok && walk.next(plan, a.shape, p)) {
+    const Extent e = plan.extents[p.b];
+    const int total = e.length + e.there;
+    const int32_t* const entries = c.table + static_cast<size_t>(p.b) * c.row_pages;
+    // lane l knows entry 32 w + l of the table: of K's window, the one before (V lags behind) and the next
+    auto window = [&](int w) {
+      const int entry = 32 * w + lane;
+      return entry < c.row_pages && entry << c.shift < total ? __ldg(entries + entry) : -1;
+    };
+    int now = p.tile0 * per_tile / 32, before = -1, here = window(now), after = window(now + 1);
+    for (int n = 0; n < 2 * p.nt && ok; ++n, ++item) {
+      // n-th tile of the piece in the order of the ring
+      bool value;
+      const int t = ring_tile<L>(n, p.nt, value);
+      const uint32_t stage = item % L::STAGES, use = item / L::STAGES;
+      const int entry = (p.tile0 + t) * per_tile, w = entry / 32;
+      if (w > now) {
+        before = here;
+        here = after;
+        now = w;
+        after = window(now + 1);
+      }
+      const int chunk = lane / per_tile, at = lane % per_tile;
+      const int id = __shfl_sync(0xffffffffu, w == now ? here : before, (entry + at) & 31);
+      const int first = (p.tile0 + t) * TOK, pages = min(per_tile, (total - first + rows - 1) >> c.shift);
+      if (use > 0) ok = wait(&bars[FREE + stage], (use - 1) & 1, ctx, 930);
+      if (!ok) break;
+      if (lane == 0) mbar_arrive_expect_tx(&bars[FULL + stage], static_cast<uint32_t>(pages << c.shift) * D * 2);
+      __syncwarp();
+      if (chunk < L::DCH && at < pages) {
+        const bool in = static_cast<unsigned>(id) < static_cast<unsigned>(c.pages);
+        bad |= !in;
+        tma_load_2d(smem + L::RING_OFF + stage * L::STAGE + chunk * SUB + (at << c.shift) * 128, value ? map_v : map_k, chunk * 64,
+                    in ? (id * c.kv_heads + p.h) << c.shift : nowhere, &bars[FULL + stage]);
+      }
+      __syncwarp();
+    }
+  }
+  if (bad) report(status, STATUS_PAGE);
+  if (!ok) {   // copies in flight land before the block goes away
+    const long long begin = clock64();
+    while (clock64() - begin < (1ll << 21)) {}
+  }
+}
+
+// ---- warps 8-11: queries, and values that rows do not see --------------------------------------------------------------
+template <int DT> __device__ __forceinline__ bool not_finite(uint32_t bits16) {
+  constexpr uint32_t E = DT == NKV_BF16 ? 0x7F80u : 0x7C00u;
+  return (bits16 & E) == E;
+}
+
+template <int DT, int D, int COPIES>
+__device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, const PageArrays& c, const TileCall& a, const Plan& plan, const Ctx& ctx) {
+  using L = Layout<D, COPIES>;
+  const int tid = threadIdx.x - 32 * SOFTMAX_WARPS, lane = tid & 31;
+  const uint32_t base = smem_u32(smem);
+  // queries: a thread has one 16-byte column of every ROWS-th row of the unit
+  constexpr int PER_ROW = D / 8, ROWS = 32 * OPERAND_WARPS / PER_ROW, AHEAD = 8, APART = L::NARROW ? QT / (COPIES > 0 ? COPIES : 1) : L::UNIT;
+  const int q_row = tid / PER_ROW, q_col = tid % PER_ROW * 8;
+  const uint32_t q_to = base + L::Q_OFF + (q_col / 64) * SUB;
+  const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;   // a negative scale is the queries' sign
+  volatile int* const stray = reinterpret_cast<volatile int*>(smem + M_STRAY);
+  Walk walk(plan, a.shape, blockIdx.x);
+  Piece p;
+  bool ok = true;
+  int pieces = 0;
+  uint32_t item = 0;    // tiles in the ring so far
+  while (ok && walk.next(plan, a.shape, p)) {
+    const Extent e = plan.extents[p.b];
+    const uint16_t* const q_head = a.q + p.b * a.q_batch + static_cast<long long>(p.h) * a.group * a.q_head + q_col;
+    // the first rows are on their way while the piece before still reads its own
+#pragma unroll 1
+    for (int row0 = q_row; row0 < L::UNIT && ok; row0 += AHEAD * ROWS) {
+      uint4 v[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int r = p.unit * L::UNIT + (row0 + k * ROWS) % APART, token = r / a.group;
+        v[k] = make_uint4(0, 0, 0, 0);
+        if (r < a.rows) {
+          const uint16_t* const src = q_head + token * a.q_token + (r - token * a.group) * a.q_head;
+          v[k] = a.q_vector ? __ldg(reinterpret_cast<const uint4*>(src)) : gather16(src);
+        }
+      }
+      if (row0 == q_row && pieces > 0) ok = wait(&bars[Q_FREE], (pieces - 1) & 1, ctx, 931);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int row = row0 + k * ROWS;
+        sts128(q_to + (row / QT) * L::DCH * SUB + sw128_offset(row % QT, q_col % 64),
+               make_uint4(v[k].x ^ flip, v[k].y ^ flip, v[k].z ^ flip, v[k].w ^ flip));
+      }
+    }
+    if (!ok) break;
+    ++pieces;
+    fence_proxy_async();
+    warp_arrive(&bars[Q_FULL], lane);
+    // ---- V tiles with tokens that some row does not see: a thread per token.  Every tile of the ring is waited for, K's and those
+    // that all rows see too: a wait tells a phase from its neighbours only.
+    const int total = e.length + e.there, masked = seen_by_all(a.shape, e, p) / TOK - p.tile0;
+    for (int n = 0; n < 2 * p.nt && ok; ++n, ++item) {
+      const uint32_t stage = item % L::STAGES;
+      ok = wait(&bars[FULL + stage], (item / L::STAGES) & 1, ctx, 932);
+      if (!ok) break;
+      bool value;
+      const int t = ring_tile<L>(n, p.nt, value);
+      if (!value || t < masked) continue;
+      const bool behind = (p.tile0 + t) * TOK + tid >= total;
+      const uint32_t row = base + L::RING_OFF + stage * L::STAGE + tid * 128;
+#pragma unroll 1
+      for (int ch = 0; ch < L::DCH; ++ch) {
+#pragma unroll 4
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t at = row + ch * SUB + ((k ^ (tid & 7)) << 4);   // (lanes of a row group take different banks)
+          if (behind) {
+            sts128(at, make_uint4(0, 0, 0, 0));
+            continue;
+          }
+          const uint4 v = lds128(at);
+          uint32_t w[4] = {v.x, v.y, v.z, v.w};
+          bool found = false;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool lo = not_finite<DT>(w[i]), hi = not_finite<DT>(w[i] >> 16);
+            found |= lo || hi;
+            w[i] &= (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
+          }
+          if (found) {
+            sts128(at, make_uint4(w[0], w[1], w[2], w[3]));
+            *stray = 1;
+          }
+        }
+      }
+      fence_proxy_async();
+      warp_arrive(&bars[CLEAN + stage], lane);
+    }
+  }
+}
+
+// ---- warp 12: MMA issue -----------------------------------------------------------------------------------------
+template <int DT, int D, int COPIES>
+__device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t tmem, const TileCall& a, const Plan& plan, const Ctx& ctx) {
+  using L = Layout<D, COPIES>;
+  constexpr int DCH = L::DCH;
+  const bool leader = elect_one();   // the whole warp runs the (uniform) control flow; one elected lane issues
+  const uint32_t base = smem_u32(smem);
+  const uint64_t q_desc = make_smem_desc_sw128(base + L::Q_OFF), k_desc = make_smem_desc_sw128(base + L::RING_OFF);
+  const uint64_t v_desc = make_smem_desc_sw128_mn(base + L::RING_OFF, SUB);
+  auto issue_s = [&](int i, uint32_t stage) {
+    const uint64_t qd = q_desc + (L::NARROW ? 0u : static_cast<uint32_t>(i * (DCH * SUB / 16))), kd = k_desc + stage * static_cast<uint32_t>(L::STAGE / 16);
+    const uint32_t d = tmem + i * 128;
+#pragma unroll
+    for (int ch = 0; ch < DCH; ++ch)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (leader) mma_bf16(d, qd + ch * (SUB / 16) + 2 * k, kd + ch * (SUB / 16) + 2 * k, idesc<DT>(TOK), ch + k > 0);
+    if (leader) mma_commit(&bars[S_FULL + i]);
+  };
+  // weights of TOK / HALVES tokens times V of them: V's rows are tokens, its columns the result's
+  auto issue_pv = [&](int i, uint32_t stage, int half, bool accumulate) {
+    constexpr int STEPS = 8 / L::HALVES;
+    const uint64_t vd = v_desc + stage * static_cast<uint32_t>(L::STAGE / 16) + half * STEPS * 128u;
+    const uint32_t d = tmem + 256 + i * 128, w = tmem + i * 128 + half * STEPS * 8;
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k)
+      if (leader) mma_bf16_ts(d, w + 8 * k, vd + 128 * k, idesc<DT>(D) | (1u << 16), accumulate || k > 0);
+    if (L::HALVES == 2 && half == 0 && leader) mma_commit(&bars[PV_HALF + i]);
+  };
+  Walk walk(plan, a.shape, blockIdx.x);
+  Piece p;
+  bool ok = true;
+  uint32_t items = 0, cleaned = 0;                 // tiles in the ring of the pieces before; phases of CLEAN, a bit per stage
+  int pieces = 0, done[2] = {0, 0}, used[2] = {0, 0};   // steps and pieces of each chain so far
+  while (ok && walk.next(plan, a.shape, p)) {
+    const Extent e = plan.extents[p.b];
+    const int n[2] = {steps_of<L>(a.shape, e, p, 0), steps_of<L>(a.shape, e, p, 1)};
+    const int longest = max(n[0], n[1]), masked = seen_by_all(a.shape, e, p) / TOK - p.tile0;   // tiles from here on are looked at
+    ok = wait(&bars[Q_FULL], pieces & 1, ctx, 933);
+    ++pieces;
+    // the first and the last chain to use a tile: each stage is waited for once and given back once
+    auto is_first = [&](int i, int step) { return L::NARROW || i == (step < n[0] ? 0 : 1); };
+    auto is_last = [&](int i, int step) { return L::NARROW || i == (step < n[1] ? 1 : 0); };
+#pragma unroll 1
+    for (int j = 0; j <= longest && ok; ++j) {
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        const int steps = i ? n[1] : n[0];
+        if (j > 0 && j - 1 < steps) {
+          const int t = tile_of<L>(i, j - 1);
+          const uint32_t item = items + place_of_v<L>(t, p.nt), stage = item % L::STAGES;
+          const uint32_t phase = ((i ? done[1] : done[0]) + j - 1) & 1;
+          if (is_first(i, j - 1)) {
+            if (t >= masked) {
+              ok = wait(&bars[CLEAN + stage], (cleaned >> stage) & 1, ctx, 934);
+              cleaned ^= 1u << stage;
+            } else {
+              ok = wait(&bars[FULL + stage], (item / L::STAGES) & 1, ctx, 935);
+            }
+          }
+          if (j == 1) {   // the first PV of a piece overwrites O: the rows of the piece before must have been read
+            const int before = i ? used[1] : used[0];
+            if (ok && before > 0) ok = wait(&bars[O_FREE + i], (before - 1) & 1, ctx, 936);
+          }
+          ok = ok && wait(&bars[P_READY + 2 * i], phase, ctx, 937);
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(i, stage, 0, j > 1);
+          if (L::HALVES == 2) {
+            ok = wait(&bars[P_READY + 2 * i + 1], phase, ctx, 938);
+            if (!ok) break;
+            tc_fence_after();
+            issue_pv(i, stage, 1, true);
+          }
+          if (j == steps && leader) mma_commit(&bars[O_DONE + i]);
+          if (is_last(i, j - 1) && leader) mma_commit(&bars[FREE + stage]);
+        }
+        if (j < steps) {
+          // S of the next step overwrites P of this one, right behind the PV that reads it: the tensor core executes one
+          // thread's MMAs in order
+          const uint32_t item = items + place_of_k<L>(tile_of<L>(i, j)), stage = item % L::STAGES;
+          if (is_first(i, j)) {
+            ok = wait(&bars[FULL + stage], (item / L::STAGES) & 1, ctx, 939);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          issue_s(i, stage);
+          if (is_last(i, j) && leader) mma_commit(&bars[FREE + stage]);
+        }
+      }
+    }
+    if (!ok) break;
+    if (leader) mma_commit(&bars[Q_FREE]);
+    items += 2 * p.nt;
+    for (int i = 0; i < 2; ++i) {
+      done[i] += n[i];
+      used[i] += n[i] > 0 ? 1 : 0;
+    }
+  }
+  if (!ok) {   // MMAs in flight end before tensor memory is given back (nobody looks at how: the launch has given up)
+    if (leader) mma_commit(&bars[DRAINED]);
+#pragma unroll 1
+    for (int i = 0; i < MOST_PARKED && !mbar_try_wait_parked(&bars[DRAINED], 0, 1000u); ++i) {}
+  }
+  __syncwarp();
+}
+
+// ---- warps 0-7: softmax -------------------------------------------------------------------------------------------
+
+// Values of column `col` that are not finite, of the tokens of a piece that were looked at and that query t sees.
+template <int DT>
+__device__ __noinline__ float strays(const PageArrays& c, const TileCall& a, Extent e, Piece p, int t, int col, int d) {
+  float sum = 0.f;
+  if (t >= e.count) return sum;
+  const int total = e.length + e.there, from = max(p.tile0, seen_by_all(a.shape, e, p) / TOK) * TOK, to = min((p.tile0 + p.nt) * TOK, total);
+  for (int first = from; first < to; first += 32) {
+    const uint32_t sees = sight_of(a, e, p.b, t, first);
+    for (int i = 0; i < 32 && first + i < to; ++i) {
+      if (!(sees >> i & 1)) continue;
+      const int at = page_of(c, p.b, first + i);
+      if (at < 0) continue;
+      const uint16_t bits = c.v[row_at(c, at, p.h, first + i, d) + col];
+      if (not_finite<DT>(bits)) sum += load_float(&bits, DT, 0);
+    }
+  }
+  return sum;
+}
+
+// barrier of the softmax warps; whether any of them passes `fails`
+__device__ __forceinline__ void softmax_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ bool softmax_any(bool fails) {
+  uint32_t any;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.or.pred q, 1, 256, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(any)
+      : "r"(static_cast<uint32_t>(fails))
+      : "memory");
+  return any != 0;
+}
+
+template <int DT, int D, int COPIES>
+__device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint32_t tmem, const PageArrays& c, const TileCall& a, const Plan& plan,
+                                             const Parts& parts, const Ctx& ctx) {
+  using L = Layout<D, COPIES>;
+  constexpr int WIDTH = L::WIDTH, GROUPS = WIDTH / 32, APART = QT / (COPIES > 0 ? COPIES : 1);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+  const int wg = warp / 4, row = tid & 127;
+  const int copy = COPIES > 1 ? row / APART : 0;
+  const uint32_t lane_sel = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+  const uint32_t o_addr = tmem + lane_sel + 256 + wg * 128;
+  const float scale = fabsf(a.scale_log2);
+  volatile int* const stray = reinterpret_cast<volatile int*>(smem + M_STRAY);
+  float2* const mls = reinterpret_cast<float2*>(smem + L::ML_OFF);
+  float* const join = reinterpret_cast<float*>(smem + L::JOIN_OFF);
+  Walk walk(plan, a.shape, blockIdx.x);
+  Piece p;
+  bool ok = true, more = true;
+  int ci = 0, pieces = 0;   // steps and pieces of this chain
+  auto place_of = [&](const Piece& pc) { return (2 * static_cast<size_t>(blockIdx.x) + (pc.tile0 == 0 ? 1 : 0)) * L::UNIT; };
+  // the row of the results that row r of a piece's kv head is
+  auto at_of = [&](const Piece& pc, int r) {
+    const int token = r / a.group;
+    return (static_cast<size_t>(pc.b) * a.tokens + token) * a.heads + pc.h * a.group + r - token * a.group;
+  };
+  while (ok && (more = walk.next(plan, a.shape, p))) {
+    const Extent e = plan.extents[p.b];
+    const int r = L::NARROW ? row % APART : p.unit * L::UNIT + wg * QT + row, token = r / a.group;
+    const bool real = r < a.rows;
+    const int clear = real ? page::sees_all_before(a.sight, e, token) : 0x7FFFFFFF;   // (rows of nobody are not masked)
+    const int clear_least = __reduce_min_sync(0xffffffffu, clear);
+    const int steps = steps_of<L>(a.shape, e, p, wg);
+    // where P' stands when the reference is set: see the top of the file
+    const float raise = DT == NKV_F16 ? 7.0f : -(RESCALE_THRESHOLD + 32 - __clz(e.length + e.there));
+    float m = NOTHING, l = 0.f;
+#pragma unroll 1
+    for (int n = 0; n < L::HALVES * steps && ok; ++n) {
+      const int half = L::HALVES == 2 ? n & 1 : 0, step = n / L::HALVES;
+      const int column = COPIES > 1 ? copy * WIDTH : half * WIDTH;   // of the tile's tokens
+      const int first = (p.tile0 + tile_of<L>(wg, step)) * TOK + column;
+      const uint32_t s_addr = tmem + lane_sel + wg * 128 + column, p_addr = tmem + lane_sel + wg * 128 + column / 2;
+      if (half == 0) {
+        ok = wait(&bars[S_FULL + wg], ci & 1, ctx, 940);
+        if (!ok) break;
+        tc_fence_after();
+      }
+      uint32_t raw[GROUPS][32];
+#pragma unroll
+      for (int k = 0; k < GROUPS; ++k) tmem_ld32_issue(s_addr + 32 * k, raw[k]);
+#pragma unroll
+      for (int k = 0; k < GROUPS; ++k) tmem_ld32_wait(raw[k]);
+      float f = scale;
+      if (first + WIDTH > clear_least) {   // some row of the warp does not see all of it
+        // scaled before they are masked: -inf times a scale of 0 would be NaN
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) {
+          const uint32_t sees = !real ? 0xFFFFFFFFu : token < e.count ? sight_of(a, e, p.b, token, first + 32 * k) : 0u;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            raw[k][j] = sees >> j & 1 ? __float_as_uint(__uint_as_float(raw[k][j]) * f) : 0xFF800000u;
+        }
+        f = 1.f;
+      }
+      float top = max32(raw[0]);
+#pragma unroll
+      for (int k = 1; k < GROUPS; ++k) top = fmaxf(top, max32(raw[k]));
+      top *= f;
+      if (__any_sync(0xffffffffu, top - m > raise + RESCALE_THRESHOLD)) {
+        // Move the reference: O and the sum are scaled by 2^(old - new).  S was issued behind PV of the step before and its commit
+        // covers both; PV of this tile's first half may still run.
+        const float m_new = fmaxf(m, top - raise), alpha = exp2f(m - m_new);
+        if (n > 0) {
+          if (half) {
+            ok = wait(&bars[PV_HALF + wg], ci & 1, ctx, 941);
+            if (!ok) break;
+            tc_fence_after();
+          }
+#pragma unroll 1
+          for (int cc = 0; cc < D / 16; ++cc) {
+            uint32_t v[16];
+            tmem_ld16(o_addr + cc * 16, v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * alpha);
+            tmem_st16(o_addr + cc * 16, v);
+          }
+          tmem_wait_st();
+        }
+        l *= alpha;
+        m = m_new;
+      }
+      // P' (16-bit pairs) replaces S, the first half's of the first columns
+      const uint64_t scale2 = pair_f32(f, f), off2 = pair_f32(-m, -m);
+      uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll
+      for (int k = 0; k < GROUPS; ++k) {
+        uint32_t packed[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float lo, hi;
+          split_f32(fma_f32x2(pair_bits(raw[k][2 * i], raw[k][2 * i + 1]), scale2, off2), lo, hi);
+          lo = exp2_fast(lo);
+          hi = exp2_fast(hi);
+          sum2[i & 1] = add_f32x2(sum2[i & 1], pair_f32(lo, hi));
+          packed[i] = pack2<DT>(lo, hi);
+        }
+        tmem_st16(p_addr + k * 16, packed);
+      }
+      if (COPIES > 1) {   // the other copies' tokens
+        constexpr uint32_t zeros[16] = {};
+#pragma unroll
+        for (int k = 1; k < COPIES; ++k)
+#pragma unroll
+          for (int g = 0; g < GROUPS; ++g)
+            tmem_st16(tmem + lane_sel + wg * 128 + ((copy + k) & (COPIES - 1)) * (WIDTH / 2) + 16 * g, zeros);
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      warp_arrive(&bars[P_READY + 2 * wg + half], lane);
+      float lo, hi;
+      split_f32(add_f32x2(sum2[0], sum2[1]), lo, hi);
+      l += lo + hi;
+      if (half == L::HALVES - 1) ++ci;
+    }
+    if (ok && steps > 0) {
+      ok = wait(&bars[O_DONE + wg], pieces & 1, ctx, 942);
+      ++pieces;
+    }
+    // ---- the rows: results, or a part of them
+    if (L::NARROW) {
+      if (softmax_any(!ok)) {   // (all of the warps take part in what follows, or none)
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      mls[tid] = make_float2(m, l);
+      softmax_sync();
+      float top = NOTHING, sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < 2 * (COPIES > 0 ? COPIES : 1); ++k) top = fmaxf(top, mls[k * APART + r].x);
+#pragma unroll
+      for (int k = 0; k < 2 * (COPIES > 0 ? COPIES : 1); ++k) sum = fmaf(mls[k * APART + r].y, exp2f(mls[k * APART + r].x - top), sum);
+      const float factor = exp2f(m - top) * (p.whole ? 1.f / sum : 1.f);
+      const bool any = sum != 0.f;      // (NaN: yes)
+      const bool look = *stray != 0;
+#pragma unroll 1
+      for (int cc = 0; cc < D / 16; ++cc) {
+        uint32_t v[16];
+        if (steps > 0) tmem_ld16(o_addr + cc * 16, v);
+        if (real)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) join[tid * 17 + j] = any && steps > 0 ? __uint_as_float(v[j]) * factor : 0.f;
+        softmax_sync();
+        for (int i = tid; i < a.rows * 16; i += 32 * SOFTMAX_WARPS) {
+          const int from = i / 16, col = i % 16;
+          float x = 0.f;
+#pragma unroll
+          for (int k = 0; k < 2 * (COPIES > 0 ? COPIES : 1); ++k) x += join[(k * APART + from) * 17 + col];
+          if (look) x += strays<DT>(c, a, e, p, from / a.group, cc * 16 + col, D);
+          if (p.whole) store_float(a.out, DT, at_of(p, from) * D + cc * 16 + col, x);
+          else parts.o[(place_of(p) + from) * D + cc * 16 + col] = x;
+        }
+        softmax_sync();
+      }
+      if (tid < APART && real) {
+        if (p.whole) a.lse[at_of(p, r)] = any ? (top + log2f(sum)) * LN2 : -INFINITY;
+        else parts.ml[place_of(p) + r] = make_float2(top, sum);
+      }
+    } else {
+      if (!ok) break;
+      tc_fence_after();
+      const float inv = 1.f / l;
+      const bool any = l != 0.f, look = *stray != 0;
+      const bool wide_out = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0, wide_part = (reinterpret_cast<uintptr_t>(parts.o) & 31) == 0;
+      float* const part = parts.o + (place_of(p) + wg * QT + row) * D;
+#pragma unroll 1
+      for (int cc = 0; cc < D / 16; ++cc) {
+        uint32_t v[16];
+        if (steps > 0) {
+          tmem_ld16(o_addr + cc * 16, v);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = 0u;
+        }
+        if (!real) continue;
+        if (look) {
+#pragma unroll 1
+          for (int j = 0; j < 16; ++j) {
+            const float x = strays<DT>(c, a, e, p, token, cc * 16 + j, D);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (i == j) v[i] = __float_as_uint(__uint_as_float(v[i]) + x);
+          }
+        }
+        if (p.whole) {
+          uint32_t o[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            o[i] = any ? pack2<DT>(__uint_as_float(v[2 * i]) * inv, __uint_as_float(v[2 * i + 1]) * inv) : 0u;
+          store32(a.out + at_of(p, r) * D + cc * 16, o, wide_out);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; j += 8) {
+            const uint32_t o[8] = {v[j], v[j + 1], v[j + 2], v[j + 3], v[j + 4], v[j + 5], v[j + 6], v[j + 7]};
+            store32(part + cc * 16 + j, o, wide_part);
+          }
+        }
+      }
+      if (real) {
+        if (p.whole) a.lse[at_of(p, r)] = any ? (m + log2f(l)) * LN2 : -INFINITY;
+        else parts.ml[place_of(p) + wg * QT + row] = make_float2(m, l);
+      }
+    }
+    if (steps > 0) {
+      tc_fence_before();
+      warp_arrive(&bars[O_FREE + wg], lane);
+    }
+  }
+  // a launch that gave up: NaN for the piece it stopped in and all later ones
+  if (!ok) {
+    while (more) {
+      const int r = L::NARROW ? tid : p.unit * L::UNIT + tid;
+      if (r < a.rows && tid < L::UNIT) {
+        if (p.whole) a.lse[at_of(p, r)] = CUDART_NAN_F;
+        else parts.ml[place_of(p) + tid] = make_float2(0.f, CUDART_NAN_F);
+      }
+      more = walk.next(plan, a.shape, p);
+    }
+  }
+}
+
+template <int DT, int D, int COPIES>
+__global__ void __launch_bounds__(THREADS, 1)
+page_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ PageArrays c,
+                 const __grid_constant__ TileCall a, Parts parts, int32_t* status) {
+  using L = Layout<D, COPIES>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(smem);
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(smem + M_SLOT);
+  volatile int* const abort_flag = reinterpret_cast<volatile int*>(smem + M_ABORT);
+  page::Extent* const extents = reinterpret_cast<page::Extent*>(smem + M_EXTENTS);
+  uint32_t* const start = reinterpret_cast<uint32_t*>(smem + M_START);
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
+  if (tid == 0) {
+    mbar_init(&bars[Q_FULL], OPERAND_WARPS);
+    mbar_init(&bars[Q_FREE], 1);
+    mbar_init(&bars[DRAINED], 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars[S_FULL + i], 1);
+      mbar_init(&bars[PV_HALF + i], 1);
+      mbar_init(&bars[O_DONE + i], 1);
+      mbar_init(&bars[O_FREE + i], QT / 32);
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(&bars[P_READY + i], QT / 32);
+    for (int i = 0; i < L::STAGES; ++i) {
+      mbar_init(&bars[FULL + i], 1);
+      mbar_init(&bars[FREE + i], 1);
+      mbar_init(&bars[CLEAN + i], OPERAND_WARPS);
+    }
+    *abort_flag = 0;
+    *reinterpret_cast<volatile int*>(smem + M_STRAY) = 0;
+    fence_barrier_init();
+    fence_proxy_async();
+  }
+  // ---- the plan
+  if (tid < a.sequences) {
+    bool bad;
+    extents[tid] = extent_of(c, a.counts, a.tokens, tid, bad);
+    if (bad) report(status, STATUS_PAGE);
+    start[tid] = 0;
+  }
+  if (warp == MMA_WARP) tmem_alloc(tmem_slot, 512);
+  __syncthreads();
+  for (int i = tid; i < a.sequences * a.shape.units; i += THREADS) {
+    const int b = i / a.shape.units, u = i % a.shape.units;
+    const uint32_t cost = page::cost_of(page::tiles_seen(a.shape, extents[b], u * L::UNIT, L::UNIT));
+    if (cost) atomicAdd(&start[b], cost);
+  }
+  __syncthreads();
+  if (warp == 0) {
+    uint32_t v[4], mine = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[k] = 4 * lane + k < a.sequences ? start[4 * lane + k] * a.shape.kv_heads : 0u;
+      mine += v[k];
+    }
+    uint32_t before = mine;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const uint32_t other = __shfl_up_sync(0xffffffffu, before, x);
+      if (lane >= x) before += other;
+    }
+    before -= mine;
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (4 * lane + k <= a.sequences) start[4 * lane + k] = before;
+      before += v[k];
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (blockIdx.x == 0) {   // for the second launch
+    for (int i = tid; i <= a.sequences; i += THREADS) {
+      if (i < a.sequences) parts.extents[i] = extents[i];
+      parts.start[i] = start[i];
+    }
+  }
+  const uint32_t tmem = *tmem_slot;
+  const Ctx ctx{abort_flag};
+  Plan plan;
+  plan.start = start;
+  plan.extents = extents;
+  plan.sequences = a.sequences;
+  plan.deal(gridDim.x);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (warp < SOFTMAX_WARPS) softmax_role<DT, D, COPIES>(smem, bars, tmem, c, a, plan, parts, ctx);
+  else if (warp < SOFTMAX_WARPS + OPERAND_WARPS) operand_role<DT, D, COPIES>(smem, bars, c, a, plan, ctx);
+  else if (warp > MMA_WARP) page_role<D, COPIES>(smem, bars, &map_k, &map_v, c, a, plan, ctx, status);
+  else mma_role<DT, D, COPIES>(smem, bars, tmem, a, plan, ctx);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
+  if (tid == 0 && *abort_flag) atomicCAS(status, 0, *abort_flag);
+}
+
+// Joins the parts of cut units and fills the rows of units that have no tiles; a thread block per (unit, kv head, sequence) and 32
+// rows, a thread per row and 16 bytes of it.
+constexpr int SLICE = 32;
+template <int DT, int D>
+__global__ void __launch_bounds__(256)
+join_parts_kernel(TileCall a, Parts parts, int runs) {
+  __shared__ uint32_t before;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Shape& s = a.shape;
+  const int slices = (min(s.unit, s.rows) + SLICE - 1) / SLICE, unit = blockIdx.x / slices, slice = blockIdx.x % slices, h = blockIdx.y, b = blockIdx.z;
+  Plan plan;
+  plan.start = parts.start;
+  plan.extents = parts.extents;
+  plan.sequences = a.sequences;
+  plan.deal(runs);
+  const Extent e = parts.extents[b];
+  const int nt = page::tiles_seen(s, e, unit * s.unit, s.unit);
+  uint32_t r0 = 0, r1 = 0;
+  if (nt > 0) {
+    if (threadIdx.x == 0) before = 0;
+    __syncthreads();
+    uint32_t mine = 0;
+    for (int u = threadIdx.x; u < unit; u += 256) mine += page::cost_of(page::tiles_seen(s, e, u * s.unit, s.unit));
+    if (mine) atomicAdd(&before, mine);
+    __syncthreads();
+    const uint32_t begin = plan.start[b] + h * ((plan.start[b + 1] - plan.start[b]) / s.kv_heads) + before + page::PIECE_TILES;
+    r0 = plan.run_of(begin);
+    r1 = plan.run_of(begin + nt - 1);
+    if (r0 == r1) return;   // one run had all of it and wrote the results
+  }
+  constexpr int PER_ROW = D / 8, ROWS = 256 / PER_ROW;
+  for (int i = threadIdx.x / PER_ROW; i < SLICE; i += ROWS) {
+    const int row = slice * SLICE + i, r = unit * s.unit + row, col = (threadIdx.x % PER_ROW) * 8;
+    if (row >= s.unit || r >= a.rows) break;
+    const int token = r / a.group;
+    const size_t at = (static_cast<size_t>(b) * a.tokens + token) * a.heads + h * a.group + r - token * a.group;
+    float top = NOTHING, sum = 0.f, acc[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) acc[k] = 0.f;
+    if (nt > 0) {
+      // the run the unit starts in has it as a piece that starts with the unit, the others as one that starts inside
+      auto place = [&](uint32_t run) { return (2 * static_cast<size_t>(run) + (run == r0 ? 1 : 0)) * s.unit + row; };
+      for (uint32_t run = r0; run <= r1; ++run) top = fmaxf(top, __ldcg(&parts.ml[place(run)]).x);
+      for (uint32_t run = r0; run <= r1; ++run) {
+        const float2 ml = __ldcg(&parts.ml[place(run)]);
+        const float4 lo = __ldcg(reinterpret_cast<const float4*>(parts.o + place(run) * D + col));
+        const float4 hi = __ldcg(reinterpret_cast<const float4*>(parts.o + place(run) * D + col + 4));
+        const float f = exp2f(ml.x - top);
+        sum = fmaf(ml.y, f, sum);
+        const float part[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] = fmaf(part[k], f, acc[k]);
+      }
+    }
+    const bool any = sum != 0.f;
+    const float inv = any ? 1.f / sum : 0.f;
+    uint32_t o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = any ? pack2<DT>(acc[2 * k] * inv, acc[2 * k + 1] * inv) : 0u;
+    *reinterpret_cast<uint4*>(a.out + at * D + col) = make_uint4(o[0], o[1], o[2], o[3]);
+    if (col == 0) a.lse[at] = any ? (top + log2f(sum)) * LN2 : -INFINITY;
+  }
+}
+
+int unit_of(int rows) { return rows > QT ? 2 * QT : QT; }
+size_t plan_bytes() { return page::MOST_SEQUENCES * sizeof(page::Extent) + (page::MOST_SEQUENCES + 1) * sizeof(uint32_t); }
+
+}  // namespace
+
+size_t page_tile_bytes(int rows, int d) {
+  return static_cast<size_t>(sm_count()) * 2 * unit_of(rows) * (d * sizeof(float) + sizeof(float2)) + plan_bytes();
+}
+
+int page_tile(const PageArrays& c, const PageCall& call, int n, int dtype, int d, void* workspace, int32_t* status, cudaStream_t stream) {
+  TileCall a;
+  static_cast<PageCall&>(a) = call;
+  const int unit = unit_of(a.rows);
+  a.sequences = n;
+  a.shape = Shape{a.sight, a.group, a.rows, unit, ceil_div(a.rows, unit), c.kv_heads};
+  // places of the list are counted in 32 bits
+  const uint64_t tiles = (static_cast<uint64_t>(c.row_pages) << c.shift) / TOK + 1 + page::PIECE_TILES, most = tiles * a.shape.units * c.kv_heads * n;
+  NKV_REQUIRE(most <= UINT32_MAX, NKV_ERR_TOO_LARGE, "page_attend: up to %llu tiles of %d x %d tokens are more than 32 bits count",
+              static_cast<unsigned long long>(most), unit, TOK);
+  const int runs = static_cast<int>(min(most, static_cast<uint64_t>(sm_count())));
+  Parts parts;
+  parts.o = static_cast<float*>(workspace);
+  parts.ml = reinterpret_cast<float2*>(parts.o + static_cast<size_t>(sm_count()) * 2 * unit * d);
+  parts.extents = reinterpret_cast<page::Extent*>(parts.ml + static_cast<size_t>(sm_count()) * 2 * unit);
+  parts.start = reinterpret_cast<uint32_t*>(parts.extents + page::MOST_SEQUENCES);
+  CUtensorMap maps[2];
+  for (int i = 0; i < 2; ++i) {
+    const uint64_t dims[2] = {static_cast<uint64_t>(d), (static_cast<uint64_t>(c.pages) * c.kv_heads) << c.shift};
+    const uint64_t strides[1] = {static_cast<uint64_t>(d) * 2};
+    const uint32_t box[2] = {64, 1u << c.shift};
+    const int rc = encode_tensor_map(&maps[i], 2, i ? c.v : c.k, 2, dims, strides, box, 128);
+    if (rc != NKV_OK) return rc;
+  }
+  auto run = [&](auto kernel, int smem) {
+    NKV_CUDA(allow_shared(reinterpret_cast<const void*>(kernel), smem));
+    kernel<<<runs, THREADS, smem, stream>>>(maps[0], maps[1], c, a, parts, status);
+    NKV_CUDA(cudaGetLastError());
+    return NKV_OK;
+  };
+  int rc = NKV_OK;
+#define NKV_PAGE_RUN(COPIES)                                                                                                             \
+  rc = d == 128 ? (dtype == NKV_BF16 ? run(page_tile_kernel<NKV_BF16, 128, COPIES>, Layout<128, COPIES>::DYNAMIC)                         \
+                                     : run(page_tile_kernel<NKV_F16, 128, COPIES>, Layout<128, COPIES>::DYNAMIC))                         \
+                : (dtype == NKV_BF16 ? run(page_tile_kernel<NKV_BF16, 64, COPIES>, Layout<64, COPIES>::DYNAMIC)                           \
+                                     : run(page_tile_kernel<NKV_F16, 64, COPIES>, Layout<64, COPIES>::DYNAMIC))
+  if (a.rows > QT) NKV_PAGE_RUN(0);
+  else if (a.rows > QT / 2) NKV_PAGE_RUN(1);
+  else if (a.rows > QT / 4) NKV_PAGE_RUN(2);
+  else NKV_PAGE_RUN(4);
+#undef NKV_PAGE_RUN
+  if (rc != NKV_OK) return rc;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(a.shape.units * ceil_div(min(unit, a.rows), SLICE), c.kv_heads, n);
+  config.blockDim = dim3(256);
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  auto join = d == 128 ? (dtype == NKV_BF16 ? join_parts_kernel<NKV_BF16, 128> : join_parts_kernel<NKV_F16, 128>)
+                       : (dtype == NKV_BF16 ? join_parts_kernel<NKV_BF16, 64> : join_parts_kernel<NKV_F16, 64>);
+  NKV_CUDA(cudaLaunchKernelEx(&config, join, a, parts, runs));
+  return NKV_OK;
+}
+
+}  // namespace nkv

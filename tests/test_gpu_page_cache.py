@@ -292,6 +292,35 @@ def test_long_sequences_are_cut_and_joined(heads, tokens, length):
     check_attention(cache, k, v, table, q, [length])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,group,tokens", [(128, 8, 1), (64, 4, 10), (128, 5, 16), (128, 2, 90)])
+def test_thread_blocks_with_many_pieces_of_many_tiles(dim, group, tokens, dtype):
+    """Rings that go round several times within a piece, and several pieces a thread block, with masked tiles at their ends."""
+    heads = 16
+    lengths = [2138 - 61 * i for i in range(31)]
+    counts = [0 if i % 8 == 5 else max(1, tokens - i % 3) for i in range(31)]
+    cache, k, v, table = made(31, 2138 + tokens, heads, dim, dtype, 64, 125, lengths)
+    spoiled(cache, k, v, table, lengths, counts)
+    q = ref.randn(31, tokens, heads * group, dim, seed=126, dtype=dtype).cuda()
+    # sequences and heads apart from one another; one of them against the formula
+    out, lse = cache.attend(q, counts=torch.tensor(counts, dtype=torch.int32).cuda())
+    ops.check_status(out.device)
+    pages = torch.cat([table, table], 0).cuda()
+    for b in (0, 1, 5, 17, 30):
+        one = PageTable.over(pages[b:b + 1].contiguous(), torch.tensor([lengths[b]], dtype=torch.int32).cuda(), pages=cache.table.pages, page=64)
+        for h in (0, 7, 15):
+            part = PageCache.over(one, cache.k_pages[:, h:h + 1].contiguous(), cache.v_pages[:, h:h + 1].contiguous())
+            rows = q[b:b + 1, :, h * group:(h + 1) * group]
+            check_attention(part, k[:, h:h + 1], v[:, h:h + 1], table[b:b + 1], rows, [lengths[b]], counts=[counts[b]])
+            alone, lse_alone = part.attend(rows, counts=torch.tensor([counts[b]], dtype=torch.int32).cuda())
+            got, lse_got = out[b:b + 1, :, h * group:(h + 1) * group], lse[b:b + 1, :, h * group:(h + 1) * group]
+            seen = lse_alone > -math.inf
+            assert torch.equal(seen, lse_got > -math.inf)
+            assert not seen.any() or ((lse_alone - lse_got).abs()[seen] <= 2.0 ** -12).all()
+            # both are within the bounds of check_attention of the formula, where values are a few units at most
+            assert ((alone.float() - got.float()).abs() <= 6 * ref.UNIT[dtype] * 6).all()
+
+
 def test_results_are_the_same_every_time():
     lengths = [500, 1, 900]
     cache, k, v, table = made(3, 1000, 2, 128, torch.bfloat16, 64, 131, lengths)
