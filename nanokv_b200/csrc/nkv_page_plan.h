@@ -59,7 +59,7 @@ NKV_PAGE_INLINE int sees_all_before(int sight, const Extent& e, int t) {
 
 // ---- attention: units of query rows of a kv head, tiles of tokens -------------------------------------------------
 constexpr int TOK = 128;             // tokens of a tile
-constexpr int MOST_SEQUENCES = 100;  // of one launch; longer batches are cut
+constexpr int MOST_SEQUENCES = 96;   // of one launch; longer batches are cut
 
 struct Shape { int sight, group, rows, unit, units, kv_heads; };   // rows of a kv head, rows of a unit, units
 

@@ -7,21 +7,28 @@
 //   wide    more than 128: units of 256 rows, two query tiles that share every K and V tile, four warps each.
 //   narrow  up to 128, one query tile; the two groups of four warps take the even and the odd tiles of its tokens, each with sums of
 //           its own.  With at most 128 / COPIES rows, COPIES of them stand in the query tile one below the other, and
-//           every copy takes its share of a tile's tokens: the weights of the others are stored as zeros.  That cuts what one
-//           thread does per tile, which is what a tile takes.  The sums of all are joined in shared memory.
+//           every copy takes a share of a tile's tokens (or of its weights' bits): the weights of the others are stored as zeros.  That
+//           cuts what one thread does per tile, which is what a tile takes.  The sums of all are joined in shared memory.
 //
 // Softmax: P' = 2^(s - m) with a reference m that follows the running maximum of the scaled scores, s; it moves when P' would pass
 // 2^8 times what it was set to.  bf16: set so that the sum of a row's P' stays below 1, O = sum P' V then below the largest |V|, any
-// number of bf16.  fp16: P' up to 2^15, so that weights down to 2^-29 of the largest keep all their bits.  P' is rounded to the cache's
-// type, as the tensor cores take it; the row sum, the maximum and O stay in fp32.
+// number of bf16.  fp16: P' up to 2^15, so that weights down to 2^-29 of the largest keep all their bits.  The row sum, the maximum and O
+// stay in fp32.  P' enters the product with V in 16 bits: fp16 rounded to nearest; bf16 as the upper half of its fp32 bits, a byte
+// permutation instead of a conversion on the unit that the exponentials need.  What is cut off is made good on average: every P' is raised
+// by the mean of it, (1 + 0.72 * 2^-8), in its exponent, and the row sum lowered again.  With four copies, two of them take the upper half of
+// P' and two the rest (2^-15 of it is left): few rows have few results, and no average to hide an unlucky weight in.
 //
 // Pending tokens that some row does not see, and whatever lies in a page behind a sequence's last token, are masked in the scores.  A weight
-// of 0 times a value that is not finite would be NaN, so four warps look at the V tiles with such tokens: values behind the
+// of 0 times a value that is not finite would be NaN, so two warps look at the V tiles with such tokens: values behind the
 // last token become 0 in shared memory, and so do values that are not finite; rows that see them get them added at the end, from memory.
+//
+// A page of K or V comes as one copy, whatever its size: the tensor map has the eight rows of a swizzle group, the 64-element chunks of a
+// row and the groups of a page as dimensions, so that a tile is its groups one behind the other, each with its chunks side by side.
 //
 // Table, lengths and counts are read by the kernel: every thread block makes the plan (nkv_page_plan.h) for itself.  The tiles of all
 // units form one list that the SMs take in equal runs; a unit that a run's end cuts leaves fp32 parts, joined by a second launch.
-// Warps: 0-7 softmax, 8-11 queries and masked values, 12 MMA issue, 13 pages.
+// Warps: 0-7 softmax, 8-9 queries and masked values, 10 MMA issue, 11 pages: 384 threads, so that 168 registers each hold a row's
+// 128 scores at once.
 #include "nkv_internal.h"
 #include "nkv_page.cuh"
 #include "nkv_tile.cuh"
@@ -38,13 +45,15 @@ using page::Walk;
 
 constexpr int QT = 128;                           // rows of a query tile
 constexpr int SUB = 128 * 128;                    // bytes of a [128 rows x 64 elements] swizzled tile
-constexpr int SOFTMAX_WARPS = 8, OPERAND_WARPS = 4, MMA_WARP = 12, THREADS = 448;
+constexpr int SOFTMAX_WARPS = 8, OPERAND_WARPS = 2, MMA_WARP = 10, THREADS = 384;
 constexpr float RESCALE_THRESHOLD = 8.0f;
+// log2(1 + 0.7213 * 2^-8) and its inverse: the mean of 1 / m over mantissas m is 0.7213, and half a bf16 step is 2^-8 of m = 1
+constexpr float CUT_LOG2 = 0.00405952f, CUT_INV = 0.99719022f;
 constexpr float NOTHING = -3e38f;                 // the reference before the first score: below all, and a number
 
 // (P_READY: chain i, half h of a tile's tokens at 2 i + h)
-enum Bar { Q_FULL = 0, Q_FREE = 1, S_FULL = 2, P_READY = 4, PV_HALF = 8, O_DONE = 10, O_FREE = 12, FULL = 14, FREE = 24, CLEAN = 34, DRAINED = 44, NUM_BARS = 45 };
-constexpr int M_SLOT = NUM_BARS * 8, M_ABORT = M_SLOT + 4, M_STRAY = M_SLOT + 8, M_EXTENTS = 384;
+enum Bar { Q_FULL = 0, Q_FREE = 1, S_FULL = 2, P_READY = 4, O_DONE = 8, O_FREE = 10, DRAINED = 12, FULL = 13, FREE = 23, LOOK = 33, CLEAN = 43, NUM_BARS = 53 };
+constexpr int M_SLOT = NUM_BARS * 8, M_ABORT = M_SLOT + 4, M_STRAY = M_SLOT + 8, M_EXTENTS = 448;
 constexpr int M_START = M_EXTENTS + page::MOST_SEQUENCES * static_cast<int>(sizeof(page::Extent)), META = 2048;
 static_assert(M_STRAY + 4 <= M_EXTENTS && M_START + 4 * (page::MOST_SEQUENCES + 1) <= META && page::MOST_SEQUENCES < 128, "meta block");
 
@@ -58,22 +67,29 @@ template <int D, int COPIES> struct Layout {
   static constexpr int Q_OFF = META;
   static constexpr int RING_OFF = Q_OFF + QTILES * DCH * SUB;
   static constexpr int ML_OFF = RING_OFF + STAGES * STAGE;             // narrow: references and sums of 256 threads
-  static constexpr int JOIN_OFF = ML_OFF + (NARROW ? 256 * 8 : 0);     // narrow: 16 columns of O of 256 threads, a row of 17 each
-  static constexpr int BYTES = JOIN_OFF + (NARROW ? 256 * 17 * 4 : 0);
+  static constexpr int JOIN_OFF = ML_OFF + (NARROW ? 256 * 8 : 0);     // narrow: columns of O of all copies of the rows
+  static constexpr int JOIN_WORDS = D == 128 ? 7424 : 11264;
+  static constexpr int BYTES = JOIN_OFF + (NARROW ? JOIN_WORDS * 4 : 0);
   static constexpr int DYNAMIC = BYTES + 1024;     // room to start on 1,024 bytes
-  static constexpr int HALVES = COPIES >= 2 ? 1 : 2, WIDTH = COPIES == 4 ? 32 : 64;   // tokens that a thread takes at a time
+  static constexpr int GROUP = DCH * 1024;         // eight rows of a K or V tile: their chunks of 64 elements side by side
 };
-static_assert(Layout<128, 0>::DYNAMIC <= 232448 && Layout<64, 0>::DYNAMIC <= 232448, "shared memory");
+static_assert(Layout<128, 0>::DYNAMIC <= 232448 && Layout<64, 0>::DYNAMIC <= 232448 && Layout<128, 1>::DYNAMIC <= 232448 &&
+                  Layout<64, 1>::DYNAMIC <= 232448,
+              "shared memory");
+static_assert(Layout<128, 1>::JOIN_WORDS >= 256 * 20, "16 columns of all rows and copies");
 
-// places of a piece's tiles in the ring: LEAD tiles of K, then a V tile and a K tile in turn
-template <class L> __device__ __forceinline__ uint32_t place_of_k(uint32_t t) { return t < L::LEAD ? t : 2 * t - L::LEAD + 1; }
-template <class L> __device__ __forceinline__ uint32_t place_of_v(uint32_t t, uint32_t nt) { return t + min(nt, L::LEAD + t); }
-// the n-th tile of a piece in the ring
+// copies of the query rows: SLICES of a tile's tokens times PARTS of a weight's bits
+template <int DT, int COPIES> constexpr int PARTS = DT == NKV_BF16 && COPIES == 4 ? 2 : 1;
+template <int DT, int COPIES> constexpr int SLICES = COPIES > 1 ? COPIES / PARTS<DT, COPIES> : 1;
+
+// The n-th tile of a piece in the ring, which holds them in the order in which they are used: LEAD tiles of K, then a tile of V and
+// one of K in turn.
 template <class L> __device__ __forceinline__ int ring_tile(int n, int nt, bool& value) {
   const int lead = min(nt, L::LEAD), k = n - lead, pairs = max(0, nt - L::LEAD);   // K ahead; V 0, K lead, V 1, ...; then V alone
   value = k >= 0 && (k >= 2 * pairs || (k & 1) == 0);
   return k < 0 ? n : k >= 2 * pairs ? k - pairs : value ? k / 2 : k / 2 + L::LEAD;
 }
+template <class L> __device__ __forceinline__ uint32_t place_of_v(int t, int nt) { return t + min(nt, L::LEAD + t); }
 
 // steps of chain i of a piece, and the tile of a step: query tile i over the tiles it sees, or every other tile
 template <class L> __device__ __forceinline__ int steps_of(const Shape& s, const Extent& e, const Piece& p, int i) {
@@ -82,9 +98,9 @@ template <class L> __device__ __forceinline__ int steps_of(const Shape& s, const
 }
 template <class L> __device__ __forceinline__ int tile_of(int i, int step) { return L::NARROW ? 2 * step + i : step; }
 
-// tokens from the first on that all rows of a unit see, where they are asked for
-__device__ __forceinline__ int seen_by_all(const Shape& s, const Extent& e, const Piece& p) {
-  return page::sees_all_before(s.sight, e, p.unit * s.unit / s.group);
+// the first tile of a piece (or one before it) with tokens that some row does not see
+__device__ __forceinline__ int first_masked(const Shape& s, const Extent& e, const Piece& p) {
+  return page::sees_all_before(s.sight, e, p.unit * s.unit / s.group) / TOK - p.tile0;
 }
 
 // A run holds at most one piece that starts inside a unit and one that starts with it and is cut: two places each.  Behind them what
@@ -101,21 +117,18 @@ struct TileCall : PageCall {
   int sequences;
 };
 
-// ---- warp 13: pages ------------------------------------------------------------------------------------------------
+// ---- warp 11: pages ------------------------------------------------------------------------------------------------
 template <int D, int COPIES>
 __device__ __forceinline__ void page_role(uint8_t* smem, uint64_t* bars, const CUtensorMap* map_k, const CUtensorMap* map_v, const PageArrays& c,
                                           const TileCall& a, const Plan& plan, const Ctx& ctx, int32_t* status) {
   using L = Layout<D, COPIES>;
   const int lane = threadIdx.x & 31, rows = 1 << c.shift, per_tile = TOK >> c.shift;
-  const int nowhere = c.pages * c.kv_heads << c.shift;   // behind the last row of the pool: read as zeros
-  if (lane == 0) {
-    prefetch_tensormap(map_k);
-    prefetch_tensormap(map_v);
-  }
+  const int groups = rows / 8, nowhere = c.pages * c.kv_heads * groups;   // groups of a page; behind the last one of the pool: read as zeros
   Walk walk(plan, a.shape, blockIdx.x);
   Piece p;
   bool ok = true, bad = false;
-  uint32_t item = 0;
+  Ring at;
+  int round = 0;        // times round the ring
   while (ok && walk.next(plan, a.shape, p)) {
     const Extent e = plan.extents[p.b];
     const int total = e.length + e.there;
@@ -126,11 +139,10 @@ __device__ __forceinline__ void page_role(uint8_t* smem, uint64_t* bars, const C
       return entry < c.row_pages && entry << c.shift < total ? __ldg(entries + entry) : -1;
     };
     int now = p.tile0 * per_tile / 32, before = -1, here = window(now), after = window(now + 1);
-    for (int n = 0; n < 2 * p.nt && ok; ++n, ++item) {
-      // n-th tile of the piece in the order of the ring
+    const int masked = first_masked(a.shape, e, p);
+    for (int n = 0; n < 2 * p.nt && ok; ++n) {
       bool value;
       const int t = ring_tile<L>(n, p.nt, value);
-      const uint32_t stage = item % L::STAGES, use = item / L::STAGES;
       const int entry = (p.tile0 + t) * per_tile, w = entry / 32;
       if (w > now) {
         before = here;
@@ -138,20 +150,24 @@ __device__ __forceinline__ void page_role(uint8_t* smem, uint64_t* bars, const C
         now = w;
         after = window(now + 1);
       }
-      const int chunk = lane / per_tile, at = lane % per_tile;
-      const int id = __shfl_sync(0xffffffffu, w == now ? here : before, (entry + at) & 31);
+      const int id = __shfl_sync(0xffffffffu, w == now ? here : before, (entry + lane) & 31);
       const int first = (p.tile0 + t) * TOK, pages = min(per_tile, (total - first + rows - 1) >> c.shift);
-      if (use > 0) ok = wait(&bars[FREE + stage], (use - 1) & 1, ctx, 930);
+      if (round > 0) ok = wait(&bars[FREE + at.stage], at.phase ^ 1, ctx, 930);
       if (!ok) break;
-      if (lane == 0) mbar_arrive_expect_tx(&bars[FULL + stage], static_cast<uint32_t>(pages << c.shift) * D * 2);
-      __syncwarp();
-      if (chunk < L::DCH && at < pages) {
-        const bool in = static_cast<unsigned>(id) < static_cast<unsigned>(c.pages);
-        bad |= !in;
-        tma_load_2d(smem + L::RING_OFF + stage * L::STAGE + chunk * SUB + (at << c.shift) * 128, value ? map_v : map_k, chunk * 64,
-                    in ? (id * c.kv_heads + p.h) << c.shift : nowhere, &bars[FULL + stage]);
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&bars[FULL + at.stage], static_cast<uint32_t>(pages << c.shift) * D * 2);
+        if (value && t >= masked) mbar_arrive(&bars[LOOK + at.stage]);
       }
       __syncwarp();
+      if (lane < pages) {
+        const bool in = static_cast<unsigned>(id) < static_cast<unsigned>(c.pages);
+        bad |= !in;
+        tma_load_4d(smem + L::RING_OFF + at.stage * L::STAGE + lane * groups * L::GROUP, value ? map_v : map_k,
+                    in ? (id * c.kv_heads + p.h) * groups : nowhere, &bars[FULL + at.stage]);
+      }
+      __syncwarp();
+      at.advance(L::STAGES);
+      round += at.stage == 0;
     }
   }
   if (bad) report(status, STATUS_PAGE);
@@ -161,10 +177,15 @@ __device__ __forceinline__ void page_role(uint8_t* smem, uint64_t* bars, const C
   }
 }
 
-// ---- warps 8-11: queries, and values that rows do not see --------------------------------------------------------------
+// ---- warps 8-9: queries, and values that rows do not see ---------------------------------------------------------------
 template <int DT> __device__ __forceinline__ bool not_finite(uint32_t bits16) {
   constexpr uint32_t E = DT == NKV_BF16 ? 0x7F80u : 0x7C00u;
   return (bits16 & E) == E;
+}
+
+// 16 bytes from memory to shared memory, or zeros
+__device__ __forceinline__ void copy16_async(uint32_t to, const void* from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
 
 template <int DT, int D, int COPIES>
@@ -173,66 +194,72 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
   const int tid = threadIdx.x - 32 * SOFTMAX_WARPS, lane = tid & 31;
   const uint32_t base = smem_u32(smem);
   // queries: a thread has one 16-byte column of every ROWS-th row of the unit
-  constexpr int PER_ROW = D / 8, ROWS = 32 * OPERAND_WARPS / PER_ROW, AHEAD = 8, APART = L::NARROW ? QT / (COPIES > 0 ? COPIES : 1) : L::UNIT;
+  constexpr int PER_ROW = D / 8, ROWS = 32 * OPERAND_WARPS / PER_ROW, APART = QT / (COPIES > 0 ? COPIES : 1);
   const int q_row = tid / PER_ROW, q_col = tid % PER_ROW * 8;
   const uint32_t q_to = base + L::Q_OFF + (q_col / 64) * SUB;
-  const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;   // a negative scale is the queries' sign
+  const bool negative = a.scale_log2 < 0.f;   // a negative scale is the queries' sign
+  const int token_step = ROWS / a.group, head_step = ROWS - token_step * a.group;
   volatile int* const stray = reinterpret_cast<volatile int*>(smem + M_STRAY);
   Walk walk(plan, a.shape, blockIdx.x);
   Piece p;
   bool ok = true;
   int pieces = 0;
-  uint32_t item = 0;    // tiles in the ring so far
+  uint32_t items = 0, looked = 0;   // tiles in the ring of the pieces before; phases of LOOK, a bit per stage
   while (ok && walk.next(plan, a.shape, p)) {
     const Extent e = plan.extents[p.b];
     const uint16_t* const q_head = a.q + p.b * a.q_batch + static_cast<long long>(p.h) * a.group * a.q_head + q_col;
-    // the first rows are on their way while the piece before still reads its own
-#pragma unroll 1
-    for (int row0 = q_row; row0 < L::UNIT && ok; row0 += AHEAD * ROWS) {
-      uint4 v[AHEAD];
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const int r = p.unit * L::UNIT + (row0 + k * ROWS) % APART, token = r / a.group;
-        v[k] = make_uint4(0, 0, 0, 0);
-        if (r < a.rows) {
-          const uint16_t* const src = q_head + token * a.q_token + (r - token * a.group) * a.q_head;
-          v[k] = a.q_vector ? __ldg(reinterpret_cast<const uint4*>(src)) : gather16(src);
-        }
-      }
-      if (row0 == q_row && pieces > 0) ok = wait(&bars[Q_FREE], (pieces - 1) & 1, ctx, 931);
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const int row = row0 + k * ROWS;
-        sts128(q_to + (row / QT) * L::DCH * SUB + sw128_offset(row % QT, q_col % 64),
-               make_uint4(v[k].x ^ flip, v[k].y ^ flip, v[k].z ^ flip, v[k].w ^ flip));
-      }
-    }
+    if (pieces > 0) ok = wait(&bars[Q_FREE], (pieces - 1) & 1, ctx, 931);
     if (!ok) break;
+    // rows of a narrow unit are the same ones every time: behind the last of them zeros stay
+    const int rows = !L::NARROW ? L::UNIT : pieces > 0 ? min(APART, a.rows) : APART;
+    auto q_place = [&](int row) { return q_to + (row / QT) * L::DCH * SUB + sw128_offset(row % QT, q_col % 64); };
+    int r = p.unit * L::UNIT + q_row, token = r / a.group, head = r - token * a.group;
+#pragma unroll 4
+    for (int row = q_row; row < rows; row += ROWS) {
+      const uint16_t* const src = q_head + token * a.q_token + head * a.q_head;
+      const bool there = r < a.rows;
+#pragma unroll
+      for (int copy = 0; copy < (COPIES > 0 ? COPIES : 1); ++copy) {
+        const uint32_t to = q_place(row + copy * APART);
+        if (a.q_vector) copy16_async(to, there ? src : a.q, there);
+        else sts128(to, there ? gather16(src) : make_uint4(0, 0, 0, 0));
+      }
+      r += ROWS;
+      token += token_step;
+      head += head_step;
+      if (head >= a.group) { head -= a.group; ++token; }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (negative)
+      for (int row = q_row; row < rows; row += ROWS)
+#pragma unroll 1
+        for (int copy = 0; copy < (COPIES > 0 ? COPIES : 1); ++copy) {
+          const uint4 v = lds128(q_place(row + copy * APART));
+          sts128(q_place(row + copy * APART), make_uint4(v.x ^ 0x80008000u, v.y ^ 0x80008000u, v.z ^ 0x80008000u, v.w ^ 0x80008000u));
+        }
     ++pieces;
     fence_proxy_async();
     warp_arrive(&bars[Q_FULL], lane);
-    // ---- V tiles with tokens that some row does not see: a thread per token.  Every tile of the ring is waited for, K's and those
-    // that all rows see too: a wait tells a phase from its neighbours only.
-    const int total = e.length + e.there, masked = seen_by_all(a.shape, e, p) / TOK - p.tile0;
-    for (int n = 0; n < 2 * p.nt && ok; ++n, ++item) {
-      const uint32_t stage = item % L::STAGES;
-      ok = wait(&bars[FULL + stage], (item / L::STAGES) & 1, ctx, 932);
+    // ---- V tiles with tokens that some row does not see: two tokens a thread.  LOOK tells that a stage waits for such a tile: a
+    // wait for FULL alone, by warps that skip all other tiles, could not tell this phase of it from an earlier one.
+    const int total = e.length + e.there;
+    for (int t = max(0, first_masked(a.shape, e, p)); t < p.nt; ++t) {
+      const uint32_t item = items + place_of_v<L>(t, p.nt), stage = item % L::STAGES;
+      ok = wait(&bars[LOOK + stage], (looked >> stage) & 1, ctx, 932) && wait(&bars[FULL + stage], (item / L::STAGES) & 1, ctx, 942);
       if (!ok) break;
-      bool value;
-      const int t = ring_tile<L>(n, p.nt, value);
-      if (!value || t < masked) continue;
-      const bool behind = (p.tile0 + t) * TOK + tid >= total;
-      const uint32_t row = base + L::RING_OFF + stage * L::STAGE + tid * 128;
+      looked ^= 1u << stage;
 #pragma unroll 1
-      for (int ch = 0; ch < L::DCH; ++ch) {
+      for (int row = tid; row < TOK; row += 32 * OPERAND_WARPS) {
+        const bool behind = (p.tile0 + t) * TOK + row >= total;
+        const uint32_t first = base + L::RING_OFF + stage * L::STAGE + (row / 8) * L::GROUP + (row & 7) * 128;
 #pragma unroll 4
-        for (int k = 0; k < 8; ++k) {
-          const uint32_t at = row + ch * SUB + ((k ^ (tid & 7)) << 4);   // (lanes of a row group take different banks)
+        for (int k = 0; k < L::DCH * 8; ++k) {
+          const uint32_t place = first + (k / 8) * 1024 + (((k & 7) ^ (row & 7)) << 4);   // (lanes of a row group take different banks)
           if (behind) {
-            sts128(at, make_uint4(0, 0, 0, 0));
+            sts128(place, make_uint4(0, 0, 0, 0));
             continue;
           }
-          const uint4 v = lds128(at);
+          const uint4 v = lds128(place);
           uint32_t w[4] = {v.x, v.y, v.z, v.w};
           bool found = false;
 #pragma unroll
@@ -242,7 +269,7 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
             w[i] &= (lo ? 0u : 0xFFFFu) | (hi ? 0u : 0xFFFF0000u);
           }
           if (found) {
-            sts128(at, make_uint4(w[0], w[1], w[2], w[3]));
+            sts128(place, make_uint4(w[0], w[1], w[2], w[3]));
             *stray = 1;
           }
         }
@@ -250,18 +277,26 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
       fence_proxy_async();
       warp_arrive(&bars[CLEAN + stage], lane);
     }
+    items += 2 * p.nt;
   }
 }
 
-// ---- warp 12: MMA issue -----------------------------------------------------------------------------------------
+// ---- warp 10: MMA issue -----------------------------------------------------------------------------------------
+// Descriptor of a K tile (K-major) or, read along its rows, of a V tile (MN-major; `leading`: from one chunk of 64 columns to the next, in
+// 16 bytes): groups of eight rows `group` bytes apart, 128-byte swizzle.
+__device__ __forceinline__ uint64_t tile_desc(uint32_t smem_addr, uint32_t leading, uint32_t group) {
+  return static_cast<uint64_t>((smem_addr >> 4) & 0x3FFF) | (static_cast<uint64_t>(leading) << 16) | (static_cast<uint64_t>(group / 16) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+
 template <int DT, int D, int COPIES>
 __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t tmem, const TileCall& a, const Plan& plan, const Ctx& ctx) {
   using L = Layout<D, COPIES>;
   constexpr int DCH = L::DCH;
   const bool leader = elect_one();   // the whole warp runs the (uniform) control flow; one elected lane issues
   const uint32_t base = smem_u32(smem);
-  const uint64_t q_desc = make_smem_desc_sw128(base + L::Q_OFF), k_desc = make_smem_desc_sw128(base + L::RING_OFF);
-  const uint64_t v_desc = make_smem_desc_sw128_mn(base + L::RING_OFF, SUB);
+  const uint64_t q_desc = make_smem_desc_sw128(base + L::Q_OFF);
+  const uint64_t k_desc = tile_desc(base + L::RING_OFF, 1, L::GROUP), v_desc = tile_desc(base + L::RING_OFF, 1024 / 16, L::GROUP);
   auto issue_s = [&](int i, uint32_t stage) {
     const uint64_t qd = q_desc + (L::NARROW ? 0u : static_cast<uint32_t>(i * (DCH * SUB / 16))), kd = k_desc + stage * static_cast<uint32_t>(L::STAGE / 16);
     const uint32_t d = tmem + i * 128;
@@ -269,49 +304,49 @@ __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t
     for (int ch = 0; ch < DCH; ++ch)
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        if (leader) mma_bf16(d, qd + ch * (SUB / 16) + 2 * k, kd + ch * (SUB / 16) + 2 * k, idesc<DT>(TOK), ch + k > 0);
+        if (leader) mma_bf16(d, qd + ch * (SUB / 16) + 2 * k, kd + ch * (1024 / 16) + 2 * k, idesc<DT>(TOK), ch + k > 0);
     if (leader) mma_commit(&bars[S_FULL + i]);
   };
-  // weights of TOK / HALVES tokens times V of them: V's rows are tokens, its columns the result's
+  // weights of half a tile's tokens times V of them: V's rows are tokens, its columns the result's
   auto issue_pv = [&](int i, uint32_t stage, int half, bool accumulate) {
-    constexpr int STEPS = 8 / L::HALVES;
-    const uint64_t vd = v_desc + stage * static_cast<uint32_t>(L::STAGE / 16) + half * STEPS * 128u;
-    const uint32_t d = tmem + 256 + i * 128, w = tmem + i * 128 + half * STEPS * 8;
+    const uint64_t vd = v_desc + stage * static_cast<uint32_t>(L::STAGE / 16) + half * static_cast<uint32_t>(8 * L::GROUP / 16);
+    const uint32_t d = tmem + 256 + i * 128, w = tmem + i * 128 + half * 32;
 #pragma unroll
-    for (int k = 0; k < STEPS; ++k)
-      if (leader) mma_bf16_ts(d, w + 8 * k, vd + 128 * k, idesc<DT>(D) | (1u << 16), accumulate || k > 0);
-    if (L::HALVES == 2 && half == 0 && leader) mma_commit(&bars[PV_HALF + i]);
+    for (int k = 0; k < 4; ++k)
+      if (leader) mma_bf16_ts(d, w + 8 * k, vd + k * (2 * L::GROUP / 16), idesc<DT>(D) | (1u << 16), accumulate || k > 0);
   };
   Walk walk(plan, a.shape, blockIdx.x);
   Piece p;
   bool ok = true;
-  uint32_t items = 0, cleaned = 0;                 // tiles in the ring of the pieces before; phases of CLEAN, a bit per stage
+  Ring at;                                         // tiles are used in the order in which they lie in the ring
+  uint32_t cleaned = 0;                            // phases of CLEAN, a bit per stage
   int pieces = 0, done[2] = {0, 0}, used[2] = {0, 0};   // steps and pieces of each chain so far
   while (ok && walk.next(plan, a.shape, p)) {
     const Extent e = plan.extents[p.b];
     const int n[2] = {steps_of<L>(a.shape, e, p, 0), steps_of<L>(a.shape, e, p, 1)};
-    const int longest = max(n[0], n[1]), masked = seen_by_all(a.shape, e, p) / TOK - p.tile0;   // tiles from here on are looked at
+    const int longest = max(n[0], n[1]), masked = first_masked(a.shape, e, p);   // V tiles from here on are looked at
     ok = wait(&bars[Q_FULL], pieces & 1, ctx, 933);
     ++pieces;
     // the first and the last chain to use a tile: each stage is waited for once and given back once
     auto is_first = [&](int i, int step) { return L::NARROW || i == (step < n[0] ? 0 : 1); };
     auto is_last = [&](int i, int step) { return L::NARROW || i == (step < n[1] ? 1 : 0); };
+    uint32_t k_stage = 0, v_stage = 0;
 #pragma unroll 1
     for (int j = 0; j <= longest && ok; ++j) {
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         const int steps = i ? n[1] : n[0];
         if (j > 0 && j - 1 < steps) {
-          const int t = tile_of<L>(i, j - 1);
-          const uint32_t item = items + place_of_v<L>(t, p.nt), stage = item % L::STAGES;
           const uint32_t phase = ((i ? done[1] : done[0]) + j - 1) & 1;
           if (is_first(i, j - 1)) {
-            if (t >= masked) {
-              ok = wait(&bars[CLEAN + stage], (cleaned >> stage) & 1, ctx, 934);
-              cleaned ^= 1u << stage;
+            v_stage = at.stage;
+            if (tile_of<L>(i, j - 1) >= masked) {
+              ok = wait(&bars[CLEAN + v_stage], (cleaned >> v_stage) & 1, ctx, 934);
+              cleaned ^= 1u << v_stage;
             } else {
-              ok = wait(&bars[FULL + stage], (item / L::STAGES) & 1, ctx, 935);
+              ok = wait(&bars[FULL + v_stage], at.phase, ctx, 935);
             }
+            at.advance(L::STAGES);
           }
           if (j == 1) {   // the first PV of a piece overwrites O: the rows of the piece before must have been read
             const int before = i ? used[1] : used[0];
@@ -320,33 +355,33 @@ __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t
           ok = ok && wait(&bars[P_READY + 2 * i], phase, ctx, 937);
           if (!ok) break;
           tc_fence_after();
-          issue_pv(i, stage, 0, j > 1);
-          if (L::HALVES == 2) {
+          issue_pv(i, v_stage, 0, j > 1);
+          if (COPIES <= 1) {
             ok = wait(&bars[P_READY + 2 * i + 1], phase, ctx, 938);
             if (!ok) break;
             tc_fence_after();
-            issue_pv(i, stage, 1, true);
           }
+          issue_pv(i, v_stage, 1, true);
           if (j == steps && leader) mma_commit(&bars[O_DONE + i]);
-          if (is_last(i, j - 1) && leader) mma_commit(&bars[FREE + stage]);
+          if (is_last(i, j - 1) && leader) mma_commit(&bars[FREE + v_stage]);
         }
         if (j < steps) {
           // S of the next step overwrites P of this one, right behind the PV that reads it: the tensor core executes one
           // thread's MMAs in order
-          const uint32_t item = items + place_of_k<L>(tile_of<L>(i, j)), stage = item % L::STAGES;
           if (is_first(i, j)) {
-            ok = wait(&bars[FULL + stage], (item / L::STAGES) & 1, ctx, 939);
+            k_stage = at.stage;
+            ok = wait(&bars[FULL + k_stage], at.phase, ctx, 939);
             if (!ok) break;
+            at.advance(L::STAGES);
             tc_fence_after();
           }
-          issue_s(i, stage);
-          if (is_last(i, j) && leader) mma_commit(&bars[FREE + stage]);
+          issue_s(i, k_stage);
+          if (is_last(i, j) && leader) mma_commit(&bars[FREE + k_stage]);
         }
       }
     }
     if (!ok) break;
     if (leader) mma_commit(&bars[Q_FREE]);
-    items += 2 * p.nt;
     for (int i = 0; i < 2; ++i) {
       done[i] += n[i];
       used[i] += n[i] > 0 ? 1 : 0;
@@ -367,7 +402,7 @@ template <int DT>
 __device__ __noinline__ float strays(const PageArrays& c, const TileCall& a, Extent e, Piece p, int t, int col, int d) {
   float sum = 0.f;
   if (t >= e.count) return sum;
-  const int total = e.length + e.there, from = max(p.tile0, seen_by_all(a.shape, e, p) / TOK) * TOK, to = min((p.tile0 + p.nt) * TOK, total);
+  const int total = e.length + e.there, from = (p.tile0 + max(0, first_masked(a.shape, e, p))) * TOK, to = min((p.tile0 + p.nt) * TOK, total);
   for (int first = from; first < to; first += 32) {
     const uint32_t sees = sight_of(a, e, p.b, t, first);
     for (int i = 0; i < 32 && first + i < to; ++i) {
@@ -400,12 +435,13 @@ template <int DT, int D, int COPIES>
 __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint32_t tmem, const PageArrays& c, const TileCall& a, const Plan& plan,
                                              const Parts& parts, const Ctx& ctx) {
   using L = Layout<D, COPIES>;
-  constexpr int WIDTH = L::WIDTH, GROUPS = WIDTH / 32, APART = QT / (COPIES > 0 ? COPIES : 1);
+  constexpr int WIDTH = TOK / SLICES<DT, COPIES>, GROUPS = WIDTH / 32, SOURCES = 2 * (COPIES > 0 ? COPIES : 1), APART = 2 * QT / SOURCES;
+  constexpr bool TWO = PARTS<DT, COPIES> == 2, CUT = DT == NKV_BF16 && !TWO;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
   const int wg = warp / 4, row = tid & 127;
-  const int copy = COPIES > 1 ? row / APART : 0;
-  const uint32_t lane_sel = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-  const uint32_t o_addr = tmem + lane_sel + 256 + wg * 128;
+  const int slice = COPIES > 1 ? row / APART % SLICES<DT, COPIES> : 0;   // (the same in all of a warp, as is whether it takes the rest)
+  const bool rest = TWO && row / APART >= SLICES<DT, COPIES>;
+  const uint32_t s_addr = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + wg * 128, o_addr = s_addr + 256;
   const float scale = fabsf(a.scale_log2);
   volatile int* const stray = reinterpret_cast<volatile int*>(smem + M_STRAY);
   float2* const mls = reinterpret_cast<float2*>(smem + L::ML_OFF);
@@ -431,19 +467,14 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
     const float raise = DT == NKV_F16 ? 7.0f : -(RESCALE_THRESHOLD + 32 - __clz(e.length + e.there));
     float m = NOTHING, l = 0.f;
 #pragma unroll 1
-    for (int n = 0; n < L::HALVES * steps && ok; ++n) {
-      const int half = L::HALVES == 2 ? n & 1 : 0, step = n / L::HALVES;
-      const int column = COPIES > 1 ? copy * WIDTH : half * WIDTH;   // of the tile's tokens
-      const int first = (p.tile0 + tile_of<L>(wg, step)) * TOK + column;
-      const uint32_t s_addr = tmem + lane_sel + wg * 128 + column, p_addr = tmem + lane_sel + wg * 128 + column / 2;
-      if (half == 0) {
-        ok = wait(&bars[S_FULL + wg], ci & 1, ctx, 940);
-        if (!ok) break;
-        tc_fence_after();
-      }
+    for (int n = 0; n < steps; ++n, ++ci) {
+      const int first = (p.tile0 + tile_of<L>(wg, n)) * TOK + slice * WIDTH;
+      ok = wait(&bars[S_FULL + wg], ci & 1, ctx, 940);
+      if (!ok) break;
+      tc_fence_after();
       uint32_t raw[GROUPS][32];
 #pragma unroll
-      for (int k = 0; k < GROUPS; ++k) tmem_ld32_issue(s_addr + 32 * k, raw[k]);
+      for (int k = 0; k < GROUPS; ++k) tmem_ld32_issue(s_addr + slice * WIDTH + 32 * k, raw[k]);
 #pragma unroll
       for (int k = 0; k < GROUPS; ++k) tmem_ld32_wait(raw[k]);
       float f = scale;
@@ -464,14 +495,9 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       top *= f;
       if (__any_sync(0xffffffffu, top - m > raise + RESCALE_THRESHOLD)) {
         // Move the reference: O and the sum are scaled by 2^(old - new).  S was issued behind PV of the step before and its commit
-        // covers both; PV of this tile's first half may still run.
+        // covers both.
         const float m_new = fmaxf(m, top - raise), alpha = exp2f(m - m_new);
         if (n > 0) {
-          if (half) {
-            ok = wait(&bars[PV_HALF + wg], ci & 1, ctx, 941);
-            if (!ok) break;
-            tc_fence_after();
-          }
 #pragma unroll 1
           for (int cc = 0; cc < D / 16; ++cc) {
             uint32_t v[16];
@@ -485,41 +511,76 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
         l *= alpha;
         m = m_new;
       }
-      // P' (16-bit pairs) replaces S, the first half's of the first columns
-      const uint64_t scale2 = pair_f32(f, f), off2 = pair_f32(-m, -m);
-      uint64_t sum2[2] = {0ull, 0ull};
+      // P' replaces S, eight scores at a time in a software pipeline: exponentials of one block beside the arguments of the next and the
+      // sums and stores of the one before.  The first half of the weights is handed over as soon as it is stored.
+      const float off = CUT ? CUT_LOG2 - m : -m;
+      const uint64_t scale2 = pair_f32(f, f), off2 = pair_f32(off, off);
+      uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull}, arg[2][4];
+      float w[2][8];
+      uint32_t packed[16];
+      auto args = [&](int b) {
 #pragma unroll
-      for (int k = 0; k < GROUPS; ++k) {
-        uint32_t packed[16];
+        for (int i = 0; i < 4; ++i)
+          arg[b & 1][i] = fma_f32x2(pair_bits(raw[b / 4][(b & 3) * 8 + 2 * i], raw[b / 4][(b & 3) * 8 + 2 * i + 1]), scale2, off2);
+      };
+      auto exps = [&](int b) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float lo, hi;
-          split_f32(fma_f32x2(pair_bits(raw[k][2 * i], raw[k][2 * i + 1]), scale2, off2), lo, hi);
-          lo = exp2_fast(lo);
-          hi = exp2_fast(hi);
-          sum2[i & 1] = add_f32x2(sum2[i & 1], pair_f32(lo, hi));
-          packed[i] = pack2<DT>(lo, hi);
+        for (int i = 0; i < 4; ++i) {
+          float x, y;
+          split_f32(arg[b & 1][i], x, y);
+          w[b & 1][2 * i] = exp2_fast(x);
+          w[b & 1][2 * i + 1] = exp2_fast(y);
         }
-        tmem_st16(p_addr + k * 16, packed);
+      };
+      auto finish = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = w[b & 1][2 * i], y = w[b & 1][2 * i + 1];
+          sum2[i] = add_f32x2(sum2[i], pair_f32(x, y));
+          if (DT == NKV_F16) {
+            packed[(b & 3) * 4 + i] = pack2<DT>(x, y);
+          } else {
+            uint32_t xb = __float_as_uint(x), yb = __float_as_uint(y);
+            if (rest) {
+              xb = __float_as_uint(x - __uint_as_float(xb & 0xFFFF0000u));
+              yb = __float_as_uint(y - __uint_as_float(yb & 0xFFFF0000u));
+            }
+            packed[(b & 3) * 4 + i] = __byte_perm(xb, yb, 0x7632);
+          }
+        }
+        if ((b & 3) == 3) {
+          tmem_st16(s_addr + slice * (WIDTH / 2) + b / 4 * 16, packed);
+          if (COPIES <= 1 && b == 7) {
+            tmem_wait_st();
+            tc_fence_before();
+            warp_arrive(&bars[P_READY + 2 * wg], lane);
+          }
+        }
+      };
+      args(0);
+#pragma unroll
+      for (int b = 0; b < 4 * GROUPS; ++b) {
+        exps(b);
+        if (b + 1 < 4 * GROUPS) args(b + 1);
+        if (b >= 1) finish(b - 1);
       }
+      finish(4 * GROUPS - 1);
       if (COPIES > 1) {   // the other copies' tokens
         constexpr uint32_t zeros[16] = {};
 #pragma unroll
-        for (int k = 1; k < COPIES; ++k)
-#pragma unroll
-          for (int g = 0; g < GROUPS; ++g)
-            tmem_st16(tmem + lane_sel + wg * 128 + ((copy + k) & (COPIES - 1)) * (WIDTH / 2) + 16 * g, zeros);
+        for (int k = GROUPS; k < 4; ++k) tmem_st16(s_addr + ((slice * GROUPS + k) & 3) * 16, zeros);
       }
       tmem_wait_st();
       tc_fence_before();
-      warp_arrive(&bars[P_READY + 2 * wg + half], lane);
-      float lo, hi;
-      split_f32(add_f32x2(sum2[0], sum2[1]), lo, hi);
-      l += lo + hi;
-      if (half == L::HALVES - 1) ++ci;
+      warp_arrive(&bars[P_READY + 2 * wg + (COPIES <= 1 ? 1 : 0)], lane);
+      float x, y;
+      split_f32(add_f32x2(add_f32x2(sum2[0], sum2[1]), add_f32x2(sum2[2], sum2[3])), x, y);
+      l += x + y;
     }
+    if (CUT) l *= CUT_INV;
+    if (rest) l = 0.f;   // (the other part's)
     if (ok && steps > 0) {
-      ok = wait(&bars[O_DONE + wg], pieces & 1, ctx, 942);
+      ok = wait(&bars[O_DONE + wg], pieces & 1, ctx, 941);
       ++pieces;
     }
     // ---- the rows: results, or a part of them
@@ -533,30 +594,66 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       softmax_sync();
       float top = NOTHING, sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < 2 * (COPIES > 0 ? COPIES : 1); ++k) top = fmaxf(top, mls[k * APART + r].x);
+      for (int k = 0; k < SOURCES; ++k) top = fmaxf(top, mls[k * APART + row % APART].x);
 #pragma unroll
-      for (int k = 0; k < 2 * (COPIES > 0 ? COPIES : 1); ++k) sum = fmaf(mls[k * APART + r].y, exp2f(mls[k * APART + r].x - top), sum);
+      for (int k = 0; k < SOURCES; ++k) sum = fmaf(mls[k * APART + row % APART].y, exp2f(mls[k * APART + row % APART].x - top), sum);
       const float factor = exp2f(m - top) * (p.whole ? 1.f / sum : 1.f);
       const bool any = sum != 0.f;      // (NaN: yes)
       const bool look = *stray != 0;
+      // As many columns at a time as there is room for, a row of them and four words apart.  Rows' results are fetched four columns a
+      // thread, neighbouring threads along a row.
+      int bits = D == 128 ? 7 : 6;
+      while (SOURCES * a.rows * ((1 << bits) + 4) > L::JOIN_WORDS) --bits;
+      const int columns = 1 << bits, stride = columns + 4;
+      float* const mine = join + (tid / APART * a.rows + r) * stride;
+      const int from0 = tid >> (bits - 2), col = (tid & (columns / 4 - 1)) * 4, more_rows = 1024 >> bits;
+      const size_t head0 = static_cast<size_t>(p.b) * a.tokens * a.heads + p.h * a.group;
 #pragma unroll 1
-      for (int cc = 0; cc < D / 16; ++cc) {
-        uint32_t v[16];
-        if (steps > 0) tmem_ld16(o_addr + cc * 16, v);
-        if (real)
+      for (int c0 = 0; c0 < D; c0 += columns) {
+#pragma unroll 1
+        for (int cc = 0; cc < columns; cc += 16) {
+          uint32_t v[16];
+          if (steps > 0) tmem_ld16(o_addr + c0 + cc, v);
+          if (real) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) join[tid * 17 + j] = any && steps > 0 ? __uint_as_float(v[j]) * factor : 0.f;
-        softmax_sync();
-        for (int i = tid; i < a.rows * 16; i += 32 * SOFTMAX_WARPS) {
-          const int from = i / 16, col = i % 16;
-          float x = 0.f;
-#pragma unroll
-          for (int k = 0; k < 2 * (COPIES > 0 ? COPIES : 1); ++k) x += join[(k * APART + from) * 17 + col];
-          if (look) x += strays<DT>(c, a, e, p, from / a.group, cc * 16 + col, D);
-          if (p.whole) store_float(a.out, DT, at_of(p, from) * D + cc * 16 + col, x);
-          else parts.o[(place_of(p) + from) * D + cc * 16 + col] = x;
+            for (int j = 0; j < 16; j += 4) {
+              float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+              if (any && steps > 0)
+                x = make_float4(__uint_as_float(v[j]) * factor, __uint_as_float(v[j + 1]) * factor, __uint_as_float(v[j + 2]) * factor,
+                                __uint_as_float(v[j + 3]) * factor);
+              *reinterpret_cast<float4*>(mine + cc + j) = x;
+            }
+          }
         }
         softmax_sync();
+#pragma unroll 1
+        for (int from = from0; from < a.rows; from += more_rows) {
+          float x[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < SOURCES; ++k) {
+            const float4 y = *reinterpret_cast<const float4*>(join + (k * a.rows + from) * stride + col);
+            x[0] += y.x;
+            x[1] += y.y;
+            x[2] += y.z;
+            x[3] += y.w;
+          }
+          const int t = from / a.group;
+          if (look)
+#pragma unroll 1
+            for (int k = 0; k < 4; ++k) {
+              const float y = strays<DT>(c, a, e, p, t, c0 + col + k, D);
+              x[0] += k == 0 ? y : 0.f;
+              x[1] += k == 1 ? y : 0.f;
+              x[2] += k == 2 ? y : 0.f;
+              x[3] += k == 3 ? y : 0.f;
+            }
+          if (p.whole)
+            *reinterpret_cast<uint2*>(a.out + (head0 + static_cast<size_t>(t) * a.heads + from - t * a.group) * D + c0 + col) =
+                make_uint2(pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]));
+          else
+            *reinterpret_cast<float4*>(parts.o + (place_of(p) + from) * D + c0 + col) = make_float4(x[0], x[1], x[2], x[3]);
+        }
+        if (c0 + columns < D) softmax_sync();
       }
       if (tid < APART && real) {
         if (p.whole) a.lse[at_of(p, r)] = any ? (top + log2f(sum)) * LN2 : -INFINITY;
@@ -569,41 +666,47 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       const bool any = l != 0.f, look = *stray != 0;
       const bool wide_out = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0, wide_part = (reinterpret_cast<uintptr_t>(parts.o) & 31) == 0;
       float* const part = parts.o + (place_of(p) + wg * QT + row) * D;
+      const size_t at = at_of(p, r);
+      uint16_t* const out = a.out + at * D;
 #pragma unroll 1
-      for (int cc = 0; cc < D / 16; ++cc) {
-        uint32_t v[16];
+      for (int cc = 0; cc < D; cc += 32) {
+        uint32_t v[32];
         if (steps > 0) {
-          tmem_ld16(o_addr + cc * 16, v);
+          tmem_ld32_issue(o_addr + cc, v);
+          tmem_ld32_wait(v);
         } else {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = 0u;
+          for (int j = 0; j < 32; ++j) v[j] = 0u;
         }
         if (!real) continue;
         if (look) {
 #pragma unroll 1
-          for (int j = 0; j < 16; ++j) {
-            const float x = strays<DT>(c, a, e, p, token, cc * 16 + j, D);
+          for (int j = 0; j < 32; ++j) {
+            const float x = strays<DT>(c, a, e, p, token, cc + j, D);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
+            for (int i = 0; i < 32; ++i)
               if (i == j) v[i] = __float_as_uint(__uint_as_float(v[i]) + x);
           }
         }
         if (p.whole) {
-          uint32_t o[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            o[i] = any ? pack2<DT>(__uint_as_float(v[2 * i]) * inv, __uint_as_float(v[2 * i + 1]) * inv) : 0u;
-          store32(a.out + at_of(p, r) * D + cc * 16, o, wide_out);
+          for (int j = 0; j < 32; j += 16) {
+            uint32_t o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              o[i] = any ? pack2<DT>(__uint_as_float(v[j + 2 * i]) * inv, __uint_as_float(v[j + 2 * i + 1]) * inv) : 0u;
+            store32(out + cc + j, o, wide_out);
+          }
         } else {
 #pragma unroll
-          for (int j = 0; j < 16; j += 8) {
+          for (int j = 0; j < 32; j += 8) {
             const uint32_t o[8] = {v[j], v[j + 1], v[j + 2], v[j + 3], v[j + 4], v[j + 5], v[j + 6], v[j + 7]};
-            store32(part + cc * 16 + j, o, wide_part);
+            store32(part + cc + j, o, wide_part);
           }
         }
       }
       if (real) {
-        if (p.whole) a.lse[at_of(p, r)] = any ? (m + log2f(l)) * LN2 : -INFINITY;
+        if (p.whole) a.lse[at] = any ? (m + log2f(l)) * LN2 : -INFINITY;
         else parts.ml[place_of(p) + wg * QT + row] = make_float2(m, l);
       }
     }
@@ -644,7 +747,6 @@ page_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     mbar_init(&bars[DRAINED], 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars[S_FULL + i], 1);
-      mbar_init(&bars[PV_HALF + i], 1);
       mbar_init(&bars[O_DONE + i], 1);
       mbar_init(&bars[O_FREE + i], QT / 32);
     }
@@ -652,6 +754,7 @@ page_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     for (int i = 0; i < L::STAGES; ++i) {
       mbar_init(&bars[FULL + i], 1);
       mbar_init(&bars[FREE + i], 1);
+      mbar_init(&bars[LOOK + i], 1);
       mbar_init(&bars[CLEAN + i], OPERAND_WARPS);
     }
     *abort_flag = 0;
@@ -659,40 +762,53 @@ page_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     fence_barrier_init();
     fence_proxy_async();
   }
-  // ---- the plan
-  if (tid < a.sequences) {
-    bool bad;
-    extents[tid] = extent_of(c, a.counts, a.tokens, tid, bad);
-    if (bad) report(status, STATUS_PAGE);
-    start[tid] = 0;
-  }
+  // ---- the plan.  Few units a sequence: one warp makes it, ahead of the barrier that the others need anyway.
   if (warp == MMA_WARP) tmem_alloc(tmem_slot, 512);
-  __syncthreads();
-  for (int i = tid; i < a.sequences * a.shape.units; i += THREADS) {
-    const int b = i / a.shape.units, u = i % a.shape.units;
-    const uint32_t cost = page::cost_of(page::tiles_seen(a.shape, extents[b], u * L::UNIT, L::UNIT));
-    if (cost) atomicAdd(&start[b], cost);
+  if (warp > MMA_WARP && lane == 0) {
+    prefetch_tensormap(&map_k);
+    prefetch_tensormap(&map_v);
   }
-  __syncthreads();
+  const bool one_warp = a.shape.units <= 4;
+  if (!one_warp) {
+    if (tid < a.sequences) {
+      bool bad;
+      extents[tid] = extent_of(c, a.counts, a.tokens, tid, bad);
+      if (bad) report(status, STATUS_PAGE);
+      start[tid] = 0;
+    }
+    __syncthreads();
+    for (int i = tid; i < a.sequences * a.shape.units; i += THREADS) {
+      const int b = i / a.shape.units, u = i % a.shape.units;
+      const uint32_t cost = page::cost_of(page::tiles_seen(a.shape, extents[b], u * L::UNIT, L::UNIT));
+      if (cost) atomicAdd(&start[b], cost);
+    }
+    __syncthreads();
+  }
   if (warp == 0) {
-    uint32_t v[4], mine = 0;
+    uint32_t carry = 0;
+    for (int b0 = 0; b0 <= a.sequences; b0 += 32) {
+      const int b = b0 + lane;
+      uint32_t cost = 0;
+      if (b < a.sequences) {
+        if (one_warp) {
+          bool bad;
+          const Extent e = extent_of(c, a.counts, a.tokens, b, bad);
+          if (bad) report(status, STATUS_PAGE);
+          extents[b] = e;
+          for (int u = 0; u < a.shape.units; ++u) cost += page::cost_of(page::tiles_seen(a.shape, e, u * L::UNIT, L::UNIT));
+        } else {
+          cost = start[b];
+        }
+        cost *= a.shape.kv_heads;
+      }
+      uint32_t upto = cost;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      v[k] = 4 * lane + k < a.sequences ? start[4 * lane + k] * a.shape.kv_heads : 0u;
-      mine += v[k];
-    }
-    uint32_t before = mine;
-#pragma unroll
-    for (int x = 1; x < 32; x <<= 1) {
-      const uint32_t other = __shfl_up_sync(0xffffffffu, before, x);
-      if (lane >= x) before += other;
-    }
-    before -= mine;
-    __syncwarp();
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (4 * lane + k <= a.sequences) start[4 * lane + k] = before;
-      before += v[k];
+      for (int x = 1; x < 32; x <<= 1) {
+        const uint32_t other = __shfl_up_sync(0xffffffffu, upto, x);
+        if (lane >= x) upto += other;
+      }
+      if (b <= a.sequences) start[b] = carry + upto - cost;
+      carry += __shfl_sync(0xffffffffu, upto, 31);
     }
   }
   tc_fence_before();
@@ -729,6 +845,7 @@ template <int DT, int D>
 __global__ void __launch_bounds__(256)
 join_parts_kernel(TileCall a, Parts parts, int runs) {
   __shared__ uint32_t before;
+  __shared__ float shared[256][11];   // (rows of an odd number of words: no two of a warp's in one bank)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Shape& s = a.shape;
   const int slices = (min(s.unit, s.rows) + SLICE - 1) / SLICE, unit = blockIdx.x / slices, slice = blockIdx.x % slices, h = blockIdx.y, b = blockIdx.z;
@@ -739,6 +856,8 @@ join_parts_kernel(TileCall a, Parts parts, int runs) {
   plan.deal(runs);
   const Extent e = parts.extents[b];
   const int nt = page::tiles_seen(s, e, unit * s.unit, s.unit);
+  const int row0 = slice * SLICE, rows = min(SLICE, min(s.unit, a.rows - unit * s.unit) - row0);
+  if (rows <= 0) return;   // (the last unit may have fewer)
   uint32_t r0 = 0, r1 = 0;
   if (nt > 0) {
     if (threadIdx.x == 0) before = 0;
@@ -752,32 +871,53 @@ join_parts_kernel(TileCall a, Parts parts, int runs) {
     r1 = plan.run_of(begin + nt - 1);
     if (r0 == r1) return;   // one run had all of it and wrote the results
   }
+  // a thread per row, 16 bytes of it and share of the parts: with few rows the threads that rows do not need share a row's parts
   constexpr int PER_ROW = D / 8, ROWS = 256 / PER_ROW;
-  for (int i = threadIdx.x / PER_ROW; i < SLICE; i += ROWS) {
-    const int row = slice * SLICE + i, r = unit * s.unit + row, col = (threadIdx.x % PER_ROW) * 8;
-    if (row >= s.unit || r >= a.rows) break;
-    const int token = r / a.group;
-    const size_t at = (static_cast<size_t>(b) * a.tokens + token) * a.heads + h * a.group + r - token * a.group;
+  int shares = 1;
+  while (shares * 2 * rows <= ROWS) shares *= 2;
+  const int col = (threadIdx.x % PER_ROW) * 8, share = threadIdx.x / PER_ROW & (shares - 1);
+  for (int i = threadIdx.x / PER_ROW / shares; i < (rows + ROWS / shares - 1) / (ROWS / shares) * (ROWS / shares); i += ROWS / shares) {
+    const int row = row0 + i, r = unit * s.unit + row, token = r / a.group;
     float top = NOTHING, sum = 0.f, acc[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) acc[k] = 0.f;
-    if (nt > 0) {
-      // the run the unit starts in has it as a piece that starts with the unit, the others as one that starts inside
-      auto place = [&](uint32_t run) { return (2 * static_cast<size_t>(run) + (run == r0 ? 1 : 0)) * s.unit + row; };
-      for (uint32_t run = r0; run <= r1; ++run) top = fmaxf(top, __ldcg(&parts.ml[place(run)]).x);
-      for (uint32_t run = r0; run <= r1; ++run) {
-        const float2 ml = __ldcg(&parts.ml[place(run)]);
-        const float4 lo = __ldcg(reinterpret_cast<const float4*>(parts.o + place(run) * D + col));
-        const float4 hi = __ldcg(reinterpret_cast<const float4*>(parts.o + place(run) * D + col + 4));
-        const float f = exp2f(ml.x - top);
-        sum = fmaf(ml.y, f, sum);
+    if (nt > 0 && i < rows) {
+#pragma unroll 2
+      for (uint32_t run = r0 + share; run <= r1; run += shares) {
+        // the run the unit starts in has it as a piece that starts with the unit, the others as one that starts inside
+        const size_t place = (2 * static_cast<size_t>(run) + (run == r0 ? 1 : 0)) * s.unit + row;
+        const float2 ml = __ldcg(&parts.ml[place]);
+        const float4 lo = __ldcg(reinterpret_cast<const float4*>(parts.o + place * D + col));
+        const float4 hi = __ldcg(reinterpret_cast<const float4*>(parts.o + place * D + col + 4));
         const float part[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        const float next = fmaxf(top, ml.x), old = exp2f(top - next), now = exp2f(ml.x - next);
+        top = next;
+        sum = fmaf(ml.y, now, sum * old);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) acc[k] = fmaf(part[k], f, acc[k]);
+        for (int k = 0; k < 8; ++k) acc[k] = fmaf(part[k], now, acc[k] * old);
       }
     }
+    if (shares > 1) {   // (one round: rows <= ROWS / shares)
+      float* const mine = shared[threadIdx.x];
+      mine[0] = top;
+      mine[1] = sum;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mine[2 + k] = acc[k];
+      __syncthreads();
+      if (share > 0) return;
+      for (int k = 1; k < shares; ++k) {
+        const float* const other = shared[threadIdx.x + k * PER_ROW];
+        const float next = fmaxf(top, other[0]), old = exp2f(top - next), now = exp2f(other[0] - next);
+        top = next;
+        sum = fmaf(other[1], now, sum * old);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = fmaf(other[2 + j], now, acc[j] * old);
+      }
+    }
+    if (i >= rows) continue;
     const bool any = sum != 0.f;
     const float inv = any ? 1.f / sum : 0.f;
+    const size_t at = (static_cast<size_t>(b) * a.tokens + token) * a.heads + h * a.group + r - token * a.group;
     uint32_t o[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) o[k] = any ? pack2<DT>(acc[2 * k] * inv, acc[2 * k + 1] * inv) : 0u;
@@ -813,10 +953,11 @@ int page_tile(const PageArrays& c, const PageCall& call, int n, int dtype, int d
   parts.start = reinterpret_cast<uint32_t*>(parts.extents + page::MOST_SEQUENCES);
   CUtensorMap maps[2];
   for (int i = 0; i < 2; ++i) {
-    const uint64_t dims[2] = {static_cast<uint64_t>(d), (static_cast<uint64_t>(c.pages) * c.kv_heads) << c.shift};
-    const uint64_t strides[1] = {static_cast<uint64_t>(d) * 2};
-    const uint32_t box[2] = {64, 1u << c.shift};
-    const int rc = encode_tensor_map(&maps[i], 2, i ? c.v : c.k, 2, dims, strides, box, 128);
+    // elements of a chunk, rows of a group, chunks of a row, groups
+    const uint64_t dims[4] = {64, 8, static_cast<uint64_t>(d) / 64, (static_cast<uint64_t>(c.pages) * c.kv_heads << c.shift) / 8};
+    const uint64_t strides[3] = {static_cast<uint64_t>(d) * 2, 128, static_cast<uint64_t>(d) * 16};
+    const uint32_t box[4] = {64, 8, static_cast<uint32_t>(d) / 64, (1u << c.shift) / 8};
+    const int rc = encode_tensor_map(&maps[i], 2, i ? c.v : c.k, 4, dims, strides, box, 128);
     if (rc != NKV_OK) return rc;
   }
   auto run = [&](auto kernel, int smem) {
