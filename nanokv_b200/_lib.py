@@ -6,6 +6,7 @@ importing the product path raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_void_p
 
 from . import build as _build
@@ -61,6 +62,12 @@ class PageCache(ctypes.Structure):
     _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p), ("table", c_void_p), ("lengths", c_void_p),
                 ("batch", c_int32), ("row_pages", c_int32), ("pages", c_int32), ("page", c_int32),
                 ("kv_heads", c_int32), ("head_dim", c_int32), ("dtype", c_int32)]
+
+
+@functools.lru_cache(maxsize=None)
+def page_caches(count: int):
+    """The array type of ``count`` of them."""
+    return PageCache * count
 
 
 class Tokens(ctypes.Structure):

@@ -66,9 +66,9 @@ template <int D, int COPIES> struct Layout {
   static constexpr int LEAD = NARROW ? 2 : 1;      // K tiles ahead of the first V tile in the ring
   static constexpr int Q_OFF = META;
   static constexpr int RING_OFF = Q_OFF + QTILES * DCH * SUB;
-  static constexpr int ML_OFF = RING_OFF + STAGES * STAGE;             // narrow: references and sums of 256 threads
-  static constexpr int JOIN_OFF = ML_OFF + (NARROW ? 256 * 8 : 0);     // narrow: columns of O of all copies of the rows
-  static constexpr int JOIN_WORDS = D == 128 ? 7424 : 11264;
+  static constexpr int ML_OFF = RING_OFF + STAGES * STAGE;             // narrow: references and sums of 256 threads, of two pieces
+  static constexpr int JOIN_OFF = ML_OFF + (NARROW ? 2 * 256 * 8 : 0);     // narrow: columns of O of all copies of the rows
+  static constexpr int JOIN_WORDS = D == 128 ? 6912 : 11264;
   static constexpr int BYTES = JOIN_OFF + (NARROW ? JOIN_WORDS * 4 : 0);
   static constexpr int DYNAMIC = BYTES + 1024;     // room to start on 1,024 bytes
   static constexpr int GROUP = DCH * 1024;         // eight rows of a K or V tile: their chunks of 64 elements side by side
@@ -103,13 +103,13 @@ __device__ __forceinline__ int first_masked(const Shape& s, const Extent& e, con
   return page::sees_all_before(s.sight, e, p.unit * s.unit / s.group) / TOK - p.tile0;
 }
 
-// A run holds at most one piece that starts inside a unit and one that starts with it and is cut: two places each.  Behind them what
-// the second launch needs of the plan.
+// A run holds at most one piece that starts inside a unit and one that starts with it and is cut: two places each.  The second launch
+// finds the latter in `cut`, with the run that has the unit's last tile.
+struct Cut { int b, h, unit, last; };   // last 0: none (a cut unit never ends in the first run)
 struct Parts {
   float* o;             // [2 runs][unit rows][D], relative to 2^m
   float2* ml;           // [2 runs][unit rows] m, row sum
-  page::Extent* extents;
-  uint32_t* start;
+  Cut* cut;             // [runs]
 };
 
 struct TileCall : PageCall {
@@ -279,6 +279,18 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
     }
     items += 2 * p.nt;
   }
+  // ---- rows of units without tiles: they see nothing
+  const int units = a.shape.units, heads = a.shape.kv_heads;
+  for (int i = blockIdx.x; i < a.sequences * units * heads; i += gridDim.x) {
+    const int h = i % heads, u = i / heads % units, b = i / heads / units, r0 = u * L::UNIT, rows = min(L::UNIT, a.rows - r0);
+    if (page::tiles_seen(a.shape, plan.extents[b], r0, L::UNIT) > 0) continue;
+    for (int k = tid; k < rows * PER_ROW; k += 32 * OPERAND_WARPS) {
+      const int r = r0 + k / PER_ROW, col = k % PER_ROW * 8, token = r / a.group;
+      const size_t at = (static_cast<size_t>(b) * a.tokens + token) * a.heads + h * a.group + r - token * a.group;
+      *reinterpret_cast<uint4*>(a.out + at * D + col) = make_uint4(0, 0, 0, 0);
+      if (col == 0) a.lse[at] = -INFINITY;
+    }
+  }
 }
 
 // ---- warp 10: MMA issue -----------------------------------------------------------------------------------------
@@ -444,12 +456,17 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
   const uint32_t s_addr = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + wg * 128, o_addr = s_addr + 256;
   const float scale = fabsf(a.scale_log2);
   volatile int* const stray = reinterpret_cast<volatile int*>(smem + M_STRAY);
-  float2* const mls = reinterpret_cast<float2*>(smem + L::ML_OFF);
   float* const join = reinterpret_cast<float*>(smem + L::JOIN_OFF);
   Walk walk(plan, a.shape, blockIdx.x);
   Piece p;
   bool ok = true, more = true;
   int ci = 0, pieces = 0;   // steps and pieces of this chain
+  int odd = 0;
+  Cut cut{0, 0, 0, 0};
+  auto note_cut = [&]() {
+    if (!p.whole && p.tile0 == 0) cut = Cut{p.b, p.h, p.unit, static_cast<int>(plan.run_of(walk.g + page::cost_of(walk.tiles) - walk.at - 1))};
+  };
+  const bool wide_out = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0, wide_part = (reinterpret_cast<uintptr_t>(parts.o) & 31) == 0;
   auto place_of = [&](const Piece& pc) { return (2 * static_cast<size_t>(blockIdx.x) + (pc.tile0 == 0 ? 1 : 0)) * L::UNIT; };
   // the row of the results that row r of a piece's kv head is
   auto at_of = [&](const Piece& pc, int r) {
@@ -584,87 +601,136 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       ++pieces;
     }
     // ---- the rows: results, or a part of them
+    note_cut();
     if (L::NARROW) {
+      // (places in turn: a warp may still read those of the piece before, not of the one before that)
+      float2* const mls = reinterpret_cast<float2*>(smem + L::ML_OFF) + odd * 256;
+      odd ^= 1;
+      mls[tid] = make_float2(m, l);
+      tc_fence_before();
       if (softmax_any(!ok)) {   // (all of the warps take part in what follows, or none)
         ok = false;
         break;
       }
       tc_fence_after();
-      mls[tid] = make_float2(m, l);
-      softmax_sync();
+      // A row has the same lane of tensor memory in both chains: a thread takes both, of half the columns.
+      const bool second = p.nt > 1;      // chain 1 had steps
       float top = NOTHING, sum = 0.f;
 #pragma unroll
       for (int k = 0; k < SOURCES; ++k) top = fmaxf(top, mls[k * APART + row % APART].x);
 #pragma unroll
       for (int k = 0; k < SOURCES; ++k) sum = fmaf(mls[k * APART + row % APART].y, exp2f(mls[k * APART + row % APART].x - top), sum);
-      const float factor = exp2f(m - top) * (p.whole ? 1.f / sum : 1.f);
-      const bool any = sum != 0.f;      // (NaN: yes)
-      const bool look = *stray != 0;
-      // As many columns at a time as there is room for, a row of them and four words apart.  Rows' results are fetched four columns a
-      // thread, neighbouring threads along a row.
-      int bits = D == 128 ? 7 : 6;
-      while (SOURCES * a.rows * ((1 << bits) + 4) > L::JOIN_WORDS) --bits;
-      const int columns = 1 << bits, stride = columns + 4;
-      float* const mine = join + (tid / APART * a.rows + r) * stride;
-      const int from0 = tid >> (bits - 2), col = (tid & (columns / 4 - 1)) * 4, more_rows = 1024 >> bits;
-      const size_t head0 = static_cast<size_t>(p.b) * a.tokens * a.heads + p.h * a.group;
+      const bool any = sum != 0.f, look = *stray != 0;      // (NaN: any)
+      const float inv = p.whole ? 1.f / sum : 1.f, f0 = exp2f(mls[row].x - top) * inv, f1 = exp2f(mls[128 + row].x - top) * inv;
+      const uint32_t o0 = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + 256 + wg * (D / 2);
+      // 16 columns of the row: both chains' together
+      auto joined = [&](int at, float (&x)[16]) {
+        uint32_t u[16], v[16];
+        tmem_ld16_issue(o0 + at, u);
+        if (second) tmem_ld16_issue(o0 + 128 + at, v);
+        tmem_ld16_wait(u);
+        if (second) tmem_ld16_wait(v);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          x[j] = __uint_as_float(u[j]) * f0;
+          if (second) x[j] = fmaf(__uint_as_float(v[j]), f1, x[j]);
+          if (!any) x[j] = 0.f;
+        }
+      };
+      const size_t row_at = at_of(p, r);
+      auto put = [&](int col, const float (&x)[16], size_t to, size_t part) {   // 16 columns of a row
+        if (p.whole) {
+          uint32_t o[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = pack2<DT>(x[2 * i], x[2 * i + 1]);
+          store32(a.out + to * D + col, o, wide_out);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; j += 8) {
+            uint32_t o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(x[j + i]);
+            store32(parts.o + part * D + col + j, o, wide_part);
+          }
+        }
+      };
+      auto add_strays = [&](int t, int col, float (&x)[16]) {
 #pragma unroll 1
-      for (int c0 = 0; c0 < D; c0 += columns) {
+        for (int j = 0; j < 16; ++j) {
+          const float y = strays<DT>(c, a, e, p, t, col + j, D);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (i == j) x[i] += y;
+        }
+      };
+      if (COPIES <= 1) {
 #pragma unroll 1
-        for (int cc = 0; cc < columns; cc += 16) {
-          uint32_t v[16];
-          if (steps > 0) tmem_ld16(o_addr + c0 + cc, v);
-          if (real) {
+        for (int cc = 0; cc < D / 2; cc += 16) {
+          float x[16];
+          joined(cc, x);
+          if (!real) continue;
+          const int col = wg * (D / 2) + cc;
+          if (look) add_strays(token, col, x);
+          put(col, x, row_at, place_of(p) + r);
+        }
+      } else {
+        // The copies of a row are other warps': through shared memory, as many columns at a time as there is room for, a row of them
+        // and four words apart.  Results are fetched 16 columns a thread.
+        int bits = D == 128 ? 6 : 5;
+        while (SOURCES * a.rows * ((1 << bits) + 4) > L::JOIN_WORDS) --bits;
+        const int columns = 1 << bits, stride = columns + 4, here = row >> (bits - 4), col = (row & (columns / 16 - 1)) * 16;
+        float* const ours = join + wg * (SOURCES / 2) * a.rows * stride;
+#pragma unroll 1
+        for (int c0 = 0; c0 < D / 2; c0 += columns) {
+#pragma unroll 1
+          for (int cc = 0; cc < columns; cc += 16) {
+            float x[16];
+            joined(c0 + cc, x);
+            float* const to = ours + (row / APART * a.rows + r) * stride + cc;
+            if (real)
+#pragma unroll
+              for (int j = 0; j < 16; j += 4) *reinterpret_cast<float4*>(to + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+          }
+          softmax_sync();
+#pragma unroll 1
+          for (int from = here; from < a.rows; from += 2048 >> bits) {
+            float x[16];
 #pragma unroll
             for (int j = 0; j < 16; j += 4) {
-              float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-              if (any && steps > 0)
-                x = make_float4(__uint_as_float(v[j]) * factor, __uint_as_float(v[j + 1]) * factor, __uint_as_float(v[j + 2]) * factor,
-                                __uint_as_float(v[j + 3]) * factor);
-              *reinterpret_cast<float4*>(mine + cc + j) = x;
-            }
-          }
-        }
-        softmax_sync();
-#pragma unroll 1
-        for (int from = from0; from < a.rows; from += more_rows) {
-          float x[4] = {0.f, 0.f, 0.f, 0.f};
+              const float* const at = ours + from * stride + col + j;
+              float4 y = *reinterpret_cast<const float4*>(at);
 #pragma unroll
-          for (int k = 0; k < SOURCES; ++k) {
-            const float4 y = *reinterpret_cast<const float4*>(join + (k * a.rows + from) * stride + col);
-            x[0] += y.x;
-            x[1] += y.y;
-            x[2] += y.z;
-            x[3] += y.w;
-          }
-          const int t = from / a.group;
-          if (look)
-#pragma unroll 1
-            for (int k = 0; k < 4; ++k) {
-              const float y = strays<DT>(c, a, e, p, t, c0 + col + k, D);
-              x[0] += k == 0 ? y : 0.f;
-              x[1] += k == 1 ? y : 0.f;
-              x[2] += k == 2 ? y : 0.f;
-              x[3] += k == 3 ? y : 0.f;
+              for (int k = 1; k < SOURCES / 2; ++k) {
+                const float4 z = *reinterpret_cast<const float4*>(at + k * a.rows * stride);
+                y = make_float4(y.x + z.x, y.y + z.y, y.z + z.z, y.w + z.w);
+              }
+              x[j] = y.x;
+              x[j + 1] = y.y;
+              x[j + 2] = y.z;
+              x[j + 3] = y.w;
             }
-          if (p.whole)
-            *reinterpret_cast<uint2*>(a.out + (head0 + static_cast<size_t>(t) * a.heads + from - t * a.group) * D + c0 + col) =
-                make_uint2(pack2<DT>(x[0], x[1]), pack2<DT>(x[2], x[3]));
-          else
-            *reinterpret_cast<float4*>(parts.o + (place_of(p) + from) * D + c0 + col) = make_float4(x[0], x[1], x[2], x[3]);
+            const int first = wg * (D / 2) + c0 + col;
+            if (look) add_strays(from / a.group, first, x);
+            put(first, x, at_of(p, from), place_of(p) + from);
+          }
+          if (c0 + columns < D / 2) softmax_sync();
         }
-        if (c0 + columns < D) softmax_sync();
       }
       if (tid < APART && real) {
-        if (p.whole) a.lse[at_of(p, r)] = any ? (top + log2f(sum)) * LN2 : -INFINITY;
+        if (p.whole) a.lse[row_at] = any ? (top + log2f(sum)) * LN2 : -INFINITY;
         else parts.ml[place_of(p) + r] = make_float2(top, sum);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&bars[O_FREE]);
+        if (second) mbar_arrive(&bars[O_FREE + 1]);
       }
     } else {
       if (!ok) break;
       tc_fence_after();
       const float inv = 1.f / l;
       const bool any = l != 0.f, look = *stray != 0;
-      const bool wide_out = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0, wide_part = (reinterpret_cast<uintptr_t>(parts.o) & 31) == 0;
       float* const part = parts.o + (place_of(p) + wg * QT + row) * D;
       const size_t at = at_of(p, r);
       uint16_t* const out = a.out + at * D;
@@ -709,10 +775,10 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
         if (p.whole) a.lse[at] = any ? (m + log2f(l)) * LN2 : -INFINITY;
         else parts.ml[place_of(p) + wg * QT + row] = make_float2(m, l);
       }
-    }
-    if (steps > 0) {
-      tc_fence_before();
-      warp_arrive(&bars[O_FREE + wg], lane);
+      if (steps > 0) {
+        tc_fence_before();
+        warp_arrive(&bars[O_FREE + wg], lane);
+      }
     }
   }
   // a launch that gave up: NaN for the piece it stopped in and all later ones
@@ -723,9 +789,11 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
         if (p.whole) a.lse[at_of(p, r)] = CUDART_NAN_F;
         else parts.ml[place_of(p) + tid] = make_float2(0.f, CUDART_NAN_F);
       }
+      note_cut();
       more = walk.next(plan, a.shape, p);
     }
   }
+  if (tid == 0) parts.cut[blockIdx.x] = cut;
 }
 
 template <int DT, int D, int COPIES>
@@ -748,7 +816,7 @@ page_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars[S_FULL + i], 1);
       mbar_init(&bars[O_DONE + i], 1);
-      mbar_init(&bars[O_FREE + i], QT / 32);
+      mbar_init(&bars[O_FREE + i], L::NARROW ? SOFTMAX_WARPS : QT / 32);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&bars[P_READY + i], QT / 32);
     for (int i = 0; i < L::STAGES; ++i) {
@@ -814,12 +882,6 @@ page_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (blockIdx.x == 0) {   // for the second launch
-    for (int i = tid; i <= a.sequences; i += THREADS) {
-      if (i < a.sequences) parts.extents[i] = extents[i];
-      parts.start[i] = start[i];
-    }
-  }
   const uint32_t tmem = *tmem_slot;
   const Ctx ctx{abort_flag};
   Plan plan;
@@ -838,39 +900,18 @@ page_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   if (tid == 0 && *abort_flag) atomicCAS(status, 0, *abort_flag);
 }
 
-// Joins the parts of cut units and fills the rows of units that have no tiles; a thread block per (unit, kv head, sequence) and 32
-// rows, a thread per row and 16 bytes of it.
-constexpr int SLICE = 32;
+// Joins the parts of cut units: a thread block per run in which a cut unit begins, and SLICE rows of the unit.
+constexpr int SLICE = 16;
 template <int DT, int D>
 __global__ void __launch_bounds__(256)
-join_parts_kernel(TileCall a, Parts parts, int runs) {
-  __shared__ uint32_t before;
+join_parts_kernel(TileCall a, Parts parts) {
   __shared__ float shared[256][11];   // (rows of an odd number of words: no two of a warp's in one bank)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Shape& s = a.shape;
-  const int slices = (min(s.unit, s.rows) + SLICE - 1) / SLICE, unit = blockIdx.x / slices, slice = blockIdx.x % slices, h = blockIdx.y, b = blockIdx.z;
-  Plan plan;
-  plan.start = parts.start;
-  plan.extents = parts.extents;
-  plan.sequences = a.sequences;
-  plan.deal(runs);
-  const Extent e = parts.extents[b];
-  const int nt = page::tiles_seen(s, e, unit * s.unit, s.unit);
-  const int row0 = slice * SLICE, rows = min(SLICE, min(s.unit, a.rows - unit * s.unit) - row0);
-  if (rows <= 0) return;   // (the last unit may have fewer)
-  uint32_t r0 = 0, r1 = 0;
-  if (nt > 0) {
-    if (threadIdx.x == 0) before = 0;
-    __syncthreads();
-    uint32_t mine = 0;
-    for (int u = threadIdx.x; u < unit; u += 256) mine += page::cost_of(page::tiles_seen(s, e, u * s.unit, s.unit));
-    if (mine) atomicAdd(&before, mine);
-    __syncthreads();
-    const uint32_t begin = plan.start[b] + h * ((plan.start[b + 1] - plan.start[b]) / s.kv_heads) + before + page::PIECE_TILES;
-    r0 = plan.run_of(begin);
-    r1 = plan.run_of(begin + nt - 1);
-    if (r0 == r1) return;   // one run had all of it and wrote the results
-  }
+  const int r0 = blockIdx.x, row0 = blockIdx.y * SLICE;
+  const int4 cut = __ldcg(reinterpret_cast<const int4*>(parts.cut) + r0);
+  const int b = cut.x, h = cut.y, unit = cut.z, r1 = cut.w, rows = min(SLICE, min(s.unit, a.rows - unit * s.unit) - row0);
+  if (r1 == 0 || rows <= 0) return;
   // a thread per row, 16 bytes of it and share of the parts: with few rows the threads that rows do not need share a row's parts
   constexpr int PER_ROW = D / 8, ROWS = 256 / PER_ROW;
   int shares = 1;
@@ -881,9 +922,9 @@ join_parts_kernel(TileCall a, Parts parts, int runs) {
     float top = NOTHING, sum = 0.f, acc[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) acc[k] = 0.f;
-    if (nt > 0 && i < rows) {
-#pragma unroll 2
-      for (uint32_t run = r0 + share; run <= r1; run += shares) {
+    if (i < rows) {
+#pragma unroll 4
+      for (int run = r0 + share; run <= r1; run += shares) {
         // the run the unit starts in has it as a piece that starts with the unit, the others as one that starts inside
         const size_t place = (2 * static_cast<size_t>(run) + (run == r0 ? 1 : 0)) * s.unit + row;
         const float2 ml = __ldcg(&parts.ml[place]);
@@ -927,12 +968,10 @@ join_parts_kernel(TileCall a, Parts parts, int runs) {
 }
 
 int unit_of(int rows) { return rows > QT ? 2 * QT : QT; }
-size_t plan_bytes() { return page::MOST_SEQUENCES * sizeof(page::Extent) + (page::MOST_SEQUENCES + 1) * sizeof(uint32_t); }
-
 }  // namespace
 
 size_t page_tile_bytes(int rows, int d) {
-  return static_cast<size_t>(sm_count()) * 2 * unit_of(rows) * (d * sizeof(float) + sizeof(float2)) + plan_bytes();
+  return static_cast<size_t>(sm_count()) * 2 * unit_of(rows) * (d * sizeof(float) + sizeof(float2)) + sm_count() * sizeof(Cut);
 }
 
 int page_tile(const PageArrays& c, const PageCall& call, int n, int dtype, int d, void* workspace, int32_t* status, cudaStream_t stream) {
@@ -949,8 +988,7 @@ int page_tile(const PageArrays& c, const PageCall& call, int n, int dtype, int d
   Parts parts;
   parts.o = static_cast<float*>(workspace);
   parts.ml = reinterpret_cast<float2*>(parts.o + static_cast<size_t>(sm_count()) * 2 * unit * d);
-  parts.extents = reinterpret_cast<page::Extent*>(parts.ml + static_cast<size_t>(sm_count()) * 2 * unit);
-  parts.start = reinterpret_cast<uint32_t*>(parts.extents + page::MOST_SEQUENCES);
+  parts.cut = reinterpret_cast<Cut*>(parts.ml + static_cast<size_t>(sm_count()) * 2 * unit);
   CUtensorMap maps[2];
   for (int i = 0; i < 2; ++i) {
     // elements of a chunk, rows of a group, chunks of a row, groups
@@ -982,14 +1020,14 @@ int page_tile(const PageArrays& c, const PageCall& call, int n, int dtype, int d
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(a.shape.units * ceil_div(min(unit, a.rows), SLICE), c.kv_heads, n);
+  config.gridDim = dim3(runs, ceil_div(min(unit, a.rows), SLICE));
   config.blockDim = dim3(256);
   config.stream = stream;
   config.attrs = &attribute;
   config.numAttrs = 1;
   auto join = d == 128 ? (dtype == NKV_BF16 ? join_parts_kernel<NKV_BF16, 128> : join_parts_kernel<NKV_F16, 128>)
                        : (dtype == NKV_BF16 ? join_parts_kernel<NKV_BF16, 64> : join_parts_kernel<NKV_F16, 64>);
-  NKV_CUDA(cudaLaunchKernelEx(&config, join, a, parts, runs));
+  NKV_CUDA(cudaLaunchKernelEx(&config, join, a, parts));
   return NKV_OK;
 }
 

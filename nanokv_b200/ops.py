@@ -881,38 +881,56 @@ def _device_ints(x: torch.Tensor | None, shape: tuple, name: str, device: torch.
     return x.data_ptr()
 
 
-def page_append(struct: _lib.PageCache, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None, *, counts=None,
-                rotation: _lib.Rotation | None = None):
-    """Pending tokens k, v [batch, tokens, kv_heads, width] put behind the settled ones (nkv_page_append) -> q rotated, or None."""
-    out = None if q is None else torch.empty_like(q, memory_format=torch.contiguous_format)
+def page_rows(x: torch.Tensor, batch: int, width: int, dtype: torch.dtype, device: torch.device, name: str) -> _lib.Tokens:
+    """Rows x [batch, tokens, heads, width] as the ABI takes them, whatever their strides but the last."""
+    shape = x.shape
+    if len(shape) != 4 or shape[0] != batch or shape[3] != width:
+        raise ValueError(f"{name} must be [{batch}, tokens, heads, {width}]; got {list(shape)}")
+    if x.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, as the cache is; got {x.dtype}")
+    if x.device != device:
+        raise (ValueError if x.is_cuda else RuntimeError)(f"{name} is on {x.device}, the cache on {device}")
+    in_batch, in_token, in_head, element = x.stride()
+    if element != 1:
+        raise ValueError(f"{name} must be contiguous along the width")
+    return _lib.Tokens(x.data_ptr(), in_batch, in_token, in_head, shape[2])
+
+
+def page_append(struct: _lib.PageCache, k: _lib.Tokens, v: _lib.Tokens, q: _lib.Tokens | None, q_out: torch.Tensor | None,
+                tokens: int, *, counts=None, rotation: _lib.Rotation | None = None, device: torch.device) -> None:
+    """Pending tokens k, v put behind the settled ones, queries q rotated to ``q_out`` (nkv_page_append); rows as ``page_rows``
+    gives them."""
     _lib.check(_lib.library().nkv_page_append(
-        struct, _rows(k, "k"), _rows(v, "v"), None if q is None else _rows(q, "q"), None if q is None else out.data_ptr(),
-        k.shape[1], _device_ints(counts, (struct.batch,), "counts", k.device), rotation, status_word(k.device).data_ptr(),
-        _raw_stream(k.device)))
-    return out
+        struct, k, v, q, None if q_out is None else q_out.data_ptr(), tokens, _device_ints(counts, (struct.batch,), "counts", device),
+        rotation, status_word(device).data_ptr(), _raw_stream(device)))
 
 
-def page_attend(struct: _lib.PageCache, q: torch.Tensor, *, counts=None, tree: torch.Tensor | None = None, causal: bool = True,
-                scale: float, status: torch.Tensor | None = None):
-    """Attention of pending queries q [batch, tokens, heads, width] (nkv_page_attend) -> (O like q, lse f32 [batch, tokens,
-    heads]).  ``tree`` i32 [tokens, words] or [batch, tokens, words]: bits of the pending tokens that each query sees."""
-    rows = _rows(q, "q")
-    batch, tokens, heads, _ = q.shape
-    words, stride = -(-tokens // 32), 0
+def page_attend_workspace(struct: _lib.PageCache, heads: int, tokens: int) -> int:
+    """Bytes of scratch of ``page_attend``."""
+    return _lib.library().nkv_page_attend_workspace_bytes(struct, heads, tokens)
+
+
+def page_attend(struct: _lib.PageCache, q: torch.Tensor, rows: _lib.Tokens, workspace_bytes: int, *, counts=None,
+                tree: torch.Tensor | None = None, causal: bool = True, scale: float, status: torch.Tensor | None = None):
+    """Attention of pending queries q [batch, tokens, heads, width], ``rows`` of them (nkv_page_attend) -> (O like q, lse f32
+    [batch, tokens, heads]).  ``tree`` i32 [tokens, words] or [batch, tokens, words]: bits of the pending tokens that each query
+    sees."""
+    device = q.device
+    batch, tokens, heads, width = q.shape
+    bits, stride = None, 0
     if tree is not None:
+        words = -(-tokens // 32)
         shared = tree.dim() == 2
-        bits = _device_ints(tree, (tokens, words) if shared else (batch, tokens, words), "tree", q.device)
+        bits = _device_ints(tree, (tokens, words) if shared else (batch, tokens, words), "tree", device)
         stride = 0 if shared else tokens * words
-    lib = _lib.library()
-    out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-    nbytes = lib.nkv_page_attend_workspace_bytes(struct, heads, tokens)
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    word = status_word(q.device) if status is None else status
-    _lib.check(lib.nkv_page_attend(
-        struct, rows, tokens, _device_ints(counts, (batch,), "counts", q.device), None if tree is None else bits, stride, int(causal),
-        float(scale), out.data_ptr(), lse.data_ptr(), word.data_ptr(), workspace.data_ptr() if nbytes else None, nbytes,
-        _raw_stream(q.device)))
+    # (new_empty with a tuple is what allocates in least time)
+    out = q.new_empty((batch, tokens, heads, width))
+    lse = q.new_empty((batch, tokens, heads), dtype=torch.float32)
+    workspace = q.new_empty(workspace_bytes, dtype=torch.uint8)
+    word = status_word(device) if status is None else status
+    _lib.check(_lib.library().nkv_page_attend(
+        struct, rows, tokens, _device_ints(counts, (batch,), "counts", device), bits, stride, causal, scale, out.data_ptr(),
+        lse.data_ptr(), word.data_ptr(), workspace.data_ptr(), workspace_bytes, _raw_stream(device)))
     return out, lse
 
 
@@ -920,10 +938,9 @@ def page_keep(structs, path: torch.Tensor, counts: torch.Tensor | None = None) -
     """Rows of the pending tokens that ``path`` i32 [batch, accepted] lists moved to the front of them, in every cache
     (nkv_page_keep)."""
     batch, accepted = structs[0].batch, path.shape[1]
-    caches = (_lib.PageCache * len(structs))(*structs)
     device = path.device
     _lib.check(_lib.library().nkv_page_keep(
-        caches, len(structs), _device_ints(path, (batch, accepted), "path", device), accepted,
+        _lib.page_caches(len(structs))(*structs), len(structs), _device_ints(path, (batch, accepted), "path", device), accepted,
         _device_ints(counts, (batch,), "counts", device), status_word(device).data_ptr(), _raw_stream(device)))
 
 
@@ -935,8 +952,7 @@ def tree_mask(parents: torch.Tensor):
     if parents.dtype != torch.int32 or parents.dim() not in (1, 2):
         raise ValueError(f"parents must be int32 [tokens] or [batch, tokens]; got {parents.dtype} {list(parents.shape)}")
     tokens = parents.shape[-1]
-    mask = torch.empty(*parents.shape, -(-tokens // 32), dtype=torch.int32, device=device)
-    depth = torch.empty_like(parents)
+    mask, depth = parents.new_empty((*parents.shape, -(-tokens // 32))), parents.new_empty(tuple(parents.shape))
     with _On(device):
         _lib.check(_lib.library().nkv_tree_mask(
             parents.data_ptr(), parents.shape[0] if parents.dim() == 2 else 1, tokens, mask.data_ptr(), depth.data_ptr(),

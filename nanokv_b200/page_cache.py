@@ -150,18 +150,13 @@ class PageCache:
                 raise ValueError(f"{name} must be contiguous, on the table's device")
         self.table, self.k_pages, self.v_pages = table, k_pages, v_pages
         self.kv_heads, self.head_dim, self.dtype, self.device = k_pages.shape[1], k_pages.shape[3], k_pages.dtype, table.device
+        self._scale, self._scratch = 1.0 / math.sqrt(self.head_dim), {}     # scratch bytes by query heads and tokens
         self._struct = _lib.PageCache(k_pages.data_ptr(), v_pages.data_ptr(), table.table.data_ptr(), table.lengths.data_ptr(),
                                       table.batch, table.table.shape[1], table.pages, table.page, self.kv_heads, self.head_dim,
                                       ops.dtype_code(self.dtype))
 
-    def _rows_of(self, x: torch.Tensor, name: str) -> int:
-        if x.dim() != 4 or x.shape[0] != self.table.batch or x.shape[3] != self.head_dim:
-            raise ValueError(f"{name} must be [{self.table.batch}, tokens, heads, {self.head_dim}]; got {list(x.shape)}")
-        if x.dtype != self.dtype:
-            raise ValueError(f"{name} must be {self.dtype}, as the cache is; got {x.dtype}")
-        if x.device != self.device:
-            raise (ValueError if x.is_cuda else RuntimeError)(f"{name} is on {x.device}, the cache on {self.device}")
-        return x.shape[1]
+    def _rows(self, x: torch.Tensor, name: str) -> _lib.Tokens:
+        return ops.page_rows(x, self._struct.batch, self.head_dim, self.dtype, self.device, name)
 
     def append(self, k: torch.Tensor, v: torch.Tensor, q: torch.Tensor | None = None, *, counts: torch.Tensor | None = None,
                rotary: Rotary | None = None, positions: torch.Tensor | None = None) -> torch.Tensor | None:
@@ -169,14 +164,15 @@ class PageCache:
         of sequence b the first ``counts[b]`` (int32 on the device; default: all).  ``rotary`` rotates the keys, and queries q [batch, tokens,
         heads, head_dim] with them, by ``positions`` i32 [batch, tokens]; default: the settled tokens' number and on, as for a chain.  Returns
         the rotated queries.  A token for which the table has no page is left out and reported (``ops.check_status``)."""
-        tokens = self._rows_of(k, "k")
-        if self._rows_of(v, "v") != tokens or k.shape[2] != self.kv_heads or v.shape[2] != self.kv_heads:
+        rows, values, queries = self._rows(k, "k"), self._rows(v, "v"), None if q is None else self._rows(q, "q")
+        tokens = k.shape[1]
+        if v.shape[1] != tokens or rows.heads != self.kv_heads or values.heads != self.kv_heads:
             raise ValueError(f"k and v must share [{self.table.batch}, tokens, {self.kv_heads}, {self.head_dim}]; got "
                              f"{list(k.shape)} and {list(v.shape)}")
         if q is not None:
             if rotary is None:
                 raise ValueError("queries are only rotated here: there is no rotation")
-            if self._rows_of(q, "q") != tokens:
+            if q.shape[1] != tokens:
                 raise ValueError(f"there are {tokens} tokens of k and {q.shape[1]} of q")
         rotation = None
         if rotary is not None:
@@ -188,7 +184,9 @@ class PageCache:
             if positions is None:
                 rotation.positions = None
         with ops._On(self.device):
-            return ops.page_append(self._struct, k, v, q, counts=counts, rotation=rotation)
+            out = None if q is None else q.new_empty(tuple(q.shape))
+            ops.page_append(self._struct, rows, values, queries, out, tokens, counts=counts, rotation=rotation, device=self.device)
+        return out
 
     def attend(self, q: torch.Tensor, *, counts: torch.Tensor | None = None, tree: torch.Tensor | None = None, causal: bool = True,
                scale: float | None = None, status: torch.Tensor | None = None):
@@ -198,12 +196,15 @@ class PageCache:
         ``tree`` i32 [tokens, words] or [batch, tokens, words], as ``ops.tree_mask`` makes it: the pending tokens that each query
         sees, as bits.  Without it each sees those up to its own (``causal``) or all of them.  A query that sees nothing, or
         lies past ``counts[b]``, gets O = 0 and lse = -inf."""
-        self._rows_of(q, "q")
+        rows = self._rows(q, "q")
         if status is not None and (status.dtype != torch.int32 or status.device != self.device or status.numel() < 1):
             raise ValueError(f"status must be int32 on {self.device}")
         with ops._On(self.device):
-            return ops.page_attend(self._struct, q, counts=counts, tree=tree, causal=causal,
-                                   scale=1.0 / math.sqrt(self.head_dim) if scale is None else scale, status=status)
+            nbytes = self._scratch.get((rows.heads, q.shape[1]))
+            if nbytes is None:
+                nbytes = self._scratch[rows.heads, q.shape[1]] = ops.page_attend_workspace(self._struct, rows.heads, q.shape[1])
+            return ops.page_attend(self._struct, q, rows, nbytes, counts=counts, tree=tree, causal=bool(causal),
+                                   scale=self._scale if scale is None else float(scale), status=status)
 
     def keep(self, path: torch.Tensor, counts: torch.Tensor | None = None) -> None:
         """``keep`` of this cache alone."""
