@@ -881,8 +881,6 @@ int nkv_page_append(const nkv_page_cache* cache, const nkv_tokens* k, const nkv_
     if (rc != NKV_OK) return rc;
     NKV_REQUIRE(rotation->rotary_dim % 16 == 0, NKV_ERR_INVALID, "page_append: rotary_dim %d must be a multiple of 16", rotation->rotary_dim);
   }
-  const int64_t units = static_cast<int64_t>(cache->batch) * tokens * (2ll * cache->kv_heads + (q ? q->heads : 0)) * (cache->head_dim / 16);
-  NKV_REQUIRE(units <= (1ll << 38), NKV_ERR_TOO_LARGE, "page_append: %d sequences of %d tokens", cache->batch, tokens);
   return page_append(*cache, *k, *v, q, q_out, tokens, counts, rotation, status_word, static_cast<cudaStream_t>(stream));
 }
 

@@ -15,28 +15,42 @@ struct Side {
   int heads, vector;   // vector: rows start on 16 bytes
 };
 
-// A thread takes two 16-byte pieces of a head row whose elements are each other's partners (or two that are only copied).
-template <int DT>
+// A thread takes two 16-byte pieces of a head row whose elements are each other's partners (or two that are only copied), of HEADS
+// heads, which share the table's entries and the page; one where the call is short of threads.  Bound: memory.  Rows of the call are
+// counted from row0 on; a launch has fewer than 2^31 threads.
+template <int DT, int HEADS>
 __global__ void __launch_bounds__(256)
-page_append_kernel(PageArrays c, Side k, Side v, Side q, uint16_t* q_out, const int32_t* counts, int batch, int tokens, int d,
-                   Rotation rot, int32_t* status) {
-  const int units = d / 16, groups = k.heads + v.heads + q.heads;
-  const long long index = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
-  if (index >= static_cast<long long>(batch) * tokens * groups * units) return;
-  const int u = static_cast<int>(index % units);
-  const long long rest = index / units;
-  int head = static_cast<int>(rest % groups);
-  const long long row = rest / groups;
-  const int b = static_cast<int>(row / tokens), t = static_cast<int>(row % tokens);
-  const int kind = head < k.heads ? 0 : head < k.heads + q.heads ? 1 : 2;   // a key's, a query's, a value's
-  head -= kind == 0 ? 0 : kind == 1 ? k.heads : k.heads + q.heads;
+page_append_kernel(PageArrays c, Side k, Side v, Side q, uint16_t* q_out, const int32_t* counts, long long row0, unsigned rows, unsigned tokens,
+                   int d, Rotation rot, int32_t* status) {
+  const unsigned units = d / 16, groups_kv = (k.heads + HEADS - 1) / HEADS, groups_q = (q.heads + HEADS - 1) / HEADS, groups = 2 * groups_kv + groups_q;
+  const unsigned index = blockIdx.x * 256 + threadIdx.x;
+  if (index >= rows * groups * units) return;
+  const unsigned u = index & (units - 1), rest = index / units, group = rest % groups;   // (units: 4 or 8)
+  const long long row = row0 + rest / groups;
+  const int b = static_cast<int>(row / tokens), t = static_cast<int>(row - static_cast<long long>(b) * tokens);
+  const int kind = group < groups_kv ? 0 : group < groups_kv + groups_q ? 1 : 2;   // keys, queries, values
+  const int head0 = (group - (kind == 0 ? 0 : kind == 1 ? groups_kv : groups_kv + groups_q)) * HEADS;
   const Side& side = kind == 0 ? k : kind == 1 ? q : v;
+  const bool turns = kind != 2 && static_cast<int>(u) < rot.dim / 16;
+  const int first = turns && rot.layout == NKV_ROTARY_HALF ? u * 8 : 16 * u;
+  const int other = turns && rot.layout == NKV_ROTARY_HALF ? first + rot.dim / 2 : first + 8;
+  // all that comes from memory first
+  const uint16_t* const from = side.x + b * side.stride_batch + t * side.stride_token + head0 * side.stride_head;
+  uint4 lo[HEADS], hi[HEADS];
+#pragma unroll
+  for (int h = 0; h < HEADS; ++h) {
+    if (HEADS > 1 && head0 + h >= side.heads) break;
+    lo[h] = load_piece<DT>(from + h * side.stride_head, first, side.vector);
+    hi[h] = load_piece<DT>(from + h * side.stride_head, other, side.vector);
+  }
   bool bad;
   const Extent e = extent_of(c, counts, tokens, b, bad);
   if (bad && t == 0 && u == 0) report(status, STATUS_PAGE);
   uint16_t* to;
+  size_t apart;
   if (kind == 1) {
-    to = q_out + (row * q.heads + head) * d;
+    to = q_out + (row * q.heads + head0) * d;
+    apart = d;
   } else {
     if (t >= e.there) return;
     const int page = page_of(c, b, e.length + t);
@@ -44,41 +58,41 @@ page_append_kernel(PageArrays c, Side k, Side v, Side q, uint16_t* q_out, const 
       report(status, STATUS_PAGE);
       return;
     }
-    to = (kind == 0 ? c.k : c.v) + row_at(c, page, head, e.length + t, d);
+    to = (kind == 0 ? c.k : c.v) + row_at(c, page, head0, e.length + t, d);
+    apart = static_cast<size_t>(d) << c.shift;
   }
-  const bool turns = kind != 2 && u < rot.dim / 16;
-  const int first = turns && rot.layout == NKV_ROTARY_HALF ? u * 8 : 16 * u;
-  const int other = turns && rot.layout == NKV_ROTARY_HALF ? first + rot.dim / 2 : first + 8;
-  const uint16_t* const from = side.x + b * side.stride_batch + t * side.stride_token + head * side.stride_head;
-  uint4 lo = load_piece<DT>(from, first, side.vector), hi = load_piece<DT>(from, other, side.vector);
-  if (turns) {
-    float2 cs[8];
-    turns_of(rot, rot.positions ? __ldg(rot.positions + row) : e.length + t, u * 8, cs);
-    float x[8], y[8];
-    Piece<DT>::unpack(lo, x);
-    Piece<DT>::unpack(hi, y);
-    if (rot.layout == NKV_ROTARY_HALF) {
+  float2 cs[8];
+  if (turns) turns_of(rot, rot.positions ? __ldg(rot.positions + row) : e.length + t, u * 8, cs);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x0 = x[i], x1 = y[i];
-        x[i] = turn_first(x0, x1, cs[i]);
-        y[i] = turn_second(x0, x1, cs[i]);
-      }
-    } else {
+  for (int h = 0; h < HEADS; ++h) {
+    if (HEADS > 1 && head0 + h >= side.heads) break;
+    if (turns) {
+      float x[8], y[8];
+      Piece<DT>::unpack(lo[h], x);
+      Piece<DT>::unpack(hi[h], y);
+      if (rot.layout == NKV_ROTARY_HALF) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x0 = x[2 * i], x1 = x[2 * i + 1], y0 = y[2 * i], y1 = y[2 * i + 1];
-        x[2 * i] = turn_first(x0, x1, cs[i]);
-        x[2 * i + 1] = turn_second(x0, x1, cs[i]);
-        y[2 * i] = turn_first(y0, y1, cs[4 + i]);
-        y[2 * i + 1] = turn_second(y0, y1, cs[4 + i]);
+        for (int i = 0; i < 8; ++i) {
+          const float x0 = x[i], x1 = y[i];
+          x[i] = turn_first(x0, x1, cs[i]);
+          y[i] = turn_second(x0, x1, cs[i]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x0 = x[2 * i], x1 = x[2 * i + 1], y0 = y[2 * i], y1 = y[2 * i + 1];
+          x[2 * i] = turn_first(x0, x1, cs[i]);
+          x[2 * i + 1] = turn_second(x0, x1, cs[i]);
+          y[2 * i] = turn_first(y0, y1, cs[4 + i]);
+          y[2 * i + 1] = turn_second(y0, y1, cs[4 + i]);
+        }
       }
+      lo[h] = Piece<DT>::pack(x);
+      hi[h] = Piece<DT>::pack(y);
     }
-    lo = Piece<DT>::pack(x);
-    hi = Piece<DT>::pack(y);
+    *reinterpret_cast<uint4*>(to + h * apart + first) = lo[h];
+    *reinterpret_cast<uint4*>(to + h * apart + other) = hi[h];
   }
-  *reinterpret_cast<uint4*>(to + first) = lo;
-  *reinterpret_cast<uint4*>(to + other) = hi;
 }
 
 // ---- keep ------------------------------------------------------------------------------------------------------
@@ -194,12 +208,21 @@ int page_append(const nkv_page_cache& c, const nkv_tokens& k, const nkv_tokens& 
   if (rotation)
     rot = Rotation{reinterpret_cast<const float2*>(rotation->table), rotation->positions, rotation->rows, rotation->rotary_dim,
                    rotation->layout};
-  const long long total = static_cast<long long>(c.batch) * tokens * (ks.heads + vs.heads + qs.heads) * (c.head_dim / 16);
-  auto kernel = c.dtype == NKV_BF16 ? page_append_kernel<NKV_BF16> : page_append_kernel<NKV_F16>;
-  kernel<<<static_cast<unsigned>((total + 255) / 256), 256, 0, stream>>>(page_arrays(c, 0), ks, vs, qs, static_cast<uint16_t*>(q_out), counts,
-                                                                         c.batch, tokens, c.head_dim, rot, status);
-  NKV_LAUNCH_CHECK("page_append_kernel");
-  return NKV_OK;
+  const long long rows = static_cast<long long>(c.batch) * tokens;
+  const int units = c.head_dim / 16;
+  auto run = [&](auto kernel, int heads) {
+    const long long per_row = static_cast<long long>(units) * (2 * ceil_div(ks.heads, heads) + ceil_div(qs.heads, heads)), most = ((1ll << 31) - 1) / per_row;
+    for (long long row0 = 0; row0 < rows; row0 += most) {
+      const long long n = min(most, rows - row0);
+      kernel<<<static_cast<unsigned>((n * per_row + 255) / 256), 256, 0, stream>>>(page_arrays(c, 0), ks, vs, qs, static_cast<uint16_t*>(q_out), counts,
+                                                                                  row0, static_cast<unsigned>(n), tokens, c.head_dim, rot, status);
+      NKV_LAUNCH_CHECK("page_append_kernel");
+    }
+    return NKV_OK;
+  };
+  const bool many = rows * units * (2 * ks.heads + qs.heads) >= 4ll * 256 * sm_count();
+  if (c.dtype == NKV_BF16) return many ? run(page_append_kernel<NKV_BF16, 4>, 4) : run(page_append_kernel<NKV_BF16, 1>, 1);
+  return many ? run(page_append_kernel<NKV_F16, 4>, 4) : run(page_append_kernel<NKV_F16, 1>, 1);
 }
 
 int page_keep(const nkv_page_cache* caches, int count, const int32_t* path, int accepted, const int32_t* counts, int32_t* status,
