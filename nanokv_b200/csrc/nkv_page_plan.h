@@ -71,8 +71,10 @@ NKV_PAGE_INLINE int tiles_seen(const Shape& s, const Extent& e, int r0, int n) {
   return (seen + TOK - 1) / TOK;
 }
 
-// A unit costs a run as much as PIECE_TILES tiles on top of its own: its queries' way in and its rows' way out.
-constexpr uint32_t PIECE_TILES = 3;
+// A unit costs a run as much as PIECE_TILES tiles on top of its own: its queries' way in and its rows' way out (2 x 4,095 causal
+// queries x 32 heads, costs of 2 / 3 / 5 / 7 / 9: 356 / 347 / 313 / 317 / 323 us; one token each of 31 sequences of up to 2,138 x 320 heads 144 /
+// 138 / 127 / 129 / 133; 99,840 tokens x 40 heads 306 / 307 / 312 / 310 / 308).
+constexpr uint32_t PIECE_TILES = 5;
 NKV_PAGE_INLINE uint32_t cost_of(int tiles) { return tiles > 0 ? tiles + PIECE_TILES : 0; }
 
 // The list of tiles: sequence by sequence, kv head by kv head, unit by unit, with PIECE_TILES places ahead of a unit's.  `runs`

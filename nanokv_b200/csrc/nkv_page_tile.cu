@@ -6,9 +6,8 @@
 //
 //   wide    more than 128: units of 256 rows, two query tiles that share every K and V tile, four warps each.
 //   narrow  up to 128, one query tile; the two groups of four warps take the even and the odd tiles of its tokens, each with sums of
-//           its own.  With at most 128 / COPIES rows, COPIES of them stand in the query tile one below the other, and
-//           every copy takes a share of a tile's tokens (or of its weights' bits): the weights of the others are stored as zeros.  That
-//           cuts what one thread does per tile, which is what a tile takes.  The sums of all are joined in shared memory.
+//           its own.  Up to 32 rows stand in the query tile four times, one below the other, and every copy takes a share of a tile's
+//           tokens or of its weights' bits: the weights of the others are stored as zeros.  The copies' sums are joined in shared memory.
 //
 // Softmax: P' = 2^(s - m) with a reference m that follows the running maximum of the scaled scores, s; it moves when P' would pass
 // 2^8 times what it was set to.  bf16: set so that the sum of a row's P' stays below 1, O = sum P' V then below the largest |V|, any
@@ -27,8 +26,8 @@
 //
 // Table, lengths and counts are read by the kernel: every thread block makes the plan (nkv_page_plan.h) for itself.  The tiles of all
 // units form one list that the SMs take in equal runs; a unit that a run's end cuts leaves fp32 parts, joined by a second launch.
-// Warps: 0-7 softmax, 8-9 queries and masked values, 10 MMA issue, 11 pages: 384 threads, so that 168 registers each hold a row's
-// 128 scores at once.
+// Warps: 0-7 softmax, 8-9 queries and masked values, 10 MMA issue, 11 pages: 384 threads, whose registers are dealt out
+// so that a softmax thread holds a row's 128 scores at once.
 #include "nkv_internal.h"
 #include "nkv_page.cuh"
 #include "nkv_tile.cuh"
@@ -458,7 +457,7 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
   volatile int* const stray = reinterpret_cast<volatile int*>(smem + M_STRAY);
   float* const join = reinterpret_cast<float*>(smem + L::JOIN_OFF);
   Walk walk(plan, a.shape, blockIdx.x);
-  Piece p;
+  Piece p = {};
   bool ok = true, more = true;
   int ci = 0, pieces = 0;   // steps and pieces of this chain
   int odd = 0;
@@ -492,8 +491,12 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       uint32_t raw[GROUPS][32];
 #pragma unroll
       for (int k = 0; k < GROUPS; ++k) tmem_ld32_issue(s_addr + slice * WIDTH + 32 * k, raw[k]);
+      if constexpr (GROUPS == 4) {
+        tmem_ld128_wait(raw[0], raw[1], raw[2], raw[3]);
+      } else {
 #pragma unroll
-      for (int k = 0; k < GROUPS; ++k) tmem_ld32_wait(raw[k]);
+        for (int k = 0; k < GROUPS; ++k) tmem_ld32_wait(raw[k]);
+      }
       float f = scale;
       if (first + WIDTH > clear_least) {   // some row of the warp does not see all of it
         // scaled before they are masked: -inf times a scale of 0 would be NaN
@@ -890,10 +893,16 @@ page_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   plan.sequences = a.sequences;
   plan.deal(gridDim.x);
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (warp < SOFTMAX_WARPS) softmax_role<DT, D, COPIES>(smem, bars, tmem, c, a, plan, parts, ctx);
-  else if (warp < SOFTMAX_WARPS + OPERAND_WARPS) operand_role<DT, D, COPIES>(smem, bars, c, a, plan, ctx);
-  else if (warp > MMA_WARP) page_role<D, COPIES>(smem, bars, &map_k, &map_v, c, a, plan, ctx, status);
-  else mma_role<DT, D, COPIES>(smem, bars, tmem, a, plan, ctx);
+  // registers: 12 warps of 168 at launch, 8 of 200 and 4 of 104 from here on
+  if (warp < SOFTMAX_WARPS) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    softmax_role<DT, D, COPIES>(smem, bars, tmem, c, a, plan, parts, ctx);
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp < SOFTMAX_WARPS + OPERAND_WARPS) operand_role<DT, D, COPIES>(smem, bars, c, a, plan, ctx);
+    else if (warp > MMA_WARP) page_role<D, COPIES>(smem, bars, &map_k, &map_v, c, a, plan, ctx, status);
+    else mma_role<DT, D, COPIES>(smem, bars, tmem, a, plan, ctx);
+  }
   tc_fence_before();
   __syncthreads();
   if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
@@ -1010,9 +1019,11 @@ int page_tile(const PageArrays& c, const PageCall& call, int n, int dtype, int d
                                      : run(page_tile_kernel<NKV_F16, 128, COPIES>, Layout<128, COPIES>::DYNAMIC))                         \
                 : (dtype == NKV_BF16 ? run(page_tile_kernel<NKV_BF16, 64, COPIES>, Layout<64, COPIES>::DYNAMIC)                           \
                                      : run(page_tile_kernel<NKV_F16, 64, COPIES>, Layout<64, COPIES>::DYNAMIC))
+  // The forms by rows (32 sequences of up to 16,411 tokens, 8 kv heads of 128, bf16): narrow against wide at 65 / 80 / 125 rows 198 / 200 /
+  // 209 against 228 / 229 / 235 us.  Four copies are for what they add to the weights' bits, and cost 1 % (5 rows 188 us, 187 without; over
+  // up to 700 tokens 32.2 and 30.1); two copies of up to 64 rows gained nothing (60 rows 199 us, 196 without).
   if (a.rows > QT) NKV_PAGE_RUN(0);
-  else if (a.rows > QT / 2) NKV_PAGE_RUN(1);
-  else if (a.rows > QT / 4) NKV_PAGE_RUN(2);
+  else if (a.rows > QT / 4) NKV_PAGE_RUN(1);
   else NKV_PAGE_RUN(4);
 #undef NKV_PAGE_RUN
   if (rc != NKV_OK) return rc;
