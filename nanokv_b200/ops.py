@@ -934,13 +934,14 @@ def page_attend(struct: _lib.PageCache, q: torch.Tensor, rows: _lib.Tokens, work
     return out, lse
 
 
-def page_keep(structs, path: torch.Tensor, counts: torch.Tensor | None = None) -> None:
+def page_keep(images, batch: int, path: torch.Tensor, counts: torch.Tensor | None = None) -> None:
     """Rows of the pending tokens that ``path`` i32 [batch, accepted] lists moved to the front of them, in every cache
-    (nkv_page_keep)."""
-    batch, accepted = structs[0].batch, path.shape[1]
+    (nkv_page_keep); ``images``: the caches' structs as bytes."""
+    accepted = path.shape[1]
     device = path.device
     _lib.check(_lib.library().nkv_page_keep(
-        _lib.page_caches(len(structs))(*structs), len(structs), _device_ints(path, (batch, accepted), "path", device), accepted,
+        _lib.page_caches(len(images)).from_buffer_copy(b"".join(images)), len(images),
+        _device_ints(path, (batch, accepted), "path", device), accepted,
         _device_ints(counts, (batch,), "counts", device), status_word(device).data_ptr(), _raw_stream(device)))
 
 

@@ -91,15 +91,16 @@ class PageTable:
             return
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("pages cannot be dealt out inside a graph capture: reserve them before")
-        entries, values = [], []
-        for b, n in enumerate(more):
-            for _ in range(n):
-                entries.append(b * self.table.shape[1] + len(self._held[b]))
-                values.append(free.pop())
-                self._held[b].append(values[-1])
+        entries = [b * self.table.shape[1] + len(self._held[b]) + i for b, n in enumerate(more) for i in range(n)]
+        taken = free[len(free) - len(entries):][::-1]
         with ops._On(self.device):
-            pairs = ops.upload(torch.tensor([entries, values], dtype=torch.int64), self.device)
+            pairs = ops.upload(torch.tensor([entries, taken], dtype=torch.int64), self.device)
             self.table.view(-1).index_copy_(0, pairs[0], pairs[1].to(torch.int32))
+        del free[len(free) - len(entries):]
+        at = 0
+        for held, n in zip(self._held, more):
+            held.extend(taken[at:at + n])
+            at += n
 
     def release(self, sequence: int) -> None:
         """A sequence emptied: its pages go back to the pool."""
@@ -114,9 +115,12 @@ class PageTable:
         self._held[sequence] = []
 
     def advance(self, counts: torch.Tensor | int) -> None:
-        """The first ``counts[b]`` pending tokens of every sequence (int32 tensor on the device, or one number for all) are settled."""
+        """The first ``counts[b]`` pending tokens of every sequence (int32 tensor on the device, or one number for all) are settled.
+        Once for all layers, behind their ``attend`` and ``keep``."""
         if isinstance(counts, torch.Tensor):
             ops._device_ints(counts, (self.batch,), "counts", self.device)
+        elif operator.index(counts) < 0:
+            raise ValueError(f"counts must not be negative; got {counts}")
         self.lengths.add_(counts)
 
 
@@ -154,6 +158,7 @@ class PageCache:
         self._struct = _lib.PageCache(k_pages.data_ptr(), v_pages.data_ptr(), table.table.data_ptr(), table.lengths.data_ptr(),
                                       table.batch, table.table.shape[1], table.pages, table.page, self.kv_heads, self.head_dim,
                                       ops.dtype_code(self.dtype))
+        self._image = bytes(self._struct)
 
     def _rows(self, x: torch.Tensor, name: str) -> _lib.Tokens:
         return ops.page_rows(x, self._struct.batch, self.head_dim, self.dtype, self.device, name)
@@ -219,9 +224,10 @@ def keep(caches, path: torch.Tensor, counts: torch.Tensor | None = None) -> None
     if not caches:
         return
     table = caches[0].table
-    if any(c.table is not table for c in caches):
-        raise ValueError("the caches of a call share one PageTable")
+    for cache in caches:
+        if cache.table is not table:
+            raise ValueError("the caches of a call share one PageTable")
     if path.dim() != 2 or path.device != table.device:
         raise ValueError(f"path must be int32 [{table.batch}, accepted] on {table.device}; got {list(path.shape)} on {path.device}")
     with ops._On(table.device):
-        ops.page_keep([c._struct for c in caches], path, counts)
+        ops.page_keep([c._image for c in caches], table.batch, path, counts)

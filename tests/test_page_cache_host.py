@@ -287,3 +287,16 @@ def test_pieces_cover_every_tile_once(plan, kind, unit):
         want = {(b, h, u, t) for b in range(n) for h in range(heads) for u in range(units)
                 for t in range(plan.tiles(kind, group, tokens, unit, lengths[b], counts[b], u))}
         assert set(seen) == want
+
+
+def test_counts_that_advance(on_host):
+    table = HostTable(2, 64, 8, 16)
+    table.advance(3)
+    table.advance(torch.tensor([1, 0], dtype=torch.int32))
+    assert table.lengths.tolist() == [4, 3]
+    for counts in (-1, torch.tensor([1, 0]), torch.tensor([1], dtype=torch.int32)):
+        with pytest.raises(ValueError, match="counts"):
+            table.advance(counts)
+    with pytest.raises(TypeError):
+        table.advance(1.5)
+    assert table.lengths.tolist() == [4, 3]
