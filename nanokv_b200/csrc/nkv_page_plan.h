@@ -77,8 +77,9 @@ NKV_PAGE_INLINE int tiles_seen(const Shape& s, const Extent& e, int r0, int n) {
 constexpr uint32_t PIECE_TILES = 5;
 NKV_PAGE_INLINE uint32_t cost_of(int tiles) { return tiles > 0 ? tiles + PIECE_TILES : 0; }
 
-// The list of tiles: sequence by sequence, kv head by kv head, unit by unit, with PIECE_TILES places ahead of a unit's.  `runs`
-// thread blocks take equal runs of it.
+// The list of tiles: sequence by sequence, kv head by kv head, unit by unit, with PIECE_TILES places ahead of a unit's.  It is cut into
+// equal runs, of which thread block i takes the i-th, and in further rounds the (blocks + i)-th and so on: blocks that work at the same
+// time then work on neighbouring parts of the list, whose keys and values the units of a kv head share in the L2 cache.
 struct Plan {
   const uint32_t* start;             // [sequences + 1]
   const Extent* extents;
@@ -99,7 +100,16 @@ struct Piece {                        // a unit, or a run's part of one
   int b, h, unit, tile0, nt, whole;   // tiles tile0 .. tile0 + nt - 1; whole: all the unit has
 };
 
-// The pieces of one run in order; every role of a thread block walks the same list.
+// Rounds of a call whose units read `bytes` of keys and values: as few as keep what one round reads within FITS, as long as a run
+// has `least` places.
+constexpr uint64_t FITS = 64ull << 20;
+NKV_PAGE_INLINE int rounds_of(uint64_t bytes, uint32_t places, int blocks, int least, int most_rounds) {
+  int rounds = 1;
+  while (rounds < most_rounds && bytes > FITS * rounds && places / blocks / (rounds + 1) >= static_cast<uint32_t>(least)) ++rounds;
+  return rounds;
+}
+
+// The pieces of one run in order.
 struct Walk {
   uint32_t g, end;
   int b, h, unit, tiles;              // the unit that g lies in, its tiles
@@ -154,6 +164,24 @@ struct Walk {
     out.whole = out.nt == tiles;
     return true;
   }
+};
+
+// The pieces of a thread block, run by run; every role of it makes the same tour.
+struct Tour {
+  int run, step, runs;                // the run at hand, from one of the block's to the next, all of them
+  Walk walk;
+  NKV_PAGE_INLINE Tour(const Plan& p, const Shape& s, int block, int blocks, int rounds)
+      : run(block), step(blocks), runs(blocks * rounds), walk(p, s, block) {}
+  NKV_PAGE_INLINE bool next(const Plan& p, const Shape& s, Piece& out) {
+    while (!walk.next(p, s, out)) {
+      if (run + step >= runs) return false;
+      run += step;
+      walk = Walk(p, s, run);
+    }
+    return true;
+  }
+  // the run that has the last tile of the unit at hand
+  NKV_PAGE_INLINE int last_run(const Plan& p) const { return static_cast<int>(p.run_of(walk.g + cost_of(walk.tiles) - walk.at - 1)); }
 };
 
 }  // namespace page

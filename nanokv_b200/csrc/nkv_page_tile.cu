@@ -40,7 +40,7 @@ using page::Piece;
 using page::Plan;
 using page::Shape;
 using page::TOK;
-using page::Walk;
+using page::Tour;
 
 constexpr int QT = 128;                           // rows of a query tile
 constexpr int SUB = 128 * 128;                    // bytes of a [128 rows x 64 elements] swizzled tile
@@ -48,13 +48,14 @@ constexpr int SOFTMAX_WARPS = 8, OPERAND_WARPS = 2, MMA_WARP = 10, THREADS = 384
 constexpr float RESCALE_THRESHOLD = 8.0f;
 // log2(1 + 0.7213 * 2^-8) and its inverse: the mean of 1 / m over mantissas m is 0.7213, and half a bf16 step is 2^-8 of m = 1
 constexpr float CUT_LOG2 = 0.00405952f, CUT_INV = 0.99719022f;
+constexpr int MOST_ROUNDS = 3, LEAST_RUN = 64;    // rounds that there is scratch for; places of a run that a cut more is worth
 constexpr float NOTHING = -3e38f;                 // the reference before the first score: below all, and a number
 
 // (P_READY: chain i, half h of a tile's tokens at 2 i + h)
 enum Bar { Q_FULL = 0, Q_FREE = 1, S_FULL = 2, P_READY = 4, O_DONE = 8, O_FREE = 10, DRAINED = 12, FULL = 13, FREE = 23, LOOK = 33, CLEAN = 43, NUM_BARS = 53 };
-constexpr int M_SLOT = NUM_BARS * 8, M_ABORT = M_SLOT + 4, M_STRAY = M_SLOT + 8, M_EXTENTS = 448;
+constexpr int M_SLOT = NUM_BARS * 8, M_ABORT = M_SLOT + 4, M_STRAY = M_SLOT + 8, M_ROUNDS = M_SLOT + 12, M_EXTENTS = 448;
 constexpr int M_START = M_EXTENTS + page::MOST_SEQUENCES * static_cast<int>(sizeof(page::Extent)), META = 2048;
-static_assert(M_STRAY + 4 <= M_EXTENTS && M_START + 4 * (page::MOST_SEQUENCES + 1) <= META && page::MOST_SEQUENCES < 128, "meta block");
+static_assert(M_ROUNDS + 4 <= M_EXTENTS && M_START + 4 * (page::MOST_SEQUENCES + 1) <= META && page::MOST_SEQUENCES < 128, "meta block");
 
 // COPIES 0: the wide form
 template <int D, int COPIES> struct Layout {
@@ -113,8 +114,10 @@ struct Parts {
 
 struct TileCall : PageCall {
   Shape shape;
-  int sequences;
+  int sequences, most_rounds;
 };
+
+__device__ __forceinline__ int plan_rounds(const uint8_t* smem) { return *reinterpret_cast<const volatile int*>(smem + M_ROUNDS); }
 
 // ---- warp 11: pages ------------------------------------------------------------------------------------------------
 template <int D, int COPIES>
@@ -123,12 +126,12 @@ __device__ __forceinline__ void page_role(uint8_t* smem, uint64_t* bars, const C
   using L = Layout<D, COPIES>;
   const int lane = threadIdx.x & 31, rows = 1 << c.shift, per_tile = TOK >> c.shift;
   const int groups = rows / 8, nowhere = c.pages * c.kv_heads * groups;   // groups of a page; behind the last one of the pool: read as zeros
-  Walk walk(plan, a.shape, blockIdx.x);
+  Tour tour(plan, a.shape, blockIdx.x, gridDim.x, plan_rounds(smem));
   Piece p;
   bool ok = true, bad = false;
   Ring at;
   int round = 0;        // times round the ring
-  while (ok && walk.next(plan, a.shape, p)) {
+  while (ok && tour.next(plan, a.shape, p)) {
     const Extent e = plan.extents[p.b];
     const int total = e.length + e.there;
     const int32_t* const entries = c.table + static_cast<size_t>(p.b) * c.row_pages;
@@ -199,12 +202,12 @@ __device__ __forceinline__ void operand_role(uint8_t* smem, uint64_t* bars, cons
   const bool negative = a.scale_log2 < 0.f;   // a negative scale is the queries' sign
   const int token_step = ROWS / a.group, head_step = ROWS - token_step * a.group;
   volatile int* const stray = reinterpret_cast<volatile int*>(smem + M_STRAY);
-  Walk walk(plan, a.shape, blockIdx.x);
+  Tour tour(plan, a.shape, blockIdx.x, gridDim.x, plan_rounds(smem));
   Piece p;
   bool ok = true;
   int pieces = 0;
   uint32_t items = 0, looked = 0;   // tiles in the ring of the pieces before; phases of LOOK, a bit per stage
-  while (ok && walk.next(plan, a.shape, p)) {
+  while (ok && tour.next(plan, a.shape, p)) {
     const Extent e = plan.extents[p.b];
     const uint16_t* const q_head = a.q + p.b * a.q_batch + static_cast<long long>(p.h) * a.group * a.q_head + q_col;
     if (pieces > 0) ok = wait(&bars[Q_FREE], (pieces - 1) & 1, ctx, 931);
@@ -326,13 +329,13 @@ __device__ __forceinline__ void mma_role(uint8_t* smem, uint64_t* bars, uint32_t
     for (int k = 0; k < 4; ++k)
       if (leader) mma_bf16_ts(d, w + 8 * k, vd + k * (2 * L::GROUP / 16), idesc<DT>(D) | (1u << 16), accumulate || k > 0);
   };
-  Walk walk(plan, a.shape, blockIdx.x);
+  Tour tour(plan, a.shape, blockIdx.x, gridDim.x, plan_rounds(smem));
   Piece p;
   bool ok = true;
   Ring at;                                         // tiles are used in the order in which they lie in the ring
   uint32_t cleaned = 0;                            // phases of CLEAN, a bit per stage
   int pieces = 0, done[2] = {0, 0}, used[2] = {0, 0};   // steps and pieces of each chain so far
-  while (ok && walk.next(plan, a.shape, p)) {
+  while (ok && tour.next(plan, a.shape, p)) {
     const Extent e = plan.extents[p.b];
     const int n[2] = {steps_of<L>(a.shape, e, p, 0), steps_of<L>(a.shape, e, p, 1)};
     const int longest = max(n[0], n[1]), masked = first_masked(a.shape, e, p);   // V tiles from here on are looked at
@@ -456,23 +459,24 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
   const float scale = fabsf(a.scale_log2);
   volatile int* const stray = reinterpret_cast<volatile int*>(smem + M_STRAY);
   float* const join = reinterpret_cast<float*>(smem + L::JOIN_OFF);
-  Walk walk(plan, a.shape, blockIdx.x);
+  Tour tour(plan, a.shape, blockIdx.x, gridDim.x, plan_rounds(smem));
   Piece p = {};
   bool ok = true, more = true;
   int ci = 0, pieces = 0;   // steps and pieces of this chain
   int odd = 0;
-  Cut cut{0, 0, 0, 0};
-  auto note_cut = [&]() {
-    if (!p.whole && p.tile0 == 0) cut = Cut{p.b, p.h, p.unit, static_cast<int>(plan.run_of(walk.g + page::cost_of(walk.tiles) - walk.at - 1))};
+  if (tid == 0)
+    for (int run = blockIdx.x; run < static_cast<int>(gridDim.x) * a.most_rounds; run += gridDim.x) parts.cut[run] = Cut{0, 0, 0, 0};
+  auto note_cut = [&]() {   // (the last piece of a run, where there is one)
+    if (tid == 0 && !p.whole && p.tile0 == 0) parts.cut[tour.run] = Cut{p.b, p.h, p.unit, tour.last_run(plan)};
   };
   const bool wide_out = (reinterpret_cast<uintptr_t>(a.out) & 31) == 0, wide_part = (reinterpret_cast<uintptr_t>(parts.o) & 31) == 0;
-  auto place_of = [&](const Piece& pc) { return (2 * static_cast<size_t>(blockIdx.x) + (pc.tile0 == 0 ? 1 : 0)) * L::UNIT; };
+  auto place_of = [&](const Piece& pc) { return (2 * static_cast<size_t>(tour.run) + (pc.tile0 == 0 ? 1 : 0)) * L::UNIT; };
   // the row of the results that row r of a piece's kv head is
   auto at_of = [&](const Piece& pc, int r) {
     const int token = r / a.group;
     return (static_cast<size_t>(pc.b) * a.tokens + token) * a.heads + pc.h * a.group + r - token * a.group;
   };
-  while (ok && (more = walk.next(plan, a.shape, p))) {
+  while (ok && (more = tour.next(plan, a.shape, p))) {
     const Extent e = plan.extents[p.b];
     const int r = L::NARROW ? row % APART : p.unit * L::UNIT + wg * QT + row, token = r / a.group;
     const bool real = r < a.rows;
@@ -793,10 +797,9 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
         else parts.ml[place_of(p) + tid] = make_float2(0.f, CUDART_NAN_F);
       }
       note_cut();
-      more = walk.next(plan, a.shape, p);
+      more = tour.next(plan, a.shape, p);
     }
   }
-  if (tid == 0) parts.cut[blockIdx.x] = cut;
 }
 
 template <int DT, int D, int COPIES>
@@ -857,6 +860,7 @@ page_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   }
   if (warp == 0) {
     uint32_t carry = 0;
+    uint64_t tokens = 0;
     for (int b0 = 0; b0 <= a.sequences; b0 += 32) {
       const int b = b0 + lane;
       uint32_t cost = 0;
@@ -871,6 +875,7 @@ page_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           cost = start[b];
         }
         cost *= a.shape.kv_heads;
+        if (cost) tokens += extents[b].length + extents[b].there;
       }
       uint32_t upto = cost;
 #pragma unroll
@@ -881,6 +886,10 @@ page_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       if (b <= a.sequences) start[b] = carry + upto - cost;
       carry += __shfl_sync(0xffffffffu, upto, 31);
     }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) tokens += __shfl_xor_sync(0xffffffffu, tokens, x);
+    if (lane == 0)
+      *reinterpret_cast<volatile int*>(smem + M_ROUNDS) = page::rounds_of(tokens * (4ull * D * a.shape.kv_heads), carry, gridDim.x, LEAST_RUN, a.most_rounds);
   }
   tc_fence_before();
   __syncthreads();
@@ -891,7 +900,7 @@ page_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   plan.start = start;
   plan.extents = extents;
   plan.sequences = a.sequences;
-  plan.deal(gridDim.x);
+  plan.deal(gridDim.x * plan_rounds(smem));
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // registers: 12 warps of 168 at launch, 8 of 200 and 4 of 104 from here on
   if (warp < SOFTMAX_WARPS) {
@@ -977,10 +986,16 @@ join_parts_kernel(TileCall a, Parts parts) {
 }
 
 int unit_of(int rows) { return rows > QT ? 2 * QT : QT; }
+// Units of a kv head that share its keys and values, in a pool larger than what a round is to read.
+int most_rounds_of(const PageArrays& c, int rows, int d) {
+  const uint64_t pool = (static_cast<uint64_t>(c.pages) * c.kv_heads << c.shift) * 4 * d;
+  return rows > unit_of(rows) && pool > page::FITS ? MOST_ROUNDS : 1;
+}
+
 }  // namespace
 
-size_t page_tile_bytes(int rows, int d) {
-  return static_cast<size_t>(sm_count()) * 2 * unit_of(rows) * (d * sizeof(float) + sizeof(float2)) + sm_count() * sizeof(Cut);
+size_t page_tile_bytes(const PageArrays& c, int rows, int d) {
+  return static_cast<size_t>(sm_count()) * most_rounds_of(c, rows, d) * (2 * unit_of(rows) * (d * sizeof(float) + sizeof(float2)) + sizeof(Cut));
 }
 
 int page_tile(const PageArrays& c, const PageCall& call, int n, int dtype, int d, void* workspace, int32_t* status, cudaStream_t stream) {
@@ -996,8 +1011,10 @@ int page_tile(const PageArrays& c, const PageCall& call, int n, int dtype, int d
   const int runs = static_cast<int>(min(most, static_cast<uint64_t>(sm_count())));
   Parts parts;
   parts.o = static_cast<float*>(workspace);
-  parts.ml = reinterpret_cast<float2*>(parts.o + static_cast<size_t>(sm_count()) * 2 * unit * d);
-  parts.cut = reinterpret_cast<Cut*>(parts.ml + static_cast<size_t>(sm_count()) * 2 * unit);
+  a.most_rounds = most_rounds_of(c, a.rows, d);
+  const size_t places = static_cast<size_t>(sm_count()) * a.most_rounds * 2 * unit;
+  parts.ml = reinterpret_cast<float2*>(parts.o + places * d);
+  parts.cut = reinterpret_cast<Cut*>(parts.ml + places);
   CUtensorMap maps[2];
   for (int i = 0; i < 2; ++i) {
     // elements of a chunk, rows of a group, chunks of a row, groups
@@ -1031,7 +1048,7 @@ int page_tile(const PageArrays& c, const PageCall& call, int n, int dtype, int d
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(runs, ceil_div(min(unit, a.rows), SLICE));
+  config.gridDim = dim3(runs * a.most_rounds, ceil_div(min(unit, a.rows), SLICE));
   config.blockDim = dim3(256);
   config.stream = stream;
   config.attrs = &attribute;

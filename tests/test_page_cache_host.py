@@ -206,6 +206,32 @@ extern "C" int pieces(int kind, int group, int tokens, int unit, int heads, int 
   }
   return found;
 }
+// the same pieces by the tours of `blocks` thread blocks, `rounds` runs each
+extern "C" int toured(int kind, int group, int tokens, int unit, int heads, int n, const int* lengths, const int* counts, int blocks, int rounds, int* out) {
+  const int rows = group * tokens;
+  const Shape s{kind, group, rows, unit, (rows + unit - 1) / unit, heads};
+  std::vector<Extent> e; std::vector<uint32_t> start(1, 0);
+  for (int b = 0; b < n; ++b) {
+    bool bad; e.push_back(extent_in(lengths[b], counts[b], tokens, 1 << 30, bad));
+    uint32_t cost = 0;
+    for (int u = 0; u < s.units; ++u) cost += cost_of(tiles_seen(s, e[b], u * unit, unit));
+    start.push_back(start.back() + cost * heads);
+  }
+  Plan p{start.data(), e.data(), n, 0, 0};
+  p.deal(blocks * rounds);
+  int found = 0;
+  for (int block = 0; block < blocks; ++block) {
+    Tour t(p, s, block, blocks, rounds);
+    Piece piece;
+    while (t.next(p, s, piece)) {
+      int* const at = out + 8 * found++;
+      at[0] = t.run; at[1] = piece.b; at[2] = piece.h; at[3] = piece.unit; at[4] = piece.tile0; at[5] = piece.nt; at[6] = piece.whole;
+      at[7] = t.last_run(p);
+    }
+  }
+  return found;
+}
+extern "C" int rounds(uint64_t bytes, uint32_t places, int blocks, int least, int most) { return rounds_of(bytes, places, blocks, least, most); }
 extern "C" int tiles(int kind, int group, int tokens, int unit, int length, int count, int u) {
   bool bad; const Extent e = extent_in(length, count, tokens, 1 << 30, bad);
   const int rows = group * tokens;
@@ -300,3 +326,35 @@ def test_counts_that_advance(on_host):
     with pytest.raises(TypeError):
         table.advance(1.5)
     assert table.lengths.tolist() == [4, 3]
+
+
+@pytest.mark.parametrize("rounds", [1, 2, 3])
+def test_tours_have_the_pieces_of_all_runs(plan, rounds):
+    import random
+    rng = random.Random(rounds)
+    for _ in range(40):
+        n, heads, blocks, group = rng.randint(1, 5), rng.randint(1, 4), rng.choice([1, 3, 20]), rng.choice([1, 3])
+        tokens = rng.randint(200, 900)
+        lengths = [rng.choice([0, 1, 128, 1000, 5000]) for _ in range(n)]
+        counts = [rng.choice([0, 1, tokens, tokens]) for _ in range(n)]
+        array = ctypes.c_int * n
+        runs, tours = (ctypes.c_int * 70000)(), (ctypes.c_int * 70000)()
+        a = plan.pieces(1, group, tokens, 256, heads, n, array(*lengths), array(*counts), blocks * rounds, runs)
+        b = plan.toured(1, group, tokens, 256, heads, n, array(*lengths), array(*counts), blocks, rounds, tours)
+        pieces = [tuple(runs[7 * i:7 * i + 7]) for i in range(a)]
+        toured = [tuple(tours[8 * i:8 * i + 7]) for i in range(b)]
+        assert sorted(pieces) == sorted(toured)
+        by_unit = {}
+        for run, sequence, h, u, *_ in pieces:
+            by_unit.setdefault((sequence, h, u), []).append(run)
+        for i in range(b):
+            run, sequence, h, u, tile0, nt, whole, last = tours[8 * i:8 * i + 8]
+            assert last == max(by_unit[sequence, h, u]) and by_unit[sequence, h, u] == list(range(min(by_unit[sequence, h, u]), last + 1))
+
+
+def test_rounds_are_as_few_as_fit(plan):
+    plan.rounds.argtypes = [ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int, ctypes.c_int, ctypes.c_int]
+    fits = 64 << 20
+    assert plan.rounds(fits, 10 ** 6, 148, 64, 3) == 1 and plan.rounds(fits + 1, 10 ** 6, 148, 64, 3) == 2
+    assert plan.rounds(100 * fits, 10 ** 6, 148, 64, 3) == 3 and plan.rounds(100 * fits, 10 ** 6, 148, 64, 1) == 1
+    assert plan.rounds(100 * fits, 148 * 127, 148, 64, 3) == 1 and plan.rounds(100 * fits, 148 * 128, 148, 64, 3) == 2
