@@ -24,6 +24,15 @@
 // A page of K or V comes as one copy, whatever its size: the tensor map has the eight rows of a swizzle group, the 64-element chunks of a
 // row and the groups of a page as dimensions, so that a tile is its groups one behind the other, each with its chunks side by side.
 //
+// Measured (kernel and join): one query token over 99,840 tokens x 40 heads 307 us (2.04 GB, 6.6 TB/s: memory); 32 trees of 16 nodes x 40 heads over
+// up to 16,411 tokens x 8 heads 191 us (5.7 TB/s); 4,680 queries x 24 heads over 24,960 tokens 1.20 ms (1,200 TFLOP/s, at the clock that the power
+// limit leaves), 2 x 4,095 causal queries x 32 heads 313 us.  What bounds the wide form: the MMA warp, whose six batches a tile pair (S and two
+// halves of PV for both query tiles, 2,048 tensor cycles) take about 3,400 cycles with the waits between them, and power: reading K and V from L2
+// instead of memory gave 10 % (rounds, below).  Small calls: two launches, the plan, and a chain of table, tile, two products, rows.
+// Tried and dropped (4,680 queries, us, kept form first): exponentials ahead of the row's maximum (1,333 / 1,390; with straight code and a fallback
+// 1,345 / 1,368); K awaited with the weights (1,333 / 1,362); two barriers per wait (1,339 / 1,393); waits without parking (no change); P
+// beside S in tensor memory for 64-wide heads (no change); two more copies' bits by a second product (batch of trees 238 / 324).
+//
 // Table, lengths and counts are read by the kernel: every thread block makes the plan (nkv_page_plan.h) for itself.  The tiles of all
 // units form one list that the SMs take in equal runs; a unit that a run's end cuts leaves fp32 parts, joined by a second launch.
 // Warps: 0-7 softmax, 8-9 queries and masked values, 10 MMA issue, 11 pages: 384 threads, whose registers are dealt out
@@ -48,7 +57,10 @@ constexpr int SOFTMAX_WARPS = 8, OPERAND_WARPS = 2, MMA_WARP = 10, THREADS = 384
 constexpr float RESCALE_THRESHOLD = 8.0f;
 // log2(1 + 0.7213 * 2^-8) and its inverse: the mean of 1 / m over mantissas m is 0.7213, and half a bf16 step is 2^-8 of m = 1
 constexpr float CUT_LOG2 = 0.00405952f, CUT_INV = 0.99719022f;
-constexpr int MOST_ROUNDS = 3, LEAST_RUN = 64;    // rounds that there is scratch for; places of a run that a cut more is worth
+// Rounds that there is scratch for, and places of a run that a cut more is worth.  4,680 queries x 24 heads over 24,960 tokens in 1 / 2 / 3 / 4 rounds:
+// 1,335 / 1,335 / 1,191 / 1,238 us, 5.06 GB read from memory in one and 0.58 in three (a run is one unit then, and a head's units go in step);
+// 1,560 x 40 heads over 98,560 x 8 in 2 / 3 / 4: 2,712 / 2,760 / 2,600.
+constexpr int MOST_ROUNDS = 3, LEAST_RUN = 64;
 constexpr float NOTHING = -3e38f;                 // the reference before the first score: below all, and a number
 
 // (P_READY: chain i, half h of a tile's tokens at 2 i + h)
