@@ -897,12 +897,12 @@ def page_rows(x: torch.Tensor, batch: int, width: int, dtype: torch.dtype, devic
 
 
 def page_append(struct: _lib.PageCache, k: _lib.Tokens, v: _lib.Tokens, q: _lib.Tokens | None, q_out: torch.Tensor | None,
-                tokens: int, *, counts=None, rotation: _lib.Rotation | None = None, device: torch.device) -> None:
+                tokens: int, *, counts=None, rotation: _lib.Rotation | None = None, device: torch.device, word: int) -> None:
     """Pending tokens k, v put behind the settled ones, queries q rotated to ``q_out`` (nkv_page_append); rows as ``page_rows``
-    gives them."""
+    gives them, ``word`` the address of a status word."""
     _lib.check(_lib.library().nkv_page_append(
-        struct, k, v, q, None if q_out is None else q_out.data_ptr(), tokens, _device_ints(counts, (struct.batch,), "counts", device),
-        rotation, status_word(device).data_ptr(), _raw_stream(device)))
+        struct, k, v, q, None if q_out is None else q_out.data_ptr(), tokens,
+        None if counts is None else _device_ints(counts, (struct.batch,), "counts", device), rotation, word, _raw_stream(device)))
 
 
 def page_attend_workspace(struct: _lib.PageCache, heads: int, tokens: int) -> int:
@@ -911,10 +911,10 @@ def page_attend_workspace(struct: _lib.PageCache, heads: int, tokens: int) -> in
 
 
 def page_attend(struct: _lib.PageCache, q: torch.Tensor, rows: _lib.Tokens, workspace_bytes: int, *, counts=None,
-                tree: torch.Tensor | None = None, causal: bool = True, scale: float, status: torch.Tensor | None = None):
+                tree: torch.Tensor | None = None, causal: bool = True, scale: float, word: int):
     """Attention of pending queries q [batch, tokens, heads, width], ``rows`` of them (nkv_page_attend) -> (O like q, lse f32
     [batch, tokens, heads]).  ``tree`` i32 [tokens, words] or [batch, tokens, words]: bits of the pending tokens that each query
-    sees."""
+    sees.  ``word``: the address of a status word."""
     device = q.device
     batch, tokens, heads, width = q.shape
     bits, stride = None, 0
@@ -927,10 +927,9 @@ def page_attend(struct: _lib.PageCache, q: torch.Tensor, rows: _lib.Tokens, work
     out = q.new_empty((batch, tokens, heads, width))
     lse = q.new_empty((batch, tokens, heads), dtype=torch.float32)
     workspace = q.new_empty(workspace_bytes, dtype=torch.uint8)
-    word = status_word(device) if status is None else status
     _lib.check(_lib.library().nkv_page_attend(
-        struct, rows, tokens, _device_ints(counts, (batch,), "counts", device), bits, stride, causal, scale, out.data_ptr(),
-        lse.data_ptr(), word.data_ptr(), workspace.data_ptr(), workspace_bytes, _raw_stream(device)))
+        struct, rows, tokens, None if counts is None else _device_ints(counts, (batch,), "counts", device), bits, stride, causal, scale,
+        out.data_ptr(), lse.data_ptr(), word, workspace.data_ptr(), workspace_bytes, _raw_stream(device)))
     return out, lse
 
 
@@ -954,8 +953,7 @@ def tree_mask(parents: torch.Tensor):
         raise ValueError(f"parents must be int32 [tokens] or [batch, tokens]; got {parents.dtype} {list(parents.shape)}")
     tokens = parents.shape[-1]
     mask, depth = parents.new_empty((*parents.shape, -(-tokens // 32))), parents.new_empty(tuple(parents.shape))
+    batch, word, stream = parents.shape[0] if parents.dim() == 2 else 1, status_word(device).data_ptr(), _raw_stream(device)
     with _On(device):
-        _lib.check(_lib.library().nkv_tree_mask(
-            parents.data_ptr(), parents.shape[0] if parents.dim() == 2 else 1, tokens, mask.data_ptr(), depth.data_ptr(),
-            status_word(device).data_ptr(), _raw_stream(device)))
+        _lib.check(_lib.library().nkv_tree_mask(parents.data_ptr(), batch, tokens, mask.data_ptr(), depth.data_ptr(), word, stream))
     return mask, depth

@@ -60,6 +60,7 @@ class PageTable:
             raise ValueError(f"a pool has at least one page; got {pages}")
         self.table, self.lengths, self.pages, self.page = table, lengths, int(pages), int(page)
         self.batch, self.device = table.shape[0], table.device
+        self.status = ops.status_word(self.device)      # what calls report into (ops.check_status)
 
     @property
     def capacity(self) -> int:
@@ -190,7 +191,8 @@ class PageCache:
                 rotation.positions = None
         with ops._On(self.device):
             out = None if q is None else q.new_empty(tuple(q.shape))
-            ops.page_append(self._struct, rows, values, queries, out, tokens, counts=counts, rotation=rotation, device=self.device)
+            ops.page_append(self._struct, rows, values, queries, out, tokens, counts=counts, rotation=rotation, device=self.device,
+                            word=self.table.status.data_ptr())
         return out
 
     def attend(self, q: torch.Tensor, *, counts: torch.Tensor | None = None, tree: torch.Tensor | None = None, causal: bool = True,
@@ -209,7 +211,8 @@ class PageCache:
             if nbytes is None:
                 nbytes = self._scratch[rows.heads, q.shape[1]] = ops.page_attend_workspace(self._struct, rows.heads, q.shape[1])
             return ops.page_attend(self._struct, q, rows, nbytes, counts=counts, tree=tree, causal=bool(causal),
-                                   scale=self._scale if scale is None else float(scale), status=status)
+                                   scale=self._scale if scale is None else float(scale),
+                                   word=(self.table.status if status is None else status).data_ptr())
 
     def keep(self, path: torch.Tensor, counts: torch.Tensor | None = None) -> None:
         """``keep`` of this cache alone."""
