@@ -744,8 +744,9 @@ int nkv_page_append(const nkv_page_cache* cache, const nkv_tokens* k, const nkv_
  * in dtype, lse f32 [batch, tokens, heads] natural log; a query that sees nothing, or only scores of -inf, or lies past counts[b] has out 0
  * and lse -inf.  What a query does not see has no part in its result, also where it is not finite; a value that it sees and that is not
  * finite leaves a result that is not finite (inf or NaN).  Weights enter the product with V in dtype, fp16 ones rounded to nearest, bf16 ones
- * cut off with their mean loss made good, of up to 32 rows a kv head (tokens * heads / kv_heads) as two numbers that leave 2^-15 of them; sums, maxima and
- * results are fp32 until they are rounded once.  workspace: nkv_page_attend_workspace_bytes(...) bytes
+ * cut off, of up to 32 rows a kv head (tokens * heads / kv_heads) as two numbers that leave 2^-15 of them; of more bf16 rows the result is divided by the
+ * sum of the weights as they were cut off, so that they add up to one.  The same query is therefore rounded otherwise in a call of more than 32 rows
+ * than in one of fewer.  Sums, maxima and results are fp32 until they are rounded once.  workspace: nkv_page_attend_workspace_bytes(...) bytes
  * of device scratch (16-byte aligned), no two calls in flight on the same.
  */
 size_t nkv_page_attend_workspace_bytes(const nkv_page_cache* cache, int heads, int tokens);

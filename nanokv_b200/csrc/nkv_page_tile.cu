@@ -13,9 +13,13 @@
 // 2^8 times what it was set to.  bf16: set so that the sum of a row's P' stays below 1, O = sum P' V then below the largest |V|, any
 // number of bf16.  fp16: P' up to 2^15, so that weights down to 2^-29 of the largest keep all their bits.  The row sum, the maximum and O
 // stay in fp32.  P' enters the product with V in 16 bits: fp16 rounded to nearest; bf16 as the upper half of its fp32 bits, a byte
-// permutation instead of a conversion on the unit that the exponentials need.  What is cut off is made good on average: every P' is raised
-// by the mean of it, (1 + 0.72 * 2^-8), in its exponent, and the row sum lowered again.  With four copies, two of them take the upper half of
-// P' and two the rest (2^-15 of it is left): few rows have few results, and no average to hide an unlucky weight in.
+// permutation instead of a conversion.  What is cut off is up to 2^-7 of a weight and, where many weights are alike, the same for all of
+// them: so rows of O are divided by the sum of the weights as they entered the product, two additions more a pair of scores, and lse
+// takes the sum of the weights in full.  (4,680 queries x 24 heads over 24,960 tokens 1,413 us, 32 trees of 16 nodes x 40 heads 232, cases in
+// turn; divided by the full sum, cut off / rounded to nearest: 1,370 / 1,389 and 226 / 227, and results up to 2^-8 off as a whole, row by row.
+// The second sum behind the weights' handing over: 1,411 and 238; from halves unpacked by shifts and masks 1,455 and 239.)  With four
+// copies, two of them take the upper half of P' and two the rest (2^-15 of it is left): few rows have few results, and no average to hide an
+// unlucky weight in.  A token's row is therefore rounded otherwise alone than as one of more than 32 rows.
 //
 // Pending tokens that some row does not see, and whatever lies in a page behind a sequence's last token, are masked in the scores.  A weight
 // of 0 times a value that is not finite would be NaN, so two warps look at the V tiles with such tokens: values behind the
@@ -55,8 +59,6 @@ constexpr int QT = 128;                           // rows of a query tile
 constexpr int SUB = 128 * 128;                    // bytes of a [128 rows x 64 elements] swizzled tile
 constexpr int SOFTMAX_WARPS = 8, OPERAND_WARPS = 2, MMA_WARP = 10, THREADS = 384;
 constexpr float RESCALE_THRESHOLD = 8.0f;
-// log2(1 + 0.7213 * 2^-8) and its inverse: the mean of 1 / m over mantissas m is 0.7213, and half a bf16 step is 2^-8 of m = 1
-constexpr float CUT_LOG2 = 0.00405952f, CUT_INV = 0.99719022f;
 // Rounds that there is scratch for, and places of a run that a cut more is worth.  4,680 queries x 24 heads over 24,960 tokens in 1 / 2 / 3 / 4 rounds:
 // 1,335 / 1,335 / 1,191 / 1,238 us, 5.06 GB read from memory in one and 0.58 in three (a run is one unit then, and a head's units go in step);
 // 1,560 x 40 heads over 98,560 x 8 in 2 / 3 / 4: 2,712 / 2,760 / 2,600.
@@ -79,7 +81,8 @@ template <int D, int COPIES> struct Layout {
   static constexpr int Q_OFF = META;
   static constexpr int RING_OFF = Q_OFF + QTILES * DCH * SUB;
   static constexpr int ML_OFF = RING_OFF + STAGES * STAGE;             // narrow: references and sums of 256 threads, of two pieces
-  static constexpr int JOIN_OFF = ML_OFF + (NARROW ? 2 * 256 * 8 : 0);     // narrow: columns of O of all copies of the rows
+  static constexpr int JOIN_OFF = ML_OFF + (NARROW ? 2 * 256 * 8 : 0);     // narrow: columns of O of all copies of the rows; of one copy what
+                                                                            // cut weights are short of, as the references
   static constexpr int JOIN_WORDS = D == 128 ? 6912 : 11264;
   static constexpr int BYTES = JOIN_OFF + (NARROW ? JOIN_WORDS * 4 : 0);
   static constexpr int DYNAMIC = BYTES + 1024;     // room to start on 1,024 bytes
@@ -195,6 +198,16 @@ __device__ __forceinline__ void page_role(uint8_t* smem, uint64_t* bars, const C
 template <int DT> __device__ __forceinline__ bool not_finite(uint32_t bits16) {
   constexpr uint32_t E = DT == NKV_BF16 ? 0x7F80u : 0x7C00u;
   return (bits16 & E) == E;
+}
+
+// lo + the lower half of two bf16 numbers, hi + the upper one, in fp32
+__device__ __forceinline__ void add_bf16x2(float& lo, float& hi, uint32_t two) {
+  asm("{\n\t.reg .b16 x, y;\n\t"
+      "mov.b32 {x, y}, %2;\n\t"
+      "add.rn.f32.bf16 %0, x, %0;\n\t"
+      "add.rn.f32.bf16 %1, y, %1;\n\t}"
+      : "+f"(lo), "+f"(hi)
+      : "r"(two));
 }
 
 // 16 bytes from memory to shared memory, or zeros
@@ -462,7 +475,7 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
                                              const Parts& parts, const Ctx& ctx) {
   using L = Layout<D, COPIES>;
   constexpr int WIDTH = TOK / SLICES<DT, COPIES>, GROUPS = WIDTH / 32, SOURCES = 2 * (COPIES > 0 ? COPIES : 1), APART = 2 * QT / SOURCES;
-  constexpr bool TWO = PARTS<DT, COPIES> == 2, CUT = DT == NKV_BF16 && !TWO;
+  constexpr bool TWO = PARTS<DT, COPIES> == 2, CUT = DT == NKV_BF16 && !TWO;   // CUT: O is divided by the sum of the weights as they are stored
   const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
   const int wg = warp / 4, row = tid & 127;
   const int slice = COPIES > 1 ? row / APART % SLICES<DT, COPIES> : 0;   // (the same in all of a warp, as is whether it takes the rest)
@@ -497,7 +510,7 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
     const int steps = steps_of<L>(a.shape, e, p, wg);
     // where P' stands when the reference is set: see the top of the file
     const float raise = DT == NKV_F16 ? 7.0f : -(RESCALE_THRESHOLD + 32 - __clz(e.length + e.there));
-    float m = NOTHING, l = 0.f;
+    float m = NOTHING, l = 0.f, stored = 0.f;   // (stored: CUT)
 #pragma unroll 1
     for (int n = 0; n < steps; ++n, ++ci) {
       const int first = (p.tile0 + tile_of<L>(wg, n)) * TOK + slice * WIDTH;
@@ -545,14 +558,15 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
           tmem_wait_st();
         }
         l *= alpha;
+        stored *= alpha;
         m = m_new;
       }
       // P' replaces S, eight scores at a time in a software pipeline: exponentials of one block beside the arguments of the next and the
       // sums and stores of the one before.  The first half of the weights is handed over as soon as it is stored.
-      const float off = CUT ? CUT_LOG2 - m : -m;
-      const uint64_t scale2 = pair_f32(f, f), off2 = pair_f32(off, off);
+      const uint64_t scale2 = pair_f32(f, f), off2 = pair_f32(-m, -m);
       uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull}, arg[2][4];
       float w[2][8];
+      float held[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       uint32_t packed[16];
       auto args = [&](int b) {
 #pragma unroll
@@ -582,6 +596,7 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
               yb = __float_as_uint(y - __uint_as_float(yb & 0xFFFF0000u));
             }
             packed[(b & 3) * 4 + i] = __byte_perm(xb, yb, 0x7632);
+            if (CUT) add_bf16x2(held[2 * i], held[2 * i + 1], packed[(b & 3) * 4 + i]);
           }
         }
         if ((b & 3) == 3) {
@@ -612,8 +627,9 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       float x, y;
       split_f32(add_f32x2(add_f32x2(sum2[0], sum2[1]), add_f32x2(sum2[2], sum2[3])), x, y);
       l += x + y;
+      if (CUT) stored += ((held[0] + held[1]) + (held[2] + held[3])) + ((held[4] + held[5]) + (held[6] + held[7]));
     }
-    if (CUT) l *= CUT_INV;
+    const float raised = CUT && l != 0.f ? l / stored : 1.f;   // what O is short of by its weights' cut-off bits
     if (rest) l = 0.f;   // (the other part's)
     if (ok && steps > 0) {
       ok = wait(&bars[O_DONE + wg], pieces & 1, ctx, 941);
@@ -626,6 +642,8 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
       float2* const mls = reinterpret_cast<float2*>(smem + L::ML_OFF) + odd * 256;
       odd ^= 1;
       mls[tid] = make_float2(m, l);
+      float* const raises = join + (mls - reinterpret_cast<float2*>(smem + L::ML_OFF));
+      if (CUT) raises[tid] = raised;
       tc_fence_before();
       if (softmax_any(!ok)) {   // (all of the warps take part in what follows, or none)
         ok = false;
@@ -640,7 +658,8 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
 #pragma unroll
       for (int k = 0; k < SOURCES; ++k) sum = fmaf(mls[k * APART + row % APART].y, exp2f(mls[k * APART + row % APART].x - top), sum);
       const bool any = sum != 0.f, look = *stray != 0;      // (NaN: any)
-      const float inv = p.whole ? 1.f / sum : 1.f, f0 = exp2f(mls[row].x - top) * inv, f1 = exp2f(mls[128 + row].x - top) * inv;
+      const float inv = p.whole ? 1.f / sum : 1.f, f0 = exp2f(mls[row].x - top) * inv * (CUT ? raises[row] : 1.f),
+                  f1 = exp2f(mls[128 + row].x - top) * inv * (CUT ? raises[128 + row] : 1.f);
       const uint32_t o0 = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + 256 + wg * (D / 2);
       // 16 columns of the row: both chains' together
       auto joined = [&](int at, float (&x)[16]) {
@@ -748,7 +767,7 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
     } else {
       if (!ok) break;
       tc_fence_after();
-      const float inv = 1.f / l;
+      const float inv = raised / l;
       const bool any = l != 0.f, look = *stray != 0;
       float* const part = parts.o + (place_of(p) + wg * QT + row) * D;
       const size_t at = at_of(p, r);
@@ -785,7 +804,9 @@ __device__ __forceinline__ void softmax_role(uint8_t* smem, uint64_t* bars, uint
         } else {
 #pragma unroll
           for (int j = 0; j < 32; j += 8) {
-            const uint32_t o[8] = {v[j], v[j + 1], v[j + 2], v[j + 3], v[j + 4], v[j + 5], v[j + 6], v[j + 7]};
+            uint32_t o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = __float_as_uint(__uint_as_float(v[j + i]) * raised);
             store32(part + cc + j, o, wide_part);
           }
         }
