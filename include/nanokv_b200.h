@@ -756,6 +756,7 @@ int nkv_page_attend(const nkv_page_cache* cache, const nkv_tokens* q, int tokens
 
 /* The accepted path of a draft: rows of pending tokens path[b][j] (DEVICE i32 [batch][accepted], ascending), j < counts[b] (DEVICE; NULL:
  * `accepted`), moved to pending places j, in all `count` caches (HOST array; they share batch, table, lengths and shape; layers).
+ * A node that does not ascend, or lies ahead of its place j, is left out and leaves status 920.
  * Lengths stay as they are: the caller adds counts to them, once for all layers. */
 int nkv_page_keep(const nkv_page_cache* caches, int count, const int32_t* path, int accepted, const int32_t* counts,
                   int32_t* status_word, void* stream);

@@ -103,8 +103,8 @@ struct Kept {
 };
 
 // A thread moves one 16-byte column of a kv head: the rows of the path lie at or behind the places they move to, in order, so
-// that none is written before it is read.  Bound: the chain length, node, page, row (one sequence 2.0 us); 32 sequences x 40 layers x 9 rows
-// of 8 heads 8.4 us.
+// that none is written before it is read; a node ahead of its place, as those behind a refused one may be, is refused as well.  Bound:
+// the chain length, node, page, row (one sequence 2.0 us); 32 sequences x 40 layers x 9 rows of 8 heads 8.4 us.
 constexpr int AT_ONCE = 8;   // rows in flight
 __global__ void __launch_bounds__(256)
 page_keep_kernel(const __grid_constant__ Kept kept, PageArrays c, const int32_t* path, int accepted, const int32_t* counts, int d,
@@ -127,7 +127,7 @@ page_keep_kernel(const __grid_constant__ Kept kept, PageArrays c, const int32_t*
       moves[i] = false;
       if (j0 + i >= e.there) continue;
       const int node = __ldg(nodes + j0 + i);
-      const bool in = node > before && node < room - e.length;
+      const bool in = node > before && node >= j0 + i && node < room - e.length;
       bad |= !in;
       if (!in) continue;
       before = node;
