@@ -763,7 +763,8 @@ int nkv_page_keep(const nkv_page_cache* caches, int count, const int32_t* path, 
 
 /* What every node of a draft sees: parents i32 [batch][tokens], each before its node, -1 for a node that follows the settled tokens ->
  * mask u32 [batch][tokens][ceil(tokens / 32)], the bits of a node and its ancestors, and depth i32 [batch][tokens], how
- * many ancestors it has.  tokens <= 4096.  A parent that does not come before its node counts as -1 and leaves status 921. */
+ * many ancestors it has.  tokens <= 4096.  A parent that does not come before its node counts as -1 and leaves status 921 (status_word NULL: is not
+ * reported). */
 int nkv_tree_mask(const int32_t* parents, int batch, int tokens, uint32_t* mask, int32_t* depth, int32_t* status_word, void* stream);
 
 #ifdef __cplusplus

@@ -940,7 +940,7 @@ int nkv_page_keep(const nkv_page_cache* caches, int count, const int32_t* path, 
 int nkv_tree_mask(const int32_t* parents, int batch, int tokens, uint32_t* mask, int32_t* depth, int32_t* status_word, void* stream) {
   NKV_REQUIRE(batch >= 0 && batch <= 65535 && tokens >= 0 && tokens <= 4096, NKV_ERR_INVALID, "tree_mask: batch=%d tokens=%d", batch, tokens);
   if (batch == 0 || tokens == 0) return NKV_OK;
-  NKV_REQUIRE(parents && mask && depth && status_word, NKV_ERR_INVALID, "tree_mask: arrays missing");
+  NKV_REQUIRE(parents && mask && depth, NKV_ERR_INVALID, "tree_mask: arrays missing");
   return tree_mask(parents, batch, tokens, mask, depth, status_word, static_cast<cudaStream_t>(stream));
 }
 

@@ -164,7 +164,7 @@ tree_mask_kernel(const int32_t* parents, int tokens, int words, uint32_t* mask, 
     bad |= !in;
     up[i] = in ? p : -1;
   }
-  if (bad) report(status, STATUS_TREE);
+  if (bad && status) report(status, STATUS_TREE);
   __syncthreads();
   const int index = blockIdx.x * 256 + threadIdx.x;
   if (index >= tokens * words) return;

@@ -226,11 +226,7 @@ def decode_rows(view: HistoryView, decoder, mean, *, rows=None, dtype=None) -> t
     out = torch.empty(n, J, dtype=dtype, device=device)
     if rows is not None:
         rows = rows.to(dtype=torch.int32).contiguous()
-    # the word is not made inside a capture: a graph would clear it on every replay (the rows that a decode
-    # could not finish are NaN without it as well)
-    word = _STATUS_WORDS.get(device)
-    if word is None and not torch.cuda.is_current_stream_capturing():
-        word = status_word(device)
+    word = _word(device)      # (the rows that a decode could not finish are NaN without it as well)
     struct = view.struct()
     _lib.check(_lib.library().nkv_decode_rows_status(
         ctypes.byref(struct), _ptr(rows), n, _ptr(decoder), dtype_code(decoder.dtype), _ptr(mean),
@@ -254,6 +250,15 @@ def status_word(device: torch.device) -> torch.Tensor:
     if key not in _STATUS_WORDS:
         _STATUS_WORDS[key] = torch.zeros(1, dtype=torch.int32, device=key)
     return _STATUS_WORDS[key]
+
+
+def _word(device: torch.device) -> torch.Tensor | None:
+    """The same, but none where there is none yet and the call is captured: made inside a capture, it would be the graph's, which
+    would clear it on every replay."""
+    word = _STATUS_WORDS.get(device)
+    if word is None and not torch.cuda.is_current_stream_capturing():
+        word = status_word(device)
+    return word
 
 
 def check_status(device=None) -> None:
@@ -933,27 +938,29 @@ def page_attend(struct: _lib.PageCache, q: torch.Tensor, rows: _lib.Tokens, work
     return out, lse
 
 
-def page_keep(images, batch: int, path: torch.Tensor, counts: torch.Tensor | None = None) -> None:
+def page_keep(images, batch: int, path: torch.Tensor, counts: torch.Tensor | None = None, *, word: int) -> None:
     """Rows of the pending tokens that ``path`` i32 [batch, accepted] lists moved to the front of them, in every cache
-    (nkv_page_keep); ``images``: the caches' structs as bytes."""
+    (nkv_page_keep); ``images``: the caches' structs as bytes, ``word``: the address of a status word."""
     accepted = path.shape[1]
     device = path.device
     _lib.check(_lib.library().nkv_page_keep(
         _lib.page_caches(len(images)).from_buffer_copy(b"".join(images)), len(images),
         _device_ints(path, (batch, accepted), "path", device), accepted,
-        _device_ints(counts, (batch,), "counts", device), status_word(device).data_ptr(), _raw_stream(device)))
+        _device_ints(counts, (batch,), "counts", device), word, _raw_stream(device)))
 
 
 def tree_mask(parents: torch.Tensor):
     """What the nodes of a draft see (nkv_tree_mask): parents i32 [tokens] or [batch, tokens], each before its node, -1 for one
     that follows the settled tokens -> (mask i32 [.., tokens, ceil(tokens / 32)] with the bits of a node and its ancestors, depth
-    i32 [.., tokens])."""
+    i32 [.., tokens]).  A parent that does not come before its node counts as -1 and is reported (``check_status``); a call that is captured
+    before its device has a status word (``status_word`` and every ``PageTable`` make it) has nowhere to report to."""
     device = _require_cuda(parents)
     if parents.dtype != torch.int32 or parents.dim() not in (1, 2):
         raise ValueError(f"parents must be int32 [tokens] or [batch, tokens]; got {parents.dtype} {list(parents.shape)}")
     tokens = parents.shape[-1]
     mask, depth = parents.new_empty((*parents.shape, -(-tokens // 32))), parents.new_empty(tuple(parents.shape))
-    batch, word, stream = parents.shape[0] if parents.dim() == 2 else 1, status_word(device).data_ptr(), _raw_stream(device)
+    batch, word, stream = parents.shape[0] if parents.dim() == 2 else 1, _word(device), _raw_stream(device)
     with _On(device):
-        _lib.check(_lib.library().nkv_tree_mask(parents.data_ptr(), batch, tokens, mask.data_ptr(), depth.data_ptr(), word, stream))
+        _lib.check(_lib.library().nkv_tree_mask(parents.data_ptr(), batch, tokens, mask.data_ptr(), depth.data_ptr(),
+                                                None if word is None else word.data_ptr(), stream))
     return mask, depth

@@ -233,4 +233,4 @@ def keep(caches, path: torch.Tensor, counts: torch.Tensor | None = None) -> None
     if path.dim() != 2 or path.device != table.device:
         raise ValueError(f"path must be int32 [{table.batch}, accepted] on {table.device}; got {list(path.shape)} on {path.device}")
     with ops._On(table.device):
-        ops.page_keep([c._image for c in caches], table.batch, path, counts)
+        ops.page_keep([c._image for c in caches], table.batch, path, counts, word=table.status.data_ptr())

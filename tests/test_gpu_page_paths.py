@@ -1,4 +1,4 @@
-"""Accepted paths with nodes that cannot be followed."""
+"""Accepted paths with nodes that cannot be followed, and what captured calls report."""
 import pytest
 import torch
 
@@ -39,3 +39,51 @@ def test_a_node_that_cannot_be_followed_moves_nothing(path, page):
     for cache in caches:
         for got, pool in ((cache.k_pages, k), (cache.v_pages, v)):
             assert torch.equal(got.cpu(), moved(pool, table, lengths, paths, counts, tokens))
+
+
+def test_a_captured_tree_mask_does_not_clear_what_others_report(monkeypatch):
+    """Captured before anything on the device has reported: the graph must not hold the device's status word, which each replay would clear."""
+    monkeypatch.setattr(ops, "_STATUS_WORDS", {})
+    parents = torch.tensor([-1, 0, 0, 2], dtype=torch.int32, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mask, depth = ops.tree_mask(parents)
+    ops.tree_mask(torch.tensor([3], dtype=torch.int32, device="cuda"))       # reports its parent
+    graph.replay()
+    assert mask.flatten().tolist() == [1, 3, 5, 13] and depth.tolist() == [0, 1, 1, 2]
+    with pytest.raises(RuntimeError, match="parent"):
+        ops.check_status("cuda:0")
+
+
+def test_a_captured_tree_mask_reports_where_there_is_a_word():
+    ops.status_word(torch.device("cuda:0"))
+    parents = torch.tensor([-1, 0], dtype=torch.int32, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        mask, _ = ops.tree_mask(parents)
+    graph.replay()
+    ops.check_status("cuda:0")
+    parents[1] = 1
+    graph.replay()
+    assert mask.flatten().tolist() == [1, 2]
+    with pytest.raises(RuntimeError, match="parent"):
+        ops.check_status("cuda:0")
+
+
+def test_a_captured_keep_reports_into_its_tables_word(monkeypatch):
+    table = PageTable(1, 64, pages=4, page=16)
+    table.reserve([40])
+    cache = PageCache(table, 1, 64)
+    x = ref.randn(1, 8, 1, 64, seed=1, dtype=torch.bfloat16).cuda()
+    cache.append(x, x)
+    path = torch.tensor([[1, 3]], dtype=torch.int32, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    word = table.status
+    monkeypatch.setattr(ops, "_STATUS_WORDS", {})
+    with torch.cuda.graph(graph):
+        cache.keep(path)
+    path[0, 1] = 0
+    graph.replay()
+    torch.cuda.synchronize()
+    assert int(word) == 920 and not ops._STATUS_WORDS
+    word.zero_()
