@@ -717,7 +717,8 @@ int nkv_block_evict(const float* weights, const int32_t* table, const int32_t* f
  * lengths are DEVICE memory, shared by the caches of all layers: a step that was captured into a graph can be replayed while
  * they grow.  The host does not see what they hold, so the kernels check it: a token without a page (an entry outside 0 .. pages-1, or
  * no entry) is not written, reads as keys and values of zero, and leaves status 920 in the status word, as do lengths, counts and paths out of
- * range; no access leaves the arrays.  Two sequences may name one page as long as neither writes to it.
+ * range; no access leaves the arrays.  Two sequences may name one page as long as neither writes to it; one pool as both keys and values can
+ * only be read.
  */
 typedef struct nkv_page_cache {
   void*    k_pages;         /* [pages][kv_heads][page][head_dim] in dtype; 16-byte aligned */

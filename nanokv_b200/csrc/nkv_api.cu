@@ -867,6 +867,7 @@ int nkv_page_append(const nkv_page_cache* cache, const nkv_tokens* k, const nkv_
   NKV_REQUIRE(tokens >= 0 && tokens <= (1 << 28), NKV_ERR_INVALID, "page_append: tokens=%d", tokens);
   if (tokens == 0 || cache->batch == 0) return NKV_OK;
   NKV_REQUIRE(k && v && k->data && v->data && status_word, NKV_ERR_INVALID, "page_append: rows or status word missing");
+  NKV_REQUIRE(cache->k_pages != cache->v_pages, NKV_ERR_INVALID, "page_append: one pool for keys and values");
   NKV_REQUIRE(k->heads == cache->kv_heads && v->heads == cache->kv_heads, NKV_ERR_INVALID, "page_append: %d and %d heads for a cache of %d",
               k->heads, v->heads, cache->kv_heads);
   if (q) {
@@ -929,8 +930,10 @@ int nkv_page_keep(const nkv_page_cache* caches, int count, const int32_t* path, 
     NKV_REQUIRE(a.batch == b.batch && a.row_pages == b.row_pages && a.pages == b.pages && a.page == b.page && a.kv_heads == b.kv_heads &&
                     a.head_dim == b.head_dim && a.table == b.table && a.lengths == b.lengths,
                 NKV_ERR_INVALID, "page_keep: cache %d does not share the table and shape of the first", i);
-    for (int j = 0; j < i; ++j)   // (its rows would be moved twice)
-      NKV_REQUIRE(caches[j].k_pages != b.k_pages && caches[j].v_pages != b.v_pages, NKV_ERR_INVALID, "page_keep: caches %d and %d are one", j, i);
+    for (int j = 0; j <= i; ++j)   // (rows of a pool that is named twice would be moved twice)
+      NKV_REQUIRE((j == i || (caches[j].k_pages != b.k_pages && caches[j].v_pages != b.v_pages && caches[j].v_pages != b.k_pages)) &&
+                      caches[j].k_pages != b.v_pages,
+                  NKV_ERR_INVALID, "page_keep: pools of caches %d and %d are one", j, i);
   }
   if (count == 0 || accepted == 0 || caches[0].batch == 0) return NKV_OK;
   NKV_REQUIRE(path && status_word, NKV_ERR_INVALID, "page_keep: path or status word missing");

@@ -1,0 +1,14 @@
+"""Calls of the paged cache that would write one place twice: refused on the host, no GPU needed."""
+from nanokv_b200 import _lib
+from test_page_cache_host import rows, status_of, struct
+
+
+def test_pools_that_are_written_twice():
+    """One pool as keys and values of a cache that is written, or of two caches of a call."""
+    one = struct(address=1024, v=1024)
+    status, text = status_of("nkv_page_append", one, rows(2), rows(2), None, None, 1, None, None, 256, None)
+    assert status == _lib.NKV_ERR_INVALID and "one pool" in text
+    crossed = (_lib.PageCache * 2)(struct(address=1024, v=2048), struct(address=2048, v=4096))
+    for caches, count in (((_lib.PageCache * 1)(one), 1), (crossed, 2)):
+        status, text = status_of("nkv_page_keep", caches, count, 256, 1, None, 256, None)
+        assert status == _lib.NKV_ERR_INVALID and "are one" in text
