@@ -5,6 +5,7 @@
 #include <cstdlib>
 #include <cstring>
 
+#include "nkv_block.cuh"
 #include "nkv_internal.h"
 #include "nkv_tc.cuh"
 
@@ -911,7 +912,8 @@ int nkv_page_attend(const nkv_page_cache* cache, const nkv_tokens* q, int tokens
   const int64_t words = (static_cast<int64_t>(tokens) + 31) / 32 * tokens;
   NKV_REQUIRE(!mask || mask_stride == 0 || mask_stride >= words, NKV_ERR_INVALID, "page_attend: masks of %lld words lie %lld apart",
               static_cast<long long>(words), static_cast<long long>(mask_stride));
-  NKV_REQUIRE(scale - scale == 0.f, NKV_ERR_INVALID, "page_attend: scale is not finite");
+  const float scale_log2 = scale * LOG2E;   // what the kernels take
+  NKV_REQUIRE(scale_log2 - scale_log2 == 0.f, NKV_ERR_INVALID, "page_attend: scale, or scale * log2(e), is not finite");
   const size_t need = page_attend_workspace_bytes(*cache, q->heads, tokens);
   NKV_REQUIRE(workspace_bytes >= need && (need == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0)), NKV_ERR_INVALID,
               "page_attend: workspace of %zu bytes is too small or not 16-byte aligned (%zu)", workspace_bytes, need);

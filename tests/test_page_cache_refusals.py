@@ -1,4 +1,6 @@
-"""Calls of the paged cache that would write one place twice: refused on the host, no GPU needed."""
+"""Calls of the paged cache that would write one place twice, or take what is no number: refused on the host, no GPU needed."""
+import pytest
+
 from nanokv_b200 import _lib
 from test_page_cache_host import rows, status_of, struct
 
@@ -12,3 +14,10 @@ def test_pools_that_are_written_twice():
     for caches, count in (((_lib.PageCache * 1)(one), 1), (crossed, 2)):
         status, text = status_of("nkv_page_keep", caches, count, 256, 1, None, 256, None)
         assert status == _lib.NKV_ERR_INVALID and "are one" in text
+
+
+@pytest.mark.parametrize("scale", [2.4e38, -3.4e38])
+def test_scales_that_are_no_number_in_base_two(scale):
+    """The kernels take scale * log2(e)."""
+    status, text = status_of("nkv_page_attend", struct(), rows(2), 1, None, None, 0, 1, scale, 256, 256, 256, None, 0, None)
+    assert status == _lib.NKV_ERR_INVALID and "finite" in text
