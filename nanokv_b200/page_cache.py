@@ -106,6 +106,7 @@ class PageTable:
     def release(self, sequence: int) -> None:
         """A sequence emptied: its pages go back to the pool."""
         free = self._own()
+        sequence = int(operator.index(sequence))      # (True would index a tensor otherwise than a list)
         if not 0 <= sequence < self.batch:
             raise ValueError(f"there are sequences 0 .. {self.batch - 1}; got {sequence}")
         if torch.cuda.is_current_stream_capturing():
