@@ -65,7 +65,7 @@ __device__ __forceinline__ uint32_t sight_of(const PageCall& a, const Extent& e,
 }
 
 // sequences [0, n) of `c` from one of the batch's on (nkv_page_tile.cu)
-size_t page_tile_bytes(const PageArrays& c, int rows, int d);
+size_t page_tile_bytes(const PageArrays& c, int n, int rows, int d);
 int page_tile(const PageArrays& c, const PageCall& a, int n, int dtype, int d, void* workspace, int32_t* status, cudaStream_t stream);
 
 }  // namespace nkv

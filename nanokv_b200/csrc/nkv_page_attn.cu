@@ -87,7 +87,8 @@ page_plain_kernel(PageArrays c, PageCall a, int32_t* status) {
 }  // namespace
 
 size_t page_attend_workspace_bytes(const nkv_page_cache& c, int heads, int tokens) {
-  return page_tile_bytes(page_arrays(c, 0), heads / c.kv_heads * tokens, c.head_dim);   // launches follow one another on the stream and share it
+  const int n = min(page::MOST_SEQUENCES, c.batch);
+  return page_tile_bytes(page_arrays(c, 0), n, heads / c.kv_heads * tokens, c.head_dim);   // launches follow one another on the stream and share it
 }
 
 int page_attend(const nkv_page_cache& c, const nkv_tokens& q, int tokens, const int32_t* counts, const uint32_t* mask,

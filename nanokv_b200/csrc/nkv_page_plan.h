@@ -108,6 +108,22 @@ NKV_PAGE_INLINE int rounds_of(uint64_t bytes, uint32_t places, int blocks, int l
   while (rounds < most_rounds && bytes > FITS * rounds && places / blocks / (rounds + 1) >= static_cast<uint32_t>(least)) ++rounds;
   return rounds;
 }
+// Of the counts that let a round read between FITS and twice that (L2 holds 126 MB), the one whose runs come closest to a whole number
+// of runs a unit: units of a kv head then start and end together and go in step.
+NKV_PAGE_INLINE int rounds_for(uint64_t bytes, uint32_t places, uint32_t units, int blocks, int least, int most_rounds) {
+  const int most = rounds_of(bytes, places, blocks, least, most_rounds);
+  int best = 0;
+  uint32_t off = UINT32_MAX;
+  for (int rounds = rounds_of(bytes / 2, places, blocks, least, most_rounds); rounds <= most; ++rounds) {
+    const uint32_t runs = static_cast<uint32_t>(rounds) * blocks, over = runs % units;
+    const uint32_t away = runs < units || units - over < over ? units - over : over;
+    if (away < off) {
+      off = away;
+      best = rounds;
+    }
+  }
+  return best;
+}
 
 // The pieces of one run in order.
 struct Walk {

@@ -59,10 +59,20 @@ constexpr int QT = 128;                           // rows of a query tile
 constexpr int SUB = 128 * 128;                    // bytes of a [128 rows x 64 elements] swizzled tile
 constexpr int SOFTMAX_WARPS = 8, OPERAND_WARPS = 2, MMA_WARP = 10, THREADS = 384;
 constexpr float RESCALE_THRESHOLD = 8.0f;
-// Rounds that there is scratch for, and places of a run that a cut more is worth.  4,680 queries x 24 heads over 24,960 tokens in 1 / 2 / 3 / 4 rounds:
-// 1,335 / 1,335 / 1,191 / 1,238 us, 5.06 GB read from memory in one and 0.58 in three (a run is one unit then, and a head's units go in step);
-// 1,560 x 40 heads over 98,560 x 8 in 2 / 3 / 4: 2,712 / 2,760 / 2,600.
-constexpr int MOST_ROUNDS = 3, LEAST_RUN = 64;
+// Rounds that there is scratch for, and places of a run that a cut more is worth.  us in 1 / 2 / 3 / 4 / 5 / 6 / 8 rounds, heads of 128, quarters
+// of a second of each in shuffled order over three states, at the power limit; queries x heads over tokens x kv heads (MB of them, units):
+//   4,680 x 24 over 24,960 x 24 (307, 456)           1,632 1,603 1,424 1,472 1,483 1,451 1,486   5.06 GB read from memory in one, 0.58 in three
+//   1,560 x 40 over 100,120 x 8 (410, 248)           3,509 3,512 3,402 3,249 3,054 3,215 3,097
+//   6,000 x 8 over 66,000 x 8 (270, 192)             1,805 1,793 1,672 1,579 1,653 1,626 1,615
+//   2,048 x 40 over 18,432 x 40, causal (377, 320)     838   815   811   802   824   819   835
+//   4 x 512 x 32 over 32,768 x 8, causal (537, 256)  1,225 1,232 1,222 1,169 1,192 1,155 1,166
+//   1,560 x 24 over 24,960 x 24 (307, 168)             604   583   577   571   594   592   626
+//   4,095 x 32 over 24,095 x 8, causal (99, 512)     1,411 1,396 1,427 1,457 1,477 1,484 1,567
+//   2 x 1,024 x 24 over 13,312 x 24 (327, 192)         402   387   408   400   419   428   456   140 places a run in one round
+//   600 x 40 over 30,600 x 40 (627, 120)               515   523   532   518   531   538   571   200 places
+//   8 x 333 x 16 over 8,500 x 16, causal (557, 256)    303   312   329   338   353   354   367   120 places
+// The rule takes 3, 5, 4, 4, 5, 3, 2, 2, 3 and 1.
+constexpr int MOST_ROUNDS = 5, LEAST_RUN = 64;
 constexpr float NOTHING = -3e38f;                 // the reference before the first score: below all, and a number
 
 // (P_READY: chain i, half h of a tile's tokens at 2 i + h)
@@ -892,7 +902,7 @@ page_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     __syncthreads();
   }
   if (warp == 0) {
-    uint32_t carry = 0;
+    uint32_t carry = 0, units = 0;
     uint64_t tokens = 0;
     for (int b0 = 0; b0 <= a.sequences; b0 += 32) {
       const int b = b0 + lane;
@@ -908,7 +918,10 @@ page_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           cost = start[b];
         }
         cost *= a.shape.kv_heads;
-        if (cost) tokens += extents[b].length + extents[b].there;
+        if (cost) {
+          tokens += extents[b].length + extents[b].there;
+          units += a.shape.units * a.shape.kv_heads;
+        }
       }
       uint32_t upto = cost;
 #pragma unroll
@@ -921,8 +934,10 @@ page_tile_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) tokens += __shfl_xor_sync(0xffffffffu, tokens, x);
+    units = __reduce_add_sync(0xffffffffu, units);
     if (lane == 0)
-      *reinterpret_cast<volatile int*>(smem + M_ROUNDS) = page::rounds_of(tokens * (4ull * D * a.shape.kv_heads), carry, gridDim.x, LEAST_RUN, a.most_rounds);
+      *reinterpret_cast<volatile int*>(smem + M_ROUNDS) =
+          page::rounds_for(tokens * (4ull * D * a.shape.kv_heads), carry, max(units, 1u), gridDim.x, LEAST_RUN, a.most_rounds);
   }
   tc_fence_before();
   __syncthreads();
@@ -1019,16 +1034,16 @@ join_parts_kernel(TileCall a, Parts parts) {
 }
 
 int unit_of(int rows) { return rows > QT ? 2 * QT : QT; }
-// Units of a kv head that share its keys and values, in a pool larger than what a round is to read.
-int most_rounds_of(const PageArrays& c, int rows, int d) {
-  const uint64_t pool = (static_cast<uint64_t>(c.pages) * c.kv_heads << c.shift) * 4 * d;
-  return rows > unit_of(rows) && pool > page::FITS ? MOST_ROUNDS : 1;
+// Units of a kv head that share its keys and values, in more of the pool than a round is to read.
+int most_rounds_of(const PageArrays& c, int n, int rows, int d) {
+  const uint64_t tokens = min(static_cast<uint64_t>(c.pages), static_cast<uint64_t>(c.row_pages) * n) << c.shift, bytes = tokens * c.kv_heads * 4 * d;
+  return rows > unit_of(rows) ? static_cast<int>(min((bytes + page::FITS - 1) / page::FITS, static_cast<uint64_t>(MOST_ROUNDS))) : 1;
 }
 
 }  // namespace
 
-size_t page_tile_bytes(const PageArrays& c, int rows, int d) {
-  return static_cast<size_t>(sm_count()) * most_rounds_of(c, rows, d) * (2 * unit_of(rows) * (d * sizeof(float) + sizeof(float2)) + sizeof(Cut));
+size_t page_tile_bytes(const PageArrays& c, int n, int rows, int d) {
+  return static_cast<size_t>(sm_count()) * most_rounds_of(c, n, rows, d) * (2 * unit_of(rows) * (d * sizeof(float) + sizeof(float2)) + sizeof(Cut));
 }
 
 int page_tile(const PageArrays& c, const PageCall& call, int n, int dtype, int d, void* workspace, int32_t* status, cudaStream_t stream) {
@@ -1044,7 +1059,7 @@ int page_tile(const PageArrays& c, const PageCall& call, int n, int dtype, int d
   const int runs = static_cast<int>(min(most, static_cast<uint64_t>(sm_count())));
   Parts parts;
   parts.o = static_cast<float*>(workspace);
-  a.most_rounds = most_rounds_of(c, a.rows, d);
+  a.most_rounds = most_rounds_of(c, n, a.rows, d);
   const size_t places = static_cast<size_t>(sm_count()) * a.most_rounds * 2 * unit;
   parts.ml = reinterpret_cast<float2*>(parts.o + places * d);
   parts.cut = reinterpret_cast<Cut*>(parts.ml + places);
