@@ -17,7 +17,7 @@ struct Side {
 
 // A thread takes two 16-byte pieces of a head row whose elements are each other's partners (or two that are only copied), of HEADS
 // heads, which share the table's entries and the page; one where the call is short of threads.  Bound: memory (24,967 tokens x 40 heads of
-// keys, values and queries: 1.55 GB in and out in 255 us, 6.1 TB/s); the smallest calls the chain of loads, length, page, store (32 tokens x 56 heads
+// keys, values and queries: 1.55 GB in and out in 270 us, 5.7 TB/s); the smallest calls the chain of loads, length, page, store (32 tokens x 56 heads
 // 2.7 us).  Rows of the call are counted from row0 on; a launch has fewer than 2^31 threads.
 template <int DT, int HEADS>
 __global__ void __launch_bounds__(256)
@@ -104,7 +104,8 @@ struct Kept {
 
 // A thread moves one 16-byte column of a kv head: the rows of the path lie at or behind the places they move to, in order, so
 // that none is written before it is read; a node ahead of its place, as those behind a refused one may be, is refused as well.  Bound:
-// the chain length, node, page, row (one sequence 2.0 us); 32 sequences x 40 layers x 9 rows of 8 heads 8.4 us.
+// the chain length, node, page, row (one sequence 2.0 us); 32 sequences x 40 layers x 9 rows of 8 heads 9.2 us over four states in turn
+// (47 MB, 5.1 TB/s), 8.2 over one, whose rows stay in L2.
 constexpr int AT_ONCE = 8;   // rows in flight
 __global__ void __launch_bounds__(256)
 page_keep_kernel(const __grid_constant__ Kept kept, PageArrays c, const int32_t* path, int accepted, const int32_t* counts, int d,
@@ -152,7 +153,7 @@ page_keep_kernel(const __grid_constant__ Kept kept, PageArrays c, const int32_t*
 // ---- tree mask --------------------------------------------------------------------------------------------------
 
 // A thread per node and word walks the node's ancestors as far as the word's first node: parents are in shared memory, and a draft is a few
-// levels deep (a chain of n nodes takes n steps).  16 nodes 2.0 us, 32 drafts of 511 nodes 3.6 us, both a launch's latency.
+// levels deep (a chain of n nodes takes n steps).  16 nodes 1.7 us, 32 drafts of 511 nodes 3.3 us, both a launch's latency.
 __global__ void __launch_bounds__(256)
 tree_mask_kernel(const int32_t* parents, int tokens, int words, uint32_t* mask, int32_t* depth, int32_t* status) {
   extern __shared__ int32_t up[];

@@ -71,9 +71,10 @@ NKV_PAGE_INLINE int tiles_seen(const Shape& s, const Extent& e, int r0, int n) {
   return (seen + TOK - 1) / TOK;
 }
 
-// A unit costs a run as much as PIECE_TILES tiles on top of its own: its queries' way in and its rows' way out (2 x 4,095 causal
-// queries x 32 heads, costs of 2 / 3 / 5 / 7 / 9: 356 / 347 / 313 / 317 / 323 us; one token each of 31 sequences of up to 2,138 x 320 heads 144 /
-// 138 / 127 / 129 / 133; 99,840 tokens x 40 heads 306 / 307 / 312 / 310 / 308).
+// A unit costs a run as much as PIECE_TILES tiles on top of its own: its queries' way in and its rows' way out (costs of 2 / 3 / 5 / 7 / 9,
+// over four states in turn, us: 2 x 4,095 causal queries x 32 heads fp16 375 / 371 / 352 / 357 / 361, bf16 372 / 368 / 348 / 354 / 358; one token each of
+// 31 sequences of up to 2,138 x 320 heads 197 / 189 / 180 / 174 / 177, of 32 of up to 4,096 x 32 heads over 8 77 / 73 / 70 / 69 / 71; 32 trees of 16 nodes
+// 240 / 236 / 235 / 238 / 238, 8 of 63 nodes over 64-wide heads 56 / 55 / 54 / 54 / 56; 99,840 tokens x 40 heads 336 to 339 with each).
 constexpr uint32_t PIECE_TILES = 5;
 NKV_PAGE_INLINE uint32_t cost_of(int tiles) { return tiles > 0 ? tiles + PIECE_TILES : 0; }
 

@@ -11,7 +11,8 @@
 //
 // Softmax: P' = 2^(s - m) with a reference m that follows the running maximum of the scaled scores, s; it moves when P' would pass
 // 2^8 times what it was set to.  bf16: set so that the sum of a row's P' stays below 1, O = sum P' V then below the largest |V|, any
-// number of bf16.  fp16: P' up to 2^15, so that weights down to 2^-29 of the largest keep all their bits.  The row sum, the maximum and O
+// number of bf16.  fp16: set to 2^7, up to 2^15 from there: weights down to 2^-21 of the largest keep all their bits (2^-29 at
+// best), smaller ones have half a step of 2^-25 where the largest has at least 2^7.  The row sum, the maximum and O
 // stay in fp32.  P' enters the product with V in 16 bits: fp16 rounded to nearest; bf16 as the upper half of its fp32 bits, a byte
 // permutation instead of a conversion.  What is cut off is up to 2^-7 of a weight and, where many weights are alike, the same for all of
 // them: so rows of O are divided by the sum of the weights as they entered the product, two additions more a pair of scores, and lse
@@ -28,13 +29,15 @@
 // A page of K or V comes as one copy, whatever its size: the tensor map has the eight rows of a swizzle group, the 64-element chunks of a
 // row and the groups of a page as dimensions, so that a tile is its groups one behind the other, each with its chunks side by side.
 //
-// Measured (kernel and join): one query token over 99,840 tokens x 40 heads 307 us (2.04 GB, 6.6 TB/s: memory); 32 trees of 16 nodes x 40 heads over
-// up to 16,411 tokens x 8 heads 191 us (5.7 TB/s); 4,680 queries x 24 heads over 24,960 tokens 1.20 ms (1,200 TFLOP/s, at the clock that the power
-// limit leaves), 2 x 4,095 causal queries x 32 heads 313 us.  What bounds the wide form: the MMA warp, whose six batches a tile pair (S and two
+// Measured (kernel and join; over three states in turn, a quarter of a second long / six calls after a second's rest: the difference is the
+// clock that the power limit leaves, one state or several are alike): one query token over 99,840 tokens x 40 heads 336 / 311 us (2.04 GB, 6.1 /
+// 6.6 TB/s: memory); 32 trees of 16 nodes x 40 heads over up to 16,411 tokens x 8 heads 233 / 199 us (4.6 / 5.4 TB/s; as many bytes of one
+// sequence 225 / 191, in pages of 64 for 16 tokens 205 / 186); 4,680 queries x 24 heads over 24,960 tokens 1.43 / 1.26 ms (1,000 / 1,140 TFLOP/s),
+// 2 x 4,095 causal queries x 32 heads 352 / 337 us.  What bounds the wide form: the MMA warp, whose six batches a tile pair (S and two
 // halves of PV for both query tiles, 2,048 tensor cycles) take about 3,400 cycles with the waits between them, and power: reading K and V from L2
 // instead of memory gave 10 % (rounds, below).  Small calls: two launches, the plan, and a chain of table, tile, two products, rows.
-// Tried and dropped (4,680 queries, us, kept form first): exponentials ahead of the row's maximum (1,333 / 1,390; with straight code and a fallback
-// 1,345 / 1,368); K awaited with the weights (1,333 / 1,362); two barriers per wait (1,339 / 1,393); waits without parking (no change); P
+// Tried and dropped (4,680 queries, us, kept form first, before the weights' second sum): exponentials ahead of the row's maximum (1,333 /
+// 1,390; with straight code and a fallback 1,345 / 1,368); K awaited with the weights (1,333 / 1,362); two barriers per wait (1,339 / 1,393); waits without parking (no change); P
 // beside S in tensor memory for 64-wide heads (no change); two more copies' bits by a second product (batch of trees 238 / 324).
 //
 // Table, lengths and counts are read by the kernel: every thread block makes the plan (nkv_page_plan.h) for itself.  The tiles of all
@@ -1084,7 +1087,7 @@ int page_tile(const PageArrays& c, const PageCall& call, int n, int dtype, int d
                                      : run(page_tile_kernel<NKV_F16, 128, COPIES>, Layout<128, COPIES>::DYNAMIC))                         \
                 : (dtype == NKV_BF16 ? run(page_tile_kernel<NKV_BF16, 64, COPIES>, Layout<64, COPIES>::DYNAMIC)                           \
                                      : run(page_tile_kernel<NKV_F16, 64, COPIES>, Layout<64, COPIES>::DYNAMIC))
-  // The forms by rows (32 sequences of up to 16,411 tokens, 8 kv heads of 128, bf16): narrow against wide at 65 / 80 / 125 rows 198 / 200 /
+  // The forms by rows (32 sequences of up to 16,411 tokens, 8 kv heads of 128, bf16, short runs, before the weights' second sum): narrow against wide at 65 / 80 / 125 rows 198 / 200 /
   // 209 against 228 / 229 / 235 us.  Four copies are for what they add to the weights' bits, and cost 1 % (5 rows 188 us, 187 without; over
   // up to 700 tokens 32.2 and 30.1); two copies of up to 64 rows gained nothing (60 rows 199 us, 196 without).
   if (a.rows > QT) NKV_PAGE_RUN(0);
