@@ -60,7 +60,9 @@ class PageTable:
             raise ValueError(f"a pool has at least one page; got {pages}")
         self.table, self.lengths, self.pages, self.page = table, lengths, int(pages), int(page)
         self.batch, self.device = table.shape[0], table.device
-        self.status = ops.status_word(self.device)      # what calls report into (ops.check_status)
+        self.status = ops._word(self.device)            # what calls report into (ops.check_status)
+        if self.status is None:
+            raise RuntimeError("the first table of a device is made outside a graph capture: its status word would be the graph's")
 
     @property
     def capacity(self) -> int:

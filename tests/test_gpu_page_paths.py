@@ -87,3 +87,21 @@ def test_a_captured_keep_reports_into_its_tables_word(monkeypatch):
     torch.cuda.synchronize()
     assert int(word) == 920 and not ops._STATUS_WORDS
     word.zero_()
+
+
+def test_the_first_table_is_not_made_inside_a_capture(monkeypatch):
+    table, lengths = torch.zeros(1, 4, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    kept = torch.ones(1, device="cuda")
+    monkeypatch.setattr(ops, "_STATUS_WORDS", {})
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept.add_(1)
+        with pytest.raises(RuntimeError, match="outside a graph capture"):
+            PageTable.over(table, lengths, pages=4, page=16)
+    assert not ops._STATUS_WORDS
+    graph.replay()
+    assert float(kept) == 2
+    PageTable.over(table, lengths, pages=4, page=16)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        kept.add_(1)
+        PageTable.over(table, lengths, pages=4, page=16)
